@@ -42,7 +42,8 @@ typedef enum {
   XRGPU_UINT8 = 6,
   XRGPU_INT64 = 7,
   XRGPU_BOOL = 8,
-  XRGPU_UNSPECIFIED = 9
+  XRGPU_UNSPECIFIED = 9,
+  XRGPU_FLOAT8_E4M3 = 10   /* extension: codes of the 8-bit key/value cache only */
 } xrgpu_dtype;
 
 /* Status codes in place of the reference's exceptions:
@@ -452,6 +453,108 @@ typedef struct {
 
 XRGPU_API int xrgpu_qmoe_workspace_size(const xrgpu_qmoe_problem* p, uint64_t* bytes);
 XRGPU_API int xrgpu_qmoe_forward(const xrgpu_qmoe_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Block-scaled serving operators (extensions; no counterpart in the reference): microscaled 4-bit
+ * floating point, and a paged key/value cache of 8-bit codes with the attention that reads it.
+ * All enqueue on `stream` and return; pointers are device pointers of the current device.
+ * ------------------------------------------------------------------------------------- */
+
+/* Microscaled 4-bit floating point. A row of K values is held in kb = ceil(K / 32) blocks of 32 (the
+ * last one padded with zeros): 32 codes of 4 bits (sign, two exponent bits, one mantissa bit: 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6), low nibble first, and one scale byte e; value = code * 2^(e - 127), e = 255: NaN.
+ *   codes  uint8 [rows, kb, 16], 16-byte aligned
+ *   scales uint8 [ceil(rows / 128), ceil(kb / 4), 32, 4, 4], 16-byte aligned: the byte of (row r, block j) at
+ *          [r / 128][j / 4][r % 32][(r % 128) / 32][j % 4], padding 0 (the tensor cores' order). */
+typedef struct {
+  int32_t dtype;     /* of the unquantised side: XRGPU_FLOAT16 or XRGPU_FLOAT32 */
+  int32_t reserved;
+  int64_t rows, K;
+  uint8_t* codes;
+  uint8_t* scales;
+} xrgpu_mxfp4_tensor;
+
+/* Bytes of the tiled scales of a [rows, K] matrix. */
+XRGPU_API int xrgpu_mxfp4_scale_bytes(int64_t rows, int64_t K, uint64_t* bytes);
+
+/* x [rows, ldx] (ldx 0: K) -> t->codes, t->scales (padding included). Per block: e = max(floor(log2 max|x|) - 2,
+ * -127) + 127, code = x * 2^(127 - e) rounded to nearest (ties to the even code), saturating at 6, sign kept; a
+ * block with a NaN or an infinity gets e = 255 and codes 0. */
+XRGPU_API int xrgpu_mxfp4_quantize(const xrgpu_mxfp4_tensor* t, const void* x, int64_t ldx, void* stream);
+
+/* The values t holds -> out [rows, K] (contiguous, t->dtype). */
+XRGPU_API int xrgpu_mxfp4_dequantize(const xrgpu_mxfp4_tensor* t, void* out, void* stream);
+
+/* Scale bytes [rows, blocks], as checkpoints hold them, -> the tiled order. */
+XRGPU_API int xrgpu_mxfp4_tile_scales(int64_t rows, int64_t blocks, const uint8_t* scales, uint8_t* tiled, void* stream);
+
+/* y[m, n] = sum_k a[m, k] * b[n, k] (+ bias[n]), both operands microscaled 4-bit, float32 sums. */
+typedef struct {
+  int32_t dtype;            /* of y and bias: XRGPU_FLOAT16 or XRGPU_FLOAT32 */
+  int32_t a_dtype;          /* XRGPU_UINT8: a holds codes; XRGPU_FLOAT16 / XRGPU_FLOAT32: quantised by the call */
+  int64_t M, K, N;
+  const void* a;            /* codes [M, kb, 16], or floats [M, lda] */
+  const uint8_t* a_scales;  /* tiled (a_dtype XRGPU_UINT8), else NULL */
+  int64_t lda;              /* row stride of float activations in elements; 0 means K */
+  const uint8_t* b;         /* codes [N, kb, 16] */
+  const uint8_t* b_scales;  /* tiled */
+  const void* bias;         /* [N] or NULL */
+  void* y;                  /* [M, ldy] */
+  int64_t ldy;              /* row stride of y in elements; 0 means N */
+} xrgpu_mxfp4_problem;
+
+/* Device scratch bytes of xrgpu_mxfp4_forward (the quantised activations; 0 for codes). */
+XRGPU_API int xrgpu_mxfp4_workspace_size(const xrgpu_mxfp4_problem* p, uint64_t* bytes);
+/* workspace: 16-byte aligned device scratch, any content; NULL: the library's per-device workspace (grown on
+ * demand). Calls sharing a workspace must not overlap on the GPU. */
+XRGPU_API int xrgpu_mxfp4_forward(const xrgpu_mxfp4_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Paged key/value cache of 8-bit codes, one float32 scale for each page of each head: value = code * scale.
+ *   k_cache, v_cache [pages, heads_kv, page, head_dim] of int8 or float8 e4m3, 16-byte aligned;
+ *   k_scale, v_scale [pages, heads_kv]; page 16, 32, 64 or 128 tokens; head_dim 64 or 128.
+ * Sequence b holds kv_len[b] tokens, token j in page page_table[b][j / page], slot j % page. The rows of a
+ * call are the LAST tokens of their sequences: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (NULL: tokens /
+ * sequences rows each), row cu_seqlens[b] + i at position kv_len[b] - n_b + i. Rows behind the last sequence
+ * are left as they were. A page id outside the pool (0x501) or lengths that do not fit (0x502: rows, table, or more
+ * new tokens than kv_len) are recorded in the device error word (xrgpu_device_error), and what they would
+ * have reached is skipped: nothing out of range is read or written. */
+typedef struct {
+  int32_t dtype;        /* T1 of q, k, v, o: XRGPU_FLOAT16 or XRGPU_FLOAT32 */
+  int32_t cache_dtype;  /* XRGPU_INT8 or XRGPU_FLOAT8_E4M3 */
+  int32_t causal;       /* attention: nonzero: a row sees the tokens up to its own position */
+  float scale;          /* attention: factor of q . k, usually head_dim^-1/2 */
+  int64_t tokens;       /* rows of q, k, v, o */
+  int64_t sequences, heads_q, heads_kv, head_dim, page, pages, max_pages;
+  int64_t window;       /* attention, causal: a row sees the last `window` tokens up to itself; 0: all */
+  int64_t q_stride, k_stride, v_stride, o_stride;  /* row strides in elements; 0: contiguous */
+  const void* q;        /* attention: [tokens, heads_q, head_dim] */
+  void* k;              /* append: new keys [tokens, heads_kv, head_dim]; read: where they go */
+  void* v;
+  void* o;              /* attention: [tokens, heads_q, head_dim] */
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* page_table;  /* [sequences, max_pages] */
+  const int32_t* cu_seqlens;  /* [sequences + 1] or NULL */
+  const int32_t* kv_len;      /* [sequences], the rows of this call included */
+} xrgpu_kv8_problem;
+
+/* Writes new keys and values into the cache. Per page and head, s = max(stored scale if the page holds older
+ * tokens of the sequence, else 0; max|x| / L), L = 127 (int8) or 448 (e4m3); new codes round(x / s), older ones
+ * round(code * s_old / s) when the scale grows, to nearest, ties to even. A NaN or an infinity makes the block's
+ * scale NaN. A page that two sequences share must not be appended to. */
+XRGPU_API int xrgpu_kv8_append(const xrgpu_kv8_problem* p, void* stream);
+
+/* The values that the cache holds for the rows' positions -> k, v. */
+XRGPU_API int xrgpu_kv8_read(const xrgpu_kv8_problem* p, void* stream);
+
+/* o[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j of the row's sequence that it sees;
+ * query head h reads key/value head h / (heads_q / heads_kv). A row that sees nothing gives zeros (cu_seqlens may
+ * hold more rows than kv_len tokens here; the first ones then see nothing). */
+XRGPU_API int xrgpu_kv8_attention_workspace_size(const xrgpu_kv8_problem* p, uint64_t* bytes);
+/* workspace as in xrgpu_mxfp4_forward. */
+XRGPU_API int xrgpu_kv8_attention(const xrgpu_kv8_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Library version string. */
 XRGPU_API const char* xrgpu_version(void);

@@ -1,0 +1,453 @@
+"""The paged 8-bit key/value cache: refusals on the CPU; append, read back and attention on the GPU against plain
+64-bit restatements (serving_reference), and a decoder layer's run of the operators together."""
+import ctypes
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import serving_reference as R
+from xrgpu_b200 import _native
+
+gpu = pytest.mark.gpu
+INT8, E4M3 = torch.int8, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def F(cuda_lib):
+    from xrgpu_b200 import functional
+    return functional
+
+
+# ------------------------------------------------------------------------------------------ refusals (no GPU)
+def _problem(**kw):
+    p = _native.Kv8Problem_()
+    p.dtype, p.cache_dtype, p.causal, p.scale = _native.FLOAT16, _native.INT8, 1, 0.125
+    p.tokens, p.sequences, p.heads_q, p.heads_kv, p.head_dim, p.page, p.pages, p.max_pages = 2, 2, 4, 2, 64, 16, 4, 2
+    for n in ("q", "k", "v", "o", "k_cache", "v_cache", "k_scale", "v_scale", "page_table", "kv_len"):
+        setattr(p, n, 4096)
+    for n, v in kw.items():
+        setattr(p, n, v)
+    return p
+
+
+BOTH = [
+    (dict(dtype=_native.INT8), "T1"), (dict(cache_dtype=_native.UINT8), "cache codes"), (dict(head_dim=80), "head_dim"),
+    (dict(page=24), "page"), (dict(page=256), "page"), (dict(tokens=-1), "geometry"), (dict(sequences=70000), "geometry"),
+    (dict(heads_kv=0), "geometry"), (dict(max_pages=1 << 30), "geometry"), (dict(tokens=3), "multiple of sequences"),
+    (dict(k_cache=4104), "aligned"), (dict(kv_len=None), "null"), (dict(page_table=None), "null"), (dict(v_scale=None), "null"),
+]
+
+
+@pytest.mark.parametrize("change,message", BOTH + [(dict(k=None), "null"), (dict(k_stride=127), "stride"), (dict(v_stride=1), "stride")])
+def test_append_refusals(cuda_lib, change, message):
+    for fn in (cuda_lib.xrgpu_kv8_append, cuda_lib.xrgpu_kv8_read):
+        assert fn(ctypes.byref(_problem(**change)), None) == _native.INVALID_ARGUMENT
+        assert message in cuda_lib.xrgpu_last_error().decode()
+
+
+@pytest.mark.parametrize("change,message", BOTH + [
+    (dict(heads_q=3), "heads_q"), (dict(heads_q=0), "heads_q"), (dict(window=-1), "window"), (dict(window=4, causal=0), "window"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=None), "null"), (dict(o=None), "null"),
+    (dict(q_stride=255), "stride"), (dict(o_stride=255), "stride"), (dict(tokens=1 << 30, sequences=1), "geometry")])
+def test_attention_refusals(cuda_lib, change, message):
+    assert cuda_lib.xrgpu_kv8_attention(ctypes.byref(_problem(**change)), None, 0, None) == _native.INVALID_ARGUMENT
+    assert message in cuda_lib.xrgpu_last_error().decode()
+
+
+def test_empty_calls_need_no_gpu(cuda_lib):
+    for change in (dict(tokens=0), dict(sequences=0, tokens=0)):
+        assert cuda_lib.xrgpu_kv8_attention(ctypes.byref(_problem(**change)), None, 0, None) == 0
+        need = ctypes.c_uint64(7)
+        assert cuda_lib.xrgpu_kv8_attention_workspace_size(ctypes.byref(_problem(**change)), ctypes.byref(need)) == 0
+        assert need.value == 0
+
+
+def test_python_refusals(F):
+    c = R.Cache([20, 3], heads=2, D=64, page=16, code=INT8)
+    q = torch.zeros(2, 4, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.attention_kv8(q, c.k, c.v, c.ks, c.vs, c.table, None, c.lens)
+    with pytest.raises(ValueError, match="int8 or float8"):
+        F.attention_kv8(q, c.k.float(), c.v, c.ks, c.vs, c.table, None, c.lens)
+    with pytest.raises(ValueError, match="page, head_dim"):
+        F.attention_kv8(q, c.k[0], c.v, c.ks, c.vs, c.table, None, c.lens)
+
+
+# ------------------------------------------------------------------------------------------ append, read back
+def _cu(new):
+    return torch.tensor([0] + list(new), dtype=torch.int32).cumsum(0).to(torch.int32)
+
+
+APPEND = [
+    # past, new per sequence
+    ([0], [1]), ([15], [1]), ([16], [1]), ([5, 0, 33], [1, 1, 1]), ([0, 7], [40, 1]), ([3, 16, 0, 100], [0, 17, 129, 2]),
+    ([31], [32]), ([250], [300]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("page,D", [(16, 64), (64, 128), (128, 64), (32, 128)])
+@pytest.mark.parametrize("past,new", APPEND)
+def test_append_is_exact(F, code, dtype, page, D, past, new):
+    c = R.Cache([a + b for a, b in zip(past, new)], heads=3, D=D, page=page, code=code, seed=page + D)
+    c.poison_tails()
+    T = sum(new)
+    g = torch.Generator().manual_seed(T)
+    k, v = (torch.randn(T, 3, D, generator=g).to(dtype) * torch.where(torch.rand(T, 3, 1, generator=g) < 0.3, 6.0, 0.5).to(dtype) for _ in range(2))
+    cu = _cu(new)
+    dev = c.cuda()
+    F.kv8_append(k.cuda(), v.cuda(), *dev, cu.cuda(), c.lens.cuda())
+    R.append(c, k, v, cu)
+    for got, want in zip(dev[:4], (c.k, c.v, c.ks, c.vs)):
+        as_bytes = lambda t: t.cpu().contiguous().view(torch.uint8 if t.element_size() == 1 else torch.int32)  # noqa: E731
+        # codes may differ in the sign of zero only (e4m3)
+        same = (as_bytes(got) == as_bytes(want)) | ((as_bytes(got) & 0x7F) + (as_bytes(want) & 0x7F) == 0 if code == E4M3 and got.element_size() == 1 else False)
+        both_nan = torch.isnan(got.cpu()) & torch.isnan(want) if got.dtype == torch.float32 else torch.tensor(False)
+        assert bool((same | both_nan).all())
+    # what the cache holds for the new tokens, rounded once to the rows' type
+    rk, rv = F.kv8_read(*dev, cu.cuda(), c.lens.cuda(), rows=T, dtype=dtype)
+    for got, which in ((rk, 0), (rv, 1)):
+        want = np.concatenate([c.tokens(b)[which][past[b]:] for b in range(len(new))])
+        assert torch.equal(got.cpu(), torch.from_numpy(want).float().to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+def test_append_borders_round_to_even(F, code):
+    """Quotients that lie on and next to the borders between codes, with scales that are no powers of two."""
+    D, L = 64, R.LIMIT[code]
+    x = torch.zeros(16, 1, D)
+    rng = np.random.default_rng(3)
+    for t in range(16):
+        a = np.float32(rng.uniform(1, 9))
+        s = np.float32(a / np.float32(L))
+        q = rng.integers(-126, 126, D) + 0.5 if code == INT8 else np.ldexp(rng.integers(8, 16, D) + 0.5, rng.integers(-5, 5, D))
+        v = (np.abs(q) * np.float64(s)).astype(np.float32)  # the float32 numbers next to the borders
+        v = np.nextafter(v, np.where(rng.random(D) < 0.5, np.float32(0), np.float32(1e9))) if t % 2 else v
+        x[t, 0] = torch.from_numpy(v.astype(np.float32))
+        x[t, 0, 0] = float(a)
+    x = x.clamp(max=float(x[:, 0, 0].max()))
+    for n in range(16):  # a page of its own for each, so that each has its own scale
+        c = R.Cache([1], heads=1, D=D, page=16, code=code, seed=n)
+        dev = c.cuda()
+        row = x[n:n + 1]
+        F.kv8_append(row.cuda(), row.cuda(), *dev, _cu([1]).cuda(), c.lens.cuda())
+        R.append(c, row, row, _cu([1]))
+        assert torch.equal(dev[0].cpu().float(), c.k.float()) and torch.equal(dev[2].cpu(), c.ks)
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+def test_append_token_by_token_rescales(F, code):
+    """Growing values rescale a page again and again; the state stays the definition's."""
+    c = R.Cache([0], heads=2, D=64, page=32, code=code, max_extra=3)
+    c.table[0, :3] = torch.tensor([2, 0, 1])
+    c = R.Cache([70], heads=2, D=64, page=32, code=code)
+    dev = c.cuda()
+    for i in range(70):
+        c.lens[0] = i + 1
+        k = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(i)) * (1.0 + 0.2 * i)
+        v = k.flip(-1) * (0.1 if i % 3 else 0.0)
+        F.kv8_append(k.cuda(), v.cuda(), *dev, _cu([1]).cuda(), c.lens.cuda())
+        R.append(c, k, v, _cu([1]))
+    ids = c.table[0, :3].long()
+    for got, want in zip(dev[:2], (c.k, c.v)):
+        w = want[ids].float().transpose(1, 2).reshape(-1, 2, 64)[:70]
+        assert torch.equal(got.cpu()[ids].float().transpose(1, 2).reshape(-1, 2, 64)[:70], w)
+    assert torch.equal(dev[2].cpu()[ids], c.ks[ids]) and torch.equal(dev[3].cpu()[ids], c.vs[ids])
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+def test_append_non_finite_poisons_its_block_only(F, code):
+    c = R.Cache([20, 18], heads=2, D=64, page=16, code=code)
+    dev = c.cuda()
+    k = torch.randn(6, 2, 64)
+    v = torch.randn(6, 2, 64)
+    k[1, 0, 3], v[5, 1, 60] = float("nan"), float("-inf")
+    cu = _cu([4, 2])
+    F.kv8_append(k.cuda(), v.cuda(), *dev, cu.cuda(), c.lens.cuda())
+    R.append(c, k, v, cu)
+    for got, want in zip(dev[2:4], (c.ks, c.vs)):
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+        assert int(torch.isnan(want).sum()) == 1
+
+
+@gpu
+def test_append_refuses_bad_pages_and_lengths(F):
+    """Bad page ids, lengths past the table, more rows than tokens: recorded, nothing written for them."""
+    F.device_error(0)
+    for change, code in ((lambda c, cu: c.table.__setitem__((0, 1), 99), 0x501), (lambda c, cu: c.table.__setitem__((0, 1), -1), 0x501),
+                         (lambda c, cu: c.lens.__setitem__(0, 3), 0x502), (lambda c, cu: c.lens.__setitem__(0, 10 ** 6), 0x502),
+                         (lambda c, cu: cu.__setitem__(1, -5), 0x502), (lambda c, cu: c.lens.__setitem__(0, -1), 0x502)):
+        c = R.Cache([20, 18], heads=1, D=64, page=16, code=INT8)
+        cu = _cu([4, 2])
+        change(c, cu)
+        dev = c.cuda()
+        k = torch.randn(6, 1, 64).cuda()
+        F.kv8_append(k, k, *dev, cu.cuda(), c.lens.cuda())
+        assert F.device_error(0) == code
+        first = c.table[1, 1].item()  # of the pages, only the second sequence's may have changed
+        keep = [i for i in range(c.k.shape[0]) if i != first]
+        assert torch.equal(dev[0].cpu()[keep], c.k[keep]) and torch.equal(dev[2].cpu()[keep], c.ks[keep])
+        F.attention_kv8(torch.randn(6, 1, 64).cuda(), *dev, cu.cuda(), c.lens.cuda())
+        F.kv8_read(*dev, cu.cuda(), c.lens.cuda(), rows=6)
+        F.device_error(0)
+    assert F.device_error(0) == 0
+
+
+@gpu
+def test_append_strided_rows_and_rows_behind_the_last_sequence(F):
+    c = R.Cache([20, 5], heads=2, D=64, page=16, code=INT8)
+    fused = torch.randn(9, 8 * 64).half()
+    k, v = fused[:, 128:256].unflatten(1, (2, 64)), fused[:, 256:384].unflatten(1, (2, 64))
+    cu = _cu([4, 3])  # two padding rows
+    dev, d2 = c.cuda(), c.cuda()
+    fd = fused.cuda()
+    F.kv8_append(fd[:, 128:256].unflatten(1, (2, 64)), fd[:, 256:384].unflatten(1, (2, 64)), *dev, cu.cuda(), c.lens.cuda())
+    R.append(c, k.contiguous(), v.contiguous(), cu)
+    assert torch.equal(dev[0].cpu(), c.k) and torch.equal(dev[1].cpu(), c.v)
+    odd = torch.zeros(9, 130 + 1, dtype=torch.float16, device="cuda")[:, 1:129].unflatten(1, (2, 64))  # no 16-byte rows
+    odd.copy_(fd[:, 128:256].unflatten(1, (2, 64)))
+    F.kv8_append(odd, fd[:, 256:384].unflatten(1, (2, 64)), *d2, cu.cuda(), c.lens.cuda())
+    assert torch.equal(d2[0].cpu(), c.k) and torch.equal(d2[1].cpu(), c.v)
+    rk, _ = F.kv8_read(*dev, cu.cuda(), c.lens.cuda(), rows=9)
+    assert bool((rk[7:] == 0).all())
+
+
+# ------------------------------------------------------------------------------------------ attention
+def _check(F, c, new, hq, dtype, *, pad=0, q=None, uniform=False, **kw):
+    cu = _cu(new)
+    T = sum(new) + pad
+    if q is None:
+        q = torch.randn(T, hq, c.D, generator=torch.Generator().manual_seed(T + hq)).to(dtype)
+    want, tol = R.attention(c, q, cu, **kw)
+    got = F.attention_kv8(q.cuda(), *c.cuda(), None if uniform else cu.cuda(), c.lens.cuda(), **kw)
+    torch.cuda.synchronize()
+    assert F.device_error(0) == 0
+    g = got.cpu().double().numpy()[:sum(new)]
+    assert np.isfinite(g).all()
+    off = np.abs(g - want[:sum(new)]) - tol[:sum(new)]
+    assert (off <= 0).all(), float(off.max())
+    return got
+
+
+LENS = [
+    # lengths, new rows
+    ([1], [1]), ([17], [1]), ([64], [1]), ([300, 1, 65], [1, 1, 1]), ([2000], [1]), ([129, 40, 16], [5, 2, 9]), ([200], [200]),
+    ([77, 530], [33, 130]), ([40, 0, 90], [40, 0, 3]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("D,page,hq,hkv", [(128, 64, 8, 2), (64, 16, 5, 1), (128, 32, 12, 1), (64, 128, 3, 3)])
+@pytest.mark.parametrize("lens,new", LENS)
+def test_attention(F, code, dtype, D, page, hq, hkv, lens, new):
+    c = R.Cache(lens, heads=hkv, D=D, page=page, code=code, seed=D + hq)
+    c.poison_tails()
+    _check(F, c, new, hq, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("window", [1, 7, 16, 100, 5000])
+@pytest.mark.parametrize("lens,new", [([150], [1]), ([333, 20], [50, 20]), ([600], [140])])
+def test_attention_window(F, dtype, window, lens, new):
+    c = R.Cache(lens, heads=2, D=128, page=32, code=INT8)
+    c.poison_tails()
+    _check(F, c, new, 8, dtype, window=window)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("lens,new", [([40], [3]), ([100, 7], [20, 7]), ([5], [9]), ([290], [150])])
+def test_attention_without_causal_mask(F, dtype, lens, new):
+    c = R.Cache(lens, heads=2, D=64, page=16, code=E4M3)
+    c.poison_tails()
+    _check(F, c, new, 4, dtype, causal=False, scale=0.05)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_that_see_nothing_are_zero(F, dtype):
+    """Empty sequences, and more rows than tokens: their first rows see nothing."""
+    c = R.Cache([0, 3, 0], heads=2, D=64, page=16, code=INT8)
+    got = _check(F, c, [2, 5, 1], 4, dtype)
+    assert bool((got[:4] == 0).all()) and bool((got[7:] == 0).all()) and bool((got[4:7] != 0).any())
+    _check(F, R.Cache([0, 50], heads=1, D=128, page=32, code=E4M3), [150, 180], 2, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("new", [[3, 2], [70, 130]])
+def test_rows_behind_the_last_sequence_are_left(F, dtype, new):
+    c = R.Cache([150, 200], heads=2, D=128, page=64, code=INT8)
+    q = torch.randn(sum(new) + 9, 8, 128, device="cuda", dtype=dtype)
+    q[sum(new):] = float("nan")
+    out = torch.full_like(q, 3.0)
+    cu = _cu(new).cuda()
+    F.attention_kv8(q, *c.cuda(), cu, c.lens.cuda(), out=out)
+    assert bool((out[sum(new):] == 3.0).all()) and bool(torch.isfinite(out[:sum(new)]).all())
+    fresh = F.attention_kv8(q, *c.cuda(), cu, c.lens.cuda())
+    assert torch.equal(fresh[:sum(new)], out[:sum(new)]) and bool((fresh[sum(new):] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_attention_extreme_scores_and_scales(F, dtype):
+    """One token that takes all the weight, scores in the thousands, and value blocks of scales 2^20 apart."""
+    c = R.Cache([500, 300], heads=1, D=64, page=16, code=INT8)
+    c.vs *= torch.exp2(torch.randint(-10, 10, c.vs.shape).float())
+    c.ks[::3] *= 40.0
+    _check(F, c, [1, 2], 4, dtype)
+    c.ks.zero_()
+    c.vs[::2] = 0.0
+    _check(F, c, [1, 2], 4, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("new", [[1, 1], [1, 150]])
+def test_nan_blocks_reach_their_readers_only(F, dtype, new):
+    c = R.Cache([100, 160], heads=2, D=64, page=16, code=INT8)
+    c.vs[c.table[0, 2], 1] = float("nan")
+    q = torch.randn(sum(new), 4, 64, device="cuda", dtype=dtype)
+    o = F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda())
+    assert bool(torch.isnan(o[0, 2:]).all()) and bool(torch.isfinite(o[0, :2]).all()) and bool(torch.isfinite(o[1:]).all())
+    c.vs[c.table[0, 2], 1] = 1.0
+    c.ks[c.table[0, 2], 0] = float("nan")
+    o = F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda())
+    assert bool(torch.isnan(o[0, :2]).all()) and bool(torch.isfinite(o[0, 2:]).all()) and bool(torch.isfinite(o[1:]).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_strides_uniform_and_repeat(F, dtype):
+    """Queries inside a fused projection, an output with padding, no cu_seqlens; the same bits on every call."""
+    c = R.Cache([90, 33], heads=2, D=64, page=16, code=INT8)
+    fused = torch.randn(6, 1000, device="cuda", dtype=dtype)
+    q = fused[:, 3:3 + 256].unflatten(1, (4, 64))
+    out = torch.zeros(6, 300, device="cuda", dtype=dtype)[:, :256].unflatten(1, (4, 64))
+    F.attention_kv8(q, *c.cuda(), None, c.lens.cuda(), out=out)
+    want = F.attention_kv8(q.contiguous(), *c.cuda(), _cu([3, 3]).cuda(), c.lens.cuda())
+    assert torch.equal(out, want)
+    _check(F, c, [3, 3], 4, dtype, q=q.cpu().contiguous(), uniform=True)
+    for _ in range(3):
+        assert torch.equal(F.attention_kv8(q, *c.cuda(), None, c.lens.cuda()), want)
+
+
+@gpu
+def test_attention_bad_pages_are_skipped(F):
+    """A bad page id is recorded and its tokens are left out; a bad length gives its rows zeros."""
+    c = R.Cache([40, 40], heads=1, D=64, page=16, code=INT8)
+    q = torch.randn(2, 2, 64, dtype=torch.float16)
+    whole = F.attention_kv8(q.cuda(), *c.cuda(), None, c.lens.cuda())
+    for bad in (-1, c.k.shape[0], 2 ** 31 - 1):
+        c.table[0, 1] = bad
+        o = F.attention_kv8(q.cuda(), *c.cuda(), None, c.lens.cuda())
+        assert F.device_error(0) == 0x501
+        assert bool(torch.isfinite(o).all()) and torch.equal(o[1], whole[1])
+    for bad in (-3, 10 ** 6):
+        c.lens[0] = bad
+        o = F.attention_kv8(q.cuda(), *c.cuda(), None, c.lens.cuda())
+        assert F.device_error(0) == 0x502 and torch.equal(o[1], whole[1])
+
+
+@gpu
+def test_offsets_past_32_bits(F):
+    """Pages whose codes lie more than 2^32 bytes into the cache."""
+    P, H, page, D = 36000, 8, 128, 128  # 4.7 GB a side
+    k = torch.zeros(P, H, page, D, dtype=torch.int8, device="cuda")
+    v = torch.zeros(P, H, page, D, dtype=torch.int8, device="cuda")
+    ks, vs = torch.ones(P, H, device="cuda"), torch.ones(P, H, device="cuda")
+    table = torch.tensor([[P - 1, 5, P - 2]], dtype=torch.int32, device="cuda")
+    kn, vn = (torch.randn(300, H, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    lens = torch.tensor([300], dtype=torch.int32, device="cuda")
+    F.kv8_append(kn, vn, k, v, ks, vs, table, None, lens)
+    small = [t[[P - 1, 5, P - 2]].contiguous() for t in (k, v, ks, vs)]
+    near = torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda")
+    for rows in (1, 200):
+        q = torch.randn(rows, 16, D, device="cuda", dtype=torch.float16)
+        o = F.attention_kv8(q, k, v, ks, vs, table, None, lens)
+        assert torch.equal(o, F.attention_kv8(q, *small, near, None, lens)) and bool((o != 0).any())
+    assert F.device_error(0) == 0
+
+
+# ------------------------------------------------------------------------------------------ together
+@gpu
+def test_graphs_share_nothing(F):
+    """A decode step (append, then attention) captured twice for two batches, replayed interleaved with new tokens."""
+    steps = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for seed, lens in ((1, [700, 40]), (2, [1300, 5])):
+        c = R.Cache([n + 40 for n in lens], heads=2, D=64, page=16, code=INT8, seed=seed)
+        dev, n = c.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+        q, k, v = (torch.randn(2, h, 64, device="cuda", dtype=torch.float16) for h in (8, 2, 2))
+
+        def step(dev=dev, n=n, q=q, k=k, v=v):
+            F.kv8_append(k, v, *dev, None, n)
+            return F.attention_kv8(q, *dev, None, n)
+
+        with torch.cuda.stream(side):
+            step()
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                o = step()
+        steps.append((c, dev, n, q, k, v, g, o, step))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, dev, n, q, k, v, g, o, step in steps:
+            n += 1
+            for t in (q, k, v):
+                t.copy_(torch.randn_like(t))
+        torch.cuda.synchronize()
+        for s in steps:
+            s[6].replay()
+        torch.cuda.synchronize()
+        for c, dev, n, q, k, v, g, o, step in steps:
+            got = o.clone()
+            assert torch.equal(got, step())  # appending the same tokens again changes nothing
+    assert F.device_error(0) == 0
+
+
+@gpu
+def test_decoder_layer_prompt_then_tokens(F):
+    """qkv projection -> append -> attention -> output projection in 4-bit floating point, a prompt and then tokens
+    one by one, against the same in float64 from the values that the cache holds."""
+    hidden, hq, hkv, D, page = 512, 8, 2, 64, 16
+    g = torch.Generator().manual_seed(5)
+    kb = hidden // 32
+    w = {n: (torch.randint(0, 256, (rows, kb, 16), generator=g, dtype=torch.uint8).cuda(), (torch.rand(rows, kb, generator=g) * 0.01).half().cuda())
+         for n, rows in (("q", hq * D), ("k", hkv * D), ("v", hkv * D))}
+    norm = torch.ones(hidden, dtype=torch.float16, device="cuda")
+    oc, osc = F.mxfp4_quantize(torch.randn(hidden, hq * D, generator=g).cuda() * 0.05)
+    o_values = F.mxfp4_dequantize(oc, osc).double().cpu().numpy()
+    c = R.Cache([60, 45], heads=hkv, D=D, page=page, code=INT8)
+    dev = c.cuda()
+    lens = [0, 0]
+    for new in ([37, 20], [1, 1], [1, 1], [3, 0]):
+        lens = [a + b for a, b in zip(lens, new)]
+        n, cu = torch.tensor(lens, dtype=torch.int32, device="cuda"), _cu(new).cuda()
+        x = torch.randn(sum(new), hidden, generator=g).half().cuda()
+        q, k, v = F.matmul_nbits_qkv(x, norm, *w["q"], *w["k"], *w["v"])
+        F.kv8_append(k.view(-1, hkv, D), v.view(-1, hkv, D), *dev, cu, n)
+        o = F.attention_kv8(q.view(-1, hq, D), *dev, cu, n)
+        y = F.matmul_mxfp4(o.view(-1, hq * D), oc, osc, dtype=torch.float32)
+        held = R.Cache.__new__(R.Cache)
+        held.__dict__.update(c.__dict__)
+        held.k, held.v, held.ks, held.vs = (t.cpu() for t in dev[:4])
+        held.lens = n.cpu()
+        want, tol = R.attention(held, q.cpu().view(-1, hq, D), cu.cpu())
+        assert (np.abs(o.cpu().double().numpy() - want) <= tol).all()
+        _, _, xo = R.mx_quantize(o.cpu().double().numpy().reshape(sum(new), -1))
+        yy = xo @ o_values.T
+        assert (np.abs(y.cpu().double().numpy() - yy) <= (hq * D / 32 + 24) * 2.0 ** -23 * (np.abs(xo) @ np.abs(o_values).T)).all()
+    assert F.device_error(0) == 0

@@ -14,6 +14,7 @@ MAX_RANK = 16
 
 # xrgpu_dtype (operators.h:9 order)
 FLOAT32, FLOAT16, INT32, UINT32, INT16, INT8, UINT8, INT64, BOOL, UNSPECIFIED = range(10)
+FLOAT8_E4M3 = 10  # extension: codes of the 8-bit key/value cache
 # xrgpu_status
 OK, INVALID_ARGUMENT, RUNTIME_ERROR, TIMEOUT, DEVICE_ERROR, UNAVAILABLE = range(6)
 # xrgpu_mmnb_path
@@ -31,6 +32,9 @@ EXPORTED = (
     "xrgpu_qkv_workspace_size",
     "xrgpu_qkv_forward", "xrgpu_bnb4_forward", "xrgpu_gather_block_quantized_forward", "xrgpu_qmoe_workspace_size",
     "xrgpu_qmoe_forward",
+    "xrgpu_mxfp4_scale_bytes", "xrgpu_mxfp4_quantize", "xrgpu_mxfp4_dequantize", "xrgpu_mxfp4_tile_scales",
+    "xrgpu_mxfp4_workspace_size", "xrgpu_mxfp4_forward", "xrgpu_kv8_append", "xrgpu_kv8_read",
+    "xrgpu_kv8_attention_workspace_size", "xrgpu_kv8_attention",
 )
 # xrgpu_activation
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_TANH, ACT_SIGMOID, ACT_SWIGLU = range(7)
@@ -122,6 +126,25 @@ class QmoeProblem_(ctypes.Structure):
                 ("fc2_scales", _vp), ("output", _vp)]
 
 
+class Mxfp4Tensor_(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("rows", _i64), ("K", _i64), ("codes", _vp),
+                ("scales", _vp)]
+
+
+class Mxfp4Problem_(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("a_dtype", ctypes.c_int32), ("M", _i64), ("K", _i64), ("N", _i64), ("a", _vp),
+                ("a_scales", _vp), ("lda", _i64), ("b", _vp), ("b_scales", _vp), ("bias", _vp), ("y", _vp), ("ldy", _i64)]
+
+
+class Kv8Problem_(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("tokens", _i64), ("sequences", _i64), ("heads_q", _i64), ("heads_kv", _i64),
+                ("head_dim", _i64), ("page", _i64), ("pages", _i64), ("max_pages", _i64), ("window", _i64),
+                ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64), ("o_stride", _i64), ("q", _vp), ("k", _vp),
+                ("v", _vp), ("o", _vp), ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp), ("v_scale", _vp),
+                ("page_table", _vp), ("cu_seqlens", _vp), ("kv_len", _vp)]
+
+
 _lib = None
 
 
@@ -178,6 +201,16 @@ def load(path: os.PathLike | None = None):
         "xrgpu_gather_block_quantized_forward": ([P(GatherProblem_), vp], ctypes.c_int),
         "xrgpu_qmoe_workspace_size": ([P(QmoeProblem_), P(u64)], ctypes.c_int),
         "xrgpu_qmoe_forward": ([P(QmoeProblem_), vp, u64, vp], ctypes.c_int),
+        "xrgpu_mxfp4_scale_bytes": ([_i64, _i64, P(u64)], ctypes.c_int),
+        "xrgpu_mxfp4_quantize": ([P(Mxfp4Tensor_), vp, _i64, vp], ctypes.c_int),
+        "xrgpu_mxfp4_dequantize": ([P(Mxfp4Tensor_), vp, vp], ctypes.c_int),
+        "xrgpu_mxfp4_tile_scales": ([_i64, _i64, vp, vp, vp], ctypes.c_int),
+        "xrgpu_mxfp4_workspace_size": ([P(Mxfp4Problem_), P(u64)], ctypes.c_int),
+        "xrgpu_mxfp4_forward": ([P(Mxfp4Problem_), vp, u64, vp], ctypes.c_int),
+        "xrgpu_kv8_append": ([P(Kv8Problem_), vp], ctypes.c_int),
+        "xrgpu_kv8_read": ([P(Kv8Problem_), vp], ctypes.c_int),
+        "xrgpu_kv8_attention_workspace_size": ([P(Kv8Problem_), P(u64)], ctypes.c_int),
+        "xrgpu_kv8_attention": ([P(Kv8Problem_), vp, u64, vp], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -1,0 +1,57 @@
+// Device helpers shared by the 8-bit cache kernels.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "mmnb_common.cuh"
+#include "mmnb_kv8.h"
+
+namespace xrgpu {
+
+struct SeqRows {
+  int row0, n, len;  // first row, number of rows, tokens of the sequence (the rows included)
+};
+
+// Rows and length of sequence b; n = 0 for lengths that do not fit (recorded in the error word).
+// Attention (rows_may_exceed) accepts more rows than tokens: the first rows then see nothing.
+__device__ __forceinline__ SeqRows seq_rows(const Kv8& p, int b, bool rows_may_exceed) {
+  SeqRows r;
+  if (p.uniform) {
+    r.n = p.tokens / p.seqs;
+    r.row0 = b * r.n;
+  } else {
+    r.row0 = p.cu[b];
+    r.n = p.cu[b + 1] - r.row0;
+  }
+  r.len = p.kv_len[b];
+  const bool bad = r.row0 < 0 || r.n < 0 || r.n > p.tokens || r.row0 > p.tokens - r.n || r.len < 0 ||
+                   static_cast<int64_t>(r.len) > (static_cast<int64_t>(p.max_pages) << p.page_log2) ||
+                   (!rows_may_exceed && r.n > r.len);
+  if (bad) {
+    record_device_error(p.err, kErrKv8Length);
+    r.row0 = r.n = r.len = 0;
+  }
+  return r;
+}
+
+// Page id of page j of sequence b, -1 (recorded) when the table holds none of the pool's.
+__device__ __forceinline__ int page_id(const Kv8& p, int b, int j) {
+  const int id = p.page_table[static_cast<int64_t>(b) * p.max_pages + j];
+  if (id < 0 || id >= p.pages) {
+    record_device_error(p.err, kErrKv8Page);
+    return -1;
+  }
+  return id;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t byte) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+
+template <bool E4M3>
+__device__ __forceinline__ float code_value(uint32_t byte) {
+  return E4M3 ? e4m3_value(byte) : static_cast<float>(static_cast<int8_t>(byte));
+}
+
+}  // namespace xrgpu

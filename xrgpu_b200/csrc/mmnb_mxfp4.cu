@@ -1,0 +1,205 @@
+// Microscaled 4-bit floating point: quantisation, dequantisation, scale layout (format: mmnb_mxfp4.h).
+//
+// Quantisation of a block: a = max |x|, E = max(floor(log2 a) - 2, -127) (2 is the exponent of the
+// largest code, 6 = 1.5 * 2^2), code = x * 2^-E rounded to nearest, ties to the even code, saturating
+// at 6, the sign of x kept. floor(log2 a) is a's exponent field, so nothing is approximated: x * 2^-E is
+// exact and the conversion rounds once. A block that holds a NaN or an infinity has scale byte 255
+// and codes 0.
+#include <cuda_fp16.h>
+
+#include "mmnb_common.cuh"
+#include "mmnb_mxfp4.h"
+
+namespace xrgpu {
+namespace {
+
+__device__ __forceinline__ int64_t scale_offset(int64_t row, int64_t blk, int64_t kb) {
+  return ((row >> 7) * ((kb + 3) >> 2) + (blk >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (blk & 3);
+}
+
+// Two codes in a byte: lo in the low nibble.
+__device__ __forceinline__ uint32_t to_e2m1x2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+
+__device__ __forceinline__ float pow2_of_byte(uint32_t e) {  // 2^(e - 127), e = 255: NaN
+  return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(e ? e << 23 : 1u << 22);
+}
+
+// Code (4 bits) to its value.
+__device__ __forceinline__ float e2m1_value(uint32_t c) {
+  const uint32_t m = c & 7u;
+  const float v = m < 4u ? 0.5f * static_cast<float>(m) : (m < 6u ? static_cast<float>(m) - 2.0f : 2.0f * static_cast<float>(m) - 8.0f);
+  return (c & 8u) ? -v : v;
+}
+
+constexpr int kQuantWarps = 8;
+constexpr int kChunk = 256;  // values of a row that a warp takes at a time: 8 a lane, 4 lanes a block
+
+// One warp a (row, chunk); rows beyond the matrix up to the tile's end only zero their scales.
+template <bool F16, bool VEC>
+__global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Quantize p, int64_t chunks, int64_t items) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kQuantWarps + (threadIdx.x >> 5); it < items;
+       it += static_cast<int64_t>(gridDim.x) * kQuantWarps) {
+    const int64_t row = it / chunks, k0 = (it % chunks) * kChunk + lane * 8;
+    float v[8];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (row < p.rows && k0 < p.K) {
+      if (VEC) {
+        if (F16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + row * p.ldx + k0);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+          }
+        } else {
+          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + row * p.ldx + k0);
+          const float4 f0 = src[0], f1 = src[1];
+          v[0] = f0.x; v[1] = f0.y; v[2] = f0.z; v[3] = f0.w;
+          v[4] = f1.x; v[5] = f1.y; v[6] = f1.z; v[7] = f1.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k0 + i < p.K) v[i] = load_f(p.x, F16, row * p.ldx + k0 + i);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);  // NaN > Inf > finite as bits
+    amax = max(amax, __shfl_xor_sync(~0u, amax, 1));
+    amax = max(amax, __shfl_xor_sync(~0u, amax, 2));
+    const uint32_t field = amax >> 23;
+    const bool bad = field == 255u;
+    const uint32_t e = bad ? 255u : (field > 2u ? field - 2u : 0u);
+    const float inv = bad ? 0.0f : __uint_as_float((254u - e) << 23);  // 2^(127 - e); e <= 252 here
+    uint32_t c = 0;
+    if (!bad) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c |= to_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+    }
+    const int64_t blk = k0 >> 5;
+    if (row < p.rows && blk < p.kb) reinterpret_cast<uint32_t*>(p.codes + (row * p.kb + blk) * 16)[lane & 3] = c;
+    // the four scale bytes of 16 lanes as one word
+    const uint32_t eb = (row < p.rows && blk < p.kb) ? e : 0u;
+    uint32_t word = eb << (8 * ((lane >> 2) & 3));
+    word |= __shfl_xor_sync(~0u, word, 4);
+    word |= __shfl_xor_sync(~0u, word, 8);
+    if ((lane & 15) == 0 && (blk >> 2) < ((p.kb + 3) >> 2)) *reinterpret_cast<uint32_t*>(p.scales + scale_offset(row, blk, p.kb)) = word;
+  }
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(256) dequantize_kernel(const Mxfp4Dequantize p) {
+  const int64_t n = p.rows * p.kb;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n * 4; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = (i >> 2) / p.kb, blk = (i >> 2) % p.kb, k0 = blk * 32 + (i & 3) * 8;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(p.codes)[i];
+    const float s = pow2_of_byte(p.scales[scale_offset(row, blk, p.kb)]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (k0 + j >= p.K) break;
+      const float v = e2m1_value((w >> (4 * j)) & 15u) * s;
+      if (F16) static_cast<__half*>(p.out)[row * p.K + k0 + j] = __float2half_rn(v);
+      else static_cast<float*>(p.out)[row * p.K + k0 + j] = v;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t kb, int64_t bytes) {
+  const int64_t tiles_k = (kb + 3) >> 2;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < bytes; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t tile = i >> 9, row = (tile / tiles_k) * 128 + ((i >> 2) & 3) * 32 + ((i >> 4) & 31), blk = (tile % tiles_k) * 4 + (i & 3);
+    dst[i] = (row < rows && blk < kb) ? src[row * kb + blk] : 0;
+  }
+}
+
+// One 32 x 32 tile of Y a CTA, values of one block of 32 at a time in shared memory.
+__global__ void __launch_bounds__(256) matmul_kernel(const Mxfp4Matmul p) {
+  __shared__ float sa[32][33], sb[32][33];
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 32, n0 = static_cast<int64_t>(blockIdx.x) * 32;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  float acc[4] = {};
+  for (int64_t blk = 0; blk < p.kb; ++blk) {
+    for (int r = ty; r < 32; r += 8) {
+      const int64_t m = m0 + r, n = n0 + r;
+      float va = 0.0f, vb = 0.0f;
+      if (m < p.M) va = e2m1_value((p.a[(m * p.kb + blk) * 16 + tx / 2] >> (4 * (tx & 1))) & 15u) * pow2_of_byte(p.a_scales[scale_offset(m, blk, p.kb)]);
+      if (n < p.N) vb = e2m1_value((p.b[(n * p.kb + blk) * 16 + tx / 2] >> (4 * (tx & 1))) & 15u) * pow2_of_byte(p.b_scales[scale_offset(n, blk, p.kb)]);
+      sa[r][tx] = va;
+      sb[r][tx] = vb;
+    }
+    __syncthreads();
+    for (int k = 0; k < 32; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(sa[ty + 8 * i][k], sb[tx][k], acc[i]);
+    __syncthreads();
+  }
+  const int64_t n = n0 + tx;
+  if (n >= p.N) return;
+  const float bias = p.bias ? load_f(p.bias, p.f16, n) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + ty + 8 * i;
+    if (m >= p.M) continue;
+    if (p.f16) static_cast<__half*>(p.y)[m * p.ldy + n] = __float2half_rn(acc[i] + bias);
+    else static_cast<float*>(p.y)[m * p.ldy + n] = acc[i] + bias;
+  }
+}
+
+int grid_for(int64_t blocks, int per_sm) {
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
+  return static_cast<int>(blocks < most ? (blocks > 0 ? blocks : 1) : most);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+cudaError_t launch_mxfp4_quantize(const Mxfp4Quantize& p, cudaStream_t s) {
+  const int64_t chunks = ceil_div(p.K, kChunk), rows = ceil_div(p.rows, 128) * 128, items = rows * chunks;
+  if (items == 0) return cudaSuccess;
+  const int grid = grid_for(ceil_div(items, kQuantWarps), 8);
+  // 16-byte loads of 8 values: the rows' starts and K in whole vectors
+  const int64_t es = p.f16 ? 2 : 4;
+  const bool vec = aligned16(p.x) && (p.ldx * es) % 16 == 0 && p.K % 8 == 0;
+  if (p.f16) {
+    if (vec) quantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    else quantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+  } else {
+    if (vec) quantize_kernel<false, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    else quantize_kernel<false, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_mxfp4_dequantize(const Mxfp4Dequantize& p, cudaStream_t s) {
+  const int64_t n = p.rows * p.kb * 4;
+  if (n == 0) return cudaSuccess;
+  const int grid = grid_for(ceil_div(n, 256), 8);
+  if (p.f16) dequantize_kernel<true><<<grid, 256, 0, s>>>(p);
+  else dequantize_kernel<false><<<grid, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_mxfp4_tile_scales(const uint8_t* scales, uint8_t* tiled, int64_t rows, int64_t kb, cudaStream_t s) {
+  const int64_t bytes = mxfp4_scale_bytes(rows, kb);
+  if (bytes == 0) return cudaSuccess;
+  tile_scales_kernel<<<grid_for(ceil_div(bytes, 256), 8), 256, 0, s>>>(scales, tiled, rows, kb, bytes);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 32)), static_cast<unsigned>(ceil_div(p.M, 32)));
+  matmul_kernel<<<grid, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace xrgpu

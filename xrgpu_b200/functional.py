@@ -298,3 +298,279 @@ def qmoe(x, router, fc1, fc1_scales, fc2, fc2_scales, *, k: int = 1, bits: int =
     check(lib.xrgpu_qmoe_workspace_size(ctypes.byref(p), ctypes.byref(need)))
     _call(lib.xrgpu_qmoe_forward, p, _workspace(need.value, dev), dev)
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Block-scaled serving operators: microscaled 4-bit floating point, and the paged key/value cache of
+# 8-bit codes with its attention (zero-copy, current CUDA stream of the tensors' device).
+_FLOATS = {torch.float32: _native.FLOAT32, torch.float16: _native.FLOAT16}
+_CACHES = {torch.int8: _native.INT8, torch.float8_e4m3fn: _native.FLOAT8_E4M3}
+
+
+def _launch(device, fn, *args):
+    """fn(*args, stream) on the current stream of `device`, with that device current."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _float_code(dtype) -> int:
+    if dtype not in _FLOATS:
+        raise ValueError(f"T1 must be float32 or float16, got {dtype}")
+    return _FLOATS[dtype]
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Elements from one row of [..., K] to the next; the rows must lie at one stride, values side by side."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+    step = want = 0
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if step == 0:
+            step = want = t.stride(d)
+        if t.stride(d) != want or step < t.shape[-1]:
+            raise ValueError(f"{name} must have its rows at one stride")
+        want *= t.shape[d]
+    return step or t.shape[-1]
+
+
+def _scale_shape(rows: int, kb: int):
+    return (-(-rows // 128), -(-kb // 4), 32, 4, 4)
+
+
+def _require_mxfp4(codes, scales, rows: int, kb: int, name: str, device):
+    for t, n in ((codes, name), (scales, name + "_scales")):
+        _require(t, n, device)
+        if t.dtype != torch.uint8:
+            raise ValueError(f"{n} must be uint8")
+    if codes.numel() != rows * kb * 16 or codes.shape[-1] != 16 or codes.dim() < 2:
+        raise ValueError(f"{name} must be [..., {kb}, 16] codes")
+    if tuple(scales.shape) != _scale_shape(rows, kb):
+        raise ValueError(f"{name}_scales must be tiled scales of shape {list(_scale_shape(rows, kb))}")
+
+
+def mxfp4_quantize(x: torch.Tensor):
+    """Microscaled 4-bit form of x [..., K] (float32 or float16; rows may be strided): (codes, scales).
+
+    codes uint8 [..., kb, 16], kb = ceil(K / 32): 32 four-bit floating-point codes a block, low nibble first, the
+    last block padded with zeros. scales uint8 [ceil(rows/128), ceil(kb/4), 32, 4, 4]: one power of two a block, in
+    the order the tensor cores take them (``mxfp4_tile_scales``). A block that holds a NaN or an infinity reads as NaN.
+    """
+    dtype = _float_code(x.dtype)
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    K = int(x.shape[-1]) if x.dim() else 0
+    if K < 1:
+        raise ValueError("x must be [..., K] with K >= 1")
+    rows, kb, ldx = x.numel() // K, -(-K // 32), _row_stride(x, "x")
+    codes = torch.empty(tuple(x.shape[:-1]) + (kb, 16), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_shape(rows, kb), dtype=torch.uint8, device=x.device)
+    t = _native.Mxfp4Tensor_(dtype, 0, rows, K, codes.data_ptr(), scales.data_ptr())
+    _launch(x.device, _native.load().xrgpu_mxfp4_quantize, ctypes.byref(t), x.data_ptr(), ldx)
+    return codes, scales
+
+
+def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, K: Optional[int] = None, dtype=torch.float32) -> torch.Tensor:
+    """The values [..., K] that microscaled codes and tiled scales hold (K defaults to 32 kb)."""
+    if codes.dim() < 2:
+        raise ValueError("codes must be [..., kb, 16]")
+    kb = int(codes.shape[-2])
+    K = kb * 32 if K is None else int(K)
+    if K < 1 or -(-K // 32) != kb:
+        raise ValueError("K does not match the codes")
+    rows = codes.numel() // (kb * 16) if kb else 0
+    code = _float_code(dtype)
+    _require_mxfp4(codes, scales, rows, kb, "codes", codes.device)
+    out = torch.empty(tuple(codes.shape[:-2]) + (K,), dtype=dtype, device=codes.device)
+    t = _native.Mxfp4Tensor_(code, 0, rows, K, codes.data_ptr(), scales.data_ptr())
+    _launch(codes.device, _native.load().xrgpu_mxfp4_dequantize, ctypes.byref(t), out.data_ptr())
+    return out
+
+
+def mxfp4_tile_scales(scales: torch.Tensor) -> torch.Tensor:
+    """Scale bytes [rows, kb] (as checkpoints hold them) in the tiled order of ``matmul_mxfp4``."""
+    if scales.dim() != 2 or scales.dtype != torch.uint8 or scales.shape[1] < 1:
+        raise ValueError("scales must be uint8 [rows, kb]")
+    _require(scales, "scales", scales.device)
+    rows, kb = int(scales.shape[0]), int(scales.shape[1])
+    tiled = torch.empty(_scale_shape(rows, kb), dtype=torch.uint8, device=scales.device)
+    _launch(scales.device, _native.load().xrgpu_mxfp4_tile_scales, rows, kb, scales.data_ptr(), tiled.data_ptr())
+    return tiled
+
+
+def matmul_mxfp4(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                 a_scales: Optional[torch.Tensor] = None, K: Optional[int] = None, dtype=None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Y = A . B^T (+ bias) with both operands in microscaled 4-bit form, float32 sums.
+
+    b [N, kb, 16] codes and b_scales (tiled), a either codes [..., kb, 16] with a_scales, or float32 / float16
+    [..., K], which the call quantises first. Y [..., N] in `dtype` (default a's, float16 for codes); bias [N] in it.
+    ``out`` may be a [..., N] view with unit column stride and rows at one stride.
+    """
+    dev = a.device
+    held = a_scales is not None
+    if b.dim() != 3:
+        raise ValueError("b must be [N, kb, 16] codes")
+    N, kb = int(b.shape[0]), int(b.shape[1])
+    p = _native.Mxfp4Problem_()
+    if held:
+        lead = tuple(a.shape[:-2])
+        M = a.numel() // (kb * 16) if kb else 0
+        K = kb * 32 if K is None else int(K)
+        _require_mxfp4(a, a_scales, M, kb, "a", dev)
+        p.a_dtype, p.a_scales = _native.UINT8, a_scales.data_ptr()
+        dtype = torch.float16 if dtype is None else dtype
+    else:
+        if not a.is_cuda:
+            raise ValueError("a must be a CUDA tensor")
+        p.a_dtype = _float_code(a.dtype)
+        lead = tuple(a.shape[:-1])
+        if K is not None and int(K) != a.shape[-1]:
+            raise ValueError("K does not match a")
+        K = int(a.shape[-1])
+        M = a.numel() // K if K else 0
+        p.lda = _row_stride(a, "a")
+        dtype = a.dtype if dtype is None else dtype
+    if K < 1 or -(-K // 32) != kb:
+        raise ValueError("a and b differ in K")
+    _require_mxfp4(b, b_scales, N, kb, "b", dev)
+    p.dtype, p.M, p.K, p.N = _float_code(dtype), M, K, N
+    if bias is not None:
+        _require(bias, "bias", dev)
+        if bias.dtype != dtype or tuple(bias.shape) != (N,):
+            raise ValueError("bias must be [N] in the output dtype")
+        p.bias = bias.data_ptr()
+    if out is None:
+        out = torch.empty(lead + (N,), dtype=dtype, device=dev)
+    else:
+        if out.dtype != dtype or out.device != dev or tuple(out.shape) != lead + (N,):
+            raise ValueError("out must be [..., N] in the output dtype on a's device")
+        p.ldy = _row_stride(out, "out")
+    p.a, p.b, p.b_scales, p.y = a.data_ptr(), b.data_ptr(), b_scales.data_ptr(), out.data_ptr()
+    ws, nbytes = None, 0
+    if not held and M:
+        nbytes = -(-M * kb * 16 // 256) * 256 + -(-M // 128) * -(-kb // 4) * 512
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, _native.load().xrgpu_mxfp4_forward, ctypes.byref(p), ws.data_ptr() if ws is not None else None, nbytes)
+    return out
+
+
+def _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, dtype):
+    dev = k_cache.device
+    if k_cache.dtype not in _CACHES or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must both be int8 or float8_e4m3fn")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache must be [pages, heads, page, head_dim]")
+    P, H, page, D = k_cache.shape
+    for t, name, dt in ((k_cache, "k_cache", k_cache.dtype), (v_cache, "v_cache", k_cache.dtype),
+                        (k_scale, "k_scale", torch.float32), (v_scale, "v_scale", torch.float32),
+                        (page_table, "page_table", torch.int32), (kv_len, "kv_len", torch.int32),
+                        (cu_seqlens, "cu_seqlens", torch.int32)):
+        if t is None and name == "cu_seqlens":
+            continue
+        _require(t, name, dev)
+        if t.dtype != dt:
+            raise ValueError(f"{name} must be {dt}")
+    if k_scale.shape != (P, H) or v_scale.shape != (P, H):
+        raise ValueError("k_scale and v_scale must be [pages, heads]")
+    B = int(kv_len.shape[0]) if kv_len.dim() == 1 else -1
+    if B < 0 or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError("page_table must be [sequences, max_pages] and kv_len [sequences]")
+    if cu_seqlens is not None and tuple(cu_seqlens.shape) != (B + 1,):
+        raise ValueError("cu_seqlens must be [sequences + 1]")
+    p = _native.Kv8Problem_()
+    p.dtype, p.cache_dtype = _float_code(dtype), _CACHES[k_cache.dtype]
+    p.sequences, p.heads_kv, p.head_dim, p.page, p.pages, p.max_pages = B, H, D, page, P, page_table.shape[1]
+    p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    p.page_table, p.kv_len = page_table.data_ptr(), kv_len.data_ptr()
+    if cu_seqlens is not None:
+        p.cu_seqlens = cu_seqlens.data_ptr()
+    return p
+
+
+def _head_rows(t, name: str, heads: Optional[int], D: int, device) -> int:
+    """Row stride of [rows, heads, D] whose rows may be strided, heads and values side by side."""
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on {device}")
+    if t.dim() != 3 or t.shape[2] != D or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [rows, heads, head_dim]")
+    H = t.shape[1]
+    if t.is_contiguous() or t.shape[0] == 0:
+        return H * D
+    if t.stride(2) != 1 or (H > 1 and t.stride(1) != D) or (t.shape[0] > 1 and t.stride(0) < H * D):
+        raise ValueError(f"{name} must have its heads and values side by side")
+    return t.stride(0) if t.shape[0] > 1 else H * D
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor, page_table: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
+               kv_len: torch.Tensor) -> None:
+    """Writes new keys and values [rows, heads, head_dim] (float32 or float16; rows may be strided) into the cache.
+
+    k_cache, v_cache [pages, heads, page, head_dim] int8 or float8_e4m3fn and k_scale, v_scale float32 [pages, heads]
+    are updated in place; page_table int32 [sequences, max_pages], cu_seqlens int32 [sequences + 1] (None: the same
+    number of rows each), kv_len int32 [sequences], the new tokens included: rows cu_seqlens[b] .. of sequence b become
+    its last tokens. One scale covers a page of a head; where a new token exceeds it, the page's older codes are
+    rescaled. A page shared by two sequences must not be appended to. Bad page ids and lengths: ``device_error``
+    0x501, 0x502, nothing written for them.
+    """
+    p = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, k.dtype)
+    dev = k_cache.device
+    p.k_stride = _head_rows(k, "k", p.heads_kv, p.head_dim, dev)
+    p.v_stride = _head_rows(v, "v", p.heads_kv, p.head_dim, dev)
+    if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+        raise ValueError("k and v must have the same rows and dtype")
+    p.tokens, p.k, p.v = k.shape[0], k.data_ptr(), v.data_ptr()
+    _launch(dev, _native.load().xrgpu_kv8_append, ctypes.byref(p))
+
+
+def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+             page_table: torch.Tensor, cu_seqlens: Optional[torch.Tensor], kv_len: torch.Tensor, *, rows: int,
+             dtype=torch.float16):
+    """The values (k, v), each [rows, heads, head_dim], that the cache holds for the last tokens of each sequence
+    (rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1; see ``kv8_append``). Rows of no sequence are zero."""
+    p = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, dtype)
+    dev = k_cache.device
+    k = torch.zeros((int(rows), p.heads_kv, p.head_dim), dtype=dtype, device=dev)
+    v = torch.zeros_like(k)
+    p.tokens, p.k, p.v = int(rows), k.data_ptr(), v.data_ptr()
+    _launch(dev, _native.load().xrgpu_kv8_read, ctypes.byref(p))
+    return k, v
+
+
+def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, page_table: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
+                  kv_len: torch.Tensor, *, scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [rows, query heads, head_dim] over the 8-bit cache (``kv8_append`` describes its tensors).
+
+    Rows cu_seqlens[b] .. are the last positions of sequence b (kv_len counts them; append first). A row sees the
+    tokens up to its own position (causal), the last `window` of them if given, or all kv_len (causal=False). Query
+    head h reads key/value head h // (query heads // heads). scale defaults to head_dim ** -0.5. A row that sees nothing
+    gives zeros; with ``out``, rows behind the last sequence are left as they were (without it they are zero).
+    """
+    p = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, q.dtype)
+    dev = k_cache.device
+    p.q_stride = _head_rows(q, "q", None, p.head_dim, dev)
+    if out is None:
+        # with cu_seqlens the rows may go on behind the last sequence
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev) if cu_seqlens is None else torch.zeros(q.shape, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("out must have q's shape and dtype")
+    p.o_stride = _head_rows(out, "out", q.shape[1], p.head_dim, dev)
+    p.tokens, p.heads_q, p.q, p.o = q.shape[0], q.shape[1], q.data_ptr(), out.data_ptr()
+    p.causal, p.window = int(bool(causal)), int(window)
+    p.scale = float(scale) if scale is not None else p.head_dim ** -0.5
+    lib = _native.load()
+    need = ctypes.c_uint64(0)
+    check(lib.xrgpu_kv8_attention_workspace_size(ctypes.byref(p), ctypes.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+    _launch(dev, lib.xrgpu_kv8_attention, ctypes.byref(p), ws.data_ptr() if ws is not None else None, need.value)
+    return out
