@@ -40,6 +40,7 @@
 #include <mutex>
 
 #include "mmnb_common.cuh"
+#include "mmnb_tcgen05.cuh"
 
 namespace xrgpu {
 namespace {
@@ -71,7 +72,6 @@ constexpr unsigned kErrWaitMma = 0x302;
 constexpr unsigned kErrWaitDequant = 0x303;
 constexpr unsigned kErrWaitEpilogue = 0x304;
 constexpr unsigned kErrDrain = 0x305;
-constexpr unsigned kSuspendHintNs = 0x989680;  // longest hardware suspension per mbarrier probe
 
 enum ZpMode : int { kZDefault = 0, kZPacked = 1, kZHalf = 2 };
 
@@ -86,13 +86,6 @@ struct GemmArgs {
 };
 
 // ------------------------------------------------------------------ tcgen05 / TMA wrappers
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
 // D[tmem_d] (+)= A[tmem_a] (128 x 16 f16, lanes = rows) * B[smem desc] (T x 16 f16, K-major)^T
 __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -103,24 +96,6 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_
       ::"r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
       : "memory");
 }
-
-// Arrives once on `bar` when every tcgen05 operation this thread issued so far has completed.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -137,18 +112,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&a)[8], uint32_t (&b)[8])
                ::"memory");
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
 __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
@@ -160,90 +123,9 @@ __device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
   return v;
 }
 
-// UMMA shared-memory descriptor, K-major operand in the 128-byte swizzle canonical layout:
-// rows of 128 bytes, 8-row atoms 1024 bytes apart (stride byte offset), version 1.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(1u) << 16;             // leading byte offset (unused for swizzled K-major)
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;     // stride byte offset
-  d |= static_cast<uint64_t>(1u) << 46;             // descriptor version
-  d |= static_cast<uint64_t>(2u) << 61;             // SWIZZLE_128B
-  return d;
-}
-
 // Instruction descriptor: f16 x f16 -> f32, both operands K-major, M = 128, N = T.
 __device__ __forceinline__ uint32_t umma_idesc(int T) {
   return (1u << 4) | (static_cast<uint32_t>(T >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
-}
-
-struct Ctl {
-  volatile int* abort;
-  unsigned* err;
-};
-
-// Non-blocking probe of an mbarrier phase (never suspends the thread).
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// mbarrier probe that may suspend the thread in hardware until the phase completes (or the
-// time hint, in ns, passes).
-__device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendHintNs)
-      : "memory");
-  return done != 0;
-}
-
-// Single-lane bounded spin for the latency-critical roles (TMA producer, MMA issuer).
-// Gives up on the abort flag or after the wait limit (raising it).
-__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, const Ctl& c, unsigned code) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const uint64_t start = global_timer_ns();
-  for (;;) {
-    if (mbar_test_wait(bar, parity)) return true;
-    if (*c.abort) return false;
-    if (global_timer_ns() - start > kWaitLimitNs) {
-      record_device_error(c.err, code);
-      *c.abort = 1;
-      return false;
-    }
-  }
-}
-
-// Whole-warp bounded wait (dequant and epilogue warps): every lane observes the phase and the
-// warp agrees on the outcome, so the .sync.aligned tcgen05 instructions after it stay
-// converged; the probes suspend the warp in hardware, leaving issue slots to the producer and
-// the MMA issuer. Gives up on the abort flag or after the wait limit (raising it).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Ctl& c, unsigned code) {
-  if (__all_sync(~0u, mbar_try_wait_suspend(bar, parity))) return true;
-  const uint64_t start = global_timer_ns();
-  for (;;) {
-    if (__all_sync(~0u, mbar_try_wait_suspend(bar, parity))) return true;
-    const bool aborted = *c.abort != 0;
-    const bool expired = global_timer_ns() - start > kWaitLimitNs;
-    if (__any_sync(~0u, aborted || expired)) {
-      if (__any_sync(~0u, expired) && (threadIdx.x & 31) == 0) {
-        record_device_error(c.err, code);
-        *c.abort = 1;
-      }
-      return false;
-    }
-  }
 }
 
 // Bounded wait that ignores the abort flag: used to drain copies / MMAs before exit.

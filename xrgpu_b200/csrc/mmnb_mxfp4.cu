@@ -42,6 +42,7 @@ constexpr int kChunk = 256;  // values of a row that a warp takes at a time: 8 a
 template <bool F16, bool VEC>
 __global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Quantize p, int64_t chunks, int64_t items) {
   const int lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's weights may start to load
   for (int64_t it = static_cast<int64_t>(blockIdx.x) * kQuantWarps + (threadIdx.x >> 5); it < items;
        it += static_cast<int64_t>(gridDim.x) * kQuantWarps) {
     const int64_t row = it / chunks, k0 = (it % chunks) * kChunk + lane * 8;
@@ -121,39 +122,6 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* src, ui
   }
 }
 
-// One 32 x 32 tile of Y a CTA, values of one block of 32 at a time in shared memory.
-__global__ void __launch_bounds__(256) matmul_kernel(const Mxfp4Matmul p) {
-  __shared__ float sa[32][33], sb[32][33];
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 32, n0 = static_cast<int64_t>(blockIdx.x) * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  float acc[4] = {};
-  for (int64_t blk = 0; blk < p.kb; ++blk) {
-    for (int r = ty; r < 32; r += 8) {
-      const int64_t m = m0 + r, n = n0 + r;
-      float va = 0.0f, vb = 0.0f;
-      if (m < p.M) va = e2m1_value((p.a[(m * p.kb + blk) * 16 + tx / 2] >> (4 * (tx & 1))) & 15u) * pow2_of_byte(p.a_scales[scale_offset(m, blk, p.kb)]);
-      if (n < p.N) vb = e2m1_value((p.b[(n * p.kb + blk) * 16 + tx / 2] >> (4 * (tx & 1))) & 15u) * pow2_of_byte(p.b_scales[scale_offset(n, blk, p.kb)]);
-      sa[r][tx] = va;
-      sb[r][tx] = vb;
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(sa[ty + 8 * i][k], sb[tx][k], acc[i]);
-    __syncthreads();
-  }
-  const int64_t n = n0 + tx;
-  if (n >= p.N) return;
-  const float bias = p.bias ? load_f(p.bias, p.f16, n) : 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty + 8 * i;
-    if (m >= p.M) continue;
-    if (p.f16) static_cast<__half*>(p.y)[m * p.ldy + n] = __float2half_rn(acc[i] + bias);
-    else static_cast<float*>(p.y)[m * p.ldy + n] = acc[i] + bias;
-  }
-}
-
 int grid_for(int64_t blocks, int per_sm) {
   const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
   return static_cast<int>(blocks < most ? (blocks > 0 ? blocks : 1) : most);
@@ -193,12 +161,6 @@ cudaError_t launch_mxfp4_tile_scales(const uint8_t* scales, uint8_t* tiled, int6
   const int64_t bytes = mxfp4_scale_bytes(rows, kb);
   if (bytes == 0) return cudaSuccess;
   tile_scales_kernel<<<grid_for(ceil_div(bytes, 256), 8), 256, 0, s>>>(scales, tiled, rows, kb, bytes);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 32)), static_cast<unsigned>(ceil_div(p.M, 32)));
-  matmul_kernel<<<grid, 256, 0, s>>>(p);
   return cudaGetLastError();
 }
 

@@ -49,6 +49,8 @@ struct Mxfp4Matmul {
   void* y;                  // [M, ldy]
   unsigned* err;
 };
-cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, cudaStream_t s);
+// early: the kernel before it on the stream writes the activations only and announces its end early, so
+// the weights may be loaded while it runs.
+cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s);
 
 }  // namespace xrgpu

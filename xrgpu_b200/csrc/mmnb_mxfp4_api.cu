@@ -86,7 +86,7 @@ int mxfp4_forward(const xrgpu_mxfp4_problem& c, void* ws, uint64_t ws_bytes, cud
     scales = q.scales;
   }
   Mxfp4Matmul p{f16, c.M, c.N, c.K, kb, c.ldy ? c.ldy : c.N, codes, scales, c.b, c.b_scales, c.bias, c.y, device_error_word()};
-  return launched(launch_mxfp4_matmul(p, s));
+  return launched(launch_mxfp4_matmul(p, c.a_dtype != XRGPU_UINT8, s));
 }
 
 }  // namespace xrgpu

@@ -1,0 +1,454 @@
+// Product of two microscaled 4-bit operands on tcgen05 tensor cores (format: mmnb_mxfp4.h):
+//   y[m, n] = sum_blocks 2^(ea + eb) sum_32 a w + bias[n].
+// The tensor cores take the codes and the scale bytes as they are (block-scaled 4-bit kind, one scale per
+// 32 values, float32 accumulators), so nothing is unpacked: a CTA streams code tiles and scale tiles into
+// shared memory, copies the scales on into tensor memory and issues the MMAs.
+//
+// Orientation. An MMA multiplies 128 rows (operand P) by T rows (operand Q). Up to 128 activation rows, P are
+// the weights, which stream once, and Q all activations (T the rows rounded up to 16); the K axis is then
+// split over a cluster of up to 8 CTAs whose float32 partial tiles meet in shared memory, summed in the
+// order of their ranks. For more rows P are the activations, so that a thread's accumulator row is a row of y.
+//
+// Roles (10 warps): warp 0 loads (one lane: TMA tiles with the 128-byte swizzle, bulk copies of scale
+// tiles), warp 1 copies scales to tensor memory and issues the MMAs (one lane), warps 2-9 drain the
+// accumulators (lane quadrant warp % 4, alternate 16-column chunks).
+//
+// Tensor memory: two accumulators of T columns at 0 and acc1, then per stage the scale columns: 4 columns
+// (32 lanes x 4 bytes x 4 row groups) for 128 rows x 128 values. A stage's columns are rewritten only when
+// its shared-memory buffer has come back, that is when the MMAs that read them are done. With T = 256 two
+// accumulators and the scales need more than the 512 columns: the accumulators then overlap, and the
+// drain starts with the shared columns, after which the next tile may start.
+//
+// Every wait is bounded as in mmnb_gemm_sm100.cu.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+
+#include "mmnb_mxfp4.h"
+#include "mmnb_tcgen05.cuh"
+
+namespace xrgpu {
+namespace {
+
+constexpr int kRows = 128;              // rows of operand P
+constexpr int kStepBytes = 128;         // codes of a row per stage: 256 values, one swizzle row
+constexpr int kScaleTile = 512;         // scale bytes of 128 rows x 128 values
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = (2 + kEpilogueWarps) * 32;
+constexpr int kTmemCols = 512;
+constexpr int kSmemBudget = 227 * 1024;
+constexpr int kPitch = kRows + 1;       // floats a column of a partial tile in shared memory
+
+constexpr unsigned kErrWaitProducer = 0x601;
+constexpr unsigned kErrWaitMma = 0x602;
+constexpr unsigned kErrWaitEpilogue = 0x603;
+constexpr unsigned kErrDrain = 0x604;
+
+struct Args {
+  int p_rows, q_rows;       // valid rows of the operands
+  int p_tiles, tiles;       // tiles along P, in all
+  int T, ksteps, k64;       // rows of Q a tile, stages along K, 64-value MMA steps along K
+  int stages, split, q_blocks;  // q_blocks: scale row blocks a Q tile spans (1 or 2)
+  int acc1, shared_cols;    // column of the second accumulator, columns that both hold
+  int tmem_cols, sf_col, sf_stage;
+  int early;                // the weights may be loaded before the previous kernel has finished
+  uint32_t q_stage, stage;  // bytes
+  int64_t tiles_k;          // scale tiles along K
+  int sp_blocks, sq_blocks; // row blocks of the scales
+  const uint8_t* sp;
+  const uint8_t* sq;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int vec;                  // rows of y start on 16 bytes
+  unsigned* err;
+};
+
+// D[128 x T] (+)= P (smem, K-major codes) . Q^T, scales in tensor memory.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                                         uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows of 16 bytes from shared memory to 4 columns, the same in all four lane quadrants.
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Shared-memory descriptor without swizzle: 8-row groups of 16-byte rows, 128 bytes apart.
+__device__ __forceinline__ uint64_t plain_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
+}
+
+// Instruction descriptor: 4-bit floats, both K-major, M = 128, N = T, scales of powers of two, K = 64;
+// `half` picks the scale bytes 0-1 (0) or 2-3 (2) of a column.
+__device__ __forceinline__ uint32_t instruction_desc(int T, uint32_t half) {
+  return (half << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(T >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(kRows >> 4) << 24) | (half << 29);
+}
+
+template <bool SWAP, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = a.stages;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  // a stage: [P tile 16 KB][Q tile T * 128][P scales 1 KB][Q scales q_blocks * 1 KB]
+  __shared__ uint64_t full[12], empty[12], accfull[2], drained[2], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accfull[b], 1);
+      mbar_init(&drained[b], kEpilogueWarps);
+    }
+    mbar_init(&done, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_slot)), "r"(a.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+  const Ctl ctl{&abort_flag, a.err};
+  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
+  const int k0 = static_cast<int>(static_cast<int64_t>(a.ksteps) * rank / a.split);
+  const int k1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.split);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load_p = [&](int s, int ks, int pt, int groups) {
+        tma_load_2d(base + s * a.stage, &map_p, ks * kStepBytes, pt * kRows, &full[s]);
+        bulk_copy_g2s(gbase + s * a.stage + kRows * kStepBytes + a.q_stage, a.sp + (pt * a.tiles_k + 2 * ks) * kScaleTile,
+                      groups * kScaleTile, &full[s]);
+      };
+      auto load_q = [&](int s, int ks, int qt, int groups) {
+        tma_load_2d(base + s * a.stage + kRows * kStepBytes, &map_q, ks * kStepBytes, qt * a.T, &full[s]);
+        const int rb = qt * a.T / kRows;
+        for (int b = 0; b < a.q_blocks && rb + b < a.sq_blocks; ++b)
+          bulk_copy_g2s(gbase + s * a.stage + kRows * kStepBytes + a.q_stage + (1 + b) * 2 * kScaleTile,
+                        a.sq + (static_cast<int64_t>(rb + b) * a.tiles_k + 2 * ks) * kScaleTile, groups * kScaleTile, &full[s]);
+      };
+      auto expect = [&](int s, int qt, int groups) {
+        const int rb = qt * a.T / kRows, blocks = 1 + min(a.q_blocks, a.sq_blocks - rb);
+        mbar_arrive_expect_tx(&full[s], kRows * kStepBytes + a.q_stage + blocks * groups * kScaleTile);
+      };
+      auto groups_of = [&](int ks) { return min(2, (a.k64 - 4 * ks + 1) >> 1); };
+      // The weights' first stages do not depend on the kernel before this one; the activations may.
+      const int pt0 = first % a.p_tiles, qt0 = first / a.p_tiles;
+      const int pre = (a.early && first < a.tiles) ? min(S, k1 - k0) : 0;
+      for (int i = 0; i < pre; ++i) {
+        expect(i, qt0, groups_of(k0 + i));
+        if (SWAP) load_p(i, k0 + i, pt0, groups_of(k0 + i));
+        else load_q(i, k0 + i, qt0, groups_of(k0 + i));
+      }
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      int g = 0, s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < a.tiles; tile += step) {
+        const int pt = tile % a.p_tiles, qt = tile / a.p_tiles;
+        for (int ks = k0; ks < k1; ++ks, ++g) {
+          const int groups = groups_of(ks);
+          if (g < pre) {
+            if (SWAP) load_q(s, ks, qt, groups);
+            else load_p(s, ks, pt, groups);
+          } else {
+            if (!thread_wait(&empty[s], ph ^ 1, ctl, kErrWaitProducer)) {
+              ok = false;
+              break;
+            }
+            expect(s, qt, groups);
+            load_p(s, ks, pt, groups);
+            load_q(s, ks, qt, groups);
+          }
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (!ok)
+        for (int h = (g > S ? g - S : 0); h < g; ++h) drain_wait(&full[h % S], (h / S) & 1, a.err, kErrDrain);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+      const uint64_t s_desc = plain_desc(base + kRows * kStepBytes + a.q_stage);
+      const uint32_t i_desc[2] = {instruction_desc(a.T, 0u), instruction_desc(a.T, 2u)};
+      int i = 0, s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
+        // Overlapping accumulators: the shared columns of tile i - 1 are out; separate ones: tile i - 2 is.
+        const int w = a.shared_cols ? i - 1 : i - 2;
+        if (w >= 0 && !thread_wait(&drained[w & 1], (w >> 1) & 1, ctl, kErrWaitMma)) break;
+        tc_fence_after();
+        const int qt = tile / a.p_tiles;
+        const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
+        const uint32_t q_first = (qt * a.T % kRows) >> 5;  // column of the tile's first row within its row block
+        for (int ks = k0; ks < k1; ++ks) {
+          if (!thread_wait(&full[s], ph, ctl, kErrWaitMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int subs = min(4, a.k64 - 4 * ks), groups = (subs + 1) >> 1;
+          const uint32_t off = static_cast<uint32_t>(s) * (a.stage >> 4);
+          const uint32_t sf = tmem + a.sf_col + s * a.sf_stage;
+          // columns: P group 0, P group 1, Q group 0 (4 a row block), Q group 1
+          for (int gr = 0; gr < groups; ++gr) {
+            scales_to_tmem(sf + 4 * gr, s_desc + off + gr * (kScaleTile >> 4));
+            for (int b = 0; b < a.q_blocks; ++b)
+              scales_to_tmem(sf + 8 + 4 * (gr * a.q_blocks + b), s_desc + off + ((1 + b) * 2 + gr) * (kScaleTile >> 4));
+          }
+          for (int j = 0; j < subs; ++j)
+            mma_mxf4(d, p_desc + off + 2 * j, q_desc + off + 2 * j, i_desc[j & 1], sf + 4 * (j >> 1),
+                     sf + 8 + 4 * (j >> 1) * a.q_blocks + q_first, ks > k0 || j > 0);
+          mma_commit(&empty[s]);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) mma_commit(&accfull[i & 1]);
+      }
+      mma_commit(&done);  // every MMA and copy of this thread has completed once `done` flips
+      drain_wait(&done, 0, a.err, kErrDrain);
+    }
+  } else {
+    const int q = warp & 3, c = (warp - 2) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
+    const int chunks = a.T >> 4, shared_chunks = (a.shared_cols + 15) >> 4;
+    int i = 0;
+    for (int tile = first; tile < a.tiles; tile += step, ++i) {
+      const int pt = tile % a.p_tiles, qt = tile / a.p_tiles, b = i & 1;
+      const int p = pt * kRows + 32 * q + lane, q0 = qt * a.T;
+      if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
+      tc_fence_after();
+      const float p_bias = (SWAP && a.split == 1 && a.bias && p < a.p_rows) ? load_f(a.bias, F16, p) : 0.0f;
+      bool told = false;
+      for (int at = c; at < chunks + 2; at += 2) {
+        if (!told && at >= shared_chunks && (shared_chunks || at >= chunks)) {
+          // what the next tile's accumulator shares with this one (or all of it) has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&drained[b]);
+          told = true;
+        }
+        if (at >= chunks) break;
+        // the second accumulator shares its first columns with the other's last ones
+        const int col = 16 * ((b || !shared_chunks) ? at : chunks - 1 - at);
+        uint32_t v[16];
+        tmem_ld16(tmem + lane_addr + (b ? a.acc1 : 0) + col, v);
+        tmem_wait_ld16(v);
+        if (a.split > 1) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            reinterpret_cast<float*>(gbase)[(col + j) * kPitch + 32 * q + lane] = __uint_as_float(v[j]);
+        } else if (SWAP) {
+          if (p < a.p_rows) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int64_t m = q0 + col + j;
+              if (m >= a.q_rows) break;
+              const float r = __uint_as_float(v[j]) + p_bias;
+              if (F16) static_cast<__half*>(a.y)[m * a.ldy + p] = __float2half_rn(r);
+              else static_cast<float*>(a.y)[m * a.ldy + p] = r;
+            }
+          }
+        } else if (p < a.p_rows) {
+          const int n0 = q0 + col;
+          float r[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            r[j] = __uint_as_float(v[j]) + ((a.bias && n0 + j < a.q_rows) ? load_f(a.bias, F16, n0 + j) : 0.0f);
+          if (a.vec && n0 + 16 <= a.q_rows) {
+            if (F16) {
+              uint32_t h[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const __half2 x = __floats2half2_rn(r[2 * j], r[2 * j + 1]);
+                h[j] = *reinterpret_cast<const uint32_t*>(&x);
+              }
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.y) + p * a.ldy + n0);
+              dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+              dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+            } else {
+              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.y) + p * a.ldy + n0);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) dst[j] = make_float4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (n0 + j >= a.q_rows) break;
+              if (F16) static_cast<__half*>(a.y)[p * a.ldy + n0 + j] = __float2half_rn(r[j]);
+              else static_cast<float*>(a.y)[p * a.ldy + n0 + j] = r[j];
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+  }
+  if (a.split > 1) {
+    // one tile a cluster: every rank sums its share of the rows of P (SWAP: columns of y) over the ranks
+    cluster_sync();
+    const int pt = first % a.p_tiles, qt = first / a.p_tiles, share = kRows / a.split, p0 = rank * share;
+    const int cols = min(a.T, a.q_rows - qt * a.T);
+    for (int e = threadIdx.x; e < share * cols; e += kThreads) {
+      // consecutive threads along the columns n of y
+      const int col = SWAP ? e / share : e % cols, row = p0 + (SWAP ? e % share : e / cols);
+      const int p = pt * kRows + row, qq = qt * a.T + col;
+      if (p >= a.p_rows) continue;
+      float r = 0.0f;
+      for (int k = 0; k < a.split; ++k) r += ld_cluster_f32(map_rank(base + (col * kPitch + row) * 4, k));
+      const int64_t m = SWAP ? qq : p, n = SWAP ? p : qq;
+      if (a.bias) r += load_f(a.bias, F16, n);
+      if (F16) static_cast<__half*>(a.y)[m * a.ldy + n] = __float2half_rn(r);
+      else static_cast<float*>(a.y)[m * a.ldy + n] = r;
+    }
+    cluster_sync();  // nobody leaves while its partial tile is being read
+  }
+}
+
+// ------------------------------------------------------------------ host side
+struct Shape {
+  bool swap;
+  int T, split;
+};
+
+// Up to 128 activation rows: all of them in one tile, K split until the CTAs cover the SMs. More: tiles of
+// 256 columns, narrower ones and a split of K where that leaves SMs idle.
+Shape choose(const Mxfp4Matmul& p, int ksteps, int sms) {
+  Shape s{p.M <= kRows, 256, 1};
+  int64_t tiles;
+  if (s.swap) {
+    s.T = static_cast<int>(align_up(p.M, 16));
+    tiles = ceil_div(p.N, kRows);
+  } else {
+    const int64_t pt = ceil_div(p.M, kRows);
+    if (pt * ceil_div(p.N, 256) < sms) s.T = 128;
+    tiles = pt * ceil_div(p.N, s.T);
+  }
+  if (s.T <= 128)
+    while (s.split < 8 && tiles * s.split * 2 <= 2 * sms && ksteps >= 4 * s.split) s.split *= 2;
+  return s;
+}
+
+template <bool SWAP, bool F16>
+cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(mxfp4_gemm_kernel<SWAP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<SWAP, F16>, mp, mq, a);
+}
+
+}  // namespace
+
+cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s) {
+  const int sms = device_sm_count();
+  Args a{};
+  a.k64 = static_cast<int>(ceil_div(p.kb, 2));
+  a.ksteps = (a.k64 + 3) / 4;
+  const Shape sh = choose(p, a.ksteps, sms);
+  a.T = sh.T;
+  a.split = sh.split;
+  a.p_rows = static_cast<int>(sh.swap ? p.N : p.M);
+  a.q_rows = static_cast<int>(sh.swap ? p.M : p.N);
+  a.p_tiles = static_cast<int>(ceil_div(a.p_rows, kRows));
+  const int64_t tiles = static_cast<int64_t>(a.p_tiles) * ceil_div(a.q_rows, a.T);
+  if (tiles > INT_MAX / 8) return cudaErrorInvalidValue;
+  a.tiles = static_cast<int>(tiles);
+  a.q_blocks = a.T > kRows ? 2 : 1;
+  a.tiles_k = ceil_div(p.kb, 4);
+  a.sp_blocks = a.p_tiles;
+  a.sq_blocks = static_cast<int>(ceil_div(a.q_rows, kRows));
+  a.sp = sh.swap ? p.b_scales : p.a_scales;
+  a.sq = sh.swap ? p.a_scales : p.b_scales;
+  a.bias = p.bias;
+  a.y = p.y;
+  a.ldy = p.ldy;
+  a.vec = (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0 && (p.ldy * (p.f16 ? 2 : 4)) % 16 == 0;
+  a.err = p.err;
+  a.early = early;
+  a.q_stage = static_cast<uint32_t>(a.T) * kStepBytes;
+  a.stage = kRows * kStepBytes + a.q_stage + (1 + a.q_blocks) * 2 * kScaleTile;
+  a.stage = (a.stage + 1023u) & ~1023u;
+  a.sf_stage = 8 + 8 * a.q_blocks;
+  const int steps = static_cast<int>(ceil_div(a.ksteps, a.split));
+  const bool one_tile = a.split > 1 || a.tiles <= sms;
+  int stages = (kSmemBudget - 2048) / static_cast<int>(a.stage);
+  if (stages > 12) stages = 12;
+  if (one_tile && stages > steps) stages = steps;
+  size_t smem = static_cast<size_t>(stages) * a.stage;
+  if (a.split > 1 && smem < static_cast<size_t>(a.T) * kPitch * 4) smem = static_cast<size_t>(a.T) * kPitch * 4;
+  smem += 1024;
+  a.stages = stages;
+  // Tensor memory: accumulators, then the stages' scales.
+  const int sf = stages * a.sf_stage;
+  const int acc = one_tile ? a.T : 2 * a.T;
+  a.shared_cols = acc + sf > kTmemCols ? acc + sf - kTmemCols : 0;
+  a.acc1 = one_tile ? 0 : a.T - a.shared_cols;
+  a.sf_col = acc - a.shared_cols;
+  a.tmem_cols = 32;
+  while (a.tmem_cols < a.sf_col + sf) a.tmem_cols *= 2;
+  // CTAs that share an SM share its 512 columns: ask for enough shared memory that no more fit than those feed.
+  const size_t least = static_cast<size_t>(kSmemBudget) / (kTmemCols / a.tmem_cols + 1) + 1024;
+  if (smem < least) smem = least;
+  const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
+
+  CUtensorMap mp, mq;
+  const uint64_t row = static_cast<uint64_t>(p.kb) * 16;
+  if (!encode_tensor_map_2d(&mp, 0, sh.swap ? p.b : p.a, row, a.p_rows, row, kStepBytes, kRows, true) ||
+      !encode_tensor_map_2d(&mq, 0, sh.swap ? p.a : p.b, row, a.q_rows, row, kStepBytes, a.T, true))
+    return cudaErrorInvalidValue;
+  if (sh.swap) return p.f16 ? launch<true, true>(mp, mq, a, grid, smem, early, s) : launch<true, false>(mp, mq, a, grid, smem, early, s);
+  return p.f16 ? launch<false, true>(mp, mq, a, grid, smem, early, s) : launch<false, false>(mp, mq, a, grid, smem, early, s);
+}
+
+}  // namespace xrgpu
