@@ -523,6 +523,8 @@ typedef struct {
   int32_t cache_dtype;  /* XRGPU_INT8 or XRGPU_FLOAT8_E4M3 */
   int32_t causal;       /* attention: nonzero: a row sees the tokens up to its own position */
   float scale;          /* attention: factor of q . k, usually head_dim^-1/2 */
+  int32_t zero_rest;    /* attention: nonzero: rows behind the last sequence are set to zero */
+  int32_t reserved;
   int64_t tokens;       /* rows of q, k, v, o */
   int64_t sequences, heads_q, heads_kv, head_dim, page, pages, max_pages;
   int64_t window;       /* attention, causal: a row sees the last `window` tokens up to itself; 0: all */
@@ -551,7 +553,8 @@ XRGPU_API int xrgpu_kv8_read(const xrgpu_kv8_problem* p, void* stream);
 
 /* o[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j of the row's sequence that it sees;
  * query head h reads key/value head h / (heads_q / heads_kv). A row that sees nothing gives zeros (cu_seqlens may
- * hold more rows than kv_len tokens here; the first ones then see nothing). */
+ * hold more rows than kv_len tokens here; the first ones then see nothing); so do the rows of a sequence whose
+ * kv_len does not fit. Tokens of a bad page id are left out. */
 XRGPU_API int xrgpu_kv8_attention_workspace_size(const xrgpu_kv8_problem* p, uint64_t* bytes);
 /* workspace as in xrgpu_mxfp4_forward. */
 XRGPU_API int xrgpu_kv8_attention(const xrgpu_kv8_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);

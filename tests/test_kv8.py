@@ -328,6 +328,27 @@ def test_nan_blocks_reach_their_readers_only(F, dtype, new):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_nan_page_at_the_edge_of_what_rows_see(F, dtype, page):
+    """A page that only some rows of a tile see (behind the causal edge, or out of the window) reaches those only."""
+    n, lens = 6, 3 * page + 2  # the last two rows are the first tokens of the last page
+    for window in (0, page):
+        for side in ("ks", "vs"):
+            c = R.Cache([lens], heads=1, D=64, page=page, code=INT8)
+            bad = 3 if window == 0 else 2
+            getattr(c, side)[c.table[0, bad], 0] = float("nan")
+            if window:
+                c.ks[c.table[0, 3], 0] = 0.02
+            q = torch.randn(n, 4, 64, device="cuda", dtype=dtype)
+            o = F.attention_kv8(q, *c.cuda(), None, c.lens.cuda(), window=window)
+            pos = torch.arange(lens - n, lens)
+            lo = (pos - window + 1).clamp(min=0) if window else torch.zeros_like(pos)
+            sees = (pos >= bad * page) & (lo < (bad + 1) * page)
+            assert torch.equal(torch.isnan(o).all(-1).all(-1).cpu(), sees) and torch.equal(torch.isnan(o).any(-1).any(-1).cpu(), sees)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_strides_uniform_and_repeat(F, dtype):
     """Queries inside a fused projection, an output with padding, no cu_seqlens; the same bits on every call."""
     c = R.Cache([90, 33], heads=2, D=64, page=16, code=INT8)
@@ -356,7 +377,7 @@ def test_attention_bad_pages_are_skipped(F):
     for bad in (-3, 10 ** 6):
         c.lens[0] = bad
         o = F.attention_kv8(q.cuda(), *c.cuda(), None, c.lens.cuda())
-        assert F.device_error(0) == 0x502 and torch.equal(o[1], whole[1])
+        assert F.device_error(0) == 0x502 and torch.equal(o[1], whole[1]) and bool((o[0] == 0).all())
 
 
 @gpu

@@ -13,9 +13,10 @@ struct SeqRows {
   int row0, n, len;  // first row, number of rows, tokens of the sequence (the rows included)
 };
 
-// Rows and length of sequence b; n = 0 for lengths that do not fit (recorded in the error word).
-// Attention (rows_may_exceed) accepts more rows than tokens: the first rows then see nothing.
-__device__ __forceinline__ SeqRows seq_rows(const Kv8& p, int b, bool rows_may_exceed) {
+// Rows and length of sequence b. Lengths that do not fit are recorded in the error word: rows outside the
+// call's give n = 0; a length outside the table's gives n = 0 (append, read) or len = 0 (attention: the rows
+// see nothing). More rows than tokens fit attention only, whose first rows then see nothing.
+__device__ __forceinline__ SeqRows seq_rows(const Kv8& p, int b, bool attention) {
   SeqRows r;
   if (p.uniform) {
     r.n = p.tokens / p.seqs;
@@ -25,12 +26,13 @@ __device__ __forceinline__ SeqRows seq_rows(const Kv8& p, int b, bool rows_may_e
     r.n = p.cu[b + 1] - r.row0;
   }
   r.len = p.kv_len[b];
-  const bool bad = r.row0 < 0 || r.n < 0 || r.n > p.tokens || r.row0 > p.tokens - r.n || r.len < 0 ||
-                   static_cast<int64_t>(r.len) > (static_cast<int64_t>(p.max_pages) << p.page_log2) ||
-                   (!rows_may_exceed && r.n > r.len);
-  if (bad) {
+  const bool bad_rows = r.row0 < 0 || r.n < 0 || r.n > p.tokens || r.row0 > p.tokens - r.n;
+  const bool bad_len = r.len < 0 || static_cast<int64_t>(r.len) > (static_cast<int64_t>(p.max_pages) << p.page_log2) ||
+                       (!attention && r.n > r.len);
+  if (bad_rows || bad_len) {
     record_device_error(p.err, kErrKv8Length);
-    r.row0 = r.n = r.len = 0;
+    r.len = 0;
+    if (bad_rows || !attention) r.row0 = r.n = 0;
   }
   return r;
 }

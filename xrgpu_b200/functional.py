@@ -560,8 +560,8 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     dev = k_cache.device
     p.q_stride = _head_rows(q, "q", None, p.head_dim, dev)
     if out is None:
-        # with cu_seqlens the rows may go on behind the last sequence
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev) if cu_seqlens is None else torch.zeros(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        p.zero_rest = 1
     elif out.dtype != q.dtype or out.shape != q.shape:
         raise ValueError("out must have q's shape and dtype")
     p.o_stride = _head_rows(out, "out", q.shape[1], p.head_dim, dev)
