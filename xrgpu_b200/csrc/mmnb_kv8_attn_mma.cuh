@@ -147,7 +147,7 @@ __device__ __forceinline__ SeqWork seq_work(const Kv8& p, int b, int rows_per_ti
   SeqWork w;
   w.r = seq_rows(p, b, true);
   const int G = p.hq / p.hkv;
-  w.tiles = (w.r.n * G + rows_per_tile - 1) / rows_per_tile;
+  w.tiles = static_cast<int64_t>(w.r.n) * G > p.few_rows ? 0 : (w.r.n * G + rows_per_tile - 1) / rows_per_tile;
   const int pos0 = w.r.len - w.r.n;  // position of the first row (may be negative)
   const int lo = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
   w.first = lo / kStep;
@@ -699,6 +699,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws,
       }
     return;
   }
+  if (w.tiles == 0) return;
   const int G = p.hq / p.hkv, rr = (row - w.r.row0) * G + h % G, tile = rr / R, r = rr % R;
   const int64_t g0 = ws.start[b] + (static_cast<int64_t>(h / G) * w.tiles + tile) * w.steps, g1 = g0 + w.steps;
   const int64_t run = run_length(ws.start[p.seqs], grid);
@@ -733,9 +734,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws,
 }
 
 // ------------------------------------------------------------------ host side
-// 8-row tiles a segment: as many as an average sequence has rows.
+// 8-row tiles a segment: as many as an average sequence has rows (or may have here).
 inline int row_tiles(const Kv8& p) {
-  const int64_t rows = ceil_div(p.tokens, p.seqs) * (p.hq / p.hkv);
+  const int64_t mean = ceil_div(p.tokens, p.seqs) * (p.hq / p.hkv), rows = mean < p.few_rows ? mean : p.few_rows;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
 

@@ -1,0 +1,551 @@
+// Attention over the paged 8-bit cache for prompts: float16 rows, tcgen05 tensor cores (layout: mmnb_kv8.h).
+//
+//   o[row, h] = sum_j softmax_j(scale * q . k_j) v_j,   k_j = code * k_scale[page], v_j = code * v_scale[page]
+//
+// A CTA takes 256 rows of one sequence and key/value head (row r is query token r / G and head r % G of its group of
+// G, so the group shares every key and value) as two tiles of 128, and passes once over the tokens they see,
+// 128 at a time. Codes are exact float16 numbers: they are widened once a CTA, in registers, on their way
+// to shared memory, and the scales stay out of them: k_scale multiplies the scores a page at a time, and
+// v_scale joins the exponent of the weights: P' = exp2(x - m + log2(v_scale 2^11 / R)), R the power of two above the
+// largest v_scale of the tokens. With m raised only when a score exceeds it by 4, P' stays below 2^15, so
+// float16 holds 2^25 of range below the largest weight times the largest scale at full precision. The normaliser is the
+// float32 sum of P' divided by the same factor, a page at a time.
+//
+// Roles (16 warps, register counts moved from the widening warps to the softmax warps):
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row. Read S from tensor memory, release it, raise m (and rescale
+//                   O, rare), write P', at the end write the row out.
+//   warps 8-11      widen keys and values: 16-byte loads a tile ahead, float16 to the 128-byte swizzle the tensor
+//                   cores read (keys K-major, values MN-major: both as they lie, no transposition).
+//   warp 12         (of 12-15) issues the MMAs (one lane): P0 V, Q0 K, P1 V, Q1 K, so that a tile's softmax runs under the
+//                   other tile's products.
+// Tensor memory: S [0, 128) (one tile's scores at a time), P' of the tiles at 128 and 192, O at 256 and 384.
+// Bounds per 128 tokens and 256 rows at D = 128, in cycles: tensor cores 2048, exponentials (16 a cycle) 2048, shared memory
+// (Q and K read for each S, V for each O, keys and values written: 256 KB) 2048.
+//
+// Every wait is bounded as in mmnb_gemm_sm100.cu.
+#include <cuda_runtime.h>
+
+#include "mmnb_kv8_attn.h"
+#include "mmnb_kv8.cuh"
+#include "mmnb_tcgen05.cuh"
+
+namespace xrgpu {
+namespace {
+
+constexpr int kTile = 128;        // rows of a tile, tokens of a step
+constexpr int kRows = 2 * kTile;  // rows of a CTA
+constexpr int kSoftmaxWarps = 8;
+constexpr int kWidenWarps = 4;
+constexpr int kThreads = (kSoftmaxWarps + kWidenWarps + 4) * 32;  // the MMA warp and three that only fill its warpgroup
+constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps;
+constexpr int kChunks = kTile / 16;
+// Registers a thread: launched with kRegs (what 16 warps can have), then moved between the warpgroups.
+constexpr int kRegs = 128, kSoftmaxRegs = 176, kWidenRegs = 112, kMmaRegs = 48;
+static_assert(256 * kSoftmaxRegs + 128 * kWidenRegs + 128 * kMmaRegs <= kThreads * kRegs, "more registers than the block has");
+constexpr float kRaise = 4.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kS = 0, kP = 128, kO = 256;  // tensor memory columns
+
+constexpr unsigned kErrMma = 0x503, kErrWiden = 0x504, kErrSoftmax = 0x505, kErrDrain = 0x506;
+
+template <int D>
+struct Smem {
+  static constexpr int kPanel = kTile * 128;                 // 128 rows of 64 float16
+  static constexpr int kOperand = kPanel * (D / 64);         // a tile of Q, K or V
+  static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kEnd = kV + 2 * kOperand;
+  static constexpr int kBytes = kEnd + 1024;
+};
+
+// What the softmax needs of 16 tokens: the factor of their scores, log2 and inverse of the values' factor.
+struct Chunk {
+  float kf, lv, iv;
+  int ok;
+};
+
+struct Bars {
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2], sfree, done;
+};
+
+// Values operand: [tokens][64] float16 panels, 64 values of D contiguous (MN-major), 128-byte swizzle: 8-token groups 1024
+// bytes apart (stride byte offset), panels kPanel apart (leading byte offset).
+template <int D>
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(Smem<D>::kPanel >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four codes to two float16x2, in order.
+template <bool E4M3>
+__device__ __forceinline__ uint2 widen4(uint32_t w) {
+  uint2 r;
+  if (E4M3) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(r.x), "=r"(r.y) : "r"(w));
+  } else {
+    w ^= 0x80808080u;  // c + 128 over 1024: the float16 number 1152 + c
+    r.x = hsub2_u32(prmt(w, 0x64646464u, 0x4140u), 0x64806480u);
+    r.y = hsub2_u32(prmt(w, 0x64646464u, 0x4342u), 0x64806480u);
+  }
+  return r;
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+struct Job {
+  int b, tile, head, rows;  // rows: of this CTA (<= 256)
+  SeqRows r;
+  int t0, t1;               // tokens seen by any row
+};
+
+template <bool E4M3, int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
+  using M = Smem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Bars bars;
+  __shared__ Chunk meta[4][kChunks];
+  __shared__ uint32_t tmem_slot, vmax_bits;
+  __shared__ int abort_flag, found_b, found_tile;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.hq / p.hkv, head = blockIdx.x % p.hkv, slot = blockIdx.x / p.hkv;
+
+  // ---- which rows: slot counts the 256-row tiles of the sequences with more than p.few_rows rows; a sequence's
+  // last rows, which see most, come first
+  if (tid == 0) found_b = -1;
+  __syncthreads();
+  if (warp == 0) {
+    int before = 0;
+    for (int b0 = 0; b0 < p.seqs; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b < p.seqs) {
+        const SeqRows r = seq_rows(p, b, true);
+        if (static_cast<int64_t>(r.n) * G > p.few_rows) n = (r.n * G + kRows - 1) / kRows;
+      }
+      int sum = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += o;
+      }
+      const int at = slot - before - (sum - n);
+      if (at >= 0 && at < n) {
+        found_b = b;
+        found_tile = n - 1 - at;
+      }
+      before += __shfl_sync(~0u, sum, 31);
+      if (before > slot) break;
+    }
+  }
+  __syncthreads();
+  if (found_b < 0) return;
+  Job job;
+  job.b = found_b;
+  job.tile = found_tile;
+  job.head = head;
+  job.r = seq_rows(p, job.b, true);
+  job.rows = min(kRows, job.r.n * G - job.tile * kRows);
+  const int pos0 = job.r.len - job.r.n;
+  {
+    const int first = pos0 + job.tile * kRows / G, last = pos0 + (job.tile * kRows + job.rows - 1) / G;
+    job.t1 = p.causal ? min(last + 1, job.r.len) : job.r.len;
+    job.t0 = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    if (job.t1 < job.t0) job.t1 = job.t0;
+  }
+  const int j0 = job.t0 / kTile, n_steps = job.t1 > job.t0 ? (job.t1 + kTile - 1) / kTile - j0 : 0;
+  const bool two = job.rows > kTile;
+
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.kfull[i], kWidenWarps);
+      mbar_init(&bars.vfull[i], kWidenWarps);
+      mbar_init(&bars.kempty[i], 1);
+      mbar_init(&bars.vempty[i], 1);
+      mbar_init(&bars.sfull[i], 1);
+      mbar_init(&bars.odone[i], 1);
+      mbar_init(&bars.pfull[i], 4);
+    }
+    mbar_init(&bars.sfree, 4);
+    mbar_init(&bars.done, 1);
+    abort_flag = 0;
+    vmax_bits = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+  const Ctl ctl{&abort_flag, p.err};
+
+  // ---- queries to shared memory (K-major, 128-byte swizzle), negated for a negative scale; the largest v_scale
+  {
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+    const bool vec = (reinterpret_cast<uintptr_t>(p.q) & 15u) == 0 && (p.qs & 7) == 0;
+    constexpr int kPer = D / 8;
+    for (int e = tid; e < kRows * kPer; e += kThreads) {
+      const int r = e / kPer, ch = e % kPer;  // 16-byte chunk ch of row r
+      uint32_t v[4] = {0, 0, 0, 0};
+      if (r < job.rows) {
+        const int rr = job.tile * kRows + r;
+        const __half* src = static_cast<const __half*>(p.q) + static_cast<int64_t>(job.r.row0 + rr / G) * p.qs + (head * G + rr % G) * D + ch * 8;
+        if (vec) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src);
+          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = static_cast<uint32_t>(__half_as_ushort(src[2 * i])) | (static_cast<uint32_t>(__half_as_ushort(src[2 * i + 1])) << 16);
+        }
+      }
+      const int row = r & (kTile - 1);
+      const uint32_t at = base + M::kQ + (r / kTile) * M::kOperand + (ch >> 3) * M::kPanel + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+      sts128(at, v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip);
+    }
+    uint32_t vm = 0;
+    for (int pg = (job.t0 >> p.page_log2) + tid; (pg << p.page_log2) < job.t1; pg += kThreads) {
+      const int id = page_id(p, job.b, pg);
+      const uint32_t bits = id < 0 ? 0u : __float_as_uint(p.v_scale[static_cast<int64_t>(id) * p.hkv + head]) & 0x7fffffffu;
+      if (bits < 0x7f800000u) vm = max(vm, bits);
+    }
+    vm = __reduce_max_sync(~0u, vm);
+    if (lane == 0 && vm) atomicMax(&vmax_bits, vm);
+    fence_async_shared();
+  }
+  __syncthreads();
+  // R: the power of two above the largest scale (exponent field + 1), and 2^11 / R
+  const uint32_t r_exp = min(max((vmax_bits >> 23) + 1u, 13u), 253u);
+  const float value_unit = __uint_as_float((r_exp - 11u) << 23);  // R 2^-11
+  const float to_unit = __uint_as_float((265u - r_exp) << 23);
+
+  if (warp < kSoftmaxWarps) {
+    regs_inc<kSoftmaxRegs>();
+    // ---------------------------------------------------------------- softmax
+    const int a = warp >> 2, q = warp & 3, row = a * kTile + q * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
+    const uint32_t s_at = tmem + lanes + kS, p_at = tmem + lanes + kP + 64 * a, o_at = tmem + lanes + kO + 128 * a;
+    const int rr = job.tile * kRows + min(row, job.rows - 1), pos = pos0 + rr / G;
+    const int hi = p.causal ? max(0, min(pos + 1, job.r.len)) : job.r.len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = a == 0 || two;
+    for (int j = 0; ok && j < n_steps; ++j) {
+      if (!warp_wait(&bars.sfull[a], j & 1, ctl, kErrSoftmax)) break;
+      tc_fence_after();
+      uint32_t x[kTile];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, x + 32 * i);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_fence_ld(x + 32 * i);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.sfree);
+
+      const Chunk* ch = meta[j & 3];
+      const int t0 = (j0 + j) * kTile;
+      bool full = t0 >= lo && t0 + kTile <= hi;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) full &= ch[c].ok != 0;
+      const bool plain = __all_sync(~0u, full);
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        float t = -INFINITY;
+        if (plain) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) t = fmaxf(t, __uint_as_float(x[16 * c + e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int tok = t0 + 16 * c + e;
+            if (tok < hi && tok >= lo && ch[c].ok) t = fmaxf(t, __uint_as_float(x[16 * c + e]));
+          }
+        }
+        const float f = t * ch[c].kf;
+        if (t > -INFINITY) top = fmaxf(top, f);
+      }
+      const bool raise = top > m + kRaise;
+      bool waited = false;
+      if (__any_sync(~0u, raise)) {
+        const float fresh = raise ? top : m;
+        const float f = raise ? (m == -INFINITY ? 0.0f : exp2_approx(m - fresh)) : 1.0f;
+        m = fresh;
+        l *= f;
+        if (j > 0) {
+          if (!warp_wait(&bars.odone[a], (j - 1) & 1, ctl, kErrSoftmax)) break;
+          waited = true;
+          tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tmem_ld32(o_at + 32 * i, o);
+            tmem_wait_ld();
+            tmem_fence_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st32(o_at + 32 * i, *reinterpret_cast<const uint32_t(*)[32]>(o));
+          }
+          tmem_wait_st();
+        }
+      }
+      const float mm = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const float kf = ch[c].kf, sub = ch[c].lv - mm;
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          float w0 = exp2_approx(fmaf(__uint_as_float(x[16 * c + e]), kf, sub));
+          float w1 = exp2_approx(fmaf(__uint_as_float(x[16 * c + e + 1]), kf, sub));
+          if (!plain) {
+            const int tok = t0 + 16 * c + e;
+            if (!(tok < hi && tok >= lo && ch[c].ok)) w0 = 0.0f;
+            if (!(tok + 1 < hi && tok + 1 >= lo && ch[c].ok)) w1 = 0.0f;
+          }
+          sum += w0 + w1;
+          x[8 * c + e / 2] = pack_half2(w0, w1);
+        }
+        if (plain || sum != 0.0f) l = fmaf(sum, ch[c].iv, l);
+      }
+      // P' may be written once the products of the step before have read it
+      if (j > 0 && !waited && !warp_wait(&bars.odone[a], (j - 1) & 1, ctl, kErrSoftmax)) break;
+      tc_fence_after();
+      tmem_st32(p_at, *reinterpret_cast<const uint32_t(*)[32]>(x));
+      tmem_st32(p_at + 32, *reinterpret_cast<const uint32_t(*)[32]>(x + 32));
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.pfull[a]);
+    }
+    if (ok && n_steps > 0) ok = warp_wait(&bars.odone[a], (n_steps - 1) & 1, ctl, kErrSoftmax);
+    tc_fence_after();
+    if (ok) {
+      const float inv = l == 0.0f ? 0.0f : value_unit / l;
+      __half* dst = static_cast<__half*>(p.o) + static_cast<int64_t>(job.r.row0 + rr / G) * p.os + (head * G + rr % G) * D;
+      const bool vec = (reinterpret_cast<uintptr_t>(p.o) & 15u) == 0 && (p.os & 7) == 0;
+#pragma unroll 1
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t o[32];
+        if (n_steps > 0) {
+          tmem_ld32(o_at + 32 * i, o);
+          tmem_wait_ld();
+          tmem_fence_ld(o);
+        }
+        if (row < job.rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              h[k] = n_steps > 0 && inv != 0.0f ? pack_half2(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv) : 0u;
+            if (vec) {
+              *reinterpret_cast<uint4*>(dst + 32 * i + e) = make_uint4(h[0], h[1], h[2], h[3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                dst[32 * i + e + 2 * k] = __ushort_as_half(static_cast<unsigned short>(h[k] & 0xffffu));
+                dst[32 * i + e + 2 * k + 1] = __ushort_as_half(static_cast<unsigned short>(h[k] >> 16));
+              }
+            }
+          }
+        }
+      }
+    }
+  } else if (warp < kMmaWarp) {
+    regs_dec<kWidenRegs>();
+    // ---------------------------------------------------------------- widen keys and values
+    constexpr int kPieces = D / 16;                                     // 16-byte pieces a row
+    constexpr int kPer = kTile * kPieces / (kWidenWarps * 32);          // pieces a thread, keys and values each
+    const int ct = tid - kSoftmaxWarps * 32, piece = ct % kPieces, row0 = ct / kPieces;
+    constexpr int kRowStep = kWidenWarps * 32 / kPieces;
+    uint4 k[kPer], v[kPer];
+    float ks = 0.0f, vs = 0.0f;  // of chunk ct (threads 0-7)
+    int okc = 0;
+    auto where = [&](int j, int row, int* id) -> int64_t {
+      const int tok = (j0 + j) * kTile + row;
+      *id = tok < job.t1 ? page_id(p, job.b, tok >> p.page_log2) : -1;
+      return (((static_cast<int64_t>(*id) * p.hkv + head) << p.page_log2) + (tok & (p.page - 1))) * D + piece * 16;
+    };
+    auto load_k = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        int id;
+        const int64_t at = where(j, row0 + i * kRowStep, &id);
+        k[i] = id >= 0 ? *reinterpret_cast<const uint4*>(p.k_cache + at) : make_uint4(0, 0, 0, 0);
+      }
+      if (ct < kChunks) {
+        int id;
+        where(j, 16 * ct, &id);
+        okc = id >= 0;
+        ks = okc ? p.k_scale[static_cast<int64_t>(id) * p.hkv + head] : 0.0f;
+        vs = okc ? p.v_scale[static_cast<int64_t>(id) * p.hkv + head] : 0.0f;
+      }
+    };
+    auto load_v = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        int id;
+        const int64_t at = where(j, row0 + i * kRowStep, &id);
+        // values of a zero scale are zero whatever their codes
+        const bool use = id >= 0 && p.v_scale[static_cast<int64_t>(id) * p.hkv + head] != 0.0f;
+        v[i] = use ? *reinterpret_cast<const uint4*>(p.v_cache + at) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto store = [&](uint32_t to, const uint4* w) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int row = row0 + i * kRowStep;
+        const uint32_t line = to + (piece >> 2) * M::kPanel + row * 128;
+        const uint2 a = widen4<E4M3>(w[i].x);
+        const uint2 b = widen4<E4M3>(w[i].y), c = widen4<E4M3>(w[i].z), d = widen4<E4M3>(w[i].w);
+        // 16-byte chunks 2 (piece % 4) and + 1; the two panels' lanes start with different ones: no bank twice
+        const int c0 = 2 * (piece & 3), odd = (piece >> 2) & 1;
+        const uint32_t at0 = line + ((c0 ^ (row & 7)) << 4), at1 = line + (((c0 + 1) ^ (row & 7)) << 4);
+        if (odd) {
+          sts128(at1, c.x, c.y, d.x, d.y);
+          sts128(at0, a.x, a.y, b.x, b.y);
+        } else {
+          sts128(at0, a.x, a.y, b.x, b.y);
+          sts128(at1, c.x, c.y, d.x, d.y);
+        }
+      }
+    };
+    if (n_steps > 0) {
+      load_k(0);
+      load_v(0);
+    }
+    for (int j = 0; j < n_steps; ++j) {
+      const int st = j & 1;
+      const uint32_t was = ((j >> 1) & 1) ^ 1;
+      if (!warp_wait(&bars.kempty[st], was, ctl, kErrWiden)) break;
+      store(base + M::kK + st * M::kOperand, k);
+      if (ct < kChunks) {
+        Chunk c;
+        const float f = vs == 0.0f ? 1.0f : fmaxf(vs * to_unit, 8.6736174e-19f);  // at least 2^-60; keeps a NaN out of fmaxf below
+        c.kf = ks * fabsf(p.scale) * kLog2e;
+        c.lv = vs != vs ? vs : __log2f(f);
+        c.iv = vs != vs ? vs : 1.0f / f;
+        c.ok = okc;
+        meta[j & 3][ct] = c;
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.kfull[st]);
+      if (j + 1 < n_steps) load_k(j + 1);
+      if (!warp_wait(&bars.vempty[st], was, ctl, kErrWiden)) break;
+      store(base + M::kV + st * M::kOperand, v);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.vfull[st]);
+      if (j + 1 < n_steps) load_v(j + 1);
+    }
+  } else {
+    regs_dec<kMmaRegs>();
+  }
+  if (warp == kMmaWarp && lane == 0) {
+    // ---------------------------------------------------------------- MMAs
+    constexpr uint32_t kF32Out = 1u << 4;
+    const uint32_t qk = kF32Out | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+    const uint32_t pv = kF32Out | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+    const uint64_t qd = umma_desc_sw128(base + M::kQ), kd = umma_desc_sw128(base + M::kK), vd = desc_mn<D>(base + M::kV);
+    int issued = 0;  // S products so far
+    bool ok = true;
+    auto scores = [&](int a, int j) {
+      if (issued > 0 && !thread_wait(&bars.sfree, (issued - 1) & 1, ctl, kErrMma)) return false;
+      tc_fence_after();
+      ++issued;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint64_t off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
+        mma_f16_ss(tmem + kS, qd + a * (M::kOperand >> 4) + off, kd + (j & 1) * (M::kOperand >> 4) + off, qk, i > 0);
+      }
+      mma_commit(&bars.sfull[a]);
+      return true;
+    };
+    auto values = [&](int a, int j) {
+      if (!thread_wait(&bars.pfull[a], j & 1, ctl, kErrMma)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < kTile / 16; ++i)
+        mma_f16_ts(tmem + kO + 128 * a, tmem + kP + 64 * a + 8 * i, vd + (j & 1) * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
+      mma_commit(&bars.odone[a]);
+      return true;
+    };
+    for (int j = -1; ok && j < n_steps; ++j) {
+      const bool more = j + 1 < n_steps;
+      if (j >= 0) {
+        ok = thread_wait(&bars.vfull[j & 1], (j >> 1) & 1, ctl, kErrMma) && values(0, j);
+        if (ok && !two) mma_commit(&bars.vempty[j & 1]);
+      }
+      if (ok && more) {
+        ok = thread_wait(&bars.kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, ctl, kErrMma) && scores(0, j + 1);
+        if (ok && !two) mma_commit(&bars.kempty[(j + 1) & 1]);
+      }
+      if (two) {
+        if (ok && j >= 0) {
+          ok = values(1, j);
+          if (ok) mma_commit(&bars.vempty[j & 1]);
+        }
+        if (ok && more) {
+          ok = scores(1, j + 1);
+          if (ok) mma_commit(&bars.kempty[(j + 1) & 1]);
+        }
+      }
+    }
+    mma_commit(&bars.done);  // every MMA issued has completed once it flips
+    drain_wait(&bars.done, 0, p.err, kErrDrain);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+template <bool E4M3, int D>
+cudaError_t launch(const Kv8& p, cudaStream_t s) {
+  const cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<E4M3, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes > 120 * 1024 ? Smem<D>::kBytes : 120 * 1024);
+  if (e != cudaSuccess) return e;
+  // one CTA an SM: it takes all tensor memory
+  const int bytes = Smem<D>::kBytes > 120 * 1024 ? Smem<D>::kBytes : 120 * 1024;
+  const int64_t G = p.hq / p.hkv, tiles = p.uniform ? ceil_div(p.tokens / p.seqs * G, kRows) * p.seqs : p.tokens * G / kRows + p.seqs;
+  attn_prompt_kernel<E4M3, D><<<static_cast<unsigned>(tiles * p.hkv), kThreads, bytes, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_attn_prompt(const Kv8& p, cudaStream_t s) {
+  if (p.D == 128) return p.e4m3 ? launch<true, 128>(p, s) : launch<false, 128>(p, s);
+  return p.e4m3 ? launch<true, 64>(p, s) : launch<false, 64>(p, s);
+}
+
+}  // namespace xrgpu
