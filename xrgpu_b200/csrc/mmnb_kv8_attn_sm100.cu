@@ -85,6 +85,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Two float32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -268,27 +284,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       if (lane == 0) mbar_arrive(&bars.sfree);
 
       const Chunk* ch = meta[j & 3];
-      const int t0 = (j0 + j) * kTile;
-      bool full = t0 >= lo && t0 + kTile <= hi;
+      const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0;
+      int oks = 0;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) full &= ch[c].ok != 0;
-      const bool plain = __all_sync(~0u, full);
+      for (int c = 0; c < kChunks; ++c) oks |= ch[c].ok << c;
+      const bool plain = __all_sync(~0u, lo_r <= 0 && hi_r >= kTile && oks == (1 << kChunks) - 1);
+      if (!plain) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int hi_c = (oks >> c) & 1 ? hi_r : 0;
+#pragma unroll
+          for (int e = 16 * c; e < 16 * c + 16; ++e)
+            if (e >= hi_c || e < lo_r) x[e] = 0xff800000u;
+        }
+      }
       float top = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        float t = -INFINITY;
-        if (plain) {
+        float t = __uint_as_float(x[16 * c]);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) t = fmaxf(t, __uint_as_float(x[16 * c + e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int tok = t0 + 16 * c + e;
-            if (tok < hi && tok >= lo && ch[c].ok) t = fmaxf(t, __uint_as_float(x[16 * c + e]));
-          }
-        }
-        const float f = t * ch[c].kf;
-        if (t > -INFINITY) top = fmaxf(top, f);
+        for (int e = 1; e < 16; ++e) t = fmaxf(t, __uint_as_float(x[16 * c + e]));
+        if (t > -INFINITY) top = fmaxf(top, t * ch[c].kf);
       }
       const bool raise = top > m + kRaise;
       bool waited = false;
@@ -317,21 +333,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       const float mm = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        const float kf = ch[c].kf, sub = ch[c].lv - mm;
-        float sum = 0.0f;
+        // a page that the row does not see keeps its factors (a NaN) to itself
+        const bool sees = plain || (((oks >> c) & 1) && 16 * c < hi_r && 16 * c + 16 > lo_r);
+        const float kf = sees ? ch[c].kf : 1.0f, sub = sees ? ch[c].lv - mm : 0.0f, iv = sees ? ch[c].iv : 0.0f;
+        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          float w0 = exp2_approx(fmaf(__uint_as_float(x[16 * c + e]), kf, sub));
-          float w1 = exp2_approx(fmaf(__uint_as_float(x[16 * c + e + 1]), kf, sub));
-          if (!plain) {
-            const int tok = t0 + 16 * c + e;
-            if (!(tok < hi && tok >= lo && ch[c].ok)) w0 = 0.0f;
-            if (!(tok + 1 < hi && tok + 1 >= lo && ch[c].ok)) w1 = 0.0f;
-          }
-          sum += w0 + w1;
-          x[8 * c + e / 2] = pack_half2(w0, w1);
+          const float2 y = fma2(make_float2(__uint_as_float(x[16 * c + e]), __uint_as_float(x[16 * c + e + 1])), make_float2(kf, kf), make_float2(sub, sub));
+          const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          sum = add2(sum, w);
+          x[8 * c + e / 2] = pack_half2(w.x, w.y);
         }
-        if (plain || sum != 0.0f) l = fmaf(sum, ch[c].iv, l);
+        l = fmaf(sum.x + sum.y, iv, l);
       }
       // P' may be written once the products of the step before have read it
       if (j > 0 && !waited && !warp_wait(&bars.odone[a], (j - 1) & 1, ctl, kErrSoftmax)) break;
@@ -385,85 +398,77 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     const int ct = tid - kSoftmaxWarps * 32, piece = ct % kPieces, row0 = ct / kPieces;
     constexpr int kRowStep = kWidenWarps * 32 / kPieces;
     uint4 k[kPer], v[kPer];
-    float ks = 0.0f, vs = 0.0f;  // of chunk ct (threads 0-7)
-    int okc = 0;
-    auto where = [&](int j, int row, int* id) -> int64_t {
-      const int tok = (j0 + j) * kTile + row;
-      *id = tok < job.t1 ? page_id(p, job.b, tok >> p.page_log2) : -1;
-      return (((static_cast<int64_t>(*id) * p.hkv + head) << p.page_log2) + (tok & (p.page - 1))) * D + piece * 16;
+    static_assert(kRowStep % 16 == 0, "a thread's rows lie at the same place of their 16-token chunks");
+    // Lane c < 8 knows chunk c of the step being loaded: where its first token's codes lie (or -1), its scales.
+    const int64_t row_bytes = (row0 & 15) * D + piece * 16;
+    int64_t chunk_base = -1;
+    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    auto find = [&](int j) {
+      const int tok = (j0 + j) * kTile + 16 * (lane & 7);
+      const int id = lane < kChunks && tok < job.t1 ? page_id(p, job.b, tok >> p.page_log2) : -1;
+      const int64_t block = static_cast<int64_t>(id) * p.hkv + head;
+      chunk_base = id < 0 ? -1 : ((block << p.page_log2) + (tok & (p.page - 1))) * D;
+      ks_next = id < 0 ? 0.0f : p.k_scale[block];
+      vs_next = id < 0 ? 0.0f : p.v_scale[block];
     };
-    auto load_k = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        int id;
-        const int64_t at = where(j, row0 + i * kRowStep, &id);
-        k[i] = id >= 0 ? *reinterpret_cast<const uint4*>(p.k_cache + at) : make_uint4(0, 0, 0, 0);
-      }
-      if (ct < kChunks) {
-        int id;
-        where(j, 16 * ct, &id);
-        okc = id >= 0;
-        ks = okc ? p.k_scale[static_cast<int64_t>(id) * p.hkv + head] : 0.0f;
-        vs = okc ? p.v_scale[static_cast<int64_t>(id) * p.hkv + head] : 0.0f;
-      }
-    };
-    auto load_v = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        int id;
-        const int64_t at = where(j, row0 + i * kRowStep, &id);
-        // values of a zero scale are zero whatever their codes
-        const bool use = id >= 0 && p.v_scale[static_cast<int64_t>(id) * p.hkv + head] != 0.0f;
-        v[i] = use ? *reinterpret_cast<const uint4*>(p.v_cache + at) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    auto store = [&](uint32_t to, const uint4* w) {
+    auto load = [&](const uint8_t* cache, int j, uint4* to) {
+      const int left = job.t1 - (j0 + j) * kTile;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int row = row0 + i * kRowStep;
-        const uint32_t line = to + (piece >> 2) * M::kPanel + row * 128;
-        const uint2 a = widen4<E4M3>(w[i].x);
-        const uint2 b = widen4<E4M3>(w[i].y), c = widen4<E4M3>(w[i].z), d = widen4<E4M3>(w[i].w);
-        // 16-byte chunks 2 (piece % 4) and + 1; the two panels' lanes start with different ones: no bank twice
-        const int c0 = 2 * (piece & 3), odd = (piece >> 2) & 1;
-        const uint32_t at0 = line + ((c0 ^ (row & 7)) << 4), at1 = line + (((c0 + 1) ^ (row & 7)) << 4);
-        if (odd) {
-          sts128(at1, c.x, c.y, d.x, d.y);
-          sts128(at0, a.x, a.y, b.x, b.y);
-        } else {
-          sts128(at0, a.x, a.y, b.x, b.y);
-          sts128(at1, c.x, c.y, d.x, d.y);
-        }
+        const int64_t at = __shfl_sync(~0u, chunk_base, row >> 4);
+        const bool use = at >= 0 && row < left;
+        to[i] = use ? *reinterpret_cast<const uint4*>(cache + at + row_bytes) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto store = [&](uint32_t to, const uint4* w) {
+      // 16-byte chunks 2 (piece % 4) and + 1; the two panels' lanes start with different ones: no bank twice
+      const int c0 = 2 * (piece & 3) + ((piece >> 2) & 1), c1 = c0 ^ 1;
+      const bool odd = (piece >> 2) & 1;
+      const uint32_t line = to + (piece >> 2) * M::kPanel + row0 * 128, at0 = line + ((c0 ^ (row0 & 7)) << 4), at1 = line + ((c1 ^ (row0 & 7)) << 4);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint2 a = widen4<E4M3>(odd ? w[i].z : w[i].x), b = widen4<E4M3>(odd ? w[i].w : w[i].y);
+        const uint2 c = widen4<E4M3>(odd ? w[i].x : w[i].z), d = widen4<E4M3>(odd ? w[i].y : w[i].w);
+        sts128(at0 + i * kRowStep * 128, a.x, a.y, b.x, b.y);
+        sts128(at1 + i * kRowStep * 128, c.x, c.y, d.x, d.y);
       }
     };
     if (n_steps > 0) {
-      load_k(0);
-      load_v(0);
+      find(0);
+      load(p.k_cache, 0, k);
+      load(p.v_cache, 0, v);
     }
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1;
       const uint32_t was = ((j >> 1) & 1) ^ 1;
+      const int here = chunk_base >= 0;
+      ks = ks_next;
+      vs = vs_next;
+      if (j + 1 < n_steps) find(j + 1);
       if (!warp_wait(&bars.kempty[st], was, ctl, kErrWiden)) break;
       store(base + M::kK + st * M::kOperand, k);
       if (ct < kChunks) {
+        // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never
+        // meets a masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
         Chunk c;
-        const float f = vs == 0.0f ? 1.0f : fmaxf(vs * to_unit, 8.6736174e-19f);  // at least 2^-60; keeps a NaN out of fmaxf below
-        c.kf = ks * fabsf(p.scale) * kLog2e;
+        const float kf = ks * fabsf(p.scale) * kLog2e, f = fmaxf(vs * to_unit, 8.6736174e-19f);
+        c.kf = kf != kf ? kf : fmaxf(kf, 1e-30f);
         c.lv = vs != vs ? vs : __log2f(f);
         c.iv = vs != vs ? vs : 1.0f / f;
-        c.ok = okc;
+        c.ok = here;
         meta[j & 3][ct] = c;
       }
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.kfull[st]);
-      if (j + 1 < n_steps) load_k(j + 1);
+      if (j + 1 < n_steps) load(p.k_cache, j + 1, k);
       if (!warp_wait(&bars.vempty[st], was, ctl, kErrWiden)) break;
       store(base + M::kV + st * M::kOperand, v);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.vfull[st]);
-      if (j + 1 < n_steps) load_v(j + 1);
+      if (j + 1 < n_steps) load(p.v_cache, j + 1, v);
     }
   } else {
     regs_dec<kMmaRegs>();
