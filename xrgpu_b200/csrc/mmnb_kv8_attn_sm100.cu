@@ -40,7 +40,7 @@ constexpr int kThreads = (kSoftmaxWarps + kWidenWarps + 4) * 32;  // the MMA war
 constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps;
 constexpr int kChunks = kTile / 16;
 // Registers a thread: launched with kRegs (what 16 warps can have), then moved between the warpgroups.
-constexpr int kRegs = 128, kSoftmaxRegs = 176, kWidenRegs = 112, kMmaRegs = 48;
+constexpr int kRegs = 128, kSoftmaxRegs = 192, kWidenRegs = 80, kMmaRegs = 48;
 static_assert(256 * kSoftmaxRegs + 128 * kWidenRegs + 128 * kMmaRegs <= kThreads * kRegs, "more registers than the block has");
 constexpr float kRaise = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -273,6 +273,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     for (int j = 0; ok && j < n_steps; ++j) {
       if (!warp_wait(&bars.sfull[a], j & 1, ctl, kErrSoftmax)) break;
       tc_fence_after();
+      const Chunk* ch = meta[j & 3];
+      const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0;
+      int oks = 0;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) oks |= ch[c].ok << c;
+      const bool plain = __all_sync(~0u, lo_r <= 0 && hi_r >= kTile && oks == (1 << kChunks) - 1);
+      if (!plain) {  // few steps: masked in tensor memory, so that the code below is one straight run
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          const int hi_c = (oks >> c) & 1 ? hi_r : 0;
+          if (__all_sync(~0u, lo_r <= 16 * c && hi_c >= 16 * c + 16)) continue;
+          uint32_t y[16];
+          tmem_ld16(s_at + 16 * c, y);
+          tmem_wait_ld16(y);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (16 * c + e >= hi_c || 16 * c + e < lo_r) y[e] = 0xff800000u;
+          tmem_st16(s_at + 16 * c, y);
+        }
+        tmem_wait_st();
+      }
       uint32_t x[kTile];
 #pragma unroll
       for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, x + 32 * i);
@@ -283,21 +304,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.sfree);
 
-      const Chunk* ch = meta[j & 3];
-      const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0;
-      int oks = 0;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) oks |= ch[c].ok << c;
-      const bool plain = __all_sync(~0u, lo_r <= 0 && hi_r >= kTile && oks == (1 << kChunks) - 1);
-      if (!plain) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int hi_c = (oks >> c) & 1 ? hi_r : 0;
-#pragma unroll
-          for (int e = 16 * c; e < 16 * c + 16; ++e)
-            if (e >= hi_c || e < lo_r) x[e] = 0xff800000u;
-        }
-      }
       float top = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
@@ -397,19 +403,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     constexpr int kPer = kTile * kPieces / (kWidenWarps * 32);          // pieces a thread, keys and values each
     const int ct = tid - kSoftmaxWarps * 32, piece = ct % kPieces, row0 = ct / kPieces;
     constexpr int kRowStep = kWidenWarps * 32 / kPieces;
-    uint4 k[kPer], v[kPer];
+    uint4 w[kPer];
     static_assert(kRowStep % 16 == 0, "a thread's rows lie at the same place of their 16-token chunks");
     // Lane c < 8 knows chunk c of the step being loaded: where its first token's codes lie (or -1), its scales.
     const int64_t row_bytes = (row0 & 15) * D + piece * 16;
     int64_t chunk_base = -1;
-    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    float ks = 0.0f, vs = 0.0f;
     auto find = [&](int j) {
       const int tok = (j0 + j) * kTile + 16 * (lane & 7);
       const int id = lane < kChunks && tok < job.t1 ? page_id(p, job.b, tok >> p.page_log2) : -1;
       const int64_t block = static_cast<int64_t>(id) * p.hkv + head;
       chunk_base = id < 0 ? -1 : ((block << p.page_log2) + (tok & (p.page - 1))) * D;
-      ks_next = id < 0 ? 0.0f : p.k_scale[block];
-      vs_next = id < 0 ? 0.0f : p.v_scale[block];
+      ks = id < 0 ? 0.0f : p.k_scale[block];
+      vs = id < 0 ? 0.0f : p.v_scale[block];
     };
     auto load = [&](const uint8_t* cache, int j, uint4* to) {
       const int left = job.t1 - (j0 + j) * kTile;
@@ -434,21 +440,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         sts128(at1 + i * kRowStep * 128, c.x, c.y, d.x, d.y);
       }
     };
+    // Operands in the order K(0), V(0), K(1), ...: each is loaded while the one before it waits for its buffer.
     if (n_steps > 0) {
       find(0);
-      load(p.k_cache, 0, k);
-      load(p.v_cache, 0, v);
+      load(p.k_cache, 0, w);
     }
-    for (int j = 0; j < n_steps; ++j) {
-      const int st = j & 1;
-      const uint32_t was = ((j >> 1) & 1) ^ 1;
-      const int here = chunk_base >= 0;
-      ks = ks_next;
-      vs = vs_next;
-      if (j + 1 < n_steps) find(j + 1);
-      if (!warp_wait(&bars.kempty[st], was, ctl, kErrWiden)) break;
-      store(base + M::kK + st * M::kOperand, k);
-      if (ct < kChunks) {
+#pragma unroll 1
+    for (int i = 0; i < 2 * n_steps; ++i) {
+      const int j = i >> 1, is_v = i & 1, st = j & 1;
+      if (!warp_wait(is_v ? &bars.vempty[st] : &bars.kempty[st], ((j >> 1) & 1) ^ 1, ctl, kErrWiden)) break;
+      store(base + (is_v ? M::kV : M::kK) + st * M::kOperand, w);
+      if (!is_v && ct < kChunks) {
         // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never
         // meets a masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
         Chunk c;
@@ -456,19 +458,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         c.kf = kf != kf ? kf : fmaxf(kf, 1e-30f);
         c.lv = vs != vs ? vs : __log2f(f);
         c.iv = vs != vs ? vs : 1.0f / f;
-        c.ok = here;
+        c.ok = chunk_base >= 0;
         meta[j & 3][ct] = c;
       }
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.kfull[st]);
-      if (j + 1 < n_steps) load(p.k_cache, j + 1, k);
-      if (!warp_wait(&bars.vempty[st], was, ctl, kErrWiden)) break;
-      store(base + M::kV + st * M::kOperand, v);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.vfull[st]);
-      if (j + 1 < n_steps) load(p.v_cache, j + 1, v);
+      if (lane == 0) mbar_arrive(is_v ? &bars.vfull[st] : &bars.kfull[st]);
+      if (is_v && j + 1 < n_steps) find(j + 1);
+      if (i + 1 < 2 * n_steps) load(is_v ? p.k_cache : p.v_cache, j + is_v, w);
     }
   } else {
     regs_dec<kMmaRegs>();
@@ -485,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       if (issued > 0 && !thread_wait(&bars.sfree, (issued - 1) & 1, ctl, kErrMma)) return false;
       tc_fence_after();
       ++issued;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < D / 16; ++i) {
         const uint64_t off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
         mma_f16_ss(tmem + kS, qd + a * (M::kOperand >> 4) + off, kd + (j & 1) * (M::kOperand >> 4) + off, qk, i > 0);
@@ -496,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     auto values = [&](int a, int j) {
       if (!thread_wait(&bars.pfull[a], j & 1, ctl, kErrMma)) return false;
       tc_fence_after();
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < kTile / 16; ++i)
         mma_f16_ts(tmem + kO + 128 * a, tmem + kP + 64 * a + 8 * i, vd + (j & 1) * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
       mma_commit(&bars.odone[a]);
