@@ -56,10 +56,11 @@ struct Smem {
   static constexpr int kBytes = kEnd + 1024;
 };
 
-// What the softmax needs of 16 tokens: the factor of their scores, log2 and inverse of the values' factor.
-struct Chunk {
-  float kf, lv, iv;
-  int ok;
+// What the softmax needs of a step's 16-token chunks: the factor of their scores, log2 and inverse of the values'
+// factor, and a bit for each chunk that holds tokens.
+struct Meta {
+  float kf[kChunks], lv[kChunks], iv[kChunks];
+  int oks;
 };
 
 struct Bars {
@@ -84,6 +85,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // Two float32 operations an instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   using M = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
-  __shared__ Chunk meta[4][kChunks];
+  __shared__ __align__(16) Meta meta[4];
   __shared__ uint32_t tmem_slot, vmax_bits;
   __shared__ int abort_flag, found_b, found_tile;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -273,11 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     for (int j = 0; ok && j < n_steps; ++j) {
       if (!warp_wait(&bars.sfull[a], j & 1, ctl, kErrSoftmax)) break;
       tc_fence_after();
-      const Chunk* ch = meta[j & 3];
-      const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0;
-      int oks = 0;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) oks |= ch[c].ok << c;
+      const Meta& mt = meta[j & 3];
+      const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0, oks = mt.oks;
       const bool plain = __all_sync(~0u, lo_r <= 0 && hi_r >= kTile && oks == (1 << kChunks) - 1);
       if (!plain) {  // few steps: masked in tensor memory, so that the code below is one straight run
 #pragma unroll 1
@@ -307,10 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       float top = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        float t = __uint_as_float(x[16 * c]);
-#pragma unroll
-        for (int e = 1; e < 16; ++e) t = fmaxf(t, __uint_as_float(x[16 * c + e]));
-        if (t > -INFINITY) top = fmaxf(top, t * ch[c].kf);
+        const float* v = reinterpret_cast<const float*>(x + 16 * c);
+        const float t = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
+                             max3(max3(v[9], v[10], v[11]), max3(v[12], v[13], v[14]), v[15]), -INFINITY);
+        top = fmaxf(top, t > -INFINITY ? t * mt.kf[c] : -INFINITY);
       }
       const bool raise = top > m + kRaise;
       bool waited = false;
@@ -341,15 +341,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       for (int c = 0; c < kChunks; ++c) {
         // a page that the row does not see keeps its factors (a NaN) to itself
         const bool sees = plain || (((oks >> c) & 1) && 16 * c < hi_r && 16 * c + 16 > lo_r);
-        const float kf = sees ? ch[c].kf : 1.0f, sub = sees ? ch[c].lv - mm : 0.0f, iv = sees ? ch[c].iv : 0.0f;
-        float2 sum = make_float2(0.0f, 0.0f);
+        const float kf = sees ? mt.kf[c] : 1.0f, sub = sees ? mt.lv[c] - mm : 0.0f, iv = sees ? mt.iv[c] : 0.0f;
+        const float2 kf2 = make_float2(kf, kf), sub2 = make_float2(sub, sub);
+        float2 w[8];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float2 y = fma2(make_float2(__uint_as_float(x[16 * c + e]), __uint_as_float(x[16 * c + e + 1])), make_float2(kf, kf), make_float2(sub, sub));
-          const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-          sum = add2(sum, w);
-          x[8 * c + e / 2] = pack_half2(w.x, w.y);
-        }
+        for (int e = 0; e < 8; ++e) w[e] = fma2(make_float2(__uint_as_float(x[16 * c + 2 * e]), __uint_as_float(x[16 * c + 2 * e + 1])), kf2, sub2);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = make_float2(exp2_approx(w[e].x), exp2_approx(w[e].y));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[8 * c + e] = pack_half2(w[e].x, w[e].y);
+        const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
         l = fmaf(sum.x + sum.y, iv, l);
       }
       // P' may be written once the products of the step before have read it
@@ -453,13 +454,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       if (!is_v && ct < kChunks) {
         // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never
         // meets a masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
-        Chunk c;
+        Meta& mt = meta[j & 3];
         const float kf = ks * fabsf(p.scale) * kLog2e, f = fmaxf(vs * to_unit, 8.6736174e-19f);
-        c.kf = kf != kf ? kf : fmaxf(kf, 1e-30f);
-        c.lv = vs != vs ? vs : __log2f(f);
-        c.iv = vs != vs ? vs : 1.0f / f;
-        c.ok = chunk_base >= 0;
-        meta[j & 3][ct] = c;
+        mt.kf[ct] = kf != kf ? kf : fmaxf(kf, 1e-30f);
+        mt.lv[ct] = vs != vs ? vs : __log2f(f);
+        mt.iv[ct] = vs != vs ? vs : 1.0f / f;
+        const int oks = __ballot_sync(0xffu, chunk_base >= 0);
+        if (ct == 0) mt.oks = oks;
       }
       fence_async_shared();
       __syncwarp();
