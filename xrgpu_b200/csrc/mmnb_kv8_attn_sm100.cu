@@ -11,14 +11,17 @@
 // float16 holds 2^25 of range below the largest weight times the largest scale at full precision. The normaliser is the
 // float32 sum of P' divided by the same factor, a page at a time.
 //
-// Roles (16 warps, register counts moved from the widening warps to the softmax warps):
-//   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row. Read S from tensor memory, release it, raise m (and rescale
-//                   O, rare), write P', at the end write the row out.
-//   warps 8-11      widen keys and values: 16-byte loads a tile ahead, float16 to the 128-byte swizzle the tensor
+// Roles (13 warps):
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row. Two passes over S in tensor memory, 64 columns at a time in
+//                   rolled loops (the whole row in registers needs straight-line code that the instruction cache does
+//                   not hold: it cost twice the time): the maximum, then P', written over the columns of S that
+//                   have been read. m is raised (and O rescaled) rarely. At the end the row is written out.
+//   warps 8-11      widen keys and values: 16-byte loads an operand ahead, float16 to the 128-byte swizzle the tensor
 //                   cores read (keys K-major, values MN-major: both as they lie, no transposition).
-//   warp 12         (of 12-15) issues the MMAs (one lane): P0 V, Q0 K, P1 V, Q1 K, so that a tile's softmax runs under the
-//                   other tile's products.
-// Tensor memory: S [0, 128) (one tile's scores at a time), P' of the tiles at 128 and 192, O at 256 and 384.
+//   warp 12         issues the MMAs (one lane), for each tile P V then Q K of the next step, whichever
+//                   tile is ready first, so that a tile's softmax runs under the other tile's products. Q K overwrites
+//                   the columns that P V reads, so it is issued only when P V has completed.
+// Tensor memory: S (and P') of the tiles at 0 and 128, O at 256 and 384.
 // Bounds per 128 tokens and 256 rows at D = 128, in cycles: tensor cores 2048, exponentials (16 a cycle) 2048, shared memory
 // (Q and K read for each S, V for each O, keys and values written: 256 KB) 2048.
 //
@@ -36,15 +39,12 @@ constexpr int kTile = 128;        // rows of a tile, tokens of a step
 constexpr int kRows = 2 * kTile;  // rows of a CTA
 constexpr int kSoftmaxWarps = 8;
 constexpr int kWidenWarps = 4;
-constexpr int kThreads = (kSoftmaxWarps + kWidenWarps + 4) * 32;  // the MMA warp and three that only fill its warpgroup
+constexpr int kThreads = (kSoftmaxWarps + kWidenWarps + 1) * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps;
 constexpr int kChunks = kTile / 16;
-// Registers a thread: launched with kRegs (what 16 warps can have), then moved between the warpgroups.
-constexpr int kRegs = 128, kSoftmaxRegs = 192, kWidenRegs = 80, kMmaRegs = 48;
-static_assert(256 * kSoftmaxRegs + 128 * kWidenRegs + 128 * kMmaRegs <= kThreads * kRegs, "more registers than the block has");
 constexpr float kRaise = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kS = 0, kP = 128, kO = 256;  // tensor memory columns
+constexpr uint32_t kS = 0, kO = 256;  // tensor memory columns (kTile a tile)
 
 constexpr unsigned kErrMma = 0x503, kErrWiden = 0x504, kErrSoftmax = 0x505, kErrDrain = 0x506;
 
@@ -64,7 +64,7 @@ struct Meta {
 };
 
 struct Bars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2], sfree, done;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2], done;
 };
 
 // Values operand: [tokens][64] float16 panels, 64 values of D contiguous (MN-major), 128-byte swizzle: 8-token groups 1024
@@ -128,11 +128,6 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 struct Job {
   int b, tile, head, rows;  // rows: of this CTA (<= 256)
   SeqRows r;
@@ -147,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   __shared__ __align__(16) Meta meta[4];
   __shared__ uint32_t tmem_slot, vmax_bits;
   __shared__ int abort_flag, found_b, found_tile;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const int G = p.hq / p.hkv, head = blockIdx.x % p.hkv, slot = blockIdx.x / p.hkv;
 
   // ---- which rows: slot counts the 256-row tiles of the sequences with more than p.few_rows rows; a sequence's
@@ -201,13 +196,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.kfull[i], kWidenWarps);
       mbar_init(&bars.vfull[i], kWidenWarps);
-      mbar_init(&bars.kempty[i], 1);
-      mbar_init(&bars.vempty[i], 1);
+      mbar_init(&bars.kempty[i], two ? 2 : 1);
+      mbar_init(&bars.vempty[i], two ? 2 : 1);
       mbar_init(&bars.sfull[i], 1);
       mbar_init(&bars.odone[i], 1);
       mbar_init(&bars.pfull[i], 4);
     }
-    mbar_init(&bars.sfree, 4);
     mbar_init(&bars.done, 1);
     abort_flag = 0;
     vmax_bits = 0;
@@ -264,11 +258,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   const float to_unit = __uint_as_float((265u - r_exp) << 23);
 
   if (warp < kSoftmaxWarps) {
-    regs_inc<kSoftmaxRegs>();
     // ---------------------------------------------------------------- softmax
     const int a = warp >> 2, q = warp & 3, row = a * kTile + q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
-    const uint32_t s_at = tmem + lanes + kS, p_at = tmem + lanes + kP + 64 * a, o_at = tmem + lanes + kO + 128 * a;
+    const uint32_t s_at = tmem + lanes + kS + kTile * a, o_at = tmem + lanes + kO + kTile * a;
     const int rr = job.tile * kRows + min(row, job.rows - 1), pos = pos0 + rr / G;
     const int hi = p.causal ? max(0, min(pos + 1, job.r.len)) : job.r.len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
     float m = -INFINITY, l = 0.0f;
@@ -279,10 +272,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       const Meta& mt = meta[j & 3];
       const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0, oks = mt.oks;
       const bool plain = __all_sync(~0u, lo_r <= 0 && hi_r >= kTile && oks == (1 << kChunks) - 1);
-      if (!plain) {  // few steps: masked in tensor memory, so that the code below is one straight run
+      int seen = (1 << kChunks) - 1;
+      if (!plain) {  // few steps: masked in tensor memory, so that the code below has no branches
+        seen = 0;
 #pragma unroll 1
         for (int c = 0; c < kChunks; ++c) {
           const int hi_c = (oks >> c) & 1 ? hi_r : 0;
+          if (16 * c < hi_c && 16 * c + 16 > lo_r) seen |= 1 << c;
           if (__all_sync(~0u, lo_r <= 16 * c && hi_c >= 16 * c + 16)) continue;
           uint32_t y[16];
           tmem_ld16(s_at + 16 * c, y);
@@ -294,35 +290,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         }
         tmem_wait_st();
       }
-      uint32_t x[kTile];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, x + 32 * i);
-      tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_fence_ld(x + 32 * i);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.sfree);
-
+      constexpr int kHalf = kTile / 2;
+      uint32_t x[kHalf];
       float top = -INFINITY;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        tmem_ld32(s_at + kHalf * h, x);
+        tmem_ld32(s_at + kHalf * h + 32, x + 32);
+        tmem_wait_ld();
+        tmem_fence_ld(x);
+        tmem_fence_ld(x + 32);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const float* v = reinterpret_cast<const float*>(x + 16 * c);
-        const float t = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
-                             max3(max3(v[9], v[10], v[11]), max3(v[12], v[13], v[14]), v[15]), -INFINITY);
-        top = fmaxf(top, t > -INFINITY ? t * mt.kf[c] : -INFINITY);
+        for (int c = 0; c < kChunks / 2; ++c) {
+          const float* v = reinterpret_cast<const float*>(x + 16 * c);
+          const float t = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
+                               max3(max3(v[9], v[10], v[11]), max3(v[12], v[13], v[14]), v[15]), -INFINITY);
+          top = fmaxf(top, t > -INFINITY ? t * mt.kf[4 * h + c] : -INFINITY);
+        }
       }
       const bool raise = top > m + kRaise;
-      bool waited = false;
       if (__any_sync(~0u, raise)) {
         const float fresh = raise ? top : m;
         const float f = raise ? (m == -INFINITY ? 0.0f : exp2_approx(m - fresh)) : 1.0f;
         m = fresh;
         l *= f;
-        if (j > 0) {
-          if (!warp_wait(&bars.odone[a], (j - 1) & 1, ctl, kErrSoftmax)) break;
-          waited = true;
-          tc_fence_after();
+        if (j > 0) {  // the products of the step before are complete: this step's scores came after them
 #pragma unroll 1
           for (int i = 0; i < D / 32; ++i) {
             uint32_t o[32];
@@ -337,27 +329,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         }
       }
       const float mm = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        tmem_ld32(s_at + kHalf * h, x);
+        tmem_ld32(s_at + kHalf * h + 32, x + 32);
+        tmem_wait_ld();
+        tmem_fence_ld(x);
+        tmem_fence_ld(x + 32);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        // a page that the row does not see keeps its factors (a NaN) to itself
-        const bool sees = plain || (((oks >> c) & 1) && 16 * c < hi_r && 16 * c + 16 > lo_r);
-        const float kf = sees ? mt.kf[c] : 1.0f, sub = sees ? mt.lv[c] - mm : 0.0f, iv = sees ? mt.iv[c] : 0.0f;
-        const float2 kf2 = make_float2(kf, kf), sub2 = make_float2(sub, sub);
-        float2 w[8];
+        for (int c = 0; c < kChunks / 2; ++c) {
+          // a page that the row does not see keeps its factors (a NaN) to itself
+          const int cc = 4 * h + c;
+          const bool sees = (seen >> cc) & 1;
+          float kf = mt.kf[cc], sub = mt.lv[cc] - mm, iv = mt.iv[cc];
+          kf = sees ? kf : 1.0f;
+          sub = sees ? sub : 0.0f;
+          iv = sees ? iv : 0.0f;
+          const float2 kf2 = make_float2(kf, kf), sub2 = make_float2(sub, sub);
+          float2 w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = fma2(make_float2(__uint_as_float(x[16 * c + 2 * e]), __uint_as_float(x[16 * c + 2 * e + 1])), kf2, sub2);
+          for (int e = 0; e < 8; ++e) w[e] = fma2(make_float2(__uint_as_float(x[16 * c + 2 * e]), __uint_as_float(x[16 * c + 2 * e + 1])), kf2, sub2);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = make_float2(exp2_approx(w[e].x), exp2_approx(w[e].y));
+          for (int e = 0; e < 8; ++e) w[e] = make_float2(exp2_approx(w[e].x), exp2_approx(w[e].y));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[8 * c + e] = pack_half2(w[e].x, w[e].y);
-        const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
-        l = fmaf(sum.x + sum.y, iv, l);
+          for (int e = 0; e < 8; ++e) x[8 * c + e] = pack_half2(w[e].x, w[e].y);
+          const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
+          l = fmaf(sum.x + sum.y, iv, l);
+        }
+        tmem_st32(s_at + 32 * h, *reinterpret_cast<const uint32_t(*)[32]>(x));
       }
-      // P' may be written once the products of the step before have read it
-      if (j > 0 && !waited && !warp_wait(&bars.odone[a], (j - 1) & 1, ctl, kErrSoftmax)) break;
-      tc_fence_after();
-      tmem_st32(p_at, *reinterpret_cast<const uint32_t(*)[32]>(x));
-      tmem_st32(p_at + 32, *reinterpret_cast<const uint32_t(*)[32]>(x + 32));
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -398,13 +398,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       }
     }
   } else if (warp < kMmaWarp) {
-    regs_dec<kWidenRegs>();
     // ---------------------------------------------------------------- widen keys and values
     constexpr int kPieces = D / 16;                                     // 16-byte pieces a row
     constexpr int kPer = kTile * kPieces / (kWidenWarps * 32);          // pieces a thread, keys and values each
     const int ct = tid - kSoftmaxWarps * 32, piece = ct % kPieces, row0 = ct / kPieces;
     constexpr int kRowStep = kWidenWarps * 32 / kPieces;
-    uint4 w[kPer];
     static_assert(kRowStep % 16 == 0, "a thread's rows lie at the same place of their 16-token chunks");
     // Lane c < 8 knows chunk c of the step being loaded: where its first token's codes lie (or -1), its scales.
     const int64_t row_bytes = (row0 & 15) * D + piece * 16;
@@ -441,17 +439,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         sts128(at1 + i * kRowStep * 128, c.x, c.y, d.x, d.y);
       }
     };
-    // Operands in the order K(0), V(0), K(1), ...: each is loaded while the one before it waits for its buffer.
+    // A step's keys and values are loaded a step ahead.
+    uint4 k[kPer], v[kPer];
     if (n_steps > 0) {
       find(0);
-      load(p.k_cache, 0, w);
+      load(p.k_cache, 0, k);
+      load(p.v_cache, 0, v);
     }
 #pragma unroll 1
-    for (int i = 0; i < 2 * n_steps; ++i) {
-      const int j = i >> 1, is_v = i & 1, st = j & 1;
-      if (!warp_wait(is_v ? &bars.vempty[st] : &bars.kempty[st], ((j >> 1) & 1) ^ 1, ctl, kErrWiden)) break;
-      store(base + (is_v ? M::kV : M::kK) + st * M::kOperand, w);
-      if (!is_v && ct < kChunks) {
+    for (int j = 0; j < n_steps; ++j) {
+      const int st = j & 1;
+      const uint32_t was = ((j >> 1) & 1) ^ 1;
+      if (!warp_wait(&bars.kempty[st], was, ctl, kErrWiden)) break;
+      store(base + M::kK + st * M::kOperand, k);
+      if (ct < kChunks) {
         // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never
         // meets a masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
         Meta& mt = meta[j & 3];
@@ -464,64 +465,91 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       }
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(is_v ? &bars.vfull[st] : &bars.kfull[st]);
-      if (is_v && j + 1 < n_steps) find(j + 1);
-      if (i + 1 < 2 * n_steps) load(is_v ? p.k_cache : p.v_cache, j + is_v, w);
+      if (lane == 0) mbar_arrive(&bars.kfull[st]);
+      if (j + 1 < n_steps) {
+        find(j + 1);
+        load(p.k_cache, j + 1, k);
+      }
+      if (!warp_wait(&bars.vempty[st], was, ctl, kErrWiden)) break;
+      store(base + M::kV + st * M::kOperand, v);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.vfull[st]);
+      if (j + 1 < n_steps) load(p.v_cache, j + 1, v);
     }
   } else {
-    regs_dec<kMmaRegs>();
-  }
-  if (warp == kMmaWarp && lane == 0) {
-    // ---------------------------------------------------------------- MMAs
+    // ---------------------------------------------------------------- MMAs (the warp stays converged, so that their operands stay in uniform registers; one lane issues)
     constexpr uint32_t kF32Out = 1u << 4;
     const uint32_t qk = kF32Out | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
     const uint32_t pv = kF32Out | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
     const uint64_t qd = umma_desc_sw128(base + M::kQ), kd = umma_desc_sw128(base + M::kK), vd = desc_mn<D>(base + M::kV);
-    int issued = 0;  // S products so far
+    // Per tile: scores issued, values issued. The next values wait for their P' and V, the next scores for K and for
+    // the completion of the values before them (they overwrite the P' those read).
+    int scores0 = 0, values0 = 0, scores1 = two ? 0 : n_steps, values1 = two ? 0 : n_steps;
+    uint64_t since = 0;
+    int idle = 0;
     bool ok = true;
-    auto scores = [&](int a, int j) {
-      if (issued > 0 && !thread_wait(&bars.sfree, (issued - 1) & 1, ctl, kErrMma)) return false;
-      tc_fence_after();
-      ++issued;
+    while (ok && (values0 < n_steps || values1 < n_steps)) {
+      bool any = false;
 #pragma unroll 1
-      for (int i = 0; i < D / 16; ++i) {
-        const uint64_t off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
-        mma_f16_ss(tmem + kS, qd + a * (M::kOperand >> 4) + off, kd + (j & 1) * (M::kOperand >> 4) + off, qk, i > 0);
-      }
-      mma_commit(&bars.sfull[a]);
-      return true;
-    };
-    auto values = [&](int a, int j) {
-      if (!thread_wait(&bars.pfull[a], j & 1, ctl, kErrMma)) return false;
-      tc_fence_after();
-#pragma unroll 1
-      for (int i = 0; i < kTile / 16; ++i)
-        mma_f16_ts(tmem + kO + 128 * a, tmem + kP + 64 * a + 8 * i, vd + (j & 1) * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
-      mma_commit(&bars.odone[a]);
-      return true;
-    };
-    for (int j = -1; ok && j < n_steps; ++j) {
-      const bool more = j + 1 < n_steps;
-      if (j >= 0) {
-        ok = thread_wait(&bars.vfull[j & 1], (j >> 1) & 1, ctl, kErrMma) && values(0, j);
-        if (ok && !two) mma_commit(&bars.vempty[j & 1]);
-      }
-      if (ok && more) {
-        ok = thread_wait(&bars.kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, ctl, kErrMma) && scores(0, j + 1);
-        if (ok && !two) mma_commit(&bars.kempty[(j + 1) & 1]);
-      }
-      if (two) {
-        if (ok && j >= 0) {
-          ok = values(1, j);
-          if (ok) mma_commit(&bars.vempty[j & 1]);
+      for (int a = 0; a < 2; ++a) {
+        const int scores = a ? scores1 : scores0, values = a ? values1 : values0;
+        if (values < scores) {
+          const int j = values, st = j & 1;
+          if (__all_sync(~0u, mbar_test_wait(&bars.pfull[a], j & 1) && mbar_test_wait(&bars.vfull[st], (j >> 1) & 1))) {
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < kTile / 16; ++i)
+              mma_f16_ts(tmem + kO + kTile * a, tmem + kS + kTile * a + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
+            mma_commit(&bars.odone[a]);
+            mma_commit(&bars.vempty[st]);
+            }
+            __syncwarp();
+            if (a) ++values1;
+            else ++values0;
+            any = true;
+          }
+        } else if (scores < n_steps) {
+          const int j = scores, st = j & 1;
+          if (__all_sync(~0u, mbar_test_wait(&bars.kfull[st], (j >> 1) & 1) && (j == 0 || mbar_test_wait(&bars.odone[a], (j - 1) & 1)))) {
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const uint64_t off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
+              mma_f16_ss(tmem + kS + kTile * a, qd + a * (M::kOperand >> 4) + off, kd + st * (M::kOperand >> 4) + off, qk, i > 0);
+            }
+            mma_commit(&bars.sfull[a]);
+            mma_commit(&bars.kempty[st]);
+            }
+            __syncwarp();
+            if (a) ++scores1;
+            else ++scores0;
+            any = true;
+          }
         }
-        if (ok && more) {
-          ok = scores(1, j + 1);
-          if (ok) mma_commit(&bars.kempty[(j + 1) & 1]);
+      }
+      idle = any ? 0 : idle + 1;
+      if (any) since = 0;
+      if (idle >= kSpins) {
+        idle = 0;
+        const uint64_t now = global_timer_ns();
+        if (since == 0) since = now;
+        const bool expired = __any_sync(~0u, now - since > kWaitLimitNs);
+        if (__any_sync(~0u, *ctl.abort != 0)) {
+          ok = false;
+        } else if (expired) {
+          if (lane == 0) {
+            record_device_error(ctl.err, kErrMma);
+            *ctl.abort = 1;
+          }
+          ok = false;
         }
       }
     }
-    mma_commit(&bars.done);  // every MMA issued has completed once it flips
+    if (elect_one()) mma_commit(&bars.done);  // every MMA issued has completed once it flips
+    __syncwarp();
     drain_wait(&bars.done, 0, p.err, kErrDrain);
   }
 

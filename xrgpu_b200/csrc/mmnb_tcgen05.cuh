@@ -100,19 +100,32 @@ __device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t pa
 }
 
 // Single-lane bounded spin for the latency-critical roles (TMA producer, MMA issuer).
-// Gives up on the abort flag or after the wait limit (raising it).
+// Gives up on the abort flag or after the wait limit (raising it); both are looked at once in
+// kSpins probes, since reading the timer takes longer than many of them.
+constexpr int kSpins = 128;
 __device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, const Ctl& c, unsigned code) {
   if (mbar_test_wait(bar, parity)) return true;
-  const uint64_t start = global_timer_ns();
+  uint64_t start = 0;
   for (;;) {
-    if (mbar_test_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < kSpins; ++i)
+      if (mbar_test_wait(bar, parity)) return true;
     if (*c.abort) return false;
-    if (global_timer_ns() - start > kWaitLimitNs) {
+    const uint64_t now = global_timer_ns();
+    if (start == 0) start = now;
+    if (now - start > kWaitLimitNs) {
       record_device_error(c.err, code);
       *c.abort = 1;
       return false;
     }
   }
+}
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r)::"memory");
+  return r != 0;
 }
 
 // Whole-warp bounded wait (dequant and epilogue warps): every lane observes the phase and the
