@@ -4,26 +4,25 @@
 //
 // A CTA takes 256 rows of one sequence and key/value head (row r is query token r / G and head r % G of its group of
 // G, so the group shares every key and value) as two tiles of 128, and passes once over the tokens they see,
-// 128 at a time. Codes are exact float16 numbers: they are widened once a CTA, in registers, on their way
+// 64 at a time. Codes are exact float16 numbers: they are widened once a CTA, in registers, on their way
 // to shared memory, and the scales stay out of them: k_scale multiplies the scores a page at a time, and
 // v_scale joins the exponent of the weights: P' = exp2(x - m + log2(v_scale 2^11 / R)), R the power of two above the
 // largest v_scale of the tokens. With m raised only when a score exceeds it by 4, P' stays below 2^15, so
 // float16 holds 2^25 of range below the largest weight times the largest scale at full precision. The normaliser is the
 // float32 sum of P' divided by the same factor, a page at a time.
 //
-// Roles (13 warps):
-//   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row. Two passes over S in tensor memory, 64 columns at a time in
-//                   rolled loops (the whole row in registers needs straight-line code that the instruction cache does
-//                   not hold: it cost twice the time): the maximum, then P', written over the columns of S that
-//                   have been read. m is raised (and O rescaled) rarely. At the end the row is written out.
-//   warps 8-11      widen keys and values: 16-byte loads an operand ahead, float16 to the 128-byte swizzle the tensor
-//                   cores read (keys K-major, values MN-major: both as they lie, no transposition).
-//   warp 12         issues the MMAs (one lane), for each tile P V then Q K of the next step, whichever
-//                   tile is ready first, so that a tile's softmax runs under the other tile's products. Q K overwrites
-//                   the columns that P V reads, so it is issued only when P V has completed.
-// Tensor memory: S (and P') of the tiles at 0 and 128, O at 256 and 384.
+// Roles (17 warps):
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row: read S, raise m (and rescale O, rare), write P' over S, at
+//                   the end write the row out.
+//   warps 8-11, 12-15  widen keys, values: 16-byte loads two steps ahead (page ids three), float16 to the 128-byte swizzle
+//                   the tensor cores read (keys K-major, values MN-major: both as they lie, no transposition).
+//   warp 16         issues the MMAs (converged, one lane elected, so that descriptors stay in uniform registers):
+//                   for each tile whichever of Q K of the next step and P V of this one is ready first.
+// Tensor memory: two S (and P') buffers of 64 columns for each tile at 0 and 128, O at 256 and 384. With two buffers the
+// scores of the next step are there when the softmax of this one ends; with one of 128 columns the softmax waited
+// for P V, Q K and both signals each step (twice the time).
 // Bounds per 128 tokens and 256 rows at D = 128, in cycles: tensor cores 2048, exponentials (16 a cycle) 2048, shared memory
-// (Q and K read for each S, V for each O, keys and values written: 256 KB) 2048.
+// (Q and K read for each S, V for each O, keys and values written: 320 KB) 2560.
 //
 // Every wait is bounded as in mmnb_gemm_sm100.cu.
 #include <cuda_runtime.h>
@@ -35,24 +34,26 @@
 namespace xrgpu {
 namespace {
 
-constexpr int kTile = 128;        // rows of a tile, tokens of a step
+constexpr int kTile = 128;        // rows of a tile
+constexpr int kStep = 64;         // tokens of a step
+constexpr int kRing = 4;          // steps of keys and of values in shared memory
 constexpr int kRows = 2 * kTile;  // rows of a CTA
 constexpr int kSoftmaxWarps = 8;
-constexpr int kWidenWarps = 4;
-constexpr int kThreads = (kSoftmaxWarps + kWidenWarps + 1) * 32;
-constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps;
-constexpr int kChunks = kTile / 16;
+constexpr int kWidenWarps = 4;    // for keys, and as many for values
+constexpr int kThreads = (kSoftmaxWarps + 2 * kWidenWarps + 1) * 32;
+constexpr int kMmaWarp = kSoftmaxWarps + 2 * kWidenWarps;
+constexpr int kChunks = kStep / 16;
 constexpr float kRaise = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kS = 0, kO = 256;  // tensor memory columns (kTile a tile)
+constexpr uint32_t kS = 0, kO = 256;  // tensor memory columns (128 a tile)
 
 constexpr unsigned kErrMma = 0x503, kErrWiden = 0x504, kErrSoftmax = 0x505, kErrDrain = 0x506;
 
 template <int D>
 struct Smem {
-  static constexpr int kPanel = kTile * 128;                 // 128 rows of 64 float16
-  static constexpr int kOperand = kPanel * (D / 64);         // a tile of Q, K or V
-  static constexpr int kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kEnd = kV + 2 * kOperand;
+  static constexpr int kQPanel = kTile * 128, kPanel = kStep * 128;  // 64 float16 of each row
+  static constexpr int kQTile = kQPanel * (D / 64), kOperand = kPanel * (D / 64);
+  static constexpr int kQ = 0, kK = 2 * kQTile, kV = kK + kRing * kOperand, kEnd = kV + kRing * kOperand;
   static constexpr int kBytes = kEnd + 1024;
 };
 
@@ -64,7 +65,8 @@ struct Meta {
 };
 
 struct Bars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2], done;
+  uint64_t kfull[kRing], kempty[kRing], vfull[kRing], vempty[kRing];
+  uint64_t sfull[2][2], pfull[2][2], odone[2][2], done;  // [tile][step % 2]
 };
 
 // Values operand: [tokens][64] float16 panels, 64 values of D contiguous (MN-major), 128-byte swizzle: 8-token groups 1024
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   using M = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
-  __shared__ __align__(16) Meta meta[4];
+  __shared__ __align__(16) Meta meta[2 * kRing];
   __shared__ uint32_t tmem_slot, vmax_bits;
   __shared__ int abort_flag, found_b, found_tile;
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
@@ -188,19 +190,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     job.t0 = p.window > 0 ? max(0, first - p.window + 1) : 0;
     if (job.t1 < job.t0) job.t1 = job.t0;
   }
-  const int j0 = job.t0 / kTile, n_steps = job.t1 > job.t0 ? (job.t1 + kTile - 1) / kTile - j0 : 0;
+  const int j0 = job.t0 / kStep, n_steps = job.t1 > job.t0 ? (job.t1 + kStep - 1) / kStep - j0 : 0;
   const bool two = job.rows > kTile;
 
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kRing; ++i) {
       mbar_init(&bars.kfull[i], kWidenWarps);
       mbar_init(&bars.vfull[i], kWidenWarps);
       mbar_init(&bars.kempty[i], two ? 2 : 1);
       mbar_init(&bars.vempty[i], two ? 2 : 1);
-      mbar_init(&bars.sfull[i], 1);
-      mbar_init(&bars.odone[i], 1);
-      mbar_init(&bars.pfull[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bars.sfull[i >> 1][i & 1], 1);
+      mbar_init(&bars.odone[i >> 1][i & 1], 1);
+      mbar_init(&bars.pfull[i >> 1][i & 1], 4);
     }
     mbar_init(&bars.done, 1);
     abort_flag = 0;
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         }
       }
       const int row = r & (kTile - 1);
-      const uint32_t at = base + M::kQ + (r / kTile) * M::kOperand + (ch >> 3) * M::kPanel + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+      const uint32_t at = base + M::kQ + (r / kTile) * M::kQTile + (ch >> 3) * M::kQPanel + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
       sts128(at, v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip);
     }
     uint32_t vm = 0;
@@ -261,52 +265,43 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     // ---------------------------------------------------------------- softmax
     const int a = warp >> 2, q = warp & 3, row = a * kTile + q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
-    const uint32_t s_at = tmem + lanes + kS + kTile * a, o_at = tmem + lanes + kO + kTile * a;
+    const uint32_t s_base = tmem + lanes + kS + 128 * a, o_at = tmem + lanes + kO + 128 * a;
     const int rr = job.tile * kRows + min(row, job.rows - 1), pos = pos0 + rr / G;
     const int hi = p.causal ? max(0, min(pos + 1, job.r.len)) : job.r.len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
     float m = -INFINITY, l = 0.0f;
     bool ok = a == 0 || two;
     for (int j = 0; ok && j < n_steps; ++j) {
-      if (!warp_wait(&bars.sfull[a], j & 1, ctl, kErrSoftmax)) break;
+      const int st = j & 1;
+      const uint32_t ph = (j >> 1) & 1, s_at = s_base + kStep * st;
+      if (!warp_wait(&bars.sfull[a][st], ph, ctl, kErrSoftmax)) break;
       tc_fence_after();
-      const Meta& mt = meta[j & 3];
-      const int t0 = (j0 + j) * kTile, lo_r = lo - t0, hi_r = hi - t0, oks = mt.oks;
-      const bool plain = __all_sync(~0u, lo_r <= 0 && hi_r >= kTile && oks == (1 << kChunks) - 1);
-      int seen = (1 << kChunks) - 1;
-      if (!plain) {  // few steps: masked in tensor memory, so that the code below has no branches
+      const Meta& mt = meta[j & (2 * kRing - 1)];
+      const int t0 = (j0 + j) * kStep, lo_r = lo - t0, hi_r = hi - t0, oks = mt.oks;
+      uint32_t x[kStep];
+      tmem_ld32(s_at, x);
+      tmem_ld32(s_at + 32, x + 32);
+      tmem_wait_ld();
+      tmem_fence_ld(x);
+      tmem_fence_ld(x + 32);
+      int seen = (1 << kChunks) - 1;  // chunks of which the row sees a token
+      if (!__all_sync(~0u, lo_r <= 0 && hi_r >= kStep && oks == (1 << kChunks) - 1)) {
         seen = 0;
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           const int hi_c = (oks >> c) & 1 ? hi_r : 0;
           if (16 * c < hi_c && 16 * c + 16 > lo_r) seen |= 1 << c;
-          if (__all_sync(~0u, lo_r <= 16 * c && hi_c >= 16 * c + 16)) continue;
-          uint32_t y[16];
-          tmem_ld16(s_at + 16 * c, y);
-          tmem_wait_ld16(y);
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (16 * c + e >= hi_c || 16 * c + e < lo_r) y[e] = 0xff800000u;
-          tmem_st16(s_at + 16 * c, y);
+          for (int e = 16 * c; e < 16 * c + 16; ++e)
+            if (e >= hi_c || e < lo_r) x[e] = 0xff800000u;
         }
-        tmem_wait_st();
       }
-      constexpr int kHalf = kTile / 2;
-      uint32_t x[kHalf];
       float top = -INFINITY;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        tmem_ld32(s_at + kHalf * h, x);
-        tmem_ld32(s_at + kHalf * h + 32, x + 32);
-        tmem_wait_ld();
-        tmem_fence_ld(x);
-        tmem_fence_ld(x + 32);
 #pragma unroll
-        for (int c = 0; c < kChunks / 2; ++c) {
-          const float* v = reinterpret_cast<const float*>(x + 16 * c);
-          const float t = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
-                               max3(max3(v[9], v[10], v[11]), max3(v[12], v[13], v[14]), v[15]), -INFINITY);
-          top = fmaxf(top, t > -INFINITY ? t * mt.kf[4 * h + c] : -INFINITY);
-        }
+      for (int c = 0; c < kChunks; ++c) {
+        const float* v = reinterpret_cast<const float*>(x + 16 * c);
+        const float t = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
+                             max3(max3(v[9], v[10], v[11]), max3(v[12], v[13], v[14]), v[15]), -INFINITY);
+        top = fmaxf(top, t > -INFINITY ? t * mt.kf[c] : -INFINITY);
       }
       const bool raise = top > m + kRaise;
       if (__any_sync(~0u, raise)) {
@@ -314,56 +309,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         const float f = raise ? (m == -INFINITY ? 0.0f : exp2_approx(m - fresh)) : 1.0f;
         m = fresh;
         l *= f;
-        if (j > 0) {  // the products of the step before are complete: this step's scores came after them
+        if (j > 0) {  // O may change once the products of the step before are complete
+          if (!warp_wait(&bars.odone[a][st ^ 1], ((j - 1) >> 1) & 1, ctl, kErrSoftmax)) break;
+          tc_fence_after();
 #pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld32(o_at + 32 * i, o);
-            tmem_wait_ld();
-            tmem_fence_ld(o);
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t o[16];
+            tmem_ld16(o_at + 16 * i, o);
+            tmem_wait_ld16(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(o_at + 32 * i, *reinterpret_cast<const uint32_t(*)[32]>(o));
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(o_at + 16 * i, o);
           }
           tmem_wait_st();
         }
       }
       const float mm = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        tmem_ld32(s_at + kHalf * h, x);
-        tmem_ld32(s_at + kHalf * h + 32, x + 32);
-        tmem_wait_ld();
-        tmem_fence_ld(x);
-        tmem_fence_ld(x + 32);
 #pragma unroll
-        for (int c = 0; c < kChunks / 2; ++c) {
-          // a page that the row does not see keeps its factors (a NaN) to itself
-          const int cc = 4 * h + c;
-          const bool sees = (seen >> cc) & 1;
-          float kf = mt.kf[cc], sub = mt.lv[cc] - mm, iv = mt.iv[cc];
-          kf = sees ? kf : 1.0f;
-          sub = sees ? sub : 0.0f;
-          iv = sees ? iv : 0.0f;
-          const float2 kf2 = make_float2(kf, kf), sub2 = make_float2(sub, sub);
-          float2 w[8];
+      for (int c = 0; c < kChunks; ++c) {
+        // a page that the row does not see keeps its factors (a NaN) to itself
+        const bool sees = (seen >> c) & 1;
+        float kf = mt.kf[c], sub = mt.lv[c] - mm, iv = mt.iv[c];
+        kf = sees ? kf : 1.0f;
+        sub = sees ? sub : 0.0f;
+        iv = sees ? iv : 0.0f;
+        const float2 kf2 = make_float2(kf, kf), sub2 = make_float2(sub, sub);
+        float2 w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = fma2(make_float2(__uint_as_float(x[16 * c + 2 * e]), __uint_as_float(x[16 * c + 2 * e + 1])), kf2, sub2);
+        for (int e = 0; e < 8; ++e) w[e] = fma2(make_float2(__uint_as_float(x[16 * c + 2 * e]), __uint_as_float(x[16 * c + 2 * e + 1])), kf2, sub2);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = make_float2(exp2_approx(w[e].x), exp2_approx(w[e].y));
+        for (int e = 0; e < 8; ++e) w[e] = make_float2(exp2_approx(w[e].x), exp2_approx(w[e].y));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[8 * c + e] = pack_half2(w[e].x, w[e].y);
-          const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
-          l = fmaf(sum.x + sum.y, iv, l);
-        }
-        tmem_st32(s_at + 32 * h, *reinterpret_cast<const uint32_t(*)[32]>(x));
+        for (int e = 0; e < 8; ++e) x[8 * c + e] = pack_half2(w[e].x, w[e].y);
+        const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
+        l = fmaf(sum.x + sum.y, iv, l);
       }
+      tmem_st32(s_at, *reinterpret_cast<const uint32_t(*)[32]>(x));
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.pfull[a]);
+      if (lane == 0) mbar_arrive(&bars.pfull[a][st]);
     }
-    if (ok && n_steps > 0) ok = warp_wait(&bars.odone[a], (n_steps - 1) & 1, ctl, kErrSoftmax);
+    if (ok && n_steps > 0) ok = warp_wait(&bars.odone[a][(n_steps - 1) & 1], ((n_steps - 1) >> 1) & 1, ctl, kErrSoftmax);
     tc_fence_after();
     if (ok) {
       const float inv = l == 0.0f ? 0.0f : value_unit / l;
@@ -398,93 +385,122 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       }
     }
   } else if (warp < kMmaWarp) {
-    // ---------------------------------------------------------------- widen keys and values
-    constexpr int kPieces = D / 16;                                     // 16-byte pieces a row
-    constexpr int kPer = kTile * kPieces / (kWidenWarps * 32);          // pieces a thread, keys and values each
-    const int ct = tid - kSoftmaxWarps * 32, piece = ct % kPieces, row0 = ct / kPieces;
+    // ---------------------------------------------------------------- widen keys or values
+    constexpr int kPieces = D / 16;                             // 16-byte pieces a row
+    constexpr int kPer = kStep * kPieces / (kWidenWarps * 32);  // pieces a thread
     constexpr int kRowStep = kWidenWarps * 32 / kPieces;
     static_assert(kRowStep % 16 == 0, "a thread's rows lie at the same place of their 16-token chunks");
-    // Lane c < 8 knows chunk c of the step being loaded: where its first token's codes lie (or -1), its scales.
-    const int64_t row_bytes = (row0 & 15) * D + piece * 16;
+    const bool keys = warp < kSoftmaxWarps + kWidenWarps;
+    const int ct = tid - (keys ? kSoftmaxWarps : kSoftmaxWarps + kWidenWarps) * 32, piece = ct % kPieces, row0 = ct / kPieces;
+    const uint8_t* cache = (keys ? p.k_cache : p.v_cache) + (row0 & 15) * D + piece * 16;
+    uint64_t* full = keys ? bars.kfull : bars.vfull;
+    uint64_t* empty = keys ? bars.kempty : bars.vempty;
+    // 16-byte chunks 2 (piece % 4) and + 1 of a row's float16 numbers; the two panels' lanes start with different ones: no bank twice
+    const bool odd = (piece >> 2) & 1;
+    const int c0 = 2 * (piece & 3) + odd, c1 = c0 ^ 1;
+    const uint32_t line = base + (keys ? M::kK : M::kV) + (piece >> 2) * M::kPanel + row0 * 128;
+    const uint32_t at0 = line + ((c0 ^ (row0 & 7)) << 4), at1 = line + ((c1 ^ (row0 & 7)) << 4);
+    // Lane c < kChunks knows chunk c of a step: its page id three steps ahead, two steps ahead where its first token's
+    // codes lie (-1: nowhere). The first thread of the keys' warps for each chunk also makes the step's factors: scales two
+    // steps ahead, factors one.
+    const bool factors = keys && ct < kChunks;
+    int id_next = -1, ok_raw = 0, ok_now = 0;
     int64_t chunk_base = -1;
-    float ks = 0.0f, vs = 0.0f;
-    auto find = [&](int j) {
-      const int tok = (j0 + j) * kTile + 16 * (lane & 7);
-      const int id = lane < kChunks && tok < job.t1 ? page_id(p, job.b, tok >> p.page_log2) : -1;
-      const int64_t block = static_cast<int64_t>(id) * p.hkv + head;
-      chunk_base = id < 0 ? -1 : ((block << p.page_log2) + (tok & (p.page - 1))) * D;
-      ks = id < 0 ? 0.0f : p.k_scale[block];
-      vs = id < 0 ? 0.0f : p.v_scale[block];
+    float ks = 0.0f, vs = 0.0f, kf = 0.0f, lv = 0.0f, iv = 0.0f;
+    auto find_page = [&](int j) {
+      const int tok = (j0 + j) * kStep + 16 * lane;
+      id_next = -1;
+      if (j < n_steps && lane < kChunks && tok < job.t1) id_next = p.page_table[static_cast<int64_t>(job.b) * p.max_pages + (tok >> p.page_log2)];
     };
-    auto load = [&](const uint8_t* cache, int j, uint4* to) {
-      const int left = job.t1 - (j0 + j) * kTile;
+    auto find = [&](int j) {
+      const int tok = (j0 + j) * kStep + 16 * lane;
+      const bool wanted = j < n_steps && lane < kChunks && tok < job.t1, use = wanted && id_next >= 0 && id_next < p.pages;
+      if (wanted && !use) record_device_error(p.err, kErrKv8Page);
+      const int64_t block = static_cast<int64_t>(id_next) * p.hkv + head;
+      chunk_base = use ? ((block << p.page_log2) + (tok & (p.page - 1))) * D : -1;
+      if (factors) {
+        ok_raw = use;
+        ks = vs = 0.0f;
+        if (use) {
+          ks = p.k_scale[block];
+          vs = p.v_scale[block];
+        }
+      }
+    };
+    // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never meets a
+    // masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
+    auto make_factors = [&] {
+      const float f = fmaxf(vs * to_unit, 8.6736174e-19f);
+      kf = ks * fabsf(p.scale) * kLog2e;
+      if (kf == kf) kf = fmaxf(kf, 1e-30f);
+      lv = vs != vs ? vs : __log2f(f);
+      iv = vs != vs ? vs : __frcp_rn(f);
+      ok_now = ok_raw;
+    };
+    auto load = [&](int j, uint4 (&to)[kPer]) {
+      const int left = job.t1 - (j0 + j) * kStep;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int row = row0 + i * kRowStep;
         const int64_t at = __shfl_sync(~0u, chunk_base, row >> 4);
-        const bool use = at >= 0 && row < left;
-        to[i] = use ? *reinterpret_cast<const uint4*>(cache + at + row_bytes) : make_uint4(0, 0, 0, 0);
+        to[i] = make_uint4(0, 0, 0, 0);
+        if (at >= 0 && row < left) to[i] = *reinterpret_cast<const uint4*>(cache + at);
       }
     };
-    auto store = [&](uint32_t to, const uint4* w) {
-      // 16-byte chunks 2 (piece % 4) and + 1; the two panels' lanes start with different ones: no bank twice
-      const int c0 = 2 * (piece & 3) + ((piece >> 2) & 1), c1 = c0 ^ 1;
-      const bool odd = (piece >> 2) & 1;
-      const uint32_t line = to + (piece >> 2) * M::kPanel + row0 * 128, at0 = line + ((c0 ^ (row0 & 7)) << 4), at1 = line + ((c1 ^ (row0 & 7)) << 4);
+    auto put = [&](int j, const uint4 (&w)[kPer]) {
+      const int st = j & (kRing - 1);
+      if (!warp_wait(&empty[st], ((j / kRing) & 1) ^ 1, ctl, kErrWiden)) return false;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const uint2 a = widen4<E4M3>(odd ? w[i].z : w[i].x), b = widen4<E4M3>(odd ? w[i].w : w[i].y);
         const uint2 c = widen4<E4M3>(odd ? w[i].x : w[i].z), d = widen4<E4M3>(odd ? w[i].y : w[i].w);
-        sts128(at0 + i * kRowStep * 128, a.x, a.y, b.x, b.y);
-        sts128(at1 + i * kRowStep * 128, c.x, c.y, d.x, d.y);
+        sts128(at0 + st * M::kOperand + i * kRowStep * 128, a.x, a.y, b.x, b.y);
+        sts128(at1 + st * M::kOperand + i * kRowStep * 128, c.x, c.y, d.x, d.y);
       }
-    };
-    // A step's keys and values are loaded a step ahead.
-    uint4 k[kPer], v[kPer];
-    if (n_steps > 0) {
-      find(0);
-      load(p.k_cache, 0, k);
-      load(p.v_cache, 0, v);
-    }
-#pragma unroll 1
-    for (int j = 0; j < n_steps; ++j) {
-      const int st = j & 1;
-      const uint32_t was = ((j >> 1) & 1) ^ 1;
-      if (!warp_wait(&bars.kempty[st], was, ctl, kErrWiden)) break;
-      store(base + M::kK + st * M::kOperand, k);
-      if (ct < kChunks) {
-        // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never
-        // meets a masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
-        Meta& mt = meta[j & 3];
-        const float kf = ks * fabsf(p.scale) * kLog2e, f = fmaxf(vs * to_unit, 8.6736174e-19f);
-        mt.kf[ct] = kf != kf ? kf : fmaxf(kf, 1e-30f);
-        mt.lv[ct] = vs != vs ? vs : __log2f(f);
-        mt.iv[ct] = vs != vs ? vs : 1.0f / f;
-        const int oks = __ballot_sync(0xffu, chunk_base >= 0);
+      if (factors) {
+        Meta& mt = meta[j & (2 * kRing - 1)];
+        mt.kf[ct] = kf;
+        mt.lv[ct] = lv;
+        mt.iv[ct] = iv;
+        const int oks = __ballot_sync((1u << kChunks) - 1, ok_now);
         if (ct == 0) mt.oks = oks;
       }
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.kfull[st]);
-      if (j + 1 < n_steps) {
-        find(j + 1);
-        load(p.k_cache, j + 1, k);
-      }
-      if (!warp_wait(&bars.vempty[st], was, ctl, kErrWiden)) break;
-      store(base + M::kV + st * M::kOperand, v);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.vfull[st]);
-      if (j + 1 < n_steps) load(p.v_cache, j + 1, v);
+      if (lane == 0) mbar_arrive(&full[st]);
+      return true;
+    };
+    uint4 w0[kPer], w1[kPer];
+    find_page(0);
+    find(0);
+    find_page(1);
+    load(0, w0);
+    if (factors) make_factors();
+    find(1);
+    find_page(2);
+    load(1, w1);
+    // step j: its data in w0 / w1, the factors its own, scales those of j + 1, page ids those of j + 2
+    auto turn = [&](int j, uint4 (&w)[kPer]) {
+      if (!put(j, w)) return false;
+      if (factors) make_factors();
+      find(j + 2);
+      find_page(j + 3);
+      load(j + 2, w);
+      return true;
+    };
+#pragma unroll 1
+    for (int j = 0; j < n_steps; j += 2) {
+      if (!turn(j, w0)) break;
+      if (j + 1 < n_steps && !turn(j + 1, w1)) break;
     }
   } else {
     // ---------------------------------------------------------------- MMAs (the warp stays converged, so that their operands stay in uniform registers; one lane issues)
     constexpr uint32_t kF32Out = 1u << 4;
-    const uint32_t qk = kF32Out | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+    const uint32_t qk = kF32Out | (static_cast<uint32_t>(kStep >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
     const uint32_t pv = kF32Out | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
     const uint64_t qd = umma_desc_sw128(base + M::kQ), kd = umma_desc_sw128(base + M::kK), vd = desc_mn<D>(base + M::kV);
     // Per tile: scores issued, values issued. The next values wait for their P' and V, the next scores for K and for
-    // the completion of the values before them (they overwrite the P' those read).
+    // the completion of the values two steps before them (they overwrite the P' those read).
     int scores0 = 0, values0 = 0, scores1 = two ? 0 : n_steps, values1 = two ? 0 : n_steps;
     uint64_t since = 0;
     int idle = 0;
@@ -495,33 +511,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       for (int a = 0; a < 2; ++a) {
         const int scores = a ? scores1 : scores0, values = a ? values1 : values0;
         if (values < scores) {
-          const int j = values, st = j & 1;
-          if (__all_sync(~0u, mbar_test_wait(&bars.pfull[a], j & 1) && mbar_test_wait(&bars.vfull[st], (j >> 1) & 1))) {
+          const int j = values, st = j & (kRing - 1), b = j & 1;
+          if (__all_sync(~0u, mbar_test_wait(&bars.pfull[a][b], (j >> 1) & 1) && mbar_test_wait(&bars.vfull[st], (j / kRing) & 1))) {
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-              mma_f16_ts(tmem + kO + kTile * a, tmem + kS + kTile * a + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
-            mma_commit(&bars.odone[a]);
-            mma_commit(&bars.vempty[st]);
+              for (int i = 0; i < kStep / 16; ++i)
+                mma_f16_ts(tmem + kO + 128 * a, tmem + kS + 128 * a + kStep * b + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
+              mma_commit(&bars.odone[a][b]);
+              mma_commit(&bars.vempty[st]);
             }
             __syncwarp();
             if (a) ++values1;
             else ++values0;
             any = true;
           }
-        } else if (scores < n_steps) {
-          const int j = scores, st = j & 1;
-          if (__all_sync(~0u, mbar_test_wait(&bars.kfull[st], (j >> 1) & 1) && (j == 0 || mbar_test_wait(&bars.odone[a], (j - 1) & 1)))) {
+        }
+        if (scores < n_steps && scores < values + 2) {
+          // its buffer held the weights of step j - 2
+          const int j = scores, st = j & (kRing - 1), b = j & 1;
+          if (__all_sync(~0u, mbar_test_wait(&bars.kfull[st], (j / kRing) & 1) && (j < 2 || mbar_test_wait(&bars.odone[a][b], ((j - 2) >> 1) & 1)))) {
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              const uint64_t off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
-              mma_f16_ss(tmem + kS + kTile * a, qd + a * (M::kOperand >> 4) + off, kd + st * (M::kOperand >> 4) + off, qk, i > 0);
-            }
-            mma_commit(&bars.sfull[a]);
-            mma_commit(&bars.kempty[st]);
+              for (int i = 0; i < D / 16; ++i) {
+                const uint64_t q_off = static_cast<uint64_t>((i >> 2) * (M::kQPanel >> 4) + 2 * (i & 3)), k_off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
+                mma_f16_ss(tmem + kS + 128 * a + kStep * b, qd + a * (M::kQTile >> 4) + q_off, kd + st * (M::kOperand >> 4) + k_off, qk, i > 0);
+              }
+              mma_commit(&bars.sfull[a][b]);
+              mma_commit(&bars.kempty[st]);
             }
             __syncwarp();
             if (a) ++scores1;
