@@ -11,13 +11,13 @@
 // float16 holds 2^25 of range below the largest weight times the largest scale at full precision. The normaliser is the
 // float32 sum of P' divided by the same factor, a page at a time.
 //
-// Roles (17 warps):
+// Roles (20 warps, registers moved between them):
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row: read S, raise m (and rescale O, rare), write P' over S, at
 //                   the end write the row out.
 //   warps 8-11, 12-15  widen keys, values: 16-byte loads two steps ahead (page ids three), float16 to the 128-byte swizzle
 //                   the tensor cores read (keys K-major, values MN-major: both as they lie, no transposition).
-//   warp 16         issues the MMAs (converged, one lane elected, so that descriptors stay in uniform registers):
-//                   for each tile whichever of Q K of the next step and P V of this one is ready first.
+//   warp 16         (of 16-19) issues the MMAs (converged, one lane elected, so that descriptors stay in uniform registers):
+//                   Q K of the next step for both tiles, then P V of this one.
 // Tensor memory: two S (and P') buffers of 64 columns for each tile at 0 and 128, O at 256 and 384. With two buffers the
 // scores of the next step are there when the softmax of this one ends; with one of 128 columns the softmax waited
 // for P V, Q K and both signals each step (twice the time).
@@ -40,9 +40,13 @@ constexpr int kRing = 4;          // steps of keys and of values in shared memor
 constexpr int kRows = 2 * kTile;  // rows of a CTA
 constexpr int kSoftmaxWarps = 8;
 constexpr int kWidenWarps = 4;    // for keys, and as many for values
-constexpr int kThreads = (kSoftmaxWarps + 2 * kWidenWarps + 1) * 32;
+constexpr int kThreads = (kSoftmaxWarps + 2 * kWidenWarps + 4) * 32;  // the MMA warp and three that only fill its warpgroup
 constexpr int kMmaWarp = kSoftmaxWarps + 2 * kWidenWarps;
 constexpr int kChunks = kStep / 16;
+// Registers a thread: 20 warps are launched with 96 (as many as an SM sub-partition's five warps can have); the
+// warpgroups then trade them.
+constexpr int kRegs = 96, kSoftmaxRegs = 112, kWidenRegs = 88, kMmaRegs = 80;
+static_assert(256 * kSoftmaxRegs + 256 * kWidenRegs + 128 * kMmaRegs <= kThreads * kRegs, "more registers than the block has");
 constexpr float kRaise = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kS = 0, kO = 256;  // tensor memory columns (128 a tile)
@@ -130,6 +134,11 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 struct Job {
   int b, tile, head, rows;  // rows: of this CTA (<= 256)
   SeqRows r;
@@ -198,8 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&bars.kfull[i], kWidenWarps);
       mbar_init(&bars.vfull[i], kWidenWarps);
-      mbar_init(&bars.kempty[i], two ? 2 : 1);
-      mbar_init(&bars.vempty[i], two ? 2 : 1);
+      mbar_init(&bars.kempty[i], 1);
+      mbar_init(&bars.vempty[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bars.sfull[i >> 1][i & 1], 1);
@@ -262,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   const float to_unit = __uint_as_float((265u - r_exp) << 23);
 
   if (warp < kSoftmaxWarps) {
+    regs_inc<kSoftmaxRegs>();
     // ---------------------------------------------------------------- softmax
     const int a = warp >> 2, q = warp & 3, row = a * kTile + q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
@@ -385,6 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       }
     }
   } else if (warp < kMmaWarp) {
+    regs_dec<kWidenRegs>();
     // ---------------------------------------------------------------- widen keys or values
     constexpr int kPieces = D / 16;                             // 16-byte pieces a row
     constexpr int kPer = kStep * kPieces / (kWidenWarps * 32);  // pieces a thread
@@ -494,76 +505,75 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       if (j + 1 < n_steps && !turn(j + 1, w1)) break;
     }
   } else {
+    regs_dec<kMmaRegs>();
+  }
+  if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- MMAs (the warp stays converged, so that their operands stay in uniform registers; one lane issues)
     constexpr uint32_t kF32Out = 1u << 4;
     const uint32_t qk = kF32Out | (static_cast<uint32_t>(kStep >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
     const uint32_t pv = kF32Out | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
     const uint64_t qd = umma_desc_sw128(base + M::kQ), kd = umma_desc_sw128(base + M::kK), vd = desc_mn<D>(base + M::kV);
-    // Per tile: scores issued, values issued. The next values wait for their P' and V, the next scores for K and for
-    // the completion of the values two steps before them (they overwrite the P' those read).
-    int scores0 = 0, values0 = 0, scores1 = two ? 0 : n_steps, values1 = two ? 0 : n_steps;
-    uint64_t since = 0;
-    int idle = 0;
-    bool ok = true;
-    while (ok && (values0 < n_steps || values1 < n_steps)) {
-      bool any = false;
+    // Step by step: scores of the next step (their buffers held the weights of the step before this one), then the values
+    // of this one. Lanes look at the barriers of a wait side by side: one probe's latency, not the sum.
+    auto wait = [&](uint64_t* bar, uint32_t parity, bool mine) {
+      uint64_t start = 0;
+      for (;;) {
 #pragma unroll 1
-      for (int a = 0; a < 2; ++a) {
-        const int scores = a ? scores1 : scores0, values = a ? values1 : values0;
-        if (values < scores) {
-          const int j = values, st = j & (kRing - 1), b = j & 1;
-          if (__all_sync(~0u, mbar_test_wait(&bars.pfull[a][b], (j >> 1) & 1) && mbar_test_wait(&bars.vfull[st], (j / kRing) & 1))) {
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int i = 0; i < kStep / 16; ++i)
-                mma_f16_ts(tmem + kO + 128 * a, tmem + kS + 128 * a + kStep * b + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
-              mma_commit(&bars.odone[a][b]);
-              mma_commit(&bars.vempty[st]);
-            }
-            __syncwarp();
-            if (a) ++values1;
-            else ++values0;
-            any = true;
-          }
-        }
-        if (scores < n_steps && scores < values + 2) {
-          // its buffer held the weights of step j - 2
-          const int j = scores, st = j & (kRing - 1), b = j & 1;
-          if (__all_sync(~0u, mbar_test_wait(&bars.kfull[st], (j / kRing) & 1) && (j < 2 || mbar_test_wait(&bars.odone[a][b], ((j - 2) >> 1) & 1)))) {
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) {
-                const uint64_t q_off = static_cast<uint64_t>((i >> 2) * (M::kQPanel >> 4) + 2 * (i & 3)), k_off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
-                mma_f16_ss(tmem + kS + 128 * a + kStep * b, qd + a * (M::kQTile >> 4) + q_off, kd + st * (M::kOperand >> 4) + k_off, qk, i > 0);
-              }
-              mma_commit(&bars.sfull[a][b]);
-              mma_commit(&bars.kempty[st]);
-            }
-            __syncwarp();
-            if (a) ++scores1;
-            else ++scores0;
-            any = true;
-          }
-        }
-      }
-      idle = any ? 0 : idle + 1;
-      if (any) since = 0;
-      if (idle >= kSpins) {
-        idle = 0;
-        const uint64_t now = global_timer_ns();
-        if (since == 0) since = now;
-        const bool expired = __any_sync(~0u, now - since > kWaitLimitNs);
-        if (__any_sync(~0u, *ctl.abort != 0)) {
-          ok = false;
-        } else if (expired) {
+        for (int i = 0; i < kSpins; ++i)
+          if (__all_sync(~0u, !mine || mbar_test_wait(bar, parity))) return true;
+        if (__any_sync(~0u, *ctl.abort != 0)) return false;
+        const uint64_t now = __shfl_sync(~0u, global_timer_ns(), 0);
+        if (start == 0) start = now;
+        if (now - start > kWaitLimitNs) {
           if (lane == 0) {
             record_device_error(ctl.err, kErrMma);
             *ctl.abort = 1;
           }
-          ok = false;
+          return false;
         }
+      }
+    };
+    const int tiles = two ? 2 : 1;
+#pragma unroll 1
+    for (int j = -1; j < n_steps; ++j) {
+      if (j + 1 < n_steps) {
+        const int t = j + 1, st = t & (kRing - 1), b = t & 1;
+        if (!wait(lane == 0 ? &bars.kfull[st] : &bars.odone[lane & 1][b], lane == 0 ? (t / kRing) & 1 : ((t - 2) >> 1) & 1,
+                  lane == 0 || (t >= 2 && (lane == 2 || (lane == 1 && two)))))
+          break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll 1
+          for (int a = 0; a < tiles; ++a) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const uint64_t q_off = static_cast<uint64_t>((i >> 2) * (M::kQPanel >> 4) + 2 * (i & 3)), k_off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
+              mma_f16_ss(tmem + kS + 128 * a + kStep * b, qd + a * (M::kQTile >> 4) + q_off, kd + st * (M::kOperand >> 4) + k_off, qk, i > 0);
+            }
+            mma_commit(&bars.sfull[a][b]);
+          }
+          mma_commit(&bars.kempty[st]);
+        }
+        __syncwarp();
+      }
+      if (j >= 0) {
+        const int st = j & (kRing - 1), b = j & 1;
+        bool ok = true;
+#pragma unroll 1
+        for (int a = 0; ok && a < tiles; ++a) {
+          ok = wait(lane == 0 ? &bars.vfull[st] : &bars.pfull[a][b], lane == 0 ? (j / kRing) & 1 : (j >> 1) & 1, lane < 2);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < kStep / 16; ++i)
+              mma_f16_ts(tmem + kO + 128 * a, tmem + kS + 128 * a + kStep * b + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
+            mma_commit(&bars.odone[a][b]);
+            if (a == tiles - 1) mma_commit(&bars.vempty[st]);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
       }
     }
     if (elect_one()) mma_commit(&bars.done);  // every MMA issued has completed once it flips
