@@ -558,22 +558,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       }
       if (j >= 0) {
         const int st = j & (kRing - 1), b = j & 1;
-        bool ok = true;
+        if (!wait(lane == 0 ? &bars.vfull[st] : &bars.pfull[lane & 1][b], lane == 0 ? (j / kRing) & 1 : (j >> 1) & 1, lane == 0 || lane == 2 || (lane == 1 && two))) break;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll 1
-        for (int a = 0; ok && a < tiles; ++a) {
-          ok = wait(lane == 0 ? &bars.vfull[st] : &bars.pfull[a][b], lane == 0 ? (j / kRing) & 1 : (j >> 1) & 1, lane < 2);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
+          for (int a = 0; a < tiles; ++a) {
 #pragma unroll
             for (int i = 0; i < kStep / 16; ++i)
               mma_f16_ts(tmem + kO + 128 * a, tmem + kS + 128 * a + kStep * b + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
             mma_commit(&bars.odone[a][b]);
-            if (a == tiles - 1) mma_commit(&bars.vempty[st]);
           }
-          __syncwarp();
+          mma_commit(&bars.vempty[st]);
         }
-        if (!ok) break;
+        __syncwarp();
       }
     }
     if (elect_one()) mma_commit(&bars.done);  // every MMA issued has completed once it flips
