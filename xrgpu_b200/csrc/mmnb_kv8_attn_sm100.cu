@@ -6,9 +6,9 @@
 // G, so the group shares every key and value) as two tiles of 128, and passes once over the tokens they see,
 // 64 at a time. Codes are exact float16 numbers: they are widened once a CTA, in registers, on their way
 // to shared memory, and the scales stay out of them: k_scale multiplies the scores a page at a time, and
-// v_scale joins the exponent of the weights: P' = exp2(x - m + log2(v_scale 2^11 / R)), R the power of two above the
-// largest v_scale of the tokens. With m raised only when a score exceeds it by 4, P' stays below 2^15, so
-// float16 holds 2^25 of range below the largest weight times the largest scale at full precision. The normaliser is the
+// v_scale joins the exponent of the weights: P' = exp2(x - m + log2(v_scale 2^7 / R)), R the power of two above the
+// largest v_scale of the tokens. With m raised only when a score exceeds it by 8, P' stays below 2^15, so
+// float16 holds 2^21 of range below the weight 1 with the largest scale at full precision. The normaliser is the
 // float32 sum of P' divided by the same factor, a page at a time.
 //
 // Roles (20 warps, registers moved between them):
@@ -16,8 +16,10 @@
 //                   the end write the row out.
 //   warps 8-11, 12-15  widen keys, values: 16-byte loads two steps ahead (page ids three), float16 to the 128-byte swizzle
 //                   the tensor cores read (keys K-major, values MN-major: both as they lie, no transposition).
-//   warp 16         (of 16-19) issues the MMAs (converged, one lane elected, so that descriptors stay in uniform registers):
-//                   Q K of the next step for both tiles, then P V of this one.
+//   warps 16-19     issue the MMAs, one each of tile 0's scores, tile 1's scores, tile 0's values, tile 1's values (one warp
+//                   for all spent 40 % of the time on its own waits; the products depend on one another through
+//                   barriers only). A warp stays converged and elects the issuing lane, so that descriptors stay in
+//                   uniform registers.
 // Tensor memory: two S (and P') buffers of 64 columns for each tile at 0 and 128, O at 256 and 384. With two buffers the
 // scores of the next step are there when the softmax of this one ends; with one of 128 columns the softmax waited
 // for P V, Q K and both signals each step (twice the time).
@@ -40,14 +42,14 @@ constexpr int kRing = 4;          // steps of keys and of values in shared memor
 constexpr int kRows = 2 * kTile;  // rows of a CTA
 constexpr int kSoftmaxWarps = 8;
 constexpr int kWidenWarps = 4;    // for keys, and as many for values
-constexpr int kThreads = (kSoftmaxWarps + 2 * kWidenWarps + 4) * 32;  // the MMA warp and three that only fill its warpgroup
+constexpr int kThreads = (kSoftmaxWarps + 2 * kWidenWarps + 4) * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + 2 * kWidenWarps;
 constexpr int kChunks = kStep / 16;
 // Registers a thread: 20 warps are launched with 96 (as many as an SM sub-partition's five warps can have); the
 // warpgroups then trade them.
 constexpr int kRegs = 96, kSoftmaxRegs = 112, kWidenRegs = 88, kMmaRegs = 80;
 static_assert(256 * kSoftmaxRegs + 256 * kWidenRegs + 128 * kMmaRegs <= kThreads * kRegs, "more registers than the block has");
-constexpr float kRaise = 4.0f;
+constexpr float kRaise = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kS = 0, kO = 256;  // tensor memory columns (128 a tile)
 
@@ -70,7 +72,8 @@ struct Meta {
 
 struct Bars {
   uint64_t kfull[kRing], kempty[kRing], vfull[kRing], vempty[kRing];
-  uint64_t sfull[2][2], pfull[2][2], odone[2][2], done;  // [tile][step % 2]
+  uint64_t sfull[2][2], pfull[2][2], odone[2][2];  // [tile][step % 2]
+  uint64_t done[4];
 };
 
 // Values operand: [tokens][64] float16 panels, 64 values of D contiguous (MN-major), 128-byte swizzle: 8-token groups 1024
@@ -207,15 +210,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&bars.kfull[i], kWidenWarps);
       mbar_init(&bars.vfull[i], kWidenWarps);
-      mbar_init(&bars.kempty[i], 1);
-      mbar_init(&bars.vempty[i], 1);
+      mbar_init(&bars.kempty[i], two ? 2 : 1);
+      mbar_init(&bars.vempty[i], two ? 2 : 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bars.sfull[i >> 1][i & 1], 1);
       mbar_init(&bars.odone[i >> 1][i & 1], 1);
       mbar_init(&bars.pfull[i >> 1][i & 1], 4);
+      mbar_init(&bars.done[i], 1);
     }
-    mbar_init(&bars.done, 1);
     abort_flag = 0;
     vmax_bits = 0;
     fence_mbar_init();
@@ -265,10 +268,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     fence_async_shared();
   }
   __syncthreads();
-  // R: the power of two above the largest scale (exponent field + 1), and 2^11 / R
+  // R: the power of two above the largest scale (exponent field + 1), and 2^7 / R
   const uint32_t r_exp = min(max((vmax_bits >> 23) + 1u, 13u), 253u);
-  const float value_unit = __uint_as_float((r_exp - 11u) << 23);  // R 2^-11
-  const float to_unit = __uint_as_float((265u - r_exp) << 23);
+  const float value_unit = __uint_as_float((r_exp - 7u) << 23);  // R 2^-7
+  const float to_unit = __uint_as_float((261u - r_exp) << 23);
 
   if (warp < kSoftmaxWarps) {
     regs_inc<kSoftmaxRegs>();
@@ -507,14 +510,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   } else {
     regs_dec<kMmaRegs>();
   }
-  if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- MMAs (the warp stays converged, so that their operands stay in uniform registers; one lane issues)
-    constexpr uint32_t kF32Out = 1u << 4;
-    const uint32_t qk = kF32Out | (static_cast<uint32_t>(kStep >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
-    const uint32_t pv = kF32Out | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
-    const uint64_t qd = umma_desc_sw128(base + M::kQ), kd = umma_desc_sw128(base + M::kK), vd = desc_mn<D>(base + M::kV);
-    // Step by step: scores of the next step (their buffers held the weights of the step before this one), then the values
-    // of this one. Lanes look at the barriers of a wait side by side: one probe's latency, not the sum.
+  if (warp >= kMmaWarp && (two || !((warp - kMmaWarp) & 1))) {
+    // ---------------------------------------------------------------- MMAs (a warp stays converged, so that their operands stay in uniform registers; one lane issues)
+    const int a = (warp - kMmaWarp) & 1, issuer = warp - kMmaWarp;
+    // Lanes 0 and 1 look at a wait's two barriers side by side: one probe's latency, not the sum.
     auto wait = [&](uint64_t* bar, uint32_t parity, bool mine) {
       uint64_t start = 0;
       for (;;) {
@@ -533,49 +532,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         }
       }
     };
-    const int tiles = two ? 2 : 1;
+    constexpr uint32_t kF32Out = 1u << 4;
+    if (issuer < 2) {  // scores; their buffer held the weights of two steps before
+      constexpr uint32_t qk = kF32Out | (static_cast<uint32_t>(kStep >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+      const uint64_t qd = umma_desc_sw128(base + M::kQ + a * M::kQTile), kd = umma_desc_sw128(base + M::kK);
 #pragma unroll 1
-    for (int j = -1; j < n_steps; ++j) {
-      if (j + 1 < n_steps) {
-        const int t = j + 1, st = t & (kRing - 1), b = t & 1;
-        if (!wait(lane == 0 ? &bars.kfull[st] : &bars.odone[lane & 1][b], lane == 0 ? (t / kRing) & 1 : ((t - 2) >> 1) & 1,
-                  lane == 0 || (t >= 2 && (lane == 2 || (lane == 1 && two)))))
-          break;
+      for (int j = 0; j < n_steps; ++j) {
+        const int st = j & (kRing - 1), b = j & 1;
+        if (!wait(lane == 0 ? &bars.kfull[st] : &bars.odone[a][b], lane == 0 ? (j / kRing) & 1 : ((j - 2) >> 1) & 1, lane == 0 || (lane == 1 && j >= 2))) break;
         tc_fence_after();
         if (elect_one()) {
-#pragma unroll 1
-          for (int a = 0; a < tiles; ++a) {
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              const uint64_t q_off = static_cast<uint64_t>((i >> 2) * (M::kQPanel >> 4) + 2 * (i & 3)), k_off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
-              mma_f16_ss(tmem + kS + 128 * a + kStep * b, qd + a * (M::kQTile >> 4) + q_off, kd + st * (M::kOperand >> 4) + k_off, qk, i > 0);
-            }
-            mma_commit(&bars.sfull[a][b]);
+          for (int i = 0; i < D / 16; ++i) {
+            const uint64_t q_off = static_cast<uint64_t>((i >> 2) * (M::kQPanel >> 4) + 2 * (i & 3)), k_off = static_cast<uint64_t>((i >> 2) * (M::kPanel >> 4) + 2 * (i & 3));
+            mma_f16_ss(tmem + kS + 128 * a + kStep * b, qd + q_off, kd + st * (M::kOperand >> 4) + k_off, qk, i > 0);
           }
+          mma_commit(&bars.sfull[a][b]);
           mma_commit(&bars.kempty[st]);
         }
         __syncwarp();
       }
-      if (j >= 0) {
+    } else {  // values
+      constexpr uint32_t pv = kF32Out | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+      const uint64_t vd = desc_mn<D>(base + M::kV);
+#pragma unroll 1
+      for (int j = 0; j < n_steps; ++j) {
         const int st = j & (kRing - 1), b = j & 1;
-        if (!wait(lane == 0 ? &bars.vfull[st] : &bars.pfull[lane & 1][b], lane == 0 ? (j / kRing) & 1 : (j >> 1) & 1, lane == 0 || lane == 2 || (lane == 1 && two))) break;
+        if (!wait(lane == 0 ? &bars.vfull[st] : &bars.pfull[a][b], lane == 0 ? (j / kRing) & 1 : (j >> 1) & 1, lane < 2)) break;
         tc_fence_after();
         if (elect_one()) {
-#pragma unroll 1
-          for (int a = 0; a < tiles; ++a) {
 #pragma unroll
-            for (int i = 0; i < kStep / 16; ++i)
-              mma_f16_ts(tmem + kO + 128 * a, tmem + kS + 128 * a + kStep * b + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
-            mma_commit(&bars.odone[a][b]);
-          }
+          for (int i = 0; i < kStep / 16; ++i)
+            mma_f16_ts(tmem + kO + 128 * a, tmem + kS + 128 * a + kStep * b + 8 * i, vd + st * (M::kOperand >> 4) + i * (2048 >> 4), pv, j > 0 || i > 0);
+          mma_commit(&bars.odone[a][b]);
           mma_commit(&bars.vempty[st]);
         }
         __syncwarp();
       }
     }
-    if (elect_one()) mma_commit(&bars.done);  // every MMA issued has completed once it flips
+    if (elect_one()) mma_commit(&bars.done[issuer]);  // every MMA that this warp issued has completed once it flips
     __syncwarp();
-    drain_wait(&bars.done, 0, p.err, kErrDrain);
+    drain_wait(&bars.done[issuer], 0, p.err, kErrDrain);
   }
 
   tc_fence_before();
