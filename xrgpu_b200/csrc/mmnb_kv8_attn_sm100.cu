@@ -405,15 +405,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     constexpr int kRowStep = kWidenWarps * 32 / kPieces;
     static_assert(kRowStep % 16 == 0, "a thread's rows lie at the same place of their 16-token chunks");
     const bool keys = warp < kSoftmaxWarps + kWidenWarps;
-    const int ct = tid - (keys ? kSoftmaxWarps : kSoftmaxWarps + kWidenWarps) * 32, piece = ct % kPieces, row0 = ct / kPieces;
+    // A lane's piece of a row is 16 codes: 16-byte chunks 2 (piece % 4) and + 1 of the row's float16 numbers in panel piece / 4.
+    // The lanes of the second panel take the neighbouring row, whose swizzle puts them on the other banks.
+    const int ct = tid - (keys ? kSoftmaxWarps : kSoftmaxWarps + kWidenWarps) * 32, piece = ct % kPieces, row0 = (ct / kPieces) ^ (piece >> 2);
     const uint8_t* cache = (keys ? p.k_cache : p.v_cache) + (row0 & 15) * D + piece * 16;
     uint64_t* full = keys ? bars.kfull : bars.vfull;
     uint64_t* empty = keys ? bars.kempty : bars.vempty;
-    // 16-byte chunks 2 (piece % 4) and + 1 of a row's float16 numbers; the two panels' lanes start with different ones: no bank twice
-    const bool odd = (piece >> 2) & 1;
-    const int c0 = 2 * (piece & 3) + odd, c1 = c0 ^ 1;
+    const int c0 = 2 * (piece & 3);
     const uint32_t line = base + (keys ? M::kK : M::kV) + (piece >> 2) * M::kPanel + row0 * 128;
-    const uint32_t at0 = line + ((c0 ^ (row0 & 7)) << 4), at1 = line + ((c1 ^ (row0 & 7)) << 4);
+    const uint32_t at0 = line + ((c0 ^ (row0 & 7)) << 4), at1 = line + (((c0 + 1) ^ (row0 & 7)) << 4);
     // Lane c < kChunks knows chunk c of a step: its page id three steps ahead, two steps ahead where its first token's
     // codes lie (-1: nowhere). The first thread of the keys' warps for each chunk also makes the step's factors: scales two
     // steps ahead, factors one.
@@ -466,8 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       if (!warp_wait(&empty[st], ((j / kRing) & 1) ^ 1, ctl, kErrWiden)) return false;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const uint2 a = widen4<E4M3>(odd ? w[i].z : w[i].x), b = widen4<E4M3>(odd ? w[i].w : w[i].y);
-        const uint2 c = widen4<E4M3>(odd ? w[i].x : w[i].z), d = widen4<E4M3>(odd ? w[i].y : w[i].w);
+        const uint2 a = widen4<E4M3>(w[i].x), b = widen4<E4M3>(w[i].y), c = widen4<E4M3>(w[i].z), d = widen4<E4M3>(w[i].w);
         sts128(at0 + st * M::kOperand + i * kRowStep * 128, a.x, a.y, b.x, b.y);
         sts128(at1 + st * M::kOperand + i * kRowStep * 128, c.x, c.y, d.x, d.y);
       }
@@ -513,25 +512,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   if (warp >= kMmaWarp && (two || !((warp - kMmaWarp) & 1))) {
     // ---------------------------------------------------------------- MMAs (a warp stays converged, so that their operands stay in uniform registers; one lane issues)
     const int a = (warp - kMmaWarp) & 1, issuer = warp - kMmaWarp;
-    // Lanes 0 and 1 look at a wait's two barriers side by side: one probe's latency, not the sum.
-    auto wait = [&](uint64_t* bar, uint32_t parity, bool mine) {
-      uint64_t start = 0;
-      for (;;) {
-#pragma unroll 1
-        for (int i = 0; i < kSpins; ++i)
-          if (__all_sync(~0u, !mine || mbar_test_wait(bar, parity))) return true;
-        if (__any_sync(~0u, *ctl.abort != 0)) return false;
-        const uint64_t now = __shfl_sync(~0u, global_timer_ns(), 0);
-        if (start == 0) start = now;
-        if (now - start > kWaitLimitNs) {
-          if (lane == 0) {
-            record_device_error(ctl.err, kErrMma);
-            *ctl.abort = 1;
-          }
-          return false;
-        }
-      }
-    };
     constexpr uint32_t kF32Out = 1u << 4;
     if (issuer < 2) {  // scores; their buffer held the weights of two steps before
       constexpr uint32_t qk = kF32Out | (static_cast<uint32_t>(kStep >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
@@ -539,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
 #pragma unroll 1
       for (int j = 0; j < n_steps; ++j) {
         const int st = j & (kRing - 1), b = j & 1;
-        if (!wait(lane == 0 ? &bars.kfull[st] : &bars.odone[a][b], lane == 0 ? (j / kRing) & 1 : ((j - 2) >> 1) & 1, lane == 0 || (lane == 1 && j >= 2))) break;
+        if (!warp_wait(&bars.kfull[st], (j / kRing) & 1, ctl, kErrMma) || (j >= 2 && !warp_wait(&bars.odone[a][b], ((j - 2) >> 1) & 1, ctl, kErrMma))) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -558,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
 #pragma unroll 1
       for (int j = 0; j < n_steps; ++j) {
         const int st = j & (kRing - 1), b = j & 1;
-        if (!wait(lane == 0 ? &bars.vfull[st] : &bars.pfull[a][b], lane == 0 ? (j / kRing) & 1 : (j >> 1) & 1, lane < 2)) break;
+        if (!warp_wait(&bars.vfull[st], (j / kRing) & 1, ctl, kErrMma) || !warp_wait(&bars.pfull[a][b], (j >> 1) & 1, ctl, kErrMma)) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
