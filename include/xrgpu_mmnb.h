@@ -523,7 +523,7 @@ typedef struct {
   int32_t cache_dtype;  /* XRGPU_INT8 or XRGPU_FLOAT8_E4M3 */
   int32_t causal;       /* attention: nonzero: a row sees the tokens up to its own position */
   float scale;          /* attention: factor of q . k, usually head_dim^-1/2 */
-  int32_t zero_rest;    /* attention: nonzero: rows behind the last sequence are set to zero */
+  int32_t zero_rest;    /* attention, read: nonzero: rows of no sequence are set to zero */
   int32_t reserved;
   int64_t tokens;       /* rows of q, k, v, o */
   int64_t sequences, heads_q, heads_kv, head_dim, page, pages, max_pages;

@@ -138,8 +138,8 @@ class Mxfp4Problem_(ctypes.Structure):
 
 class Kv8Problem_(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32), ("causal", ctypes.c_int32),
-                ("scale", ctypes.c_float), ("zero_rest", ctypes.c_int32), ("reserved", ctypes.c_int32), ("tokens", _i64), ("sequences", _i64), ("heads_q", _i64), ("heads_kv", _i64),
-                ("head_dim", _i64), ("page", _i64), ("pages", _i64), ("max_pages", _i64), ("window", _i64),
+                ("scale", ctypes.c_float), ("zero_rest", ctypes.c_int32), ("reserved", ctypes.c_int32), ("tokens", _i64),
+                ("sequences", _i64), ("heads_q", _i64), ("heads_kv", _i64), ("head_dim", _i64), ("page", _i64), ("pages", _i64), ("max_pages", _i64), ("window", _i64),
                 ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64), ("o_stride", _i64), ("q", _vp), ("k", _vp),
                 ("v", _vp), ("o", _vp), ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp), ("v_scale", _vp),
                 ("page_table", _vp), ("cu_seqlens", _vp), ("kv_len", _vp)]

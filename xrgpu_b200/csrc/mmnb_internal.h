@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -28,6 +29,19 @@ struct Problem {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t align_up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
+
+// Lets `Kernel` use up to `bytes` of dynamic shared memory on the current device (asked of the runtime once a device).
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<int> allowed[64];
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  const cudaError_t f = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (f == cudaSuccess && dev >= 0 && dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
+  return f;
+}
 
 // Number of SMs of the current device (cached per device).
 int device_sm_count();

@@ -170,44 +170,47 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const Kv8 p) {
   }
 }
 
-// One warp a (row, head, side): finds the row's sequence and copies its values out.
-template <bool E4M3, bool F16>
-__global__ void __launch_bounds__(256) read_kernel(const Kv8 p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int row = static_cast<int>(warp / p.hkv), head = static_cast<int>(warp % p.hkv);
-  if (row >= p.tokens) return;
-  int b = -1;
-  if (p.uniform) {
-    b = row / (p.tokens / p.seqs);
-    if (b >= p.seqs) return;
-  } else {
-    for (int b0 = 0; b0 < p.seqs && b < 0; b0 += 32) {
-      const bool here = b0 + lane < p.seqs && p.cu[b0 + lane] <= row && row < p.cu[b0 + lane + 1];
-      const unsigned m = __ballot_sync(~0u, here);
-      if (m) b = b0 + __ffs(m) - 1;
-    }
-    if (b < 0) return;
+// The sequence of a row (found by a warp), -1 if it belongs to none.
+__device__ __forceinline__ int sequence_of(const Kv8& p, int row, int lane) {
+  if (p.uniform) return row / (p.tokens / p.seqs);
+  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
+    const bool here = b0 + lane < p.seqs && p.cu[b0 + lane] <= row && row < p.cu[b0 + lane + 1];
+    const unsigned m = __ballot_sync(~0u, here);
+    if (m) return b0 + __ffs(m) - 1;
   }
-  const SeqRows r = seq_rows(p, b, false);
-  if (r.n == 0) return;
-  const int pos = r.len - r.n + (row - r.row0), id = page_id(p, b, pos >> p.page_log2);
-  if (id < 0) return;
+  return -1;
+}
+
+// One warp a (row, side), all heads: PER codes a lane.
+template <bool E4M3, bool F16, int PER>
+__global__ void __launch_bounds__(256) read_kernel(const Kv8 p) {
+  constexpr int D = 32 * PER;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= p.tokens) return;
   const bool side_v = blockIdx.y != 0;
-  const int64_t block = static_cast<int64_t>(id) * p.hkv + head;
-  const float s = (side_v ? p.v_scale : p.k_scale)[block];
-  const uint8_t* codes = (side_v ? p.v_cache : p.k_cache) + ((block << p.page_log2) + (pos & (p.page - 1))) * p.D;
+  const int b = sequence_of(p, row, lane);
+  const SeqRows r = b < 0 ? SeqRows{0, 0, 0} : seq_rows(p, b, false);
+  const int pos = r.len - r.n + (row - r.row0), id = r.n ? page_id(p, b, pos >> p.page_log2) : -1;
+  if (id < 0 && !p.zero_rest) return;
+  const int64_t block = static_cast<int64_t>(id) * p.hkv;
+  const float* scales = (side_v ? p.v_scale : p.k_scale) + block;
+  const uint8_t* codes = (side_v ? p.v_cache : p.k_cache) + ((block << p.page_log2) + (pos & (p.page - 1))) * D + lane * PER;
   void* dst = side_v ? p.v : p.k;
-  const int64_t at = static_cast<int64_t>(row) * (side_v ? p.vs : p.ks) + head * p.D;
-  for (int d = lane * 2; d < p.D; d += 64) {
-    const uint32_t w = *reinterpret_cast<const uint16_t*>(codes + d);
-    const float a = code_value<E4M3>(w & 255u) * s, c = code_value<E4M3>(w >> 8) * s;
-    if (F16) {
-      static_cast<__half*>(dst)[at + d] = __float2half_rn(a);
-      static_cast<__half*>(dst)[at + d + 1] = __float2half_rn(c);
-    } else {
-      static_cast<float*>(dst)[at + d] = a;
-      static_cast<float*>(dst)[at + d + 1] = c;
+  int64_t at = static_cast<int64_t>(row) * (side_v ? p.vs : p.ks) + lane * PER;
+#pragma unroll 4
+  for (int h = 0; h < p.hkv; ++h, at += D) {
+    uint32_t w = 0;
+    float s = 0.0f;
+    if (id >= 0) {
+      const uint8_t* src = codes + (static_cast<int64_t>(h) << p.page_log2) * D;
+      w = PER == 4 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
+      s = scales[h];
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const float v = id < 0 ? 0.0f : code_value<E4M3>((w >> (8 * e)) & 255u) * s;
+      if (F16) static_cast<__half*>(dst)[at + e] = __float2half_rn(v);
+      else static_cast<float*>(dst)[at + e] = v;
     }
   }
 }
@@ -239,12 +242,16 @@ cudaError_t launch_kv8_append(const Kv8& p, cudaStream_t s) {
 
 cudaError_t launch_kv8_read(const Kv8& p, cudaStream_t s) {
   if (p.tokens == 0 || p.seqs == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.tokens) * p.hkv + 7) / 8), 2);
-  switch ((p.e4m3 ? 2 : 0) | (p.f16 ? 1 : 0)) {
-    case 0: read_kernel<false, false><<<grid, 256, 0, s>>>(p); break;
-    case 1: read_kernel<false, true><<<grid, 256, 0, s>>>(p); break;
-    case 2: read_kernel<true, false><<<grid, 256, 0, s>>>(p); break;
-    default: read_kernel<true, true><<<grid, 256, 0, s>>>(p); break;
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.tokens) + 7) / 8), 2);
+  switch ((p.D == 128 ? 4 : 0) | (p.e4m3 ? 2 : 0) | (p.f16 ? 1 : 0)) {
+    case 0: read_kernel<false, false, 2><<<grid, 256, 0, s>>>(p); break;
+    case 1: read_kernel<false, true, 2><<<grid, 256, 0, s>>>(p); break;
+    case 2: read_kernel<true, false, 2><<<grid, 256, 0, s>>>(p); break;
+    case 3: read_kernel<true, true, 2><<<grid, 256, 0, s>>>(p); break;
+    case 4: read_kernel<false, false, 4><<<grid, 256, 0, s>>>(p); break;
+    case 5: read_kernel<false, true, 4><<<grid, 256, 0, s>>>(p); break;
+    case 6: read_kernel<true, false, 4><<<grid, 256, 0, s>>>(p); break;
+    default: read_kernel<true, true, 4><<<grid, 256, 0, s>>>(p); break;
   }
   return cudaGetLastError();
 }

@@ -22,7 +22,7 @@ struct Kv8 {
   int f16;       // rows: 1 float16, 0 float32
   int e4m3;      // codes: 1 e4m3, 0 int8
   int causal;
-  int zero_rest; // attention: rows of no sequence are set to zero
+  int zero_rest; // attention, read back: rows of no sequence are set to zero
   int few_rows;  // attention: sequences with more rows (tokens x query heads a key/value head) are the prompt kernel's
   int uniform;   // cu_seqlens absent: tokens / sequences rows each
   int tokens, seqs, hq, hkv, D, page, page_log2, pages, max_pages, window;

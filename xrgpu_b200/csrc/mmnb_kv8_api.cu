@@ -33,6 +33,7 @@ int convert(const xrgpu_kv8_problem* c, Need need, Kv8* out) {
   p.hkv = static_cast<int>(c->heads_kv); p.D = static_cast<int>(c->head_dim);
   p.page = static_cast<int>(c->page); p.pages = static_cast<int>(c->pages); p.max_pages = static_cast<int>(c->max_pages);
   while ((1 << p.page_log2) < p.page) ++p.page_log2;
+  p.zero_rest = c->zero_rest != 0;
   p.uniform = c->cu_seqlens == nullptr;
   if (p.uniform && p.seqs > 0 && p.tokens % p.seqs) return fail("tokens must be a multiple of sequences without cu_seqlens");
   const int64_t kv_row = c->heads_kv * c->head_dim;
@@ -42,7 +43,7 @@ int convert(const xrgpu_kv8_problem* c, Need need, Kv8* out) {
     if (c->window < 0 || c->window > INT_MAX) return fail("window must be >= 0");
     if (c->window > 0 && !c->causal) return fail("a window needs causal attention");
     if (!(c->scale >= -3.4028234e38f && c->scale <= 3.4028234e38f)) return fail("scale must be finite");
-    p.hq = static_cast<int>(c->heads_q); p.window = static_cast<int>(c->window); p.causal = c->causal != 0; p.zero_rest = c->zero_rest != 0; p.scale = c->scale;
+    p.hq = static_cast<int>(c->heads_q); p.window = static_cast<int>(c->window); p.causal = c->causal != 0; p.scale = c->scale;
     const int64_t q_row = c->heads_q * c->head_dim;
     p.qs = c->q_stride ? c->q_stride : q_row;
     p.os = c->o_stride ? c->o_stride : q_row;

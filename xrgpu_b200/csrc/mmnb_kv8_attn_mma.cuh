@@ -744,7 +744,7 @@ template <bool E4M3, int D, int NT, bool F32>
 cudaError_t launch_nt(const Kv8& p, void* ws, cudaStream_t s) {
   using C = Traits<E4M3, D, NT, F32>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<E4M3, D, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  cudaError_t e = allow_smem<attn_mma_kernel<E4M3, D, NT, F32>>(C::kSmem);
   if (e != cudaSuccess) return e;
   const int grid = device_sm_count();
   Workspace w{static_cast<int64_t*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + starts_bytes(p.seqs))};

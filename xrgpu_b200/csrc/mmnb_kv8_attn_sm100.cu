@@ -565,10 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
 
 template <bool E4M3, int D>
 cudaError_t launch(const Kv8& p, cudaStream_t s) {
-  const cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<E4M3, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes > 120 * 1024 ? Smem<D>::kBytes : 120 * 1024);
-  if (e != cudaSuccess) return e;
   // one CTA an SM: it takes all tensor memory
-  const int bytes = Smem<D>::kBytes > 120 * 1024 ? Smem<D>::kBytes : 120 * 1024;
+  constexpr int bytes = Smem<D>::kBytes > 120 * 1024 ? Smem<D>::kBytes : 120 * 1024;
+  const cudaError_t e = allow_smem<attn_prompt_kernel<E4M3, D>>(bytes);
+  if (e != cudaSuccess) return e;
   const int64_t G = p.hq / p.hkv, tiles = p.uniform ? ceil_div(p.tokens / p.seqs * G, kRows) * p.seqs : p.tokens * G / kRows + p.seqs;
   attn_prompt_kernel<E4M3, D><<<static_cast<unsigned>(tiles * p.hkv), kThreads, bytes, s>>>(p);
   return cudaGetLastError();

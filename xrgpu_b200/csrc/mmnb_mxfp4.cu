@@ -28,11 +28,10 @@ __device__ __forceinline__ float pow2_of_byte(uint32_t e) {  // 2^(e - 127), e =
   return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(e ? e << 23 : 1u << 22);
 }
 
-// Code (4 bits) to its value.
+// Code (4 bits) to its value: exponent and mantissa bits in place of a float32's make 2^-126 of it (the code
+// without exponent a subnormal, so exactly), the sign bit goes to the top.
 __device__ __forceinline__ float e2m1_value(uint32_t c) {
-  const uint32_t m = c & 7u;
-  const float v = m < 4u ? 0.5f * static_cast<float>(m) : (m < 6u ? static_cast<float>(m) - 2.0f : 2.0f * static_cast<float>(m) - 8.0f);
-  return (c & 8u) ? -v : v;
+  return __uint_as_float(((c & 7u) << 22) | ((c & 8u) << 28)) * __uint_as_float(253u << 23);
 }
 
 constexpr int kQuantWarps = 8;
@@ -51,7 +50,7 @@ __global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Q
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     if (row < p.rows && k0 < p.K) {
-      if (VEC) {
+      if (VEC && k0 + 8 <= p.K) {
         if (F16) {
           const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + row * p.ldx + k0);
           const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -97,19 +96,41 @@ __global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Q
   }
 }
 
-template <bool F16>
-__global__ void __launch_bounds__(256) dequantize_kernel(const Mxfp4Dequantize p) {
-  const int64_t n = p.rows * p.kb;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n * 4; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = (i >> 2) / p.kb, blk = (i >> 2) % p.kb, k0 = blk * 32 + (i & 3) * 8;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(p.codes)[i];
+// Four lanes a block, 8 values each; one word of four scales serves 16 lanes.
+template <bool F16, bool VEC>
+__global__ void __launch_bounds__(kQuantWarps * 32) dequantize_kernel(const Mxfp4Dequantize p, int64_t chunks, int64_t items) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kQuantWarps + (threadIdx.x >> 5); it < items;
+       it += static_cast<int64_t>(gridDim.x) * kQuantWarps) {
+    const int64_t row = it / chunks, k0 = (it % chunks) * kChunk + lane * 8, blk = k0 >> 5;
+    if (blk >= p.kb || k0 >= p.K) continue;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(p.codes + (row * p.kb + blk) * 16)[lane & 3];
     const float s = pow2_of_byte(p.scales[scale_offset(row, blk, p.kb)]);
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (k0 + j >= p.K) break;
-      const float v = e2m1_value((w >> (4 * j)) & 15u) * s;
-      if (F16) static_cast<__half*>(p.out)[row * p.K + k0 + j] = __float2half_rn(v);
-      else static_cast<float*>(p.out)[row * p.K + k0 + j] = v;
+    for (int j = 0; j < 8; ++j) v[j] = e2m1_value((w >> (4 * j)) & 15u) * s;
+    const int64_t at = row * p.K + k0;
+    if (VEC) {
+      if (F16) {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          h[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (k0 + j >= p.K) break;
+        if (F16) static_cast<__half*>(p.out)[at + j] = __float2half_rn(v[j]);
+        else static_cast<float*>(p.out)[at + j] = v[j];
+      }
     }
   }
 }
@@ -135,9 +156,9 @@ cudaError_t launch_mxfp4_quantize(const Mxfp4Quantize& p, cudaStream_t s) {
   const int64_t chunks = ceil_div(p.K, kChunk), rows = ceil_div(p.rows, 128) * 128, items = rows * chunks;
   if (items == 0) return cudaSuccess;
   const int grid = grid_for(ceil_div(items, kQuantWarps), 8);
-  // 16-byte loads of 8 values: the rows' starts and K in whole vectors
+  // 16-byte loads of 8 values (a ragged end of a row is loaded one by one): the rows start on 16 bytes
   const int64_t es = p.f16 ? 2 : 4;
-  const bool vec = aligned16(p.x) && (p.ldx * es) % 16 == 0 && p.K % 8 == 0;
+  const bool vec = aligned16(p.x) && (p.ldx * es) % 16 == 0;
   if (p.f16) {
     if (vec) quantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
     else quantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
@@ -149,11 +170,17 @@ cudaError_t launch_mxfp4_quantize(const Mxfp4Quantize& p, cudaStream_t s) {
 }
 
 cudaError_t launch_mxfp4_dequantize(const Mxfp4Dequantize& p, cudaStream_t s) {
-  const int64_t n = p.rows * p.kb * 4;
-  if (n == 0) return cudaSuccess;
-  const int grid = grid_for(ceil_div(n, 256), 8);
-  if (p.f16) dequantize_kernel<true><<<grid, 256, 0, s>>>(p);
-  else dequantize_kernel<false><<<grid, 256, 0, s>>>(p);
+  const int64_t chunks = ceil_div(p.K, kChunk), items = p.rows * chunks;
+  if (items == 0) return cudaSuccess;
+  const int grid = grid_for(ceil_div(items, kQuantWarps), 8);
+  const bool vec = aligned16(p.out) && p.K % 8 == 0;
+  if (p.f16) {
+    if (vec) dequantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    else dequantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+  } else {
+    if (vec) dequantize_kernel<false, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    else dequantize_kernel<false, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+  }
   return cudaGetLastError();
 }
 

@@ -364,7 +364,7 @@ Shape choose(const Mxfp4Matmul& p, int ksteps, int sms) {
 
 template <bool SWAP, bool F16>
 cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(mxfp4_gemm_kernel<SWAP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t e = allow_smem<mxfp4_gemm_kernel<SWAP, F16>>(kSmemBudget - 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);

@@ -307,13 +307,33 @@ _FLOATS = {torch.float32: _native.FLOAT32, torch.float16: _native.FLOAT16}
 _CACHES = {torch.int8: _native.INT8, torch.float8_e4m3fn: _native.FLOAT8_E4M3}
 
 
-def _launch(device, fn, *args):
-    """fn(*args, stream) on the current stream of `device`, with that device current."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+# Handle of a device's current stream, without the Stream object around it (these calls are launch-bound).
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _launch(index: int, fn, *args):
+    """fn(*args, stream) on the current stream of device `index`, with that device current."""
+    if torch.cuda.current_device() == index:
+        check(fn(*args, _current_stream(index)))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            check(fn(*args, _current_stream(index)))
+
+
+def _device_of(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return index
+
+
+def _on(t: torch.Tensor, name: str, dtype, index: int):
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be a CUDA tensor on cuda:{index}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
 
 
 def _float_code(dtype) -> int:
@@ -344,14 +364,12 @@ def _scale_shape(rows: int, kb: int):
     return (-(-rows // 128), -(-kb // 4), 32, 4, 4)
 
 
-def _require_mxfp4(codes, scales, rows: int, kb: int, name: str, device):
-    for t, n in ((codes, name), (scales, name + "_scales")):
-        _require(t, n, device)
-        if t.dtype != torch.uint8:
-            raise ValueError(f"{n} must be uint8")
+def _require_mxfp4(codes, scales, rows: int, kb: int, name: str, index: int):
+    _on(codes, name, torch.uint8, index)
+    _on(scales, name + "_scales", torch.uint8, index)
     if codes.numel() != rows * kb * 16 or codes.shape[-1] != 16 or codes.dim() < 2:
         raise ValueError(f"{name} must be [..., {kb}, 16] codes")
-    if tuple(scales.shape) != _scale_shape(rows, kb):
+    if scales.shape != _scale_shape(rows, kb):
         raise ValueError(f"{name}_scales must be tiled scales of shape {list(_scale_shape(rows, kb))}")
 
 
@@ -363,16 +381,15 @@ def mxfp4_quantize(x: torch.Tensor):
     the order the tensor cores take them (``mxfp4_tile_scales``). A block that holds a NaN or an infinity reads as NaN.
     """
     dtype = _float_code(x.dtype)
-    if not x.is_cuda:
-        raise ValueError("x must be a CUDA tensor")
-    K = int(x.shape[-1]) if x.dim() else 0
+    index = _device_of(x, "x")
+    K = x.shape[-1] if x.dim() else 0
     if K < 1:
         raise ValueError("x must be [..., K] with K >= 1")
     rows, kb, ldx = x.numel() // K, -(-K // 32), _row_stride(x, "x")
-    codes = torch.empty(tuple(x.shape[:-1]) + (kb, 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_shape(rows, kb), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((*x.shape[:-1], kb, 16), dtype=torch.uint8)
+    scales = x.new_empty(_scale_shape(rows, kb), dtype=torch.uint8)
     t = _native.Mxfp4Tensor_(dtype, 0, rows, K, codes.data_ptr(), scales.data_ptr())
-    _launch(x.device, _native.load().xrgpu_mxfp4_quantize, ctypes.byref(t), x.data_ptr(), ldx)
+    _launch(index, _native.load().xrgpu_mxfp4_quantize, ctypes.byref(t), x.data_ptr(), ldx)
     return codes, scales
 
 
@@ -385,11 +402,11 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, K: Optional[i
     if K < 1 or -(-K // 32) != kb:
         raise ValueError("K does not match the codes")
     rows = codes.numel() // (kb * 16) if kb else 0
-    code = _float_code(dtype)
-    _require_mxfp4(codes, scales, rows, kb, "codes", codes.device)
-    out = torch.empty(tuple(codes.shape[:-2]) + (K,), dtype=dtype, device=codes.device)
+    code, index = _float_code(dtype), _device_of(codes, "codes")
+    _require_mxfp4(codes, scales, rows, kb, "codes", index)
+    out = codes.new_empty((*codes.shape[:-2], K), dtype=dtype)
     t = _native.Mxfp4Tensor_(code, 0, rows, K, codes.data_ptr(), scales.data_ptr())
-    _launch(codes.device, _native.load().xrgpu_mxfp4_dequantize, ctypes.byref(t), out.data_ptr())
+    _launch(index, _native.load().xrgpu_mxfp4_dequantize, ctypes.byref(t), out.data_ptr())
     return out
 
 
@@ -397,10 +414,11 @@ def mxfp4_tile_scales(scales: torch.Tensor) -> torch.Tensor:
     """Scale bytes [rows, kb] (as checkpoints hold them) in the tiled order of ``matmul_mxfp4``."""
     if scales.dim() != 2 or scales.dtype != torch.uint8 or scales.shape[1] < 1:
         raise ValueError("scales must be uint8 [rows, kb]")
-    _require(scales, "scales", scales.device)
-    rows, kb = int(scales.shape[0]), int(scales.shape[1])
-    tiled = torch.empty(_scale_shape(rows, kb), dtype=torch.uint8, device=scales.device)
-    _launch(scales.device, _native.load().xrgpu_mxfp4_tile_scales, rows, kb, scales.data_ptr(), tiled.data_ptr())
+    index = _device_of(scales, "scales")
+    _on(scales, "scales", torch.uint8, index)
+    rows, kb = scales.shape
+    tiled = scales.new_empty(_scale_shape(rows, kb))
+    _launch(index, _native.load().xrgpu_mxfp4_tile_scales, rows, kb, scales.data_ptr(), tiled.data_ptr())
     return tiled
 
 
@@ -413,92 +431,89 @@ def matmul_mxfp4(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias:
     [..., K], which the call quantises first. Y [..., N] in `dtype` (default a's, float16 for codes); bias [N] in it.
     ``out`` may be a [..., N] view with unit column stride and rows at one stride.
     """
-    dev = a.device
+    index = _device_of(a, "a")
     held = a_scales is not None
     if b.dim() != 3:
         raise ValueError("b must be [N, kb, 16] codes")
-    N, kb = int(b.shape[0]), int(b.shape[1])
-    p = _native.Mxfp4Problem_()
+    N, kb = b.shape[0], b.shape[1]
+    lda = ldy = nbytes = 0
+    bias_ptr = scales_ptr = ws = None
     if held:
-        lead = tuple(a.shape[:-2])
+        lead = a.shape[:-2]
         M = a.numel() // (kb * 16) if kb else 0
         K = kb * 32 if K is None else int(K)
-        _require_mxfp4(a, a_scales, M, kb, "a", dev)
-        p.a_dtype, p.a_scales = _native.UINT8, a_scales.data_ptr()
+        _require_mxfp4(a, a_scales, M, kb, "a", index)
+        a_code, scales_ptr = _native.UINT8, a_scales.data_ptr()
         dtype = torch.float16 if dtype is None else dtype
     else:
-        if not a.is_cuda:
-            raise ValueError("a must be a CUDA tensor")
-        p.a_dtype = _float_code(a.dtype)
-        lead = tuple(a.shape[:-1])
-        if K is not None and int(K) != a.shape[-1]:
+        a_code = _float_code(a.dtype)
+        lead = a.shape[:-1]
+        if K is not None and K != a.shape[-1]:
             raise ValueError("K does not match a")
-        K = int(a.shape[-1])
+        K = a.shape[-1]
         M = a.numel() // K if K else 0
-        p.lda = _row_stride(a, "a")
+        lda = _row_stride(a, "a")
         dtype = a.dtype if dtype is None else dtype
     if K < 1 or -(-K // 32) != kb:
         raise ValueError("a and b differ in K")
-    _require_mxfp4(b, b_scales, N, kb, "b", dev)
-    p.dtype, p.M, p.K, p.N = _float_code(dtype), M, K, N
+    _require_mxfp4(b, b_scales, N, kb, "b", index)
+    code = _float_code(dtype)
     if bias is not None:
-        _require(bias, "bias", dev)
-        if bias.dtype != dtype or tuple(bias.shape) != (N,):
+        _on(bias, "bias", dtype, index)
+        if bias.shape != (N,):
             raise ValueError("bias must be [N] in the output dtype")
-        p.bias = bias.data_ptr()
+        bias_ptr = bias.data_ptr()
     if out is None:
-        out = torch.empty(lead + (N,), dtype=dtype, device=dev)
+        out = a.new_empty((*lead, N), dtype=dtype)
     else:
-        if out.dtype != dtype or out.device != dev or tuple(out.shape) != lead + (N,):
+        if out.dtype != dtype or out.get_device() != index or out.shape != (*lead, N):
             raise ValueError("out must be [..., N] in the output dtype on a's device")
-        p.ldy = _row_stride(out, "out")
-    p.a, p.b, p.b_scales, p.y = a.data_ptr(), b.data_ptr(), b_scales.data_ptr(), out.data_ptr()
-    ws, nbytes = None, 0
+        ldy = _row_stride(out, "out")
+    p = _native.Mxfp4Problem_(code, a_code, M, K, N, a.data_ptr(), scales_ptr, lda, b.data_ptr(), b_scales.data_ptr(), bias_ptr,
+                              out.data_ptr(), ldy)
     if not held and M:
         nbytes = -(-M * kb * 16 // 256) * 256 + -(-M // 128) * -(-kb // 4) * 512
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, _native.load().xrgpu_mxfp4_forward, ctypes.byref(p), ws.data_ptr() if ws is not None else None, nbytes)
+        scratch = a.new_empty(nbytes, dtype=torch.uint8)
+        ws = scratch.data_ptr()
+    _launch(index, _native.load().xrgpu_mxfp4_forward, ctypes.byref(p), ws, nbytes)
     return out
 
 
 def _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, dtype):
-    dev = k_cache.device
-    if k_cache.dtype not in _CACHES or v_cache.dtype != k_cache.dtype:
+    """The cache's part of a call, checked, and its device."""
+    code = k_cache.dtype
+    if code not in _CACHES:
         raise ValueError("k_cache and v_cache must both be int8 or float8_e4m3fn")
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError("k_cache and v_cache must be [pages, heads, page, head_dim]")
+    index = _device_of(k_cache, "k_cache")
     P, H, page, D = k_cache.shape
-    for t, name, dt in ((k_cache, "k_cache", k_cache.dtype), (v_cache, "v_cache", k_cache.dtype),
-                        (k_scale, "k_scale", torch.float32), (v_scale, "v_scale", torch.float32),
-                        (page_table, "page_table", torch.int32), (kv_len, "kv_len", torch.int32),
-                        (cu_seqlens, "cu_seqlens", torch.int32)):
-        if t is None and name == "cu_seqlens":
-            continue
-        _require(t, name, dev)
-        if t.dtype != dt:
-            raise ValueError(f"{name} must be {dt}")
+    _on(k_cache, "k_cache", code, index)
+    _on(v_cache, "v_cache", code, index)
+    _on(k_scale, "k_scale", torch.float32, index)
+    _on(v_scale, "v_scale", torch.float32, index)
+    _on(page_table, "page_table", torch.int32, index)
+    _on(kv_len, "kv_len", torch.int32, index)
     if k_scale.shape != (P, H) or v_scale.shape != (P, H):
         raise ValueError("k_scale and v_scale must be [pages, heads]")
-    B = int(kv_len.shape[0]) if kv_len.dim() == 1 else -1
-    if B < 0 or page_table.dim() != 2 or page_table.shape[0] != B:
+    if kv_len.dim() != 1 or page_table.dim() != 2 or page_table.shape[0] != kv_len.shape[0]:
         raise ValueError("page_table must be [sequences, max_pages] and kv_len [sequences]")
-    if cu_seqlens is not None and tuple(cu_seqlens.shape) != (B + 1,):
-        raise ValueError("cu_seqlens must be [sequences + 1]")
-    p = _native.Kv8Problem_()
-    p.dtype, p.cache_dtype = _float_code(dtype), _CACHES[k_cache.dtype]
-    p.sequences, p.heads_kv, p.head_dim, p.page, p.pages, p.max_pages = B, H, D, page, P, page_table.shape[1]
-    p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-    p.page_table, p.kv_len = page_table.data_ptr(), kv_len.data_ptr()
+    B, cu = kv_len.shape[0], None
     if cu_seqlens is not None:
-        p.cu_seqlens = cu_seqlens.data_ptr()
-    return p
+        _on(cu_seqlens, "cu_seqlens", torch.int32, index)
+        if cu_seqlens.shape != (B + 1,):
+            raise ValueError("cu_seqlens must be [sequences + 1]")
+        cu = cu_seqlens.data_ptr()
+    p = _native.Kv8Problem_(_float_code(dtype), _CACHES[code], 0, 0.0, 0, 0, 0, B, 0, H, D, page, P, page_table.shape[1], 0, 0, 0, 0, 0,
+                            None, None, None, None, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                            v_scale.data_ptr(), page_table.data_ptr(), cu, kv_len.data_ptr())
+    return p, index, H, D
 
 
-def _head_rows(t, name: str, heads: Optional[int], D: int, device) -> int:
+def _head_rows(t, name: str, heads: Optional[int], D: int, index: int) -> int:
     """Row stride of [rows, heads, D] whose rows may be strided, heads and values side by side."""
-    if not t.is_cuda or t.device != device:
-        raise ValueError(f"{name} must be a CUDA tensor on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be a CUDA tensor on cuda:{index}")
     if t.dim() != 3 or t.shape[2] != D or (heads is not None and t.shape[1] != heads):
         raise ValueError(f"{name} must be [rows, heads, head_dim]")
     H = t.shape[1]
@@ -521,14 +536,13 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     rescaled. A page shared by two sequences must not be appended to. Bad page ids and lengths: ``device_error``
     0x501, 0x502, nothing written for them.
     """
-    p = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, k.dtype)
-    dev = k_cache.device
-    p.k_stride = _head_rows(k, "k", p.heads_kv, p.head_dim, dev)
-    p.v_stride = _head_rows(v, "v", p.heads_kv, p.head_dim, dev)
+    p, index, H, D = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, k.dtype)
+    p.k_stride = _head_rows(k, "k", H, D, index)
+    p.v_stride = _head_rows(v, "v", H, D, index)
     if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
         raise ValueError("k and v must have the same rows and dtype")
     p.tokens, p.k, p.v = k.shape[0], k.data_ptr(), v.data_ptr()
-    _launch(dev, _native.load().xrgpu_kv8_append, ctypes.byref(p))
+    _launch(index, _native.load().xrgpu_kv8_append, ctypes.byref(p))
 
 
 def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -536,12 +550,11 @@ def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
              dtype=torch.float16):
     """The values (k, v), each [rows, heads, head_dim], that the cache holds for the last tokens of each sequence
     (rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1; see ``kv8_append``). Rows of no sequence are zero."""
-    p = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, dtype)
-    dev = k_cache.device
-    k = torch.zeros((int(rows), p.heads_kv, p.head_dim), dtype=dtype, device=dev)
-    v = torch.zeros_like(k)
-    p.tokens, p.k, p.v = int(rows), k.data_ptr(), v.data_ptr()
-    _launch(dev, _native.load().xrgpu_kv8_read, ctypes.byref(p))
+    p, index, H, D = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, dtype)
+    k = k_scale.new_empty((int(rows), H, D), dtype=dtype)
+    v = torch.empty_like(k)
+    p.tokens, p.k, p.v, p.zero_rest = int(rows), k.data_ptr(), v.data_ptr(), 1
+    _launch(index, _native.load().xrgpu_kv8_read, ctypes.byref(p))
     return k, v
 
 
@@ -556,21 +569,21 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     head h reads key/value head h // (query heads // heads). scale defaults to head_dim ** -0.5. A row that sees nothing
     gives zeros; with ``out``, rows behind the last sequence are left as they were (without it they are zero).
     """
-    p = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, q.dtype)
-    dev = k_cache.device
-    p.q_stride = _head_rows(q, "q", None, p.head_dim, dev)
+    p, index, H, D = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, q.dtype)
+    p.q_stride = _head_rows(q, "q", None, D, index)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         p.zero_rest = 1
-    elif out.dtype != q.dtype or out.shape != q.shape:
-        raise ValueError("out must have q's shape and dtype")
-    p.o_stride = _head_rows(out, "out", q.shape[1], p.head_dim, dev)
+    else:
+        if out.dtype != q.dtype or out.shape != q.shape:
+            raise ValueError("out must have q's shape and dtype")
+        p.o_stride = _head_rows(out, "out", q.shape[1], D, index)
     p.tokens, p.heads_q, p.q, p.o = q.shape[0], q.shape[1], q.data_ptr(), out.data_ptr()
     p.causal, p.window = int(bool(causal)), int(window)
-    p.scale = float(scale) if scale is not None else p.head_dim ** -0.5
+    p.scale = float(scale) if scale is not None else D ** -0.5
     lib = _native.load()
     need = ctypes.c_uint64(0)
     check(lib.xrgpu_kv8_attention_workspace_size(ctypes.byref(p), ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-    _launch(dev, lib.xrgpu_kv8_attention, ctypes.byref(p), ws.data_ptr() if ws is not None else None, need.value)
+    ws = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    _launch(index, lib.xrgpu_kv8_attention, ctypes.byref(p), ws.data_ptr() if ws is not None else None, need.value)
     return out
