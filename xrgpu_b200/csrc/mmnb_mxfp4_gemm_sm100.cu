@@ -38,7 +38,7 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = (2 + kEpilogueWarps) * 32;
 constexpr int kTmemCols = 512;
 constexpr int kSmemBudget = 227 * 1024;
-constexpr int kPitch = kRows + 1;       // floats a column of a partial tile in shared memory
+constexpr int kPitch = kRows + 4;       // floats a column of a partial tile in shared memory
 
 constexpr unsigned kErrWaitProducer = 0x601;
 constexpr unsigned kErrWaitMma = 0x602;
@@ -93,11 +93,11 @@ __device__ __forceinline__ uint32_t instruction_desc(int T, uint32_t half) {
          (static_cast<uint32_t>(kRows >> 4) << 24) | (half << 29);
 }
 
-template <bool SWAP, bool F16>
+template <bool SWAP, bool F16, int QB>
 __global__ void __launch_bounds__(kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
   extern __shared__ uint8_t smem_raw[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int S = a.stages;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
@@ -191,50 +191,60 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int h = (g > S ? g - S : 0); h < g; ++h) drain_wait(&full[h % S], (h / S) & 1, a.err, kErrDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
-      const uint64_t s_desc = plain_desc(base + kRows * kStepBytes + a.q_stage);
-      const uint32_t i_desc[2] = {instruction_desc(a.T, 0u), instruction_desc(a.T, 2u)};
-      int i = 0, s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
-        // Overlapping accumulators: the shared columns of tile i - 1 are out; separate ones: tile i - 2 is.
-        const int w = a.shared_cols ? i - 1 : i - 2;
-        if (w >= 0 && !thread_wait(&drained[w & 1], (w >> 1) & 1, ctl, kErrWaitMma)) break;
-        tc_fence_after();
-        const int qt = tile / a.p_tiles;
-        const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
-        const uint32_t q_first = (qt * a.T % kRows) >> 5;  // column of the tile's first row within its row block
-        for (int ks = k0; ks < k1; ++ks) {
-          if (!thread_wait(&full[s], ph, ctl, kErrWaitMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const int subs = min(4, a.k64 - 4 * ks), groups = (subs + 1) >> 1;
-          const uint32_t off = static_cast<uint32_t>(s) * (a.stage >> 4);
-          const uint32_t sf = tmem + a.sf_col + s * a.sf_stage;
-          // columns: P group 0, P group 1, Q group 0 (4 a row block), Q group 1
-          for (int gr = 0; gr < groups; ++gr) {
-            scales_to_tmem(sf + 4 * gr, s_desc + off + gr * (kScaleTile >> 4));
-            for (int b = 0; b < a.q_blocks; ++b)
-              scales_to_tmem(sf + 8 + 4 * (gr * a.q_blocks + b), s_desc + off + ((1 + b) * 2 + gr) * (kScaleTile >> 4));
-          }
-          for (int j = 0; j < subs; ++j)
-            mma_mxf4(d, p_desc + off + 2 * j, q_desc + off + 2 * j, i_desc[j & 1], sf + 4 * (j >> 1),
-                     sf + 8 + 4 * (j >> 1) * a.q_blocks + q_first, ks > k0 || j > 0);
-          mma_commit(&empty[s]);
-          if (++s == S) {
-            s = 0;
-            ph ^= 1;
-          }
+    // The warp stays converged and elects the issuing lane, so that descriptors stay in uniform registers: with one
+    // lane in a branch of its own each tcgen05 instruction took 100 cycles to issue (a step 1700 instead of 600).
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+    const uint64_t s_desc = plain_desc(base + kRows * kStepBytes + a.q_stage);
+    const uint32_t i_desc0 = instruction_desc(a.T, 0u), i_desc1 = instruction_desc(a.T, 2u);
+    int i = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
+      // Overlapping accumulators: the shared columns of tile i - 1 are out; separate ones: tile i - 2 is.
+      const int w = a.shared_cols ? i - 1 : i - 2;
+      if (w >= 0 && !warp_spin(&drained[w & 1], (w >> 1) & 1, ctl, kErrWaitMma)) break;
+      const int qt = tile / a.p_tiles;
+      const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
+      const uint32_t q_first = (qt * a.T % kRows) >> 5;  // column of the tile's first row within its row block
+      for (int ks = k0; ks < k1; ++ks) {
+        if (!warp_spin(&full[s], ph, ctl, kErrWaitMma)) {
+          ok = false;
+          break;
         }
-        if (ok) mma_commit(&accfull[i & 1]);
+        tc_fence_after();
+        const int subs = a.k64 - 4 * ks;  // 64-value MMA steps left
+        const uint32_t off = static_cast<uint32_t>(s) * (a.stage >> 4);
+        const uint32_t sf = tmem + a.sf_col + s * a.sf_stage;
+        if (elect_one()) {
+          // columns: P group 0, P group 1, Q group 0 (4 a row block), Q group 1
+#pragma unroll
+          for (int gr = 0; gr < 2; ++gr) {
+            if (gr == 1 && subs <= 2) break;
+            scales_to_tmem(sf + 4 * gr, s_desc + off + gr * (kScaleTile >> 4));
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+              scales_to_tmem(sf + 8 + 4 * (gr * QB + b), s_desc + off + ((1 + b) * 2 + gr) * (kScaleTile >> 4));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j > 0 && j >= subs) break;
+            mma_mxf4(d, p_desc + off + 2 * j, q_desc + off + 2 * j, (j & 1) ? i_desc1 : i_desc0, sf + 4 * (j >> 1),
+                     sf + 8 + 4 * (j >> 1) * QB + q_first, ks > k0 || j > 0);
+          }
+          mma_commit(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == S) {
+          s = 0;
+          ph ^= 1;
+        }
       }
-      mma_commit(&done);  // every MMA and copy of this thread has completed once `done` flips
-      drain_wait(&done, 0, a.err, kErrDrain);
+      if (ok && elect_one()) mma_commit(&accfull[i & 1]);
+      __syncwarp();
     }
+    if (elect_one()) mma_commit(&done);  // every MMA and copy of this warp has completed once `done` flips
+    __syncwarp();
+    drain_wait(&done, 0, a.err, kErrDrain);
   } else {
     const int q = warp & 3, c = (warp - 2) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
@@ -321,18 +331,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     // one tile a cluster: every rank sums its share of the rows of P (SWAP: columns of y) over the ranks
     cluster_sync();
     const int pt = first % a.p_tiles, qt = first / a.p_tiles, share = kRows / a.split, p0 = rank * share;
-    const int cols = min(a.T, a.q_rows - qt * a.T);
-    for (int e = threadIdx.x; e < share * cols; e += kThreads) {
-      // consecutive threads along the columns n of y
-      const int col = SWAP ? e / share : e % cols, row = p0 + (SWAP ? e % share : e / cols);
-      const int p = pt * kRows + row, qq = qt * a.T + col;
-      if (p >= a.p_rows) continue;
-      float r = 0.0f;
-      for (int k = 0; k < a.split; ++k) r += ld_cluster_f32(map_rank(base + (col * kPitch + row) * 4, k));
-      const int64_t m = SWAP ? qq : p, n = SWAP ? p : qq;
-      if (a.bias) r += load_f(a.bias, F16, n);
-      if (F16) static_cast<__half*>(a.y)[m * a.ldy + n] = __float2half_rn(r);
-      else static_cast<float*>(a.y)[m * a.ldy + n] = r;
+    const int cols = min(a.T, a.q_rows - qt * a.T), quads = share / 4;
+    for (int e = threadIdx.x; e < quads * cols; e += kThreads) {
+      // four rows of P a thread; consecutive threads along the columns n of y
+      const int col = SWAP ? e / quads : e % cols, row = p0 + 4 * (SWAP ? e % quads : e / cols);
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < a.split) v[k] = ld_cluster_f32x4(map_rank(base + (col * kPitch + row) * 4, k));
+      float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < a.split) {
+          r[0] += v[k].x;
+          r[1] += v[k].y;
+          r[2] += v[k].z;
+          r[3] += v[k].w;
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = pt * kRows + row + i, qq = qt * a.T + col;
+        if (p >= a.p_rows) break;
+        const int64_t m = SWAP ? qq : p, n = SWAP ? p : qq;
+        const float y = a.bias ? r[i] + load_f(a.bias, F16, n) : r[i];
+        if (F16) static_cast<__half*>(a.y)[m * a.ldy + n] = __float2half_rn(y);
+        else static_cast<float*>(a.y)[m * a.ldy + n] = y;
+      }
     }
     cluster_sync();  // nobody leaves while its partial tile is being read
   }
@@ -362,9 +386,9 @@ Shape choose(const Mxfp4Matmul& p, int ksteps, int sms) {
   return s;
 }
 
-template <bool SWAP, bool F16>
+template <bool SWAP, bool F16, int QB>
 cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
-  cudaError_t e = allow_smem<mxfp4_gemm_kernel<SWAP, F16>>(kSmemBudget - 1024);
+  cudaError_t e = allow_smem<mxfp4_gemm_kernel<SWAP, F16, QB>>(kSmemBudget - 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
@@ -385,7 +409,7 @@ cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, 
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<SWAP, F16>, mp, mq, a);
+  return cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<SWAP, F16, QB>, mp, mq, a);
 }
 
 }  // namespace
@@ -425,6 +449,11 @@ cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s
   int stages = (kSmemBudget - 2048) / static_cast<int>(a.stage);
   if (stages > 12) stages = 12;
   if (one_tile && stages > steps) stages = steps;
+  if (a.split > 1) {  // all CTAs at once: those that share an SM share its memory
+    const int together = static_cast<int>(ceil_div(static_cast<int64_t>(a.tiles) * a.split, sms));
+    const int fit = (kSmemBudget / together - 2048) / static_cast<int>(a.stage);
+    if (stages > fit && fit >= 2) stages = fit;
+  }
   size_t smem = static_cast<size_t>(stages) * a.stage;
   if (a.split > 1 && smem < static_cast<size_t>(a.T) * kPitch * 4) smem = static_cast<size_t>(a.T) * kPitch * 4;
   smem += 1024;
@@ -447,8 +476,9 @@ cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s
   if (!encode_tensor_map_2d(&mp, 0, sh.swap ? p.b : p.a, row, a.p_rows, row, kStepBytes, kRows, true) ||
       !encode_tensor_map_2d(&mq, 0, sh.swap ? p.a : p.b, row, a.q_rows, row, kStepBytes, a.T, true))
     return cudaErrorInvalidValue;
-  if (sh.swap) return p.f16 ? launch<true, true>(mp, mq, a, grid, smem, early, s) : launch<true, false>(mp, mq, a, grid, smem, early, s);
-  return p.f16 ? launch<false, true>(mp, mq, a, grid, smem, early, s) : launch<false, false>(mp, mq, a, grid, smem, early, s);
+  if (sh.swap) return p.f16 ? launch<true, true, 1>(mp, mq, a, grid, smem, early, s) : launch<true, false, 1>(mp, mq, a, grid, smem, early, s);
+  if (a.q_blocks == 1) return p.f16 ? launch<false, true, 1>(mp, mq, a, grid, smem, early, s) : launch<false, false, 1>(mp, mq, a, grid, smem, early, s);
+  return p.f16 ? launch<false, true, 2>(mp, mq, a, grid, smem, early, s) : launch<false, false, 2>(mp, mq, a, grid, smem, early, s);
 }
 
 }  // namespace xrgpu

@@ -128,6 +128,26 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// Bounded spin of a converged warp (latency-critical, unlike warp_wait).
+__device__ __forceinline__ bool warp_spin(uint64_t* bar, uint32_t parity, const Ctl& c, unsigned code) {
+  uint64_t start = 0;
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < kSpins; ++i)
+      if (__all_sync(~0u, mbar_test_wait(bar, parity))) return true;
+    if (__any_sync(~0u, *c.abort != 0)) return false;
+    const uint64_t now = __shfl_sync(~0u, global_timer_ns(), 0);
+    if (start == 0) start = now;
+    if (now - start > kWaitLimitNs) {
+      if ((threadIdx.x & 31) == 0) {
+        record_device_error(c.err, code);
+        *c.abort = 1;
+      }
+      return false;
+    }
+  }
+}
+
 // Whole-warp bounded wait (dequant and epilogue warps): every lane observes the phase and the
 // warp agrees on the outcome, so the .sync.aligned tcgen05 instructions after it stay
 // converged; the probes suspend the warp in hardware, leaving issue slots to the producer and
@@ -227,9 +247,9 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
