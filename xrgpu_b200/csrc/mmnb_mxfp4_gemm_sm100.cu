@@ -14,7 +14,8 @@
 // accumulators (lane quadrant warp % 4, alternate 16-column chunks).
 //
 // Tensor memory: two accumulators of T columns at 0 and acc1, then per stage the scale columns: 4 columns
-// (32 lanes x 4 bytes x 4 row groups) for 128 rows x 128 values. A stage's columns are rewritten only when
+// (32 lanes x 4 bytes x 4 row groups) for 128 rows x 128 values. Q tiles begin at a row block (one tile, or T a multiple of
+// 128), so that their scales begin at a column that is a multiple of 4: other starts are not taken. A stage's columns are rewritten only when
 // its shared-memory buffer has come back, that is when the MMAs that read them are done. With T = 256 two
 // accumulators and the scales need more than the 512 columns: the accumulators then overlap, and the
 // drain starts with the shared columns, after which the next tile may start.
@@ -38,7 +39,7 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = (2 + kEpilogueWarps) * 32;
 constexpr int kTmemCols = 512;
 constexpr int kSmemBudget = 227 * 1024;
-constexpr int kPitch = kRows + 4;       // floats a column of a partial tile in shared memory
+constexpr int kPitch = kRows;           // floats a column of a partial tile in shared memory
 
 constexpr unsigned kErrWaitProducer = 0x601;
 constexpr unsigned kErrWaitMma = 0x602;
@@ -203,9 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Overlapping accumulators: the shared columns of tile i - 1 are out; separate ones: tile i - 2 is.
       const int w = a.shared_cols ? i - 1 : i - 2;
       if (w >= 0 && !warp_spin(&drained[w & 1], (w >> 1) & 1, ctl, kErrWaitMma)) break;
-      const int qt = tile / a.p_tiles;
       const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
-      const uint32_t q_first = (qt * a.T % kRows) >> 5;  // column of the tile's first row within its row block
       for (int ks = k0; ks < k1; ++ks) {
         if (!warp_spin(&full[s], ph, ctl, kErrWaitMma)) {
           ok = false;
@@ -229,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 4; ++j) {
             if (j > 0 && j >= subs) break;
             mma_mxf4(d, p_desc + off + 2 * j, q_desc + off + 2 * j, (j & 1) ? i_desc1 : i_desc0, sf + 4 * (j >> 1),
-                     sf + 8 + 4 * (j >> 1) * QB + q_first, ks > k0 || j > 0);
+                     sf + 8 + 4 * (j >> 1) * QB, ks > k0 || j > 0);
           }
           mma_commit(&empty[s]);
         }
@@ -328,13 +327,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
   }
   if (a.split > 1) {
-    // one tile a cluster: every rank sums its share of the rows of P (SWAP: columns of y) over the ranks
+    // one tile a cluster: every rank sums its share of the columns over the ranks (128 floats of a column lie together),
+    // in their order; y's rows run along P for SWAP, else the sums turn round in shared memory
     cluster_sync();
-    const int pt = first % a.p_tiles, qt = first / a.p_tiles, share = kRows / a.split, p0 = rank * share;
-    const int cols = min(a.T, a.q_rows - qt * a.T), quads = share / 4;
-    for (int e = threadIdx.x; e < quads * cols; e += kThreads) {
-      // four rows of P a thread; consecutive threads along the columns n of y
-      const int col = SWAP ? e / quads : e % cols, row = p0 + 4 * (SWAP ? e % quads : e / cols);
+    const int pt = first % a.p_tiles, qt = first / a.p_tiles;
+    const int cols = min(a.T, a.q_rows - qt * a.T), share = (cols + a.split - 1) / a.split;
+    const int col0 = rank * share, mine = max(0, min(share, cols - col0));
+    float* turned = reinterpret_cast<float*>(gbase) + a.T * kPitch;  // [128][share + 1]
+    for (int e = threadIdx.x; e < mine * (kRows / 4); e += kThreads) {
+      const int col = col0 + e / (kRows / 4), row = 4 * (e % (kRows / 4));
       float4 v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -348,14 +349,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           r[2] += v[k].z;
           r[3] += v[k].w;
         }
+      if (SWAP) {
+        const int64_t n = pt * kRows + row, at = static_cast<int64_t>(qt * a.T + col) * a.ldy + n;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int p = pt * kRows + row + i, qq = qt * a.T + col;
-        if (p >= a.p_rows) break;
-        const int64_t m = SWAP ? qq : p, n = SWAP ? p : qq;
-        const float y = a.bias ? r[i] + load_f(a.bias, F16, n) : r[i];
-        if (F16) static_cast<__half*>(a.y)[m * a.ldy + n] = __float2half_rn(y);
-        else static_cast<float*>(a.y)[m * a.ldy + n] = y;
+        for (int i = 0; i < 4; ++i) {
+          if (n + i >= a.p_rows) break;
+          const float y = a.bias ? r[i] + load_f(a.bias, F16, n + i) : r[i];
+          if (F16) static_cast<__half*>(a.y)[at + i] = __float2half_rn(y);
+          else static_cast<float*>(a.y)[at + i] = y;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turned[(row + i) * (share + 1) + col - col0] = r[i];
+      }
+    }
+    if (!SWAP) {
+      __syncthreads();
+      const int rows = min(kRows, a.p_rows - pt * kRows);
+      for (int e = threadIdx.x; e < rows * mine; e += kThreads) {
+        const int row = e / mine, col = e % mine;
+        const int64_t n = qt * a.T + col0 + col, at = static_cast<int64_t>(pt * kRows + row) * a.ldy + n;
+        const float r = turned[row * (share + 1) + col], y = a.bias ? r + load_f(a.bias, F16, n) : r;
+        if (F16) static_cast<__half*>(a.y)[at] = __float2half_rn(y);
+        else static_cast<float*>(a.y)[at] = y;
       }
     }
     cluster_sync();  // nobody leaves while its partial tile is being read
@@ -368,21 +384,25 @@ struct Shape {
   int T, split;
 };
 
-// Up to 128 activation rows: all of them in one tile, K split until the CTAs cover the SMs. More: tiles of
-// 256 columns, narrower ones and a split of K where that leaves SMs idle.
+// Up to 128 activation rows: all of them in one tile. K is split while the CTAs find an SM each (narrow tiles: 1.6
+// CTAs an SM, they run side by side); beyond that a split costs more than it gives. Measured (us, split 1 / 2 / 4 / 8):
+// 1 x 4096 x 4096 9.4 / 7.6 / 6.4 / 6.9; 16 x 14336 x 4096 10.1 / 8.6 / 13.2 / 18.7; 128 x 4096 x 4096 11.9 / 10.9 / 8.9 / 12.4.
+// More rows: tiles of 128 or 256 columns by rounds x (columns + 128), a step's fixed cost being that of 128 columns:
+// 256 x 14336 x 4096 19.1 (128) / 15.9 (256), 512 x 4096 x 4096 12.6 / 15.3; narrow ones split like the above.
 Shape choose(const Mxfp4Matmul& p, int ksteps, int sms) {
   Shape s{p.M <= kRows, 256, 1};
-  int64_t tiles;
+  int64_t tiles, most = sms;
   if (s.swap) {
     s.T = static_cast<int>(align_up(p.M, 16));
     tiles = ceil_div(p.N, kRows);
+    if (s.T <= 64) most = sms * 8 / 5;
   } else {
-    const int64_t pt = ceil_div(p.M, kRows);
-    if (pt * ceil_div(p.N, 256) < sms) s.T = 128;
-    tiles = pt * ceil_div(p.N, s.T);
+    const int64_t pt = ceil_div(p.M, kRows), narrow = pt * ceil_div(p.N, 128), wide = pt * ceil_div(p.N, 256);
+    if (ceil_div(narrow, sms) * (128 + 128) < ceil_div(wide, sms) * (256 + 128)) s.T = 128;
+    tiles = s.T == 128 ? narrow : wide;
   }
   if (s.T <= 128)
-    while (s.split < 8 && tiles * s.split * 2 <= 2 * sms && ksteps >= 4 * s.split) s.split *= 2;
+    while (s.split < 8 && tiles * s.split * 2 <= most && ksteps >= 4 * s.split) s.split *= 2;
   return s;
 }
 
@@ -455,7 +475,8 @@ cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s
     if (stages > fit && fit >= 2) stages = fit;
   }
   size_t smem = static_cast<size_t>(stages) * a.stage;
-  if (a.split > 1 && smem < static_cast<size_t>(a.T) * kPitch * 4) smem = static_cast<size_t>(a.T) * kPitch * 4;
+  const size_t partial = (static_cast<size_t>(a.T) * kPitch + kRows * (ceil_div(a.T, a.split) + 1)) * 4;
+  if (a.split > 1 && smem < partial) smem = partial;
   smem += 1024;
   a.stages = stages;
   // Tensor memory: accumulators, then the stages' scales.
