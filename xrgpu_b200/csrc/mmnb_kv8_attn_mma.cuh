@@ -17,7 +17,7 @@
 // as pairs of float16 numbers (22 bits) and signed codes.
 //
 // Order in memory. A step is 32 tokens of keys and values, copied by a warp with 16-byte cp.async into its own ring
-// of kStages buffers. 16-byte chunk c of row r lies at c ^ f(r), f(r) = (r & 7) ^ 4 (r & 1) for 128-byte rows (two
+// of two or three buffers. 16-byte chunk c of row r lies at c ^ f(r), f(r) = (r & 7) ^ 4 (r & 1) for 128-byte rows (two
 // 64-byte rows share a line, see chunk_at): copies and both operand reads touch all banks once.
 //
 // Balance. The steps of all segments form one sequence; every CTA takes an equal run of it, found from the
@@ -33,10 +33,7 @@
 namespace xrgpu {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32;    // tokens a warp takes at a time
-constexpr int kStages = 3;
 constexpr float kRaise = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -165,15 +162,18 @@ struct Workspace {
 __host__ __device__ inline int64_t part_floats(int rows, int D) { return static_cast<int64_t>(rows) * (D + 2); }
 __host__ __device__ inline int64_t starts_bytes(int seqs) { return (static_cast<int64_t>(seqs) + 1) * 8 / 256 * 256 + 256; }
 
-__device__ __forceinline__ int64_t run_length(int64_t total, int grid) {
+// Steps of a CTA's run: an equal share, one a warp at least.
+__device__ __forceinline__ int64_t run_length(int64_t total, int grid, int warps) {
   const int64_t q = (total + grid - 1) / grid;
-  return q < kWarps ? kWarps : q;
+  return q < warps ? warps : q;
 }
 
 // ------------------------------------------------------------------ main kernel
 template <bool E4M3, int D, int NT, bool F32>
 struct Traits {
   static constexpr int kRows = 8 * NT;
+  // One tile of rows leaves registers for 12 warps, whose rings then hold two steps; more rows for 8 with three.
+  static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = kWarps * 32, kStages = NT == 1 ? 2 : 3;
   static constexpr int kK = D / 16;                   // k steps of the scores
   static constexpr int kMt = D / 16;                  // 16-dim tiles of the output
   static constexpr int kTile = kStep * D;             // bytes of a step's keys (or values)
@@ -188,8 +188,9 @@ struct Traits {
 };
 
 template <bool E4M3, int D, int NT, bool F32>
-__global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Workspace ws) {
+__global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mma_kernel(const Kv8 p, Workspace ws) {
   using C = Traits<E4M3, D, NT, F32>;
+  constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t scan[kWarps + 1];
   __shared__ int64_t found_at;
@@ -208,11 +209,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Work
   float* warp_m = reinterpret_cast<float*>(row_lo + R);                              // [kWarps][R]
   float* warp_l = warp_m + kWarps * R;
 
-  // ---- all steps, this CTA's run of them, and the sequence it starts in
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
-    const int b = b0 + tid;
-    int64_t v = b < p.seqs ? seq_total(p, seq_work(p, b, R)) : 0, sum = v;
+  // ---- all steps, this CTA's run of them, and the sequence it starts in (kThreads sequences at a time; a second pass
+  // finds the start among more)
+  auto prefix = [&](int64_t v, int64_t* all) {  // exclusive prefix sum over the threads, and the sum
+    int64_t sum = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t o = __shfl_up_sync(~0u, sum, d);
@@ -220,40 +220,41 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Work
     }
     if (lane == 31) scan[warp] = sum;
     __syncthreads();
-    int64_t all = 0;
+    int64_t before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) sum += scan[w];
-      all += scan[w];
+      if (w < warp) before += scan[w];
+      total += scan[w];
     }
-    if (blockIdx.x == 0 && b < p.seqs) ws.start[b] = total + sum - v;
+    *all = total;
+    return before + sum - v;
+  };
+  int64_t total = 0, mine_v = 0, mine_at = 0;
+  for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
+    const int b = b0 + tid;
+    int64_t all;
+    mine_v = b < p.seqs ? seq_total(p, seq_work(p, b, R)) : 0;
+    mine_at = total + prefix(mine_v, &all);
+    if (blockIdx.x == 0 && b < p.seqs) ws.start[b] = mine_at;
     total += all;
     __syncthreads();
   }
   if (blockIdx.x == 0 && tid == 0) ws.start[p.seqs] = total;
-  const int64_t run = run_length(total, gridDim.x);
+  const int64_t run = run_length(total, gridDim.x, kWarps);
   const int64_t begin = run * blockIdx.x, end = begin + run < total ? begin + run : total;
   if (begin >= end) return;
-  {
+  if (p.seqs <= kThreads) {
+    if (mine_v > 0 && begin >= mine_at && begin < mine_at + mine_v) {
+      found_b = tid;
+      found_at = mine_at;
+    }
+    __syncthreads();
+  } else {
     int64_t before = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
       const int b = b0 + tid;
-      const int64_t v = b < p.seqs ? seq_total(p, seq_work(p, b, R)) : 0;
-      int64_t sum = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t o = __shfl_up_sync(~0u, sum, d);
-        if (lane >= d) sum += o;
-      }
-      if (lane == 31) scan[warp] = sum;
-      __syncthreads();
-      int64_t all = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) sum += scan[w];
-        all += scan[w];
-      }
-      const int64_t at = before + sum - v;
+      int64_t all;
+      const int64_t v = b < p.seqs ? seq_total(p, seq_work(p, b, R)) : 0, at = before + prefix(v, &all);
       if (v > 0 && begin >= at && begin < at + v) {
         found_b = b;
         found_at = at;
@@ -279,11 +280,75 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Work
     const int s1 = static_cast<int>(end - seg_at < w.steps ? end - seg_at : w.steps);
     const int rows = min(R, w.r.n * G - tile * R);
 
-    // ---- rows of the segment: queries as operand fragments, limits
+    // What the first and the last row see (limits grow with the row): steps in which every row sees every token need no mask.
+    auto sees_to = [&](int r) {
+      const int pos = w.r.len - w.r.n + r / G;
+      return max(0, p.causal ? min(pos + 1, w.r.len) : w.r.len);
+    };
+    auto sees_from = [&](int r) { return p.window > 0 ? max(0, w.r.len - w.r.n + r / G - p.window + 1) : 0; };
+    const int row_first = tile * R, row_last = row_first + rows - 1;
+    const int all_hi = sees_to(row_first), any_hi = sees_to(row_last), any_lo = sees_from(row_first), all_lo = sees_from(row_last);
+
+    // ---- this warp's steps: s0 + warp, + kWarps, ... Page ids come 16 steps at a time: lane i holds the first page
+    // of step i of the batch, lane 16 + i the second one (pages of 16 tokens).
+    const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kWarps - 1) / kWarps : 0;
+    const int64_t head_block = static_cast<int64_t>(head) << p.page_log2;
+    int ids = -1;
+    auto issue = [&](int i) {
+      if (i < mine) {
+        if ((i & 15) == 0) {
+          const int t = (w.first + s0 + warp + (i + (lane & 15)) * kWarps) * kStep + (lane >> 4) * 16;
+          ids = -1;
+          if (i + (lane & 15) < mine && t < w.r.len && (lane < 16 || p.page == 16)) ids = page_id(p, b, t >> p.page_log2);
+        }
+        const int t0 = (w.first + s0 + warp + i * kWarps) * kStep;
+        const int id0 = __shfl_sync(~0u, ids, i & 15);
+        const int id1 = p.page == 16 ? __shfl_sync(~0u, ids, 16 + (i & 15)) : id0;
+        const uint32_t st = ring + (i % kStages) * C::kStage;
+        const int upto = min(any_hi, w.r.len) - t0;  // rows of the step that hold tokens
+        constexpr int kPerRow = D / 16, kRowsAt = 32 / kPerRow, kCopies = kStep / kRowsAt;
+        const int cr = lane / kPerRow, cc = lane % kPerRow;
+        if (p.page != 16 && upto >= kStep && id0 >= 0) {
+          // a whole step within one page: 32 rows in a row, at fixed distances on both sides (the swizzle repeats every
+          // 8 rows)
+          const int64_t off = ((static_cast<int64_t>(id0) * p.hkv << p.page_log2) + head_block + (t0 & (p.page - 1)) + cr) * D + cc * 16;
+          const uint8_t* ks = p.k_cache + off;
+          const uint8_t* vs = p.v_cache + off;
+          const uint32_t even = st + chunk_at<D>(cr, cc), odd = st + chunk_at<D>(cr + kRowsAt, cc) - kRowsAt * D;
+#pragma unroll
+          for (int j = 0; j < kCopies; ++j) {
+            const uint32_t to = ((j * kRowsAt & 7) ? odd : even) + j * kRowsAt * D;
+            cp_async16(to, ks + j * kRowsAt * D, 16);
+            cp_async16(to + C::kTile, vs + j * kRowsAt * D, 16);
+          }
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < kCopies; ++j) {
+            const int r = j * kRowsAt + cr;
+            const int id = r < 16 ? id0 : id1;
+            const bool ok = r < upto && id >= 0;
+            const int64_t off = ((static_cast<int64_t>(ok ? id : 0) * p.hkv << p.page_log2) + head_block + ((t0 + r) & (p.page - 1))) * D + cc * 16;
+            cp_async16(st + chunk_at<D>(r, cc), p.k_cache + (ok ? off : 0), ok ? 16 : 0);
+            cp_async16(st + C::kTile + chunk_at<D>(r, cc), p.v_cache + (ok ? off : 0), ok ? 16 : 0);
+          }
+        }
+        if (lane < 4) {
+          const int id = (lane & 1) ? id1 : id0;
+          const uint32_t at_m = st + 2 * C::kTile + lane * 4;
+          if (id >= 0) cp_async4(at_m, ((lane & 2) ? p.v_scale : p.k_scale) + static_cast<int64_t>(id) * p.hkv + head);
+          else *reinterpret_cast<float*>(ring_ptr + (i % kStages) * C::kStage + 2 * C::kTile + lane * 4) = 0.0f;
+          if (lane < 2) *reinterpret_cast<int*>(ring_ptr + (i % kStages) * C::kStage + 2 * C::kTile + 16 + lane * 4) = id >= 0;
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+    // ---- rows of the segment, while the first steps are under way: queries as operand fragments, limits
     if (tid < R) {
-      const int r = tile * R + min(tid, rows - 1), pos = w.r.len - w.r.n + r / G;
-      row_hi[tid] = max(0, p.causal ? min(pos + 1, w.r.len) : w.r.len);
-      row_lo[tid] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      row_hi[tid] = sees_to(min(row_first + tid, row_last));
+      row_lo[tid] = sees_from(min(row_first + tid, row_last));
     }
     for (int r = warp; r < R; r += kWarps) {
       const int rr = tile * R + r;
@@ -326,10 +391,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Work
       }
     }
     __syncthreads();
-    // steps in which every row sees every token need no mask
-    const int all_hi = row_hi[0], all_lo = row_lo[rows - 1];  // limits grow with the row
-    const int any_hi = row_hi[rows - 1], any_lo = row_lo[0];
-
     float m[NT][2], l[NT][2], fac[NT][2], cor[NT][2], O[C::kMt][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -355,47 +416,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Work
         qr[s][1] = v.y;
       }
     }
-
-    // ---- this warp's steps: s0 + warp, + kWarps, ... Page ids come 16 steps at a time: lane i holds the first page
-    // of step i of the batch, lane 16 + i the second one (pages of 16 tokens).
-    const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kWarps - 1) / kWarps : 0;
-    const int64_t head_block = static_cast<int64_t>(head) << p.page_log2;
-    int ids = -1;
-    auto issue = [&](int i) {
-      if (i < mine) {
-        if ((i & 15) == 0) {
-          const int t = (w.first + s0 + warp + (i + (lane & 15)) * kWarps) * kStep + (lane >> 4) * 16;
-          ids = -1;
-          if (i + (lane & 15) < mine && t < w.r.len && (lane < 16 || p.page == 16)) ids = page_id(p, b, t >> p.page_log2);
-        }
-        const int t0 = (w.first + s0 + warp + i * kWarps) * kStep;
-        const int id0 = __shfl_sync(~0u, ids, i & 15);
-        const int id1 = p.page == 16 ? __shfl_sync(~0u, ids, 16 + (i & 15)) : id0;
-        const uint32_t st = ring + (i % kStages) * C::kStage;
-        const int upto = min(any_hi, w.r.len) - t0;  // rows of the step that hold tokens
-        constexpr int kPerRow = D / 16, kRowsAt = 32 / kPerRow;
-        const int cr = lane / kPerRow, cc = lane % kPerRow;
-#pragma unroll
-        for (int j = 0; j < kStep / kRowsAt; ++j) {
-          const int r = j * kRowsAt + cr;
-          const int id = r < 16 ? id0 : id1;
-          const bool ok = r < upto && id >= 0;
-          const int64_t off = ((static_cast<int64_t>(ok ? id : 0) * p.hkv << p.page_log2) + head_block + ((t0 + r) & (p.page - 1))) * D + cc * 16;
-          cp_async16(st + chunk_at<D>(r, cc), p.k_cache + (ok ? off : 0), ok ? 16 : 0);
-          cp_async16(st + C::kTile + chunk_at<D>(r, cc), p.v_cache + (ok ? off : 0), ok ? 16 : 0);
-        }
-        if (lane < 4) {
-          const int id = (lane & 1) ? id1 : id0;
-          const uint32_t at_m = st + 2 * C::kTile + lane * 4;
-          if (id >= 0) cp_async4(at_m, ((lane & 2) ? p.v_scale : p.k_scale) + static_cast<int64_t>(id) * p.hkv + head);
-          else *reinterpret_cast<float*>(ring_ptr + (i % kStages) * C::kStage + 2 * C::kTile + lane * 4) = 0.0f;
-          if (lane < 2) *reinterpret_cast<int*>(ring_ptr + (i % kStages) * C::kStage + 2 * C::kTile + 16 + lane * 4) = id >= 0;
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
 
     for (int i = 0; i < mine; ++i) {
       issue(i + kStages - 1);
@@ -672,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const Kv8 p, Work
 
 // Joins the partial results of the segments that were cut: a warp a (row, query head).
 template <int D, bool F32>
-__global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws, int R, int grid) {
+__global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws, int R, int grid, int warps) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t id = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
@@ -702,7 +722,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws,
   if (w.tiles == 0) return;
   const int G = p.hq / p.hkv, rr = (row - w.r.row0) * G + h % G, tile = rr / R, r = rr % R;
   const int64_t g0 = ws.start[b] + (static_cast<int64_t>(h / G) * w.tiles + tile) * w.steps, g1 = g0 + w.steps;
-  const int64_t run = run_length(ws.start[p.seqs], grid);
+  const int64_t run = run_length(ws.start[p.seqs], grid, warps);
   const int c0 = static_cast<int>(g0 / run), c1 = static_cast<int>((g1 - 1) / run);
   if (c0 == c1) return;
   auto part_of = [&](int k) { return ws.part + (static_cast<int64_t>(k) * 2 + (g0 >= run * k ? 1 : 0)) * part_floats(R, D); };
@@ -748,7 +768,7 @@ cudaError_t launch_nt(const Kv8& p, void* ws, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   const int grid = device_sm_count();
   Workspace w{static_cast<int64_t*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + starts_bytes(p.seqs))};
-  attn_mma_kernel<E4M3, D, NT, F32><<<grid, kThreads, C::kSmem, s>>>(p, w);
+  attn_mma_kernel<E4M3, D, NT, F32><<<grid, C::kThreads, C::kSmem, s>>>(p, w);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.tokens) * p.hq + 7) / 8));
@@ -759,7 +779,7 @@ cudaError_t launch_nt(const Kv8& p, void* ws, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<D, F32>, p, w, C::kRows, grid);
+  return cudaLaunchKernelEx(&cfg, combine_kernel<D, F32>, p, w, C::kRows, grid, C::kWarps);
 }
 
 template <bool E4M3, int D, bool F32>
