@@ -4,6 +4,7 @@
 namespace xrgpu {
 
 uint64_t kv8_attn_mma_workspace(const Kv8& p) {
+  if (cluster_split(p)) return 0;
   return static_cast<uint64_t>(starts_bytes(p.seqs) + 2ll * device_sm_count() * part_floats(8 * row_tiles(p), p.D) * 4);
 }
 

@@ -22,12 +22,15 @@
 //
 // Balance. The steps of all segments form one sequence; every CTA takes an equal run of it, found from the
 // lengths on the device. A segment that lies inside one CTA's run is finished there, one that is cut leaves
-// partial results (m, l, O) in the workspace, which combine_kernel joins in the order of the CTAs.
+// partial results (m, l, O) in the workspace, which combine_kernel joins in the order of the CTAs. Where few short
+// segments leave most SMs idle, a cluster of up to 8 CTAs shares each segment instead and joins it through shared
+// memory: one launch (one token of one sequence of 2048: 16 -> 11 us).
 #pragma once
 
 #include <cstdint>
 
 #include "mmnb_kv8.cuh"
+#include "mmnb_tcgen05.cuh"
 #include "mmnb_kv8_attn.h"
 
 namespace xrgpu {
@@ -169,7 +172,7 @@ __device__ __forceinline__ int64_t run_length(int64_t total, int grid, int warps
 }
 
 // ------------------------------------------------------------------ main kernel
-template <bool E4M3, int D, int NT, bool F32>
+template <bool E4M3, int D, int NT, bool F32, bool CL = false>
 struct Traits {
   static constexpr int kRows = 8 * NT;
   // One tile of rows leaves registers for 12 warps, whose rings then hold two steps; more rows for 8 with three.
@@ -184,12 +187,13 @@ struct Traits {
   static constexpr bool kRaw = !E4M3 && !F32;
   static constexpr int kMerge = kRows * D * 4;        // a warp's O in shared memory, over its ring
   static constexpr int kWarpBytes = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kSmem = kWarps * kWarpBytes + kQ + kRows * 16 + kWarps * kRows * 8 + 64;
+  static constexpr int kJoin = CL ? kRows * (D + 2) * 4 : 0;  // the CTA's (O, m, l), read by its cluster
+  static constexpr int kSmem = kWarps * kWarpBytes + kQ + kRows * 16 + kWarps * kRows * 8 + 64 + kJoin;
 };
 
-template <bool E4M3, int D, int NT, bool F32>
-__global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mma_kernel(const Kv8 p, Workspace ws) {
-  using C = Traits<E4M3, D, NT, F32>;
+template <bool E4M3, int D, int NT, bool F32, bool CL>
+__global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mma_kernel(const Kv8 p, Workspace ws, int split) {
+  using C = Traits<E4M3, D, NT, F32, CL>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t scan[kWarps + 1];
@@ -208,6 +212,7 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mm
   int* row_lo = row_hi + R;                                                          // [R] first token seen
   float* warp_m = reinterpret_cast<float*>(row_lo + R);                              // [kWarps][R]
   float* warp_l = warp_m + kWarps * R;
+  float* join = reinterpret_cast<float*>(smem + C::kSmem - C::kJoin);                // [R][D], [R] m, [R] l
 
   // ---- all steps, this CTA's run of them, and the sequence it starts in (kThreads sequences at a time; a second pass
   // finds the start among more)
@@ -229,6 +234,49 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mm
     *all = total;
     return before + sum - v;
   };
+  int64_t begin = 0, end = 0;
+  int rank = 0;
+  if (CL) {
+    // cluster `slot` takes a (row tile, head): the slot-th of the tiles of all sequences in order
+    rank = static_cast<int>(cluster_rank());
+    const int slot = blockIdx.x / split / p.hkv;
+    int before = 0;
+    if (tid == 0) found_b = -1;
+    __syncthreads();
+    for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
+      const int b = b0 + tid;
+      const int tiles = b < p.seqs ? seq_work(p, b, R).tiles : 0;
+      int64_t all;
+      const int at = before + static_cast<int>(prefix(tiles, &all));
+      if (slot >= at && slot < at + tiles) {
+        found_b = b;
+        found_at = slot - at;
+      }
+      before += static_cast<int>(all);
+      __syncthreads();
+    }
+    if (p.zero_rest && blockIdx.x == 0) {  // few rows here: a thread looks for each row's sequence
+      for (int row = tid; row < p.tokens; row += kThreads) {
+        bool owned = false;
+        for (int b = 0; b < p.seqs && !owned; ++b) {
+          const SeqRows r = seq_rows(p, b, true);
+          owned = row >= r.row0 && row < r.row0 + r.n;
+        }
+        if (!owned)
+          for (int d = 0; d < p.hq * D; ++d) {
+            if (F32) static_cast<float*>(p.o)[row * p.os + d] = 0.0f;
+            else static_cast<__half*>(p.o)[row * p.os + d] = __half(0.0f);
+          }
+      }
+    }
+    if (found_b >= 0) {
+      const SeqWork w = seq_work(p, found_b, R);
+      const int64_t seg_at = (static_cast<int64_t>(blockIdx.x / split % p.hkv) * w.tiles + found_at) * w.steps;
+      begin = seg_at + static_cast<int64_t>(w.steps) * rank / split;
+      end = seg_at + static_cast<int64_t>(w.steps) * (rank + 1) / split;
+      for (int e = tid; e < R * (D + 2); e += kThreads) join[e] = e >= R * D && e < R * D + R ? -INFINITY : 0.0f;  // of a rank without steps
+    }
+  } else {
   int64_t total = 0, mine_v = 0, mine_at = 0;
   for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
     const int b = b0 + tid;
@@ -241,7 +289,8 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mm
   }
   if (blockIdx.x == 0 && tid == 0) ws.start[p.seqs] = total;
   const int64_t run = run_length(total, gridDim.x, kWarps);
-  const int64_t begin = run * blockIdx.x, end = begin + run < total ? begin + run : total;
+  begin = run * blockIdx.x;
+  end = begin + run < total ? begin + run : total;
   if (begin >= end) return;
   if (p.seqs <= kThreads) {
     if (mine_v > 0 && begin >= mine_at && begin < mine_at + mine_v) {
@@ -264,9 +313,11 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mm
       if (before > begin) break;
     }
   }
+  }
+  __syncthreads();
   int b = found_b;
-  int64_t seq_at = found_at;
-  SeqWork w = seq_work(p, b, R);
+  int64_t seq_at = CL ? 0 : found_at;
+  SeqWork w = b < 0 ? SeqWork{} : seq_work(p, b, R);
 
   for (int64_t at = begin; at < end;) {
     while (at >= seq_at + seq_total(p, w)) {  // on to the next sequence that has rows
@@ -664,7 +715,13 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mm
         o.z = fmaf(f, v.z, o.z);
         o.w = fmaf(f, v.w, o.w);
       }
-      if (whole) {
+      if (CL) {
+        *reinterpret_cast<float4*>(join + r * D + d) = o;
+        if (d == 0) {
+          join[R * D + r] = mm;
+          join[R * D + R + r] = ll;
+        }
+      } else if (whole) {
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
         const int rr = tile * R + r;
         const int64_t oat = static_cast<int64_t>(w.r.row0 + rr / G) * p.os + (head * G + rr % G) * D + d;
@@ -688,12 +745,54 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mm
     __syncthreads();
     at = seg_at + s1;
   }
+  if (CL) {
+    cluster_sync();
+    if (b >= 0) {
+      const int tile = static_cast<int>(found_at), head = blockIdx.x / split % p.hkv, rows = min(R, w.r.n * G - tile * R);
+      const uint32_t at = smem_u32(join);
+      for (int e = rank * kThreads + tid; e < rows * (D / 4); e += split * kThreads) {
+        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+        float mk[8], lk[8], mm = -INFINITY, ll = 0.0f;
+        float4 v[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < split) {
+            const uint32_t there = map_rank(at, k);
+            v[k] = ld_cluster_f32x4(there + (r * D + d) * 4);
+            mk[k] = ld_cluster_f32(there + (R * D + r) * 4);
+            lk[k] = ld_cluster_f32(there + (R * D + R + r) * 4);
+          }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < split) mm = fmaxf(mm, mk[k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < split) {
+            const float f = mk[k] == mm ? 1.0f : exp2_approx(mk[k] - mm);
+            ll = fmaf(f, lk[k], ll);
+            o.x = fmaf(f, v[k].x, o.x);
+            o.y = fmaf(f, v[k].y, o.y);
+            o.z = fmaf(f, v[k].z, o.z);
+            o.w = fmaf(f, v[k].w, o.w);
+          }
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+        const int rr = tile * R + r;
+        const int64_t oat = static_cast<int64_t>(w.r.row0 + rr / G) * p.os + (head * G + rr % G) * D + d;
+        const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (F32) static_cast<float*>(p.o)[oat + i] = y[i];
+          else static_cast<__half*>(p.o)[oat + i] = __float2half_rn(y[i]);
+        }
+      }
+    }
+    cluster_sync();  // nobody leaves while its part is being read
+  }
 }
 
 // Joins the partial results of the segments that were cut: a warp a (row, query head).
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws, int R, int grid, int warps) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t id = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int row = static_cast<int>(id / p.hq), h = static_cast<int>(id % p.hq);
@@ -709,6 +808,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Kv8 p, Workspace ws,
     }
   }
   const SeqWork w = b < 0 ? SeqWork{} : seq_work(p, b, R);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int PER = D / 32;
   const int64_t oat = static_cast<int64_t>(row) * p.os + h * D + lane * PER;
   if (w.r.n == 0) {  // a row of no sequence
@@ -760,15 +860,47 @@ inline int row_tiles(const Kv8& p) {
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
 
+// CTAs of a cluster that share a segment, 0: equal runs over all SMs. Clusters take a call whose segments, at least two
+// CTAs each, find an SM for every CTA, and whose tables hold at most four steps a warp.
+inline int cluster_split(const Kv8& p) {
+  if (row_tiles(p) != 1) return 0;
+  const int64_t G = p.hq / p.hkv, slots = p.uniform ? ceil_div(p.tokens / p.seqs * G, 8) * p.seqs : p.tokens * G / 8 + p.seqs;
+  int split = 8;
+  while (split > 1 && slots * p.hkv * split > device_sm_count()) split /= 2;
+  const int64_t steps = ceil_div(static_cast<int64_t>(p.max_pages) << p.page_log2, kStep);
+  return split > 1 && steps <= 4ll * 12 * split ? split : 0;
+}
+
+template <bool E4M3, int D, bool F32>
+cudaError_t launch_cluster(const Kv8& p, int split, cudaStream_t s) {
+  using C = Traits<E4M3, D, 1, F32, true>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  const cudaError_t e = allow_smem<attn_mma_kernel<E4M3, D, 1, F32, true>>(C::kSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t G = p.hq / p.hkv, slots = p.uniform ? ceil_div(p.tokens / p.seqs * G, 8) * p.seqs : p.tokens * G / 8 + p.seqs;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(slots * p.hkv * split));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_mma_kernel<E4M3, D, 1, F32, true>, p, Workspace{}, split);
+}
+
 template <bool E4M3, int D, int NT, bool F32>
 cudaError_t launch_nt(const Kv8& p, void* ws, cudaStream_t s) {
   using C = Traits<E4M3, D, NT, F32>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  cudaError_t e = allow_smem<attn_mma_kernel<E4M3, D, NT, F32>>(C::kSmem);
+  cudaError_t e = allow_smem<attn_mma_kernel<E4M3, D, NT, F32, false>>(C::kSmem);
   if (e != cudaSuccess) return e;
   const int grid = device_sm_count();
   Workspace w{static_cast<int64_t*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + starts_bytes(p.seqs))};
-  attn_mma_kernel<E4M3, D, NT, F32><<<grid, C::kThreads, C::kSmem, s>>>(p, w);
+  attn_mma_kernel<E4M3, D, NT, F32, false><<<grid, C::kThreads, C::kSmem, s>>>(p, w, 1);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.tokens) * p.hq + 7) / 8));
@@ -784,6 +916,7 @@ cudaError_t launch_nt(const Kv8& p, void* ws, cudaStream_t s) {
 
 template <bool E4M3, int D, bool F32>
 cudaError_t launch_rows(const Kv8& p, void* ws, cudaStream_t s) {
+  if (const int split = cluster_split(p)) return launch_cluster<E4M3, D, F32>(p, split, s);
   switch (row_tiles(p)) {
     case 1: return launch_nt<E4M3, D, 1, F32>(p, ws, s);
     case 2: return launch_nt<E4M3, D, 2, F32>(p, ws, s);
