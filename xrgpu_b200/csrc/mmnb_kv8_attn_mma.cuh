@@ -175,8 +175,10 @@ __device__ __forceinline__ int64_t run_length(int64_t total, int grid, int warps
 template <bool E4M3, int D, int NT, bool F32, bool CL = false>
 struct Traits {
   static constexpr int kRows = 8 * NT;
-  // One tile of rows leaves registers for 12 warps, whose rings then hold two steps; more rows for 8 with three.
-  static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = kWarps * 32, kStages = NT == 1 ? 2 : 3;
+  // One tile of rows leaves registers for 12 warps an SM, whose rings then hold two steps: two CTAs of 6, so that one
+  // streams while the other is between segments; 12 together in a cluster. More rows: 8 warps with three steps.
+  static constexpr int kWarps = NT == 1 ? (CL ? 12 : 6) : 8, kThreads = kWarps * 32, kStages = NT == 1 ? 2 : 3;
+  static constexpr int kCtas = NT == 1 && !CL ? 2 : 1;  // an SM
   static constexpr int kK = D / 16;                   // k steps of the scores
   static constexpr int kMt = D / 16;                  // 16-dim tiles of the output
   static constexpr int kTile = kStep * D;             // bytes of a step's keys (or values)
@@ -192,7 +194,7 @@ struct Traits {
 };
 
 template <bool E4M3, int D, int NT, bool F32, bool CL>
-__global__ void __launch_bounds__(Traits<E4M3, D, NT, F32>::kThreads, 1) attn_mma_kernel(const Kv8 p, Workspace ws, int split) {
+__global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits<E4M3, D, NT, F32, CL>::kCtas) attn_mma_kernel(const Kv8 p, Workspace ws, int split) {
   using C = Traits<E4M3, D, NT, F32, CL>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -895,10 +897,10 @@ cudaError_t launch_cluster(const Kv8& p, int split, cudaStream_t s) {
 template <bool E4M3, int D, int NT, bool F32>
 cudaError_t launch_nt(const Kv8& p, void* ws, cudaStream_t s) {
   using C = Traits<E4M3, D, NT, F32>;
-  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  static_assert((C::kSmem + 1024) * C::kCtas <= 228 * 1024, "shared memory");
   cudaError_t e = allow_smem<attn_mma_kernel<E4M3, D, NT, F32, false>>(C::kSmem);
   if (e != cudaSuccess) return e;
-  const int grid = device_sm_count();
+  const int grid = device_sm_count() * C::kCtas;
   Workspace w{static_cast<int64_t*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + starts_bytes(p.seqs))};
   attn_mma_kernel<E4M3, D, NT, F32, false><<<grid, C::kThreads, C::kSmem, s>>>(p, w, 1);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
