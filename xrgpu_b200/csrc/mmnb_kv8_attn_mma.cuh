@@ -862,10 +862,11 @@ inline int row_tiles(const Kv8& p) {
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
 
-// CTAs of a cluster that share a segment, 0: equal runs over all SMs. Clusters take a call whose segments, at least two
-// CTAs each, find an SM for every CTA, and whose tables hold at most four steps a warp.
+// CTAs of a cluster that share a segment, 0: equal runs over all SMs. Clusters take a call whose segments of 8 rows, at
+// least two CTAs each, find an SM for every CTA, and whose tables hold at most four steps a warp: there latency counts,
+// and segments of more rows would only run fewer CTAs and more code (7 x 5 float32 rows of 5 heads a group: 31 us as
+// segments of 32).
 inline int cluster_split(const Kv8& p) {
-  if (row_tiles(p) != 1) return 0;
   const int64_t G = p.hq / p.hkv, slots = p.uniform ? ceil_div(p.tokens / p.seqs * G, 8) * p.seqs : p.tokens * G / 8 + p.seqs;
   int split = 8;
   while (split > 1 && slots * p.hkv * split > device_sm_count()) split /= 2;
