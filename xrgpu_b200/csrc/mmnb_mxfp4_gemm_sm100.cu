@@ -94,6 +94,39 @@ __device__ __forceinline__ uint32_t instruction_desc(int T, uint32_t half) {
          (static_cast<uint32_t>(kRows >> 4) << 24) | (half << 29);
 }
 
+// 16 accumulators of a row of y from column n0 on, plus bias.
+template <bool F16>
+__device__ __forceinline__ void store_row(const Args& a, int p, int n0, const uint32_t (&v)[16]) {
+  float r[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    r[j] = __uint_as_float(v[j]) + ((a.bias && n0 + j < a.q_rows) ? load_f(a.bias, F16, n0 + j) : 0.0f);
+  if (a.vec && n0 + 16 <= a.q_rows) {
+    if (F16) {
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const __half2 x = __floats2half2_rn(r[2 * j], r[2 * j + 1]);
+        h[j] = *reinterpret_cast<const uint32_t*>(&x);
+      }
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.y) + p * a.ldy + n0);
+      dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+      dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+    } else {
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.y) + p * a.ldy + n0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[j] = make_float4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (n0 + j >= a.q_rows) break;
+      if (F16) static_cast<__half*>(a.y)[p * a.ldy + n0 + j] = __float2half_rn(r[j]);
+      else static_cast<float*>(a.y)[p * a.ldy + n0 + j] = r[j];
+    }
+  }
+}
+
 template <bool SWAP, bool F16, int QB>
 __global__ void __launch_bounds__(kThreads, 1)
     mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
@@ -286,35 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else if (p < a.p_rows) {
-          const int n0 = q0 + col;
-          float r[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            r[j] = __uint_as_float(v[j]) + ((a.bias && n0 + j < a.q_rows) ? load_f(a.bias, F16, n0 + j) : 0.0f);
-          if (a.vec && n0 + 16 <= a.q_rows) {
-            if (F16) {
-              uint32_t h[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const __half2 x = __floats2half2_rn(r[2 * j], r[2 * j + 1]);
-                h[j] = *reinterpret_cast<const uint32_t*>(&x);
-              }
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.y) + p * a.ldy + n0);
-              dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-              dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
-            } else {
-              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.y) + p * a.ldy + n0);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) dst[j] = make_float4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (n0 + j >= a.q_rows) break;
-              if (F16) static_cast<__half*>(a.y)[p * a.ldy + n0 + j] = __float2half_rn(r[j]);
-              else static_cast<float*>(a.y)[p * a.ldy + n0 + j] = r[j];
-            }
-          }
+          store_row<F16>(a, p, q0 + col, v);
         }
       }
     }
@@ -378,6 +383,227 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ------------------------------------------------------------------ pairs of CTAs
+// For many rows: a cluster of two CTAs on one 256 x 256 tile. Each holds its 128 rows of P and half of Q's 256 rows; the
+// first one's MMAs (cta_group::2) read both halves from both shared memories, so that a CTA loads and reads 256 rows
+// a step instead of 384 for the same product (alone, a step of 256 values is bound by shared memory at 768 cycles).
+// Each CTA keeps the accumulators of its own rows and all scales it needs. The second CTA passes on the arrival of its
+// loads (peer), the MMAs' completion goes to both.
+__device__ __forceinline__ void mma2_mxf4(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                                          uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void scales2_to_tmem(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Arrives on `bar` of both CTAs when the tcgen05 operations issued so far have completed.
+__device__ __forceinline__ void mma2_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// Arrives on `bar` of CTA `rank`. Relaxed: it passes on a completion (loads, tensor-memory reads), no writes of this
+// thread, and the release form costs 1500 cycles here.
+__device__ __forceinline__ void arrive_at(uint64_t* bar, uint32_t rank) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_u32(bar), rank)) : "memory");
+}
+constexpr int kStages2 = 6;
+constexpr uint32_t kStage2 = 2 * kRows * kStepBytes + 6 * kScaleTile;  // P, Q half, P scales, Q scales of both blocks
+constexpr int kSfStage2 = 24, kShared2 = kStages2 * kSfStage2;         // scale columns; columns that both accumulators hold
+constexpr int kAcc2 = 256 - kShared2, kSfCol2 = 512 - kStages2 * kSfStage2;
+static_assert(kShared2 % 16 == 0 && kAcc2 + 256 == kSfCol2, "tensor memory map");
+
+template <bool F16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    mxfp4_gemm2_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kStages2], empty[kStages2], peer[kStages2], accfull[2], drained[2], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const int rank = static_cast<int>(cluster_rank());
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages2; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&peer[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accfull[b], 1);
+      mbar_init(&drained[b], 2 * kEpilogueWarps);  // of both CTAs
+    }
+    mbar_init(&done, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are there
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+  const Ctl ctl{&abort_flag, a.err};
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      int g = 0, s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < a.tiles; tile += step) {
+        const int pb = 2 * (tile % a.p_tiles) + rank, q0 = 2 * (tile / a.p_tiles);  // row blocks
+        const int blocks = (pb < a.sp_blocks) + 1 + (q0 + 1 < a.sq_blocks);
+        for (int ks = 0; ks < a.ksteps; ++ks, ++g) {
+          if (!thread_wait(&empty[s], ph ^ 1, ctl, kErrWaitProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t groups = min(2, (a.k64 - 4 * ks + 1) >> 1) * kScaleTile;
+          const uint32_t at = base + s * kStage2;
+          uint8_t* sc = gbase + s * kStage2 + 2 * kRows * kStepBytes;
+          mbar_arrive_expect_tx(&full[s], 2 * kRows * kStepBytes + blocks * groups);
+          tma_load_2d(at, &map_p, ks * kStepBytes, pb * kRows, &full[s]);
+          tma_load_2d(at + kRows * kStepBytes, &map_q, ks * kStepBytes, (q0 + rank) * kRows, &full[s]);
+          if (pb < a.sp_blocks) bulk_copy_g2s(sc, a.sp + (pb * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
+          bulk_copy_g2s(sc + 2 * kScaleTile, a.sq + (q0 * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
+          if (q0 + 1 < a.sq_blocks) bulk_copy_g2s(sc + 4 * kScaleTile, a.sq + ((q0 + 1) * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
+          if (++s == kStages2) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (!ok)
+        for (int h = (g > kStages2 ? g - kStages2 : 0); h < g; ++h) drain_wait(&full[h % kStages2], (h / kStages2) & 1, a.err, kErrDrain);
+    }
+  } else if (warp == 1 && rank == 1) {
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < a.tiles; tile += step)
+      for (int ks = 0; ks < a.ksteps; ++ks) {
+        if (!warp_spin(&full[s], ph, ctl, kErrWaitMma)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) arrive_at(&peer[s], 0);
+        __syncwarp();
+        if (++s == kStages2) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+  } else if (warp == 1) {
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+    const uint64_t s_desc = plain_desc(base + 2 * kRows * kStepBytes);
+    const uint32_t wide = static_cast<uint32_t>(kRows >> 4) << 24;  // M = 256
+    const uint32_t i_desc0 = instruction_desc(256, 0u) + wide, i_desc1 = instruction_desc(256, 2u) + wide;
+    int i = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    // both CTAs' loads (lanes look at one barrier each), or both CTAs' drains
+    auto wait = [&](uint64_t* x, uint64_t* y, uint32_t parity) {
+      uint64_t start = 0;
+      for (;;) {
+#pragma unroll 1
+        for (int n = 0; n < kSpins; ++n)
+          if (__all_sync(~0u, mbar_test_wait((lane & 1) ? y : x, parity))) return true;
+        if (__any_sync(~0u, *ctl.abort != 0)) return false;
+        const uint64_t now = __shfl_sync(~0u, global_timer_ns(), 0);
+        if (start == 0) start = now;
+        if (now - start > kWaitLimitNs) {
+          if (lane == 0) {
+            record_device_error(a.err, kErrWaitMma);
+            *ctl.abort = 1;
+          }
+          return false;
+        }
+      }
+    };
+    for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
+      if (i > 0 && !wait(&drained[(i - 1) & 1], &drained[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
+      const uint32_t d = tmem + ((i & 1) ? kAcc2 : 0);
+      for (int ks = 0; ks < a.ksteps; ++ks) {
+        if (!wait(&full[s], &peer[s], ph)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int subs = a.k64 - 4 * ks;
+        const uint32_t off = static_cast<uint32_t>(s) * (kStage2 >> 4);
+        const uint32_t sf = tmem + kSfCol2 + s * kSfStage2;
+        if (elect_one()) {
+#pragma unroll
+          for (int gr = 0; gr < 2; ++gr) {
+            if (gr == 1 && subs <= 2) break;
+            scales2_to_tmem(sf + 4 * gr, s_desc + off + gr * (kScaleTile >> 4));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) scales2_to_tmem(sf + 8 + 4 * (gr * 2 + b), s_desc + off + ((1 + b) * 2 + gr) * (kScaleTile >> 4));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j > 0 && j >= subs) break;
+            mma2_mxf4(d, p_desc + off + 2 * j, q_desc + off + 2 * j, (j & 1) ? i_desc1 : i_desc0, sf + 4 * (j >> 1), sf + 8 + 8 * (j >> 1), ks > 0 || j > 0);
+          }
+          mma2_commit(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == kStages2) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (ok && elect_one()) mma2_commit(&accfull[i & 1]);
+      __syncwarp();
+    }
+    if (elect_one()) mma2_commit(&done);
+    __syncwarp();
+    drain_wait(&done, 0, a.err, kErrDrain);
+  } else {
+    const int q = warp & 3, c = (warp - 2) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
+    constexpr int kChunks = 16, kSharedChunks = kShared2 / 16;
+    int i = 0;
+    for (int tile = first; tile < a.tiles; tile += step, ++i) {
+      const int b = i & 1, p = (2 * (tile % a.p_tiles) + rank) * kRows + 32 * q + lane, q0 = tile / a.p_tiles * 256;
+      if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
+      tc_fence_after();
+      bool told = false;
+      for (int at = c; at < kChunks; at += 2) {
+        if (!told && at >= kSharedChunks) {  // what the next tile's accumulator shares with this one has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(&drained[b], 0);
+          told = true;
+        }
+        const int col = 16 * (b ? at : kChunks - 1 - at);
+        uint32_t v[16];
+        tmem_ld16(tmem + lane_addr + (b ? kAcc2 : 0) + col, v);
+        tmem_wait_ld16(v);
+        if (p < a.p_rows) store_row<F16>(a, p, q0 + col, v);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA's memory goes while the other may read or signal it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
 // ------------------------------------------------------------------ host side
 struct Shape {
   bool swap;
@@ -432,6 +658,53 @@ cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, 
   return cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<SWAP, F16, QB>, mp, mq, a);
 }
 
+// Pairs take a call that fills three quarters of the SMs with 256 x 256 tiles.
+bool pairs_pay(const Mxfp4Matmul& p, int sms) {
+  return ceil_div(p.M, 256) * ceil_div(p.N, 256) * 2 * 4 >= static_cast<int64_t>(sms) * 3;
+}
+
+template <bool F16>
+cudaError_t launch_pairs(const Mxfp4Matmul& p, Args a, bool early, cudaStream_t s) {
+  constexpr int smem = kStages2 * kStage2 + 1024;
+  cudaError_t e = allow_smem<mxfp4_gemm2_kernel<F16>>(smem);
+  if (e != cudaSuccess) return e;
+  a.T = 256;
+  a.split = 1;
+  a.p_rows = static_cast<int>(p.M);
+  a.q_rows = static_cast<int>(p.N);
+  a.p_tiles = static_cast<int>(ceil_div(p.M, 256));
+  const int64_t tiles = a.p_tiles * ceil_div(p.N, 256);
+  if (tiles > INT_MAX / 8) return cudaErrorInvalidValue;
+  a.tiles = static_cast<int>(tiles);
+  a.tiles_k = ceil_div(p.kb, 4);
+  a.sp_blocks = static_cast<int>(ceil_div(p.M, kRows));
+  a.sq_blocks = static_cast<int>(ceil_div(p.N, kRows));
+  a.sp = p.a_scales;
+  a.sq = p.b_scales;
+  a.bias = p.bias;
+  a.y = p.y;
+  a.ldy = p.ldy;
+  a.vec = (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0 && (p.ldy * (p.f16 ? 2 : 4)) % 16 == 0;
+  a.err = p.err;
+  CUtensorMap mp, mq;
+  const uint64_t row = static_cast<uint64_t>(p.kb) * 16;
+  if (!encode_tensor_map_2d(&mp, 0, p.a, row, a.p_rows, row, kStepBytes, kRows, true) ||
+      !encode_tensor_map_2d(&mq, 0, p.b, row, a.q_rows, row, kStepBytes, kRows, true))
+    return cudaErrorInvalidValue;
+  const int pairs = device_sm_count() / 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * (a.tiles < pairs ? a.tiles : pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, mxfp4_gemm2_kernel<F16>, mp, mq, a);
+}
+
 }  // namespace
 
 cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s) {
@@ -439,6 +712,7 @@ cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s
   Args a{};
   a.k64 = static_cast<int>(ceil_div(p.kb, 2));
   a.ksteps = (a.k64 + 3) / 4;
+  if (pairs_pay(p, sms)) return p.f16 ? launch_pairs<true>(p, a, early, s) : launch_pairs<false>(p, a, early, s);
   const Shape sh = choose(p, a.ksteps, sms);
   a.T = sh.T;
   a.split = sh.split;
