@@ -172,7 +172,7 @@ def _bound(a, w, y, dtype, K):
 
 SHAPES = [(1, 1, 1), (1, 8, 32), (1, 128, 256), (2, 129, 288), (7, 250, 544), (16, 128, 4096), (17, 384, 1024), (33, 1003, 100),
           (64, 256, 1056), (65, 130, 800), (127, 64, 512), (128, 257, 2080), (129, 255, 260), (200, 640, 384), (300, 520, 1312), (1, 4096, 14336),
-          (1200, 5900, 544), (1300, 10300, 288)]
+          (1200, 5900, 544), (1300, 10300, 288), (20, 57001, 64)]
 
 
 @gpu

@@ -16,9 +16,8 @@
 // Tensor memory: two accumulators of T columns at 0 and acc1, then per stage the scale columns: 4 columns
 // (32 lanes x 4 bytes x 4 row groups) for 128 rows x 128 values. Q tiles begin at a row block (one tile, or T a multiple of
 // 128), so that their scales begin at a column that is a multiple of 4: other starts are not taken. A stage's columns are rewritten only when
-// its shared-memory buffer has come back, that is when the MMAs that read them are done. With T = 256 two
-// accumulators and the scales need more than the 512 columns: the accumulators then overlap, and the
-// drain starts with the shared columns, after which the next tile may start.
+// its shared-memory buffer has come back, that is when the MMAs that read them are done. Only tiles of up to 128 columns
+// take turns on a CTA (more rows than that go to pairs of CTAs before they need a second round).
 //
 // Every wait is bounded as in mmnb_gemm_sm100.cu.
 #include <cuda.h>
@@ -49,9 +48,10 @@ constexpr unsigned kErrDrain = 0x604;
 struct Args {
   int p_rows, q_rows;       // valid rows of the operands
   int p_tiles, tiles;       // tiles along P, in all
+  int whole;                // pairs: tiles from this one on are halves
   int T, ksteps, k64;       // rows of Q a tile, stages along K, 64-value MMA steps along K
   int stages, split, q_blocks;  // q_blocks: scale row blocks a Q tile spans (1 or 2)
-  int acc1, shared_cols;    // column of the second accumulator, columns that both hold
+  int acc1;                 // column of the second accumulator
   int tmem_cols, sf_col, sf_stage;
   int early;                // the weights may be loaded before the previous kernel has finished
   uint32_t q_stage, stage;  // bytes
@@ -234,9 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t ph = 0;
     bool ok = true;
     for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
-      // Overlapping accumulators: the shared columns of tile i - 1 are out; separate ones: tile i - 2 is.
-      const int w = a.shared_cols ? i - 1 : i - 2;
-      if (w >= 0 && !warp_spin(&drained[w & 1], (w >> 1) & 1, ctl, kErrWaitMma)) break;
+      if (i >= 2 && !warp_spin(&drained[i & 1], ((i - 2) >> 1) & 1, ctl, kErrWaitMma)) break;
       const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
       for (int ks = k0; ks < k1; ++ks) {
         if (!warp_spin(&full[s], ph, ctl, kErrWaitMma)) {
@@ -280,7 +278,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int q = warp & 3, c = (warp - 2) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
-    const int chunks = a.T >> 4, shared_chunks = (a.shared_cols + 15) >> 4;
     int i = 0;
     for (int tile = first; tile < a.tiles; tile += step, ++i) {
       const int pt = tile % a.p_tiles, qt = tile / a.p_tiles, b = i & 1;
@@ -288,18 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
       tc_fence_after();
       const float p_bias = (SWAP && a.split == 1 && a.bias && p < a.p_rows) ? load_f(a.bias, F16, p) : 0.0f;
-      bool told = false;
-      for (int at = c; at < chunks + 2; at += 2) {
-        if (!told && at >= shared_chunks && (shared_chunks || at >= chunks)) {
-          // what the next tile's accumulator shares with this one (or all of it) has been read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&drained[b]);
-          told = true;
-        }
-        if (at >= chunks) break;
-        // the second accumulator shares its first columns with the other's last ones
-        const int col = 16 * ((b || !shared_chunks) ? at : chunks - 1 - at);
+      for (int col = 16 * c; col < a.T; col += 32) {
         uint32_t v[16];
         tmem_ld16(tmem + lane_addr + (b ? a.acc1 : 0) + col, v);
         tmem_wait_ld16(v);
@@ -322,6 +308,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           store_row<F16>(a, p, q0 + col, v);
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&drained[b]);
     }
   }
 
@@ -385,9 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------ pairs of CTAs
 // For many rows: a cluster of two CTAs on one 256 x 256 tile. Each holds its 128 rows of P and half of Q's 256 rows; the
-// first one's MMAs (cta_group::2) read both halves from both shared memories, so that a CTA loads and reads 256 rows
-// a step instead of 384 for the same product (alone, a step of 256 values is bound by shared memory at 768 cycles).
-// Each CTA keeps the accumulators of its own rows and all scales it needs. The second CTA passes on the arrival of its
+// first one's MMAs (cta_group::2) read both halves from both shared memories, so that a CTA loads 256 rows a step instead
+// of 384 for the same product. What bounds it are these loads from L2, 35 KB a CTA and step (10 TB/s in all): 8192 x
+// 28672 x 8192 takes 776 us, and 507 with the loads left out. The scale copies and the order of the tiles (bands of 8 tiles
+// of P: 787 -> 810 us) make no difference.
+// Tensor memory: two overlapping accumulators of 256 columns (they and the scales need more than the 512 columns); the
+// drain first takes the shared columns into registers, then the next tile may start (waiting for their stores: 73 -> 66
+// us at 2048 x 14336 x 4096). Each CTA keeps the accumulators of its own rows and all scales it needs. The second CTA passes on the arrival of its
 // loads (peer), the MMAs' completion goes to both.
 __device__ __forceinline__ void mma2_mxf4(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
                                           uint32_t sb, uint32_t accumulate) {
@@ -416,6 +409,17 @@ constexpr uint32_t kStage2 = 2 * kRows * kStepBytes + 6 * kScaleTile;  // P, Q h
 constexpr int kSfStage2 = 24, kShared2 = kStages2 * kSfStage2;         // scale columns; columns that both accumulators hold
 constexpr int kAcc2 = 256 - kShared2, kSfCol2 = 512 - kStages2 * kSfStage2;
 static_assert(kShared2 % 16 == 0 && kAcc2 + 256 == kSfCol2, "tensor memory map");
+
+// Tile `t` of a pair: from a.whole on each index is one half (128 rows of Q) of a tile.
+struct Tile2 {
+  int pt, q0;  // row blocks: pair of P, first of Q
+  bool half;
+};
+__device__ __forceinline__ Tile2 tile2(const Args& a, int t) {
+  const bool half = t >= a.whole;
+  const int whole = half ? a.whole + ((t - a.whole) >> 1) : t;
+  return {whole % a.p_tiles, 2 * (whole / a.p_tiles) + (half ? (t - a.whole) & 1 : 0), half};
+}
 
 template <bool F16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -461,8 +465,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint32_t ph = 0;
       bool ok = true;
       for (int tile = first; ok && tile < a.tiles; tile += step) {
-        const int pb = 2 * (tile % a.p_tiles) + rank, q0 = 2 * (tile / a.p_tiles);  // row blocks
-        const int blocks = (pb < a.sp_blocks) + 1 + (q0 + 1 < a.sq_blocks);
+        const Tile2 t = tile2(a, tile);
+        const int pb = 2 * t.pt + rank, q0 = t.q0, q_row = q0 * kRows + rank * (t.half ? kRows / 2 : kRows);
+        const bool two = !t.half && q0 + 1 < a.sq_blocks;
+        const int blocks = (pb < a.sp_blocks) + (q0 < a.sq_blocks) + two;
         for (int ks = 0; ks < a.ksteps; ++ks, ++g) {
           if (!thread_wait(&empty[s], ph ^ 1, ctl, kErrWaitProducer)) {
             ok = false;
@@ -473,10 +479,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint8_t* sc = gbase + s * kStage2 + 2 * kRows * kStepBytes;
           mbar_arrive_expect_tx(&full[s], 2 * kRows * kStepBytes + blocks * groups);
           tma_load_2d(at, &map_p, ks * kStepBytes, pb * kRows, &full[s]);
-          tma_load_2d(at + kRows * kStepBytes, &map_q, ks * kStepBytes, (q0 + rank) * kRows, &full[s]);
+          tma_load_2d(at + kRows * kStepBytes, &map_q, ks * kStepBytes, q_row, &full[s]);  // a half uses the first 64 rows
           if (pb < a.sp_blocks) bulk_copy_g2s(sc, a.sp + (pb * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
-          bulk_copy_g2s(sc + 2 * kScaleTile, a.sq + (q0 * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
-          if (q0 + 1 < a.sq_blocks) bulk_copy_g2s(sc + 4 * kScaleTile, a.sq + ((q0 + 1) * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
+          if (q0 < a.sq_blocks) bulk_copy_g2s(sc + 2 * kScaleTile, a.sq + (q0 * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
+          if (two) bulk_copy_g2s(sc + 4 * kScaleTile, a.sq + ((q0 + 1) * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
           if (++s == kStages2) {
             s = 0;
             ph ^= 1;
@@ -507,7 +513,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
     const uint64_t s_desc = plain_desc(base + 2 * kRows * kStepBytes);
     const uint32_t wide = static_cast<uint32_t>(kRows >> 4) << 24;  // M = 256
-    const uint32_t i_desc0 = instruction_desc(256, 0u) + wide, i_desc1 = instruction_desc(256, 2u) + wide;
     int i = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -533,6 +538,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
       if (i > 0 && !wait(&drained[(i - 1) & 1], &drained[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
       const uint32_t d = tmem + ((i & 1) ? kAcc2 : 0);
+      const int T = tile >= a.whole ? 128 : 256;
+      const uint32_t i_desc0 = instruction_desc(T, 0u) + wide, i_desc1 = instruction_desc(T, 2u) + wide;
       for (int ks = 0; ks < a.ksteps; ++ks) {
         if (!wait(&full[s], &peer[s], ph)) {
           ok = false;
@@ -575,22 +582,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr int kChunks = 16, kSharedChunks = kShared2 / 16;
     int i = 0;
     for (int tile = first; tile < a.tiles; tile += step, ++i) {
-      const int b = i & 1, p = (2 * (tile % a.p_tiles) + rank) * kRows + 32 * q + lane, q0 = tile / a.p_tiles * 256;
+      const Tile2 t = tile2(a, tile);
+      const int b = i & 1, p = (2 * t.pt + rank) * kRows + 32 * q + lane, q0 = t.q0 * kRows;
       if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
       tc_fence_after();
-      bool told = false;
-      for (int at = c; at < kChunks; at += 2) {
-        if (!told && at >= kSharedChunks) {  // what the next tile's accumulator shares with this one has been read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(&drained[b], 0);
-          told = true;
-        }
-        const int col = 16 * (b ? at : kChunks - 1 - at);
+      // What the next tile's accumulator shares with this one is read before anything is stored: the next tile's MMAs
+      // wait for it.
+      constexpr int kHeld = (kSharedChunks + 1) / 2;
+      const int chunks = t.half ? kChunks / 2 : kChunks;
+      auto column = [&](int chunk) { return 16 * (b ? chunk : chunks - 1 - chunk); };
+      uint32_t held[kHeld][16];
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h)
+        if (c + 2 * h < chunks) tmem_ld16(tmem + lane_addr + (b ? kAcc2 : 0) + column(c + 2 * h), held[h]);
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) tmem_wait_ld16(held[h]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(&drained[b], 0);
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h)
+        if (p < a.p_rows && c + 2 * h < chunks) store_row<F16>(a, p, q0 + column(c + 2 * h), held[h]);
+#pragma unroll 1
+      for (int at = c + 2 * kHeld; at < chunks; at += 2) {
         uint32_t v[16];
-        tmem_ld16(tmem + lane_addr + (b ? kAcc2 : 0) + col, v);
+        tmem_ld16(tmem + lane_addr + (b ? kAcc2 : 0) + column(at), v);
         tmem_wait_ld16(v);
-        if (p < a.p_rows) store_row<F16>(a, p, q0 + col, v);
+        if (p < a.p_rows) store_row<F16>(a, p, q0 + column(at), v);
       }
     }
   }
@@ -658,9 +676,11 @@ cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, 
   return cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<SWAP, F16, QB>, mp, mq, a);
 }
 
-// Pairs take a call that fills three quarters of the SMs with 256 x 256 tiles.
+// Pairs take what would need a second round of 128 x 256 tiles. Measured (us with the launch, one CTA a tile / pairs):
+// 256 x 14336 x 4096 20.5 / 20.6, 1024 x 4096 x 14336 36.9 / 38.9, 1152 x 4096 x 4096 (144 tiles) 18.4 / 24.6;
+// 2048 x 14336 x 4096 78.8 / 66, 4096 x 8192 x 8192 132 / 124, 8192 x 28672 x 8192 852 / 776.
 bool pairs_pay(const Mxfp4Matmul& p, int sms) {
-  return ceil_div(p.M, 256) * ceil_div(p.N, 256) * 2 * 4 >= static_cast<int64_t>(sms) * 3;
+  return p.M > kRows && ceil_div(p.M, kRows) * ceil_div(p.N, 256) > sms;
 }
 
 template <bool F16>
@@ -675,7 +695,11 @@ cudaError_t launch_pairs(const Mxfp4Matmul& p, Args a, bool early, cudaStream_t 
   a.p_tiles = static_cast<int>(ceil_div(p.M, 256));
   const int64_t tiles = a.p_tiles * ceil_div(p.N, 256);
   if (tiles > INT_MAX / 8) return cudaErrorInvalidValue;
-  a.tiles = static_cast<int>(tiles);
+  // A last round with few tiles takes them in halves (2048 x 14336 x 4096, 448 tiles on 74 pairs: 69.7 -> 67.6 us).
+  const int pairs = device_sm_count() / 2, rest = static_cast<int>(tiles % pairs);
+  const bool halve = tiles > pairs && 2 * rest <= pairs;
+  a.whole = static_cast<int>(halve ? tiles - rest : tiles);
+  a.tiles = static_cast<int>(halve ? tiles + rest : tiles);
   a.tiles_k = ceil_div(p.kb, 4);
   a.sp_blocks = static_cast<int>(ceil_div(p.M, kRows));
   a.sq_blocks = static_cast<int>(ceil_div(p.N, kRows));
@@ -691,7 +715,6 @@ cudaError_t launch_pairs(const Mxfp4Matmul& p, Args a, bool early, cudaStream_t 
   if (!encode_tensor_map_2d(&mp, 0, p.a, row, a.p_rows, row, kStepBytes, kRows, true) ||
       !encode_tensor_map_2d(&mq, 0, p.b, row, a.q_rows, row, kStepBytes, kRows, true))
     return cudaErrorInvalidValue;
-  const int pairs = device_sm_count() / 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (a.tiles < pairs ? a.tiles : pairs));
   cfg.blockDim = dim3(kThreads);
@@ -755,10 +778,8 @@ cudaError_t launch_mxfp4_matmul(const Mxfp4Matmul& p, bool early, cudaStream_t s
   a.stages = stages;
   // Tensor memory: accumulators, then the stages' scales.
   const int sf = stages * a.sf_stage;
-  const int acc = one_tile ? a.T : 2 * a.T;
-  a.shared_cols = acc + sf > kTmemCols ? acc + sf - kTmemCols : 0;
-  a.acc1 = one_tile ? 0 : a.T - a.shared_cols;
-  a.sf_col = acc - a.shared_cols;
+  a.acc1 = one_tile ? 0 : a.T;
+  a.sf_col = a.acc1 + a.T;
   a.tmem_cols = 32;
   while (a.tmem_cols < a.sf_col + sf) a.tmem_cols *= 2;
   // CTAs that share an SM share its 512 columns: ask for enough shared memory that no more fit than those feed.
