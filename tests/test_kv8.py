@@ -142,6 +142,27 @@ def test_append_borders_round_to_even(F, code):
 
 @gpu
 @pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("size", [2.0 ** -149, 2.0 ** -142, 2.0 ** -130, 1e-30, 2.0 ** -58, 2.0 ** -52, 1e25, 3e38])
+def test_append_extreme_magnitudes(F, code, size):
+    """Scales that are subnormal, or whose reciprocals leave the normal range; older codes under them."""
+    g = torch.Generator().manual_seed(7)
+    for past in (0, 9):
+        c = R.Cache([past + 40], heads=2, D=64, page=32, code=code)
+        if past:
+            c.ks[c.table[0, 0]] = float(np.float32(size * 2.0 ** -9))
+            c.vs[c.table[0, 0]] = float(np.float32(size * 2.0 ** -7))
+        dev = c.cuda()
+        k, v = ((torch.rand(40, 2, 64, generator=g, dtype=torch.float64) * 2 - 1) * size * f for f in (1.0, 250.0 if size < 1e30 else 0.3))
+        k, v = k.float(), v.float()
+        F.kv8_append(k.cuda(), v.cuda(), *dev, _cu([40]).cuda(), c.lens.cuda())
+        R.append(c, k, v, _cu([40]))
+        for i in (0, 1):
+            assert torch.equal(dev[i + 2].cpu(), (c.ks, c.vs)[i])
+            assert torch.equal(dev[i].cpu().float(), (c.k, c.v)[i].float())
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
 def test_append_token_by_token_rescales(F, code):
     """Growing values rescale a page again and again; the state stays the definition's."""
     c = R.Cache([0], heads=2, D=64, page=32, code=code, max_extra=3)

@@ -17,12 +17,12 @@ namespace {
 
 constexpr int kThreads = 128;
 
-// Codes round(x / s) of 8 values, s > 0 and finite, |x| <= L s up to rounding. A product with 1 / s lies within 2 ulp of
+// Codes round(x / s) of 8 values, s > 0 and finite, |x| <= L s up to s's rounding. A product with 1 / s lies within 2 ulp of
 // x / s (inv = 0, where that would leave the normal range: a division). Only where a border between two codes is nearer
 // than that is the remainder looked at; the inputs being short numbers, a third of the warps have such a value. (A
 // division a value costs 40 instructions and bounded the kernel: 20 us for 17 M values.)
 template <bool E4M3>
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, float inv) {
+__device__ __forceinline__ uint2 codes8(float (&v)[8], float s, float inv) {
   uint32_t w[2] = {0, 0};
   float q[8];
   if (inv != 0.0f) {
@@ -30,7 +30,10 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, float inv)
     for (int e = 0; e < 8; ++e) q[e] = v[e] * inv;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = v[e] / s;
+    for (int e = 0; e < 8; ++e) {
+      if (!E4M3) v[e] = fminf(fmaxf(v[e], -127.0f * s), 127.0f * s);  // a subnormal s may be far below |x| / 127
+      q[e] = v[e] / s;
+    }
   }
   if (E4M3) {
     uint32_t least = ~0u;
@@ -51,7 +54,6 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, float inv)
       w[e >> 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(q[e], q[e + 1]), __NV_SATFINITE, __NV_E4M3)) << (8 * (e & 2));
   } else {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the rounded integer
-    const float h = 0.5f * s;
     float most = 0.0f;
     uint32_t t[8];
 #pragma unroll
@@ -61,12 +63,13 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, float inv)
       q[e] = fmaf(kMagic - m, s, v[e]);  // the remainder, exactly
       most = fmaxf(most, fabsf(q[e]));
     }
-    if (!(most < h)) {
+    if (!(most + most < s)) {  // twice the remainder: half of a subnormal s would be rounded
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool odd = t[e] & 1u;
-        if (q[e] > h || (q[e] == h && odd)) ++t[e];
-        else if (q[e] < -h || (q[e] == -h && odd)) --t[e];
+        const float r = q[e] + q[e];
+        if (r > s || (r == s && odd)) ++t[e];
+        else if (r < -s || (r == -s && odd)) --t[e];
       }
     }
 #pragma unroll
