@@ -509,7 +509,7 @@ XRGPU_API int xrgpu_mxfp4_workspace_size(const xrgpu_mxfp4_problem* p, uint64_t*
  * demand). Calls sharing a workspace must not overlap on the GPU. */
 XRGPU_API int xrgpu_mxfp4_forward(const xrgpu_mxfp4_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
 
-/* Paged key/value cache of 8-bit codes, one float32 scale for each page of each head: value = code * scale.
+/* Paged key/value cache of 8-bit codes, one float32 scale >= 0 for each page of each head: value = code * scale.
  *   k_cache, v_cache [pages, heads_kv, page, head_dim] of int8 or float8 e4m3, 16-byte aligned;
  *   k_scale, v_scale [pages, heads_kv]; page 16, 32, 64 or 128 tokens; head_dim 64 or 128.
  * Sequence b holds kv_len[b] tokens, token j in page page_table[b][j / page], slot j % page. The rows of a

@@ -320,6 +320,22 @@ def test_rows_behind_the_last_sequence_are_left(F, dtype, new):
 
 
 @gpu
+def test_rows_without_sequences_are_zero(F):
+    c = R.Cache([3], heads=2, D=64, page=16, code=INT8).cuda()
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table, cu = none.view(0, 4), torch.zeros(1, dtype=torch.int32, device="cuda")
+    junk = [torch.full((5, 4, 64), float("nan"), device="cuda") for _ in range(3)]  # what the allocator hands out next
+    del junk
+    q = torch.randn(5, 4, 64, device="cuda")
+    assert not F.attention_kv8(q, *c[:4], table, cu, none).any()
+    k, v = F.kv8_read(*c[:4], table, cu, none, rows=5, dtype=torch.float32)
+    assert not k.any() and not v.any()
+    out = torch.ones_like(q)
+    F.attention_kv8(q, *c[:4], table, cu, none, out=out)
+    assert bool((out == 1).all())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_attention_extreme_scores_and_scales(F, dtype):
     """One token that takes all the weight, scores in the thousands, and value blocks of scales 2^20 apart."""

@@ -20,7 +20,7 @@ constexpr int kThreads = 128;
 // Codes round(x / s) of 8 values, s > 0 and finite, |x| <= L s up to s's rounding. A product with 1 / s lies within 2 ulp of
 // x / s (inv = 0, where that would leave the normal range: a division). Only where a border between two codes is nearer
 // than that is the remainder looked at; the inputs being short numbers, a third of the warps have such a value. (A
-// division a value costs 40 instructions and bounded the kernel: 20 us for 17 M values.)
+// division a value costs 40 instructions and bounded the kernel: 20 us for 11 M values.)
 template <bool E4M3>
 __device__ __forceinline__ uint2 codes8(float (&v)[8], float s, float inv) {
   uint32_t w[2] = {0, 0};
@@ -180,8 +180,8 @@ __device__ __forceinline__ int touched_pages(const Kv8& p, int b) {
 }
 
 // CTA (slot, two blocks): slot counts the touched pages of all sequences in order; two warps each take a block (a head's K
-// or V), so that two share the search for the sequence. Five sequences of 1700 tokens, 8 heads of 128 halves, pages of 32, e4m3
-// (52 MB): 12.8 us, 4.1 TB/s (a warp a block 13.9, four 14.5); 64 single tokens into pages of 64: 3.5 us (3.9, 4.2), a chain
+// or V), so that two share the search for the sequence. 5400 tokens of five sequences, 8 heads of 128 halves, pages of 32, e4m3
+// (33 MB): 12.8 us, 2.6 TB/s (a warp a block 13.9, four 14.5); 64 single tokens into pages of 64: 3.5 us (3.9, 4.2), a chain
 // of dependent loads. Bound by latency and instructions (half of the issue slots). Held in registers between the passes,
 // the values cost more occupancy than reading them again from the L1 cache does (15.6 us).
 template <bool E4M3, bool F16, bool VEC, int D>
@@ -292,8 +292,8 @@ __device__ __forceinline__ int sequence_of(const Kv8& p, int row, int lane) {
   return -1;
 }
 
-// One warp a (row, side), all heads: PER codes a lane. 8500 rows of 8 heads of 128 halves (52 MB): 8.7 us, 6.0 TB/s from a warm
-// L2 (13.2 with halves stored one by one).
+// One warp a (row, side), all heads: PER codes a lane. 5500 rows of 8 heads of 128 halves (34 MB): 8.7 us, 3.9 TB/s (13.2 with
+// halves stored one by one).
 template <bool E4M3, bool F16, int PER, bool VEC>
 __global__ void __launch_bounds__(256) read_kernel(const Kv8 p) {
   constexpr int D = 32 * PER;

@@ -72,6 +72,13 @@ int launched(cudaError_t e) {
   return XRGPU_OK;
 }
 
+// Without sequences every row belongs to none.
+cudaError_t zero_rows(const Kv8& p, void* rows, int64_t stride, int heads, cudaStream_t s) {
+  const size_t es = p.f16 ? 2 : 4, width = static_cast<size_t>(heads) * p.D * es;
+  if (!rows || !p.zero_rest || !p.tokens || p.seqs) return cudaSuccess;
+  return cudaMemset2DAsync(rows, static_cast<size_t>(stride) * es, 0, width, p.tokens, s);
+}
+
 }  // namespace
 }  // namespace xrgpu
 
@@ -89,8 +96,12 @@ int xrgpu_kv8_read(const xrgpu_kv8_problem* c, void* stream) {
   xrgpu::Kv8 p;
   const int st = xrgpu::convert(c, xrgpu::kRead, &p);
   if (st) return st;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = xrgpu::zero_rows(p, p.k, p.ks, p.hkv, s);
+  if (e == cudaSuccess) e = xrgpu::zero_rows(p, p.v, p.vs, p.hkv, s);
+  if (e != cudaSuccess) return xrgpu::launched(e);
   p.err = xrgpu::device_error_word();
-  return xrgpu::launched(xrgpu::launch_kv8_read(p, static_cast<cudaStream_t>(stream)));
+  return xrgpu::launched(xrgpu::launch_kv8_read(p, s));
 }
 
 int xrgpu_kv8_attention_workspace_size(const xrgpu_kv8_problem* c, uint64_t* bytes) {
@@ -105,7 +116,7 @@ int xrgpu_kv8_attention(const xrgpu_kv8_problem* c, void* ws, uint64_t ws_bytes,
   xrgpu::Kv8 p;
   int st = xrgpu::convert(c, xrgpu::kAttention, &p);
   if (st) return st;
-  if (!p.tokens || !p.seqs) return XRGPU_OK;
+  if (!p.tokens || !p.seqs) return xrgpu::launched(xrgpu::zero_rows(p, p.o, p.os, p.hq, static_cast<cudaStream_t>(stream)));
   const uint64_t need = xrgpu::kv8_attention_workspace(p);
   if (need) {
     if (!ws) {

@@ -1,4 +1,4 @@
-"""Zero-copy PyTorch entry points over the C ABI (``xrgpu_mmnb_forward``).
+"""Zero-copy PyTorch entry points over the C ABI (``xrgpu_mmnb_forward``, ``xrgpu_mxfp4_*``, ``xrgpu_kv8_*``, ...).
 
 Tensors stay on the device; the kernels run on the current torch CUDA stream. torch
 supplies device memory and streams only: every numerical step runs in this package's
