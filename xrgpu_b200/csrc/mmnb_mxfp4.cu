@@ -37,14 +37,35 @@ __device__ __forceinline__ float e2m1_value(uint32_t c) {
 constexpr int kQuantWarps = 8;
 constexpr int kChunk = 256;  // values of a row that a warp takes at a time: 8 a lane, 4 lanes a block
 
+// The (row, chunk) pairs of a warp, in order, a grid's warps apart. Stepped by its quotient and remainder: a 64-bit division
+// an item made 2048 x 14336 halves take 23.8 us (dequantised 19.9).
+struct Walk {
+  int64_t row, rows_step;
+  int chunk, chunk_step;
+  __device__ explicit Walk(int chunks) {
+    const unsigned n = static_cast<unsigned>(chunks), at = blockIdx.x * kQuantWarps + (threadIdx.x >> 5), step = gridDim.x * kQuantWarps;
+    row = at / n;
+    chunk = static_cast<int>(at % n);
+    rows_step = step / n;
+    chunk_step = static_cast<int>(step % n);
+  }
+  __device__ void next(int chunks) {
+    row += rows_step;
+    chunk += chunk_step;
+    if (chunk >= chunks) {
+      chunk -= chunks;
+      ++row;
+    }
+  }
+};
+
 // One warp a (row, chunk); rows beyond the matrix up to the tile's end only zero their scales.
 template <bool F16, bool VEC>
-__global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Quantize p, int64_t chunks, int64_t items) {
+__global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Quantize p, int chunks, int64_t rows) {
   const int lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's weights may start to load
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kQuantWarps + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * kQuantWarps) {
-    const int64_t row = it / chunks, k0 = (it % chunks) * kChunk + lane * 8;
+  for (Walk w(chunks); w.row < rows; w.next(chunks)) {
+    const int64_t row = w.row, k0 = static_cast<int64_t>(w.chunk) * kChunk + lane * 8;
     float v[8];
     uint32_t amax = 0;
 #pragma unroll
@@ -98,11 +119,10 @@ __global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Q
 
 // Four lanes a block, 8 values each; one word of four scales serves 16 lanes.
 template <bool F16, bool VEC>
-__global__ void __launch_bounds__(kQuantWarps * 32) dequantize_kernel(const Mxfp4Dequantize p, int64_t chunks, int64_t items) {
+__global__ void __launch_bounds__(kQuantWarps * 32) dequantize_kernel(const Mxfp4Dequantize p, int chunks) {
   const int lane = threadIdx.x & 31;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kQuantWarps + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * kQuantWarps) {
-    const int64_t row = it / chunks, k0 = (it % chunks) * kChunk + lane * 8, blk = k0 >> 5;
+  for (Walk at_item(chunks); at_item.row < p.rows; at_item.next(chunks)) {
+    const int64_t row = at_item.row, k0 = static_cast<int64_t>(at_item.chunk) * kChunk + lane * 8, blk = k0 >> 5;
     if (blk >= p.kb || k0 >= p.K) continue;
     const uint32_t w = reinterpret_cast<const uint32_t*>(p.codes + (row * p.kb + blk) * 16)[lane & 3];
     const float s = pow2_of_byte(p.scales[scale_offset(row, blk, p.kb)]);
@@ -160,11 +180,11 @@ cudaError_t launch_mxfp4_quantize(const Mxfp4Quantize& p, cudaStream_t s) {
   const int64_t es = p.f16 ? 2 : 4;
   const bool vec = aligned16(p.x) && (p.ldx * es) % 16 == 0;
   if (p.f16) {
-    if (vec) quantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
-    else quantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    if (vec) quantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks), rows);
+    else quantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks), rows);
   } else {
-    if (vec) quantize_kernel<false, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
-    else quantize_kernel<false, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    if (vec) quantize_kernel<false, true><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks), rows);
+    else quantize_kernel<false, false><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks), rows);
   }
   return cudaGetLastError();
 }
@@ -175,11 +195,11 @@ cudaError_t launch_mxfp4_dequantize(const Mxfp4Dequantize& p, cudaStream_t s) {
   const int grid = grid_for(ceil_div(items, kQuantWarps), 8);
   const bool vec = aligned16(p.out) && p.K % 8 == 0;
   if (p.f16) {
-    if (vec) dequantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
-    else dequantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    if (vec) dequantize_kernel<true, true><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks));
+    else dequantize_kernel<true, false><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks));
   } else {
-    if (vec) dequantize_kernel<false, true><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
-    else dequantize_kernel<false, false><<<grid, kQuantWarps * 32, 0, s>>>(p, chunks, items);
+    if (vec) dequantize_kernel<false, true><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks));
+    else dequantize_kernel<false, false><<<grid, kQuantWarps * 32, 0, s>>>(p, static_cast<int>(chunks));
   }
   return cudaGetLastError();
 }
