@@ -319,6 +319,105 @@ def test_rows_behind_the_last_sequence_are_left(F, dtype, new):
     assert torch.equal(fresh[:sum(new)], out[:sum(new)]) and bool((fresh[sum(new):] == 0).all())
 
 
+# Calls with enough rows for the prompt kernel: the key/value heads that it takes.
+def _heads(new, G, D):
+    B = len(new)
+    rows = -(-sum(new) // B) * G
+    heads = 1
+    while B * heads * rows * D < 6500 * 128 * -(-(B * heads * -(-rows // 256)) // 148):
+        heads += 1
+    assert rows > 64
+    return heads
+
+
+PROMPTS = [
+    ([200], [200], {}), ([77, 530], [33, 130], {}), ([700, 30, 1], [260, 30, 1], {}), ([40, 0, 290], [40, 0, 150], {}),
+    ([333, 20], [150, 20], {"window": 100}), ([300], [140], {"window": 7}), ([333, 300], [100, 260], {"window": 1}),
+    ([200, 7], [120, 7], {"causal": False, "scale": 0.05}), ([90], [150], {"causal": False}), ([290], [150], {"scale": -0.1}),
+    ([0, 50], [150, 180], {}),  # more rows than tokens
+]
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("D,page,G", [(128, 64, 4), (64, 16, 5), (128, 32, 2), (64, 128, 3)])
+@pytest.mark.parametrize("lens,new,kw", PROMPTS)
+def test_prompts(F, code, D, page, G, lens, new, kw):
+    heads = _heads(new, G, D)
+    c = R.Cache(lens, heads=heads, D=D, page=page, code=code, seed=D + G)
+    c.poison_tails()
+    _check(F, c, new, G * heads, torch.float16, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+def test_prompts_extreme_scores_and_scales(F, code):
+    new = [260, 150]
+    heads = _heads(new, 4, 64)
+    c = R.Cache([500, 300], heads=heads, D=64, page=16, code=code)
+    c.vs *= torch.exp2(torch.randint(-10, 10, c.vs.shape, generator=torch.Generator().manual_seed(1)).float())
+    c.ks[::3] *= 40.0
+    _check(F, c, new, 4 * heads, torch.float16)
+    c.ks.zero_()
+    c.vs[::2] = 0.0
+    _check(F, c, new, 4 * heads, torch.float16)
+
+
+@gpu
+def test_prompts_leave_rows_and_repeat(F):
+    """Strided queries and results, rows behind the last sequence, no cu_seqlens, the same bits on every call."""
+    new = [130, 130]
+    heads = _heads(new, 2, 128)
+    c = R.Cache([150, 200], heads=heads, D=128, page=64, code=INT8)
+    dev, hq, n = c.cuda(), 2 * heads, 260
+    wide = torch.randn(n + 9, hq * 128 + 24, device="cuda", dtype=torch.float16)
+    wide[n:] = float("nan")
+    q = wide[:, 3:3 + hq * 128].unflatten(1, (hq, 128))
+    out = torch.full((n + 9, hq * 128 + 40), 3.0, device="cuda", dtype=torch.float16)[:, 5:5 + hq * 128].unflatten(1, (hq, 128))
+    F.attention_kv8(q, *dev, _cu(new).cuda(), c.lens.cuda(), out=out)
+    assert bool((out[n:] == 3.0).all()) and bool(torch.isfinite(out[:n]).all())
+    fresh = F.attention_kv8(q, *dev, _cu(new).cuda(), c.lens.cuda())
+    assert torch.equal(fresh[:n], out[:n]) and bool((fresh[n:] == 0).all())
+    assert torch.equal(F.attention_kv8(q[:n].contiguous(), *dev, None, c.lens.cuda()), out[:n])
+    _check(F, c, new, hq, torch.float16, q=q[:n].cpu().contiguous(), uniform=True)
+
+
+@gpu
+def test_prompts_nan_blocks_reach_their_readers_only(F):
+    new = [1, 170]
+    heads = _heads(new, 2, 64)
+    c = R.Cache([100, 180], heads=heads, D=64, page=16, code=INT8)
+    q = torch.randn(sum(new), 2 * heads, 64, device="cuda", dtype=torch.float16)
+    for side, keep in (("vs", 1.0), ("ks", 0.02)):
+        for b, rows in ((0, slice(0, 1)), (1, slice(1 + 22, 171))):  # page 2 of the prompt: its rows from position 32 on
+            at = getattr(c, side)
+            at[c.table[b, 2], 1] = float("nan")
+            o = F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda())
+            nan = torch.isnan(o)
+            want = torch.zeros_like(nan)
+            want[rows, 2:4] = True
+            assert torch.equal(nan, want)
+            at[c.table[b, 2], 1] = keep
+
+
+@gpu
+def test_prompts_bad_pages_are_skipped(F):
+    new = [150, 150]
+    heads = _heads(new, 2, 64)
+    c = R.Cache([170, 170], heads=heads, D=64, page=16, code=INT8)
+    q = torch.randn(300, 2 * heads, 64, device="cuda", dtype=torch.float16)
+    whole = F.attention_kv8(q, *c.cuda(), None, c.lens.cuda())
+    for bad in (-1, c.k.shape[0], 2 ** 31 - 1):
+        c.table[0, 1] = bad
+        o = F.attention_kv8(q, *c.cuda(), None, c.lens.cuda())
+        assert F.device_error(0) == 0x501
+        assert bool(torch.isfinite(o).all()) and torch.equal(o[150:], whole[150:])
+    for bad in (-3, 10 ** 6):
+        c.lens[0] = bad
+        o = F.attention_kv8(q, *c.cuda(), None, c.lens.cuda())
+        assert F.device_error(0) == 0x502 and torch.equal(o[150:], whole[150:]) and bool((o[:150] == 0).all())
+
+
 @gpu
 def test_rows_without_sequences_are_zero(F):
     c = R.Cache([3], heads=2, D=64, page=16, code=INT8).cuda()

@@ -28,17 +28,20 @@ __device__ __forceinline__ float pow2_of_byte(uint32_t e) {  // 2^(e - 127), e =
   return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(e ? e << 23 : 1u << 22);
 }
 
-// Code (4 bits) to its value: exponent and mantissa bits in place of a float32's make 2^-126 of it (the code
-// without exponent a subnormal, so exactly), the sign bit goes to the top.
-__device__ __forceinline__ float e2m1_value(uint32_t c) {
-  return __uint_as_float(((c & 7u) << 22) | ((c & 8u) << 28)) * __uint_as_float(253u << 23);
+// The two values of a byte of codes.
+__device__ __forceinline__ float2 from_e2m1x2(uint32_t byte) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(r) : "r"(byte));
+  return __half22float2(*reinterpret_cast<const __half2*>(&r));
 }
 
 constexpr int kQuantWarps = 8;
-constexpr int kChunk = 256;  // values of a row that a warp takes at a time: 8 a lane, 4 lanes a block
+constexpr int kPer = 16;           // values of a lane: two lanes a block
+constexpr int kChunk = 32 * kPer;  // values of a row that a warp takes at a time
 
-// The (row, chunk) pairs of a warp, in order, a grid's warps apart. Stepped by its quotient and remainder: a 64-bit division
-// an item made 2048 x 14336 halves take 23.8 us (dequantised 19.9).
+// The (row, chunk) pairs of a warp, in order, a grid's warps apart, stepped by its quotient and remainder. What bounds
+// these kernels is instructions, not their bytes: 2048 x 14336 halves (74 MB) took 23.8 us (dequantised 19.9) with a 64-bit division
+// an item, 22.4 (18.1) without, 14.2 (17.0; 5.2 and 4.4 TB/s) with 16 values a lane instead of 8 and maxima of pairs of halves.
 struct Walk {
   int64_t row, rows_step;
   int chunk, chunk_step;
@@ -65,88 +68,100 @@ __global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Q
   const int lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's weights may start to load
   for (Walk w(chunks); w.row < rows; w.next(chunks)) {
-    const int64_t row = w.row, k0 = static_cast<int64_t>(w.chunk) * kChunk + lane * 8;
-    float v[8];
+    const int64_t row = w.row, k0 = static_cast<int64_t>(w.chunk) * kChunk + lane * kPer;
+    float v[kPer];
     uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int i = 0; i < kPer; ++i) v[i] = 0.0f;
     if (row < p.rows && k0 < p.K) {
-      if (VEC && k0 + 8 <= p.K) {
-        if (F16) {
-          const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + row * p.ldx + k0);
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      if (VEC && k0 + kPer <= p.K) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.x) + (row * p.ldx + k0) * (F16 ? 2 : 4));
+        uint4 raw[F16 ? 2 : 4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        for (int i = 0; i < (F16 ? 2 : 4); ++i) raw[i] = src[i];
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(raw);
+        if (F16) {
+          __half2 m = __float2half2_rn(0.0f);  // pairs as they are: half the instructions
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i) {
+            const __half2 h = *reinterpret_cast<const __half2*>(&u[i]);
+            m = __hmax2_nan(m, __habs2(h));
+            const float2 f = __half22float2(h);
             v[2 * i] = f.x;
             v[2 * i + 1] = f.y;
           }
+          amax = __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))) & 0x7fffffffu;
         } else {
-          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + row * p.ldx + k0);
-          const float4 f0 = src[0], f1 = src[1];
-          v[0] = f0.x; v[1] = f0.y; v[2] = f0.z; v[3] = f0.w;
-          v[4] = f1.x; v[5] = f1.y; v[6] = f1.z; v[7] = f1.w;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) v[i] = __uint_as_float(u[F16 ? 0 : i]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kPer; ++i)
           if (k0 + i < p.K) v[i] = load_f(p.x, F16, row * p.ldx + k0 + i);
       }
     }
+    if (!(F16 && VEC) || k0 + kPer > p.K) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);  // NaN > Inf > finite as bits
+      for (int i = 0; i < kPer; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);  // NaN > Inf > finite as bits
+    }
     amax = max(amax, __shfl_xor_sync(~0u, amax, 1));
-    amax = max(amax, __shfl_xor_sync(~0u, amax, 2));
     const uint32_t field = amax >> 23;
     const bool bad = field == 255u;
     const uint32_t e = bad ? 255u : (field > 2u ? field - 2u : 0u);
     const float inv = bad ? 0.0f : __uint_as_float((254u - e) << 23);  // 2^(127 - e); e <= 252 here
-    uint32_t c = 0;
+    uint32_t c[2] = {0, 0};
     if (!bad) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c |= to_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+      for (int i = 0; i < kPer / 2; ++i) c[i >> 2] |= to_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * (i & 3));
     }
     const int64_t blk = k0 >> 5;
-    if (row < p.rows && blk < p.kb) reinterpret_cast<uint32_t*>(p.codes + (row * p.kb + blk) * 16)[lane & 3] = c;
-    // the four scale bytes of 16 lanes as one word
+    if (row < p.rows && blk < p.kb) *reinterpret_cast<uint2*>(p.codes + (row * p.kb + blk) * 16 + (lane & 1) * 8) = make_uint2(c[0], c[1]);
+    // the four scale bytes of 8 lanes as one word
     const uint32_t eb = (row < p.rows && blk < p.kb) ? e : 0u;
-    uint32_t word = eb << (8 * ((lane >> 2) & 3));
+    uint32_t word = eb << (8 * ((lane >> 1) & 3));
+    word |= __shfl_xor_sync(~0u, word, 2);
     word |= __shfl_xor_sync(~0u, word, 4);
-    word |= __shfl_xor_sync(~0u, word, 8);
-    if ((lane & 15) == 0 && (blk >> 2) < ((p.kb + 3) >> 2)) *reinterpret_cast<uint32_t*>(p.scales + scale_offset(row, blk, p.kb)) = word;
+    if ((lane & 7) == 0 && (blk >> 2) < ((p.kb + 3) >> 2)) *reinterpret_cast<uint32_t*>(p.scales + scale_offset(row, blk, p.kb)) = word;
   }
 }
 
-// Four lanes a block, 8 values each; one word of four scales serves 16 lanes.
+// The same pieces: two lanes a block.
 template <bool F16, bool VEC>
 __global__ void __launch_bounds__(kQuantWarps * 32) dequantize_kernel(const Mxfp4Dequantize p, int chunks) {
   const int lane = threadIdx.x & 31;
   for (Walk at_item(chunks); at_item.row < p.rows; at_item.next(chunks)) {
-    const int64_t row = at_item.row, k0 = static_cast<int64_t>(at_item.chunk) * kChunk + lane * 8, blk = k0 >> 5;
+    const int64_t row = at_item.row, k0 = static_cast<int64_t>(at_item.chunk) * kChunk + lane * kPer, blk = k0 >> 5;
     if (blk >= p.kb || k0 >= p.K) continue;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(p.codes + (row * p.kb + blk) * 16)[lane & 3];
+    const uint2 w = *reinterpret_cast<const uint2*>(p.codes + (row * p.kb + blk) * 16 + (lane & 1) * 8);
     const float s = pow2_of_byte(p.scales[scale_offset(row, blk, p.kb)]);
-    float v[8];
+    float v[kPer];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = e2m1_value((w >> (4 * j)) & 15u) * s;
+    for (int j = 0; j < kPer / 2; ++j) {
+      const float2 f = from_e2m1x2(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u);
+      v[2 * j] = f.x * s;
+      v[2 * j + 1] = f.y * s;
+    }
     const int64_t at = row * p.K + k0;
-    if (VEC) {
+    if (VEC && k0 + kPer <= p.K) {
       if (F16) {
-        uint32_t h[4];
+        uint32_t h[kPer / 2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kPer / 2; ++j) {
           const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
           h[j] = *reinterpret_cast<const uint32_t*>(&x);
         }
-        *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at);
+        dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
       } else {
         float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+        for (int j = 0; j < kPer / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kPer; ++j) {
         if (k0 + j >= p.K) break;
         if (F16) static_cast<__half*>(p.out)[at + j] = __float2half_rn(v[j]);
         else static_cast<float*>(p.out)[at + j] = v[j];
@@ -176,7 +191,7 @@ cudaError_t launch_mxfp4_quantize(const Mxfp4Quantize& p, cudaStream_t s) {
   const int64_t chunks = ceil_div(p.K, kChunk), rows = ceil_div(p.rows, 128) * 128, items = rows * chunks;
   if (items == 0) return cudaSuccess;
   const int grid = grid_for(ceil_div(items, kQuantWarps), 8);
-  // 16-byte loads of 8 values (a ragged end of a row is loaded one by one): the rows start on 16 bytes
+  // 16-byte loads (a ragged end of a row is loaded one by one): the rows start on 16 bytes
   const int64_t es = p.f16 ? 2 : 4;
   const bool vec = aligned16(p.x) && (p.ldx * es) % 16 == 0;
   if (p.f16) {
