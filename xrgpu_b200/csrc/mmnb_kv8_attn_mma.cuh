@@ -24,7 +24,10 @@
 // lengths on the device. A segment that lies inside one CTA's run is finished there, one that is cut leaves
 // partial results (m, l, O) in the workspace, which combine_kernel joins in the order of the CTAs. Where few short
 // segments leave most SMs idle, a cluster of up to 8 CTAs shares each segment instead and joins it through shared
-// memory: one launch (one token of one sequence of 2048: 16 -> 11 us).
+// memory: one launch (one token of one sequence of 2048: 16 -> 10 us).
+//
+// Bound by the cache's stream, then by the instructions that widen its codes: one token of each of 32 ragged sequences (64 heads on 8
+// of 128, int8, 584 MB) 115 us, 5.1 TB/s; 64 sequences of 8192 200 us, 5.4 TB/s.
 #pragma once
 
 #include <cstdint>
