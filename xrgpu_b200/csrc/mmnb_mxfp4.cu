@@ -41,7 +41,8 @@ constexpr int kChunk = 32 * kPer;  // values of a row that a warp takes at a tim
 
 // The (row, chunk) pairs of a warp, in order, a grid's warps apart, stepped by its quotient and remainder. What bounds
 // these kernels is instructions, not their bytes: 2048 x 14336 halves (74 MB) took 23.8 us (dequantised 19.9) with a 64-bit division
-// an item, 22.4 (18.1) without, 14.2 (17.0; 5.2 and 4.4 TB/s) with 16 values a lane instead of 8 and maxima of pairs of halves.
+// an item, 22.4 (18.1) without, 14.2 (17.0) with 16 values a lane instead of 8 and maxima of pairs of halves; 14.0 (5.3 TB/s)
+// dequantised with the 16 in two pieces.
 struct Walk {
   int64_t row, rows_step;
   int chunk, chunk_step;
@@ -126,45 +127,54 @@ __global__ void __launch_bounds__(kQuantWarps * 32) quantize_kernel(const Mxfp4Q
   }
 }
 
-// The same pieces: two lanes a block.
+// The same chunks as two pieces of 8 values a lane, so that a warp writes a whole range at a time.
 template <bool F16, bool VEC>
 __global__ void __launch_bounds__(kQuantWarps * 32) dequantize_kernel(const Mxfp4Dequantize p, int chunks) {
+  constexpr int kPieces = 2, kEach = kPer / kPieces;
   const int lane = threadIdx.x & 31;
   for (Walk at_item(chunks); at_item.row < p.rows; at_item.next(chunks)) {
-    const int64_t row = at_item.row, k0 = static_cast<int64_t>(at_item.chunk) * kChunk + lane * kPer, blk = k0 >> 5;
-    if (blk >= p.kb || k0 >= p.K) continue;
-    const uint2 w = *reinterpret_cast<const uint2*>(p.codes + (row * p.kb + blk) * 16 + (lane & 1) * 8);
-    const float s = pow2_of_byte(p.scales[scale_offset(row, blk, p.kb)]);
-    float v[kPer];
+    const int64_t row = at_item.row, first = static_cast<int64_t>(at_item.chunk) * kChunk + lane * kEach;
+    uint32_t w[kPieces];
+    float s[kPieces];
 #pragma unroll
-    for (int j = 0; j < kPer / 2; ++j) {
-      const float2 f = from_e2m1x2(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u);
-      v[2 * j] = f.x * s;
-      v[2 * j + 1] = f.y * s;
+    for (int i = 0; i < kPieces; ++i) {
+      const int64_t k0 = first + i * 32 * kEach, blk = k0 >> 5;
+      if (k0 >= p.K) continue;
+      w[i] = reinterpret_cast<const uint32_t*>(p.codes + (row * p.kb + blk) * 16)[lane & 3];
+      s[i] = pow2_of_byte(p.scales[scale_offset(row, blk, p.kb)]);
     }
-    const int64_t at = row * p.K + k0;
-    if (VEC && k0 + kPer <= p.K) {
-      if (F16) {
-        uint32_t h[kPer / 2];
 #pragma unroll
-        for (int j = 0; j < kPer / 2; ++j) {
-          const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-          h[j] = *reinterpret_cast<const uint32_t*>(&x);
-        }
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at);
-        dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
-      } else {
-        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+    for (int i = 0; i < kPieces; ++i) {
+      const int64_t k0 = first + i * 32 * kEach, at = row * p.K + k0;
+      if (k0 >= p.K) continue;
+      float v[kEach];
 #pragma unroll
-        for (int j = 0; j < kPer / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      for (int j = 0; j < kEach / 2; ++j) {
+        const float2 f = from_e2m1x2((w[i] >> (8 * j)) & 255u);
+        v[2 * j] = f.x * s[i];
+        v[2 * j + 1] = f.y * s[i];
       }
-    } else {
+      if (VEC) {  // K is a multiple of 8
+        if (F16) {
+          uint32_t h[4];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        if (k0 + j >= p.K) break;
-        if (F16) static_cast<__half*>(p.out)[at + j] = __float2half_rn(v[j]);
-        else static_cast<float*>(p.out)[at + j] = v[j];
+          for (int j = 0; j < 4; ++j) {
+            const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            h[j] = *reinterpret_cast<const uint32_t*>(&x);
+          }
+          *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        } else {
+          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+          dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+          dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          if (k0 + j >= p.K) break;
+          if (F16) static_cast<__half*>(p.out)[at + j] = __float2half_rn(v[j]);
+          else static_cast<float*>(p.out)[at + j] = v[j];
+        }
       }
     }
   }
