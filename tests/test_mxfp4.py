@@ -290,3 +290,27 @@ def test_refusals_on_device(F):
         F.matmul_mxfp4(x, c, s, out=torch.zeros(4, 5, device="cuda", dtype=torch.float16))
     with pytest.raises(ValueError, match="CUDA tensor"):
         F.matmul_mxfp4(x, c.cpu(), s)
+
+
+@pytest.mark.parametrize("a_blocks,b_blocks,rows", [(4, 2, 2), (2, 4, 4), (6, 5, 100)])
+@pytest.mark.parametrize("given_k", [False, True])
+def test_held_activations_of_another_k_are_refused(F, monkeypatch, a_blocks, b_blocks, rows, given_k):
+    """Codes of another number of blocks than the weights': refused on the host, nothing is launched. Their tiled scales'
+    shape may well be the one expected, and so may their number of bytes."""
+    calls = []
+    monkeypatch.setattr(F, "_device_of", lambda t, name: t.get_device())  # tensors on the CPU, as far as the launch
+    monkeypatch.setattr(F, "_launch", lambda *args: calls.append(args))
+    z = lambda *shape: torch.zeros(*shape, dtype=torch.uint8)  # noqa: E731
+    tiles = lambda r, kb: z(-(-r // 128), -(-kb // 4), 32, 4, 4)  # noqa: E731
+    K = b_blocks * 32 if given_k else None
+    b, b_scales = z(8, b_blocks, 16), tiles(8, b_blocks)
+    for scales in (tiles(rows, a_blocks), tiles(rows, b_blocks), tiles(rows * a_blocks // b_blocks, b_blocks)):
+        with pytest.raises(ValueError, match="differ in K"):
+            F.matmul_mxfp4(z(rows, a_blocks, 16), b, b_scales, a_scales=scales, K=K)
+    for shape in ((rows * b_blocks * 16,), (rows, b_blocks * 16), (rows, b_blocks, 8, 2)):
+        with pytest.raises(ValueError):
+            F.matmul_mxfp4(z(*shape), b, b_scales, a_scales=tiles(rows, b_blocks), K=K)
+    assert not calls
+    y = F.matmul_mxfp4(z(1, rows, b_blocks, 16), b, b_scales, a_scales=tiles(rows, b_blocks), K=K)
+    p = calls[0][2]._obj
+    assert y.shape == (1, rows, 8) and (p.M, p.N, p.K) == (rows, 8, b_blocks * 32) and len(calls) == 1

@@ -367,7 +367,7 @@ def _scale_shape(rows: int, kb: int):
 def _require_mxfp4(codes, scales, rows: int, kb: int, name: str, index: int):
     _on(codes, name, torch.uint8, index)
     _on(scales, name + "_scales", torch.uint8, index)
-    if codes.numel() != rows * kb * 16 or codes.shape[-1] != 16 or codes.dim() < 2:
+    if codes.dim() < 2 or tuple(codes.shape[-2:]) != (kb, 16) or codes.numel() != rows * kb * 16:
         raise ValueError(f"{name} must be [..., {kb}, 16] codes")
     if scales.shape != _scale_shape(rows, kb):
         raise ValueError(f"{name}_scales must be tiled scales of shape {list(_scale_shape(rows, kb))}")
@@ -439,6 +439,10 @@ def matmul_mxfp4(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias:
     lda = ldy = nbytes = 0
     bias_ptr = scales_ptr = ws = None
     if held:
+        if a.dim() < 2 or a.shape[-1] != 16:
+            raise ValueError("a must be [..., kb, 16] codes")
+        if a.shape[-2] != kb:
+            raise ValueError("a and b differ in K")
         lead = a.shape[:-2]
         M = a.numel() // (kb * 16) if kb else 0
         K = kb * 32 if K is None else int(K)
