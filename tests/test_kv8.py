@@ -608,3 +608,20 @@ def test_decoder_layer_prompt_then_tokens(F):
         yy = xo @ o_values.T
         assert (np.abs(y.cpu().double().numpy() - yy) <= (hq * D / 32 + 24) * 2.0 ** -23 * (np.abs(xo) @ np.abs(o_values).T)).all()
     assert F.device_error(0) == 0
+
+
+# ------------------------------------------------------------------------------------------ limits of what rows see
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30, 64])
+@pytest.mark.parametrize("lens,new", [([5], [9]), ([5, 60], [9, 3]), ([50], [180]), ([0, 50], [150, 180])])
+def test_the_largest_windows_see_everything(F, dtype, window, lens, new):
+    """Windows of as many tokens as a sequence holds are none, also where the first rows lie before the first token."""
+    G, D = 4, 64
+    heads = _heads(new, G, D) if max(new) > 100 else 2  # the long ones reach the prompt kernel with float16 rows
+    c = R.Cache(lens, heads=heads, D=D, page=16, code=INT8)
+    c.poison_tails()
+    got = _check(F, c, new, G * heads, dtype, window=window)
+    assert bool((got != 0).any())
+    q = torch.randn(sum(new), G * heads, D, generator=torch.Generator().manual_seed(sum(new) + G * heads)).to(dtype)
+    assert torch.equal(got, F.attention_kv8(q.cuda(), *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=0))

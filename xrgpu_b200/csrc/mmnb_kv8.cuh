@@ -47,6 +47,12 @@ __device__ __forceinline__ int page_id(const Kv8& p, int b, int j) {
   return id;
 }
 
+// First token that the row at position pos sees (a position before the first token is negative, a window may be
+// INT_MAX: their difference need not fit an int).
+__device__ __forceinline__ int window_from(const Kv8& p, int pos) {
+  return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
 __device__ __forceinline__ float e4m3_value(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
 }

@@ -151,9 +151,7 @@ __device__ __forceinline__ SeqWork seq_work(const Kv8& p, int b, int rows_per_ti
   w.r = seq_rows(p, b, true);
   const int G = p.hq / p.hkv;
   w.tiles = static_cast<int64_t>(w.r.n) * G > p.few_rows ? 0 : (w.r.n * G + rows_per_tile - 1) / rows_per_tile;
-  const int pos0 = w.r.len - w.r.n;  // position of the first row (may be negative)
-  const int lo = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
-  w.first = lo / kStep;
+  w.first = window_from(p, w.r.len - w.r.n) / kStep;
   w.steps = max(1, (w.r.len + kStep - 1) / kStep - w.first);
   return w;
 }
@@ -341,7 +339,7 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
       const int pos = w.r.len - w.r.n + r / G;
       return max(0, p.causal ? min(pos + 1, w.r.len) : w.r.len);
     };
-    auto sees_from = [&](int r) { return p.window > 0 ? max(0, w.r.len - w.r.n + r / G - p.window + 1) : 0; };
+    auto sees_from = [&](int r) { return window_from(p, w.r.len - w.r.n + r / G); };
     const int row_first = tile * R, row_last = row_first + rows - 1;
     const int all_hi = sees_to(row_first), any_hi = sees_to(row_last), any_lo = sees_from(row_first), all_lo = sees_from(row_last);
 

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   {
     const int first = pos0 + job.tile * kRows / G, last = pos0 + (job.tile * kRows + job.rows - 1) / G;
     job.t1 = p.causal ? min(last + 1, job.r.len) : job.r.len;
-    job.t0 = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    job.t0 = window_from(p, first);
     if (job.t1 < job.t0) job.t1 = job.t0;
   }
   const int j0 = job.t0 / kStep, n_steps = job.t1 > job.t0 ? (job.t1 + kStep - 1) / kStep - j0 : 0;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
     const uint32_t s_base = tmem + lanes + kS + 128 * a, o_at = tmem + lanes + kO + 128 * a;
     const int rr = job.tile * kRows + min(row, job.rows - 1), pos = pos0 + rr / G;
-    const int hi = p.causal ? max(0, min(pos + 1, job.r.len)) : job.r.len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    const int hi = p.causal ? max(0, min(pos + 1, job.r.len)) : job.r.len, lo = window_from(p, pos);
     float m = -INFINITY, l = 0.0f;
     bool ok = a == 0 || two;
     for (int j = 0; ok && j < n_steps; ++j) {
