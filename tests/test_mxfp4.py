@@ -314,3 +314,30 @@ def test_held_activations_of_another_k_are_refused(F, monkeypatch, a_blocks, b_b
     y = F.matmul_mxfp4(z(1, rows, b_blocks, 16), b, b_scales, a_scales=tiles(rows, b_blocks), K=K)
     p = calls[0][2]._obj
     assert y.shape == (1, rows, 8) and (p.M, p.N, p.K) == (rows, 8, b_blocks * 32) and len(calls) == 1
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1150, 4300, 4130), (1200, 5900, 96), (2240, 9000, 1056), (300, 14000, 8224), (4100, 2300, 2080), (129, 37900, 544)])
+def test_product_of_pairs_is_exact_again_and_again(F, M, N, K):
+    """Products by pairs of CTAs (whole and halved last rounds, ragged edges, many and few steps along K) whose sums are exact in
+    float32, with new operands in the same buffers each time: a tile read before its loads have landed, or
+    overwritten before it was read, would show."""
+    assert -(-M // 128) * -(-N // 256) > 148
+    kb = -(-K // 32)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    held = []
+    for rows in (M, N):
+        held += [torch.empty(rows, kb, 16, dtype=torch.uint8, device="cuda"), torch.empty(-(-rows // 128), -(-kb // 4), 32, 4, 4, dtype=torch.uint8, device="cuda")]
+    out = torch.empty(M, N, device="cuda")
+    for _ in range(6):
+        for i, rows in ((0, M), (2, N)):
+            x = torch.randint(0, 256, (rows, kb, 16), generator=g, dtype=torch.uint8, device="cuda")
+            if K % 32:  # padding of the last block is zero codes
+                x[:, -1, K % 32 // 2:] = 0
+            held[i].copy_(x)
+            held[i + 1].copy_(F.mxfp4_tile_scales(torch.randint(127, 129, (rows, kb), generator=g, dtype=torch.uint8, device="cuda")))
+        out.fill_(float("nan"))
+        F.matmul_mxfp4(held[0], held[2], held[3], a_scales=held[1], K=K, dtype=torch.float32, out=out)
+        a, w = (F.mxfp4_dequantize(held[i], held[i + 1], K=K).double() for i in (0, 2))
+        assert torch.equal(out.double(), a @ w.t())  # below 2^24 quarters
+    assert F.device_error(0) == 0

@@ -20,7 +20,7 @@
 // take turns on a CTA (more rows than that go to pairs of CTAs before they need a second round).
 //
 // Measured (codes in, GPU time): 1 x 4096 x 4096 6.3 us (latency), 16 x 14336 x 4096 8.5 us (31 MB, 3.7 TB/s: latency, then the
-// weights' stream), 2048 x 14336 x 4096 61 us (3.9 PFLOP/s), 8192 x 28672 x 8192 776 us (5.0 PFLOP/s, bound by loads from L2).
+// weights' stream), 2048 x 14336 x 4096 59 us (4.1 PFLOP/s), 8192 x 28672 x 8192 671 us (5.7 PFLOP/s, bound by loads from L2).
 //
 // Every wait is bounded as in mmnb_gemm_sm100.cu.
 #include <cuda.h>
@@ -378,13 +378,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ------------------------------------------------------------------ pairs of CTAs
 // For many rows: a cluster of two CTAs on one 256 x 256 tile. Each holds its 128 rows of P and half of Q's 256 rows; the
 // first one's MMAs (cta_group::2) read both halves from both shared memories, so that a CTA loads 256 rows a step instead
-// of 384 for the same product. What bounds it are these loads from L2, 35 KB a CTA and step (10 TB/s in all): 8192 x
-// 28672 x 8192 takes 776 us, and 507 with the loads left out. The scale copies and the order of the tiles (bands of 8 tiles
-// of P: 787 -> 810 us) make no difference.
+// of 384 for the same product. What bounds it are these loads from L2, 35 KB a CTA and step (12 TB/s in all): 8192 x
+// 28672 x 8192 takes 671 us (5.7 PFLOP/s); with the loads left out it was 507.
 // Tensor memory: two overlapping accumulators of 256 columns (they and the scales need more than the 512 columns); the
 // drain first takes the shared columns into registers, then the next tile may start (waiting for their stores: 73 -> 66
-// us at 2048 x 14336 x 4096). Each CTA keeps the accumulators of its own rows and all scales it needs. The second CTA passes on the arrival of its
-// loads (peer), the MMAs' completion goes to both.
+// us at 2048 x 14336 x 4096). Each CTA keeps the accumulators of its own rows and all scales it needs.
+// Signals between the two. Both CTAs' loads complete on the first one's `full` (the scales too are tensor copies: only those
+// may signal the pair's other CTA), which expects the bytes of both. The MMAs' completion goes to both. The second CTA's
+// epilogue warps meet at its own `drained`, and its warp 1 passes that on with a release at cluster scope. What the
+// first CTA waits for it acquires at cluster scope.
 __device__ __forceinline__ void mma2_mxf4(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
                                           uint32_t sb, uint32_t accumulate) {
   asm volatile(
@@ -402,13 +404,32 @@ __device__ __forceinline__ void mma2_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
 }
-// Arrives on `bar` of CTA `rank`. Relaxed: it passes on a completion (loads, tensor-memory reads), no writes of this
-// thread, and the release form costs 1500 cycles here.
+// Arrives on `bar` of CTA `rank`, after all that this thread has done and observed.
 __device__ __forceinline__ void arrive_at(uint64_t* bar, uint32_t rank) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_u32(bar), rank)) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_u32(bar), rank)) : "memory");
+}
+// A probe that acquires at cluster scope what the phase stands for (those of a wait are the CTA's).
+__device__ __forceinline__ bool acquire_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done != 0;
+}
+// Loads a tile into this CTA's shared memory, its bytes counted by `bar`, the shared::cluster address of a barrier of either CTA.
+__device__ __forceinline__ void tma2_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 constexpr int kStages2 = 6;
-constexpr uint32_t kStage2 = 2 * kRows * kStepBytes + 6 * kScaleTile;  // P, Q half, P scales, Q scales of both blocks
+constexpr uint32_t kStage2 = 2 * kRows * kStepBytes + 6 * kScaleTile;  // P, Q half, P scales, Q scales of both blocks: a CTA's bytes
 constexpr int kSfStage2 = 24, kShared2 = kStages2 * kSfStage2;         // scale columns; columns that both accumulators hold
 constexpr int kAcc2 = 256 - kShared2, kSfCol2 = 512 - kStages2 * kSfStage2;
 static_assert(kShared2 % 16 == 0 && kAcc2 + 256 == kSfCol2, "tensor memory map");
@@ -426,24 +447,23 @@ __device__ __forceinline__ Tile2 tile2(const Args& a, int t) {
 
 template <bool F16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    mxfp4_gemm2_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
+    mxfp4_gemm2_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                       const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq, const Args a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kStages2], empty[kStages2], peer[kStages2], accfull[2], drained[2], done;
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint64_t full[kStages2], empty[kStages2], accfull[2], drained[2], done;
+  __shared__ uint32_t tmem_slot, fills[2];  // stages that each CTA's loads were issued for (in the first CTA)
   __shared__ int abort_flag;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  uint8_t* gbase = smem_raw + (base - raw);
   const int rank = static_cast<int>(cluster_rank());
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages2; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&peer[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accfull[b], 1);
-      mbar_init(&drained[b], 2 * kEpilogueWarps);  // of both CTAs
+      mbar_init(&drained[b], kEpilogueWarps + (rank == 0));  // the first CTA's: and the second CTA
     }
     mbar_init(&done, 1);
     abort_flag = 0;
@@ -469,49 +489,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int tile = first; ok && tile < a.tiles; tile += step) {
         const Tile2 t = tile2(a, tile);
-        const int pb = 2 * t.pt + rank, q0 = t.q0, q_row = q0 * kRows + rank * (t.half ? kRows / 2 : kRows);
-        const bool two = !t.half && q0 + 1 < a.sq_blocks;
-        const int blocks = (pb < a.sp_blocks) + (q0 < a.sq_blocks) + two;
+        const int pb = 2 * t.pt + rank, q_row = t.q0 * kRows + rank * (t.half ? kRows / 2 : kRows);
+        const int sp_tile = static_cast<int>(pb * a.tiles_k), sq_tile = static_cast<int>(t.q0 * a.tiles_k), tiles_k = static_cast<int>(a.tiles_k);
         for (int ks = 0; ks < a.ksteps; ++ks, ++g) {
           if (!thread_wait(&empty[s], ph ^ 1, ctl, kErrWaitProducer)) {
             ok = false;
             break;
           }
-          const uint32_t groups = min(2, (a.k64 - 4 * ks + 1) >> 1) * kScaleTile;
-          const uint32_t at = base + s * kStage2;
-          uint8_t* sc = gbase + s * kStage2 + 2 * kRows * kStepBytes;
-          mbar_arrive_expect_tx(&full[s], 2 * kRows * kStepBytes + blocks * groups);
-          tma_load_2d(at, &map_p, ks * kStepBytes, pb * kRows, &full[s]);
-          tma_load_2d(at + kRows * kStepBytes, &map_q, ks * kStepBytes, q_row, &full[s]);  // a half uses the first 64 rows
-          if (pb < a.sp_blocks) bulk_copy_g2s(sc, a.sp + (pb * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
-          if (q0 < a.sq_blocks) bulk_copy_g2s(sc + 2 * kScaleTile, a.sq + (q0 * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
-          if (two) bulk_copy_g2s(sc + 4 * kScaleTile, a.sq + ((q0 + 1) * a.tiles_k + 2 * ks) * kScaleTile, groups, &full[s]);
+          // Every copy counts whole (what lies outside the operands is filled with zeros). A second scale tile behind the
+          // last one along K is not used.
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStage2);
+          const uint32_t at = base + s * kStage2, sc = at + 2 * kRows * kStepBytes, bar = map_rank(smem_u32(&full[s]), 0);
+          tma2_load_2d(at, &map_p, ks * kStepBytes, pb * kRows, bar);
+          tma2_load_2d(at + kRows * kStepBytes, &map_q, ks * kStepBytes, q_row, bar);  // a half uses the first 64 rows
+          tma2_load_2d(sc, &map_sp, 0, sp_tile + 2 * ks, bar);
+          tma2_load_2d(sc + 2 * kScaleTile, &map_sq, 0, sq_tile + 2 * ks, bar);
+          tma2_load_2d(sc + 4 * kScaleTile, &map_sq, 0, sq_tile + tiles_k + 2 * ks, bar);
           if (++s == kStages2) {
             s = 0;
             ph ^= 1;
           }
         }
       }
-      if (!ok)
-        for (int h = (g > kStages2 ? g - kStages2 : 0); h < g; ++h) drain_wait(&full[h % kStages2], (h / kStages2) & 1, a.err, kErrDrain);
+      st_cluster_u32(map_rank(smem_u32(&fills[rank]), 0), g);
     }
   } else if (warp == 1 && rank == 1) {
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    for (int tile = first; ok && tile < a.tiles; tile += step)
-      for (int ks = 0; ks < a.ksteps; ++ks) {
-        if (!warp_spin(&full[s], ph, ctl, kErrWaitMma)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) arrive_at(&peer[s], 0);
-        __syncwarp();
-        if (++s == kStages2) {
-          s = 0;
-          ph ^= 1;
-        }
-      }
+    // passes on that this CTA's accumulators have been read (its epilogue warps have stores under way, which a release of
+    // theirs would wait for)
+    int i = 0;
+    for (int tile = first; tile < a.tiles; tile += step, ++i) {
+      if (!warp_spin(&drained[i & 1], (i >> 1) & 1, ctl, kErrWaitMma)) break;
+      if (lane == 0) arrive_at(&drained[i & 1], 0);
+      __syncwarp();
+    }
   } else if (warp == 1) {
     const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
     const uint64_t s_desc = plain_desc(base + 2 * kRows * kStepBytes);
@@ -519,32 +529,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int i = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    // both CTAs' loads (lanes look at one barrier each), or both CTAs' drains
-    auto wait = [&](uint64_t* x, uint64_t* y, uint32_t parity) {
-      uint64_t start = 0;
-      for (;;) {
-#pragma unroll 1
-        for (int n = 0; n < kSpins; ++n)
-          if (__all_sync(~0u, mbar_test_wait((lane & 1) ? y : x, parity))) return true;
-        if (__any_sync(~0u, *ctl.abort != 0)) return false;
-        const uint64_t now = __shfl_sync(~0u, global_timer_ns(), 0);
-        if (start == 0) start = now;
-        if (now - start > kWaitLimitNs) {
-          if (lane == 0) {
-            record_device_error(a.err, kErrWaitMma);
-            *ctl.abort = 1;
-          }
-          return false;
-        }
-      }
+    // both CTAs' loads, or both CTAs' drains
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return warp_spin(bar, parity, ctl, kErrWaitMma) && __all_sync(~0u, acquire_cluster(bar, parity));
     };
     for (int tile = first; ok && tile < a.tiles; tile += step, ++i) {
-      if (i > 0 && !wait(&drained[(i - 1) & 1], &drained[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
+      if (i > 0 && !wait(&drained[(i - 1) & 1], ((i - 1) >> 1) & 1)) break;
       const uint32_t d = tmem + ((i & 1) ? kAcc2 : 0);
       const int T = tile >= a.whole ? 128 : 256;
       const uint32_t i_desc0 = instruction_desc(T, 0u) + wide, i_desc1 = instruction_desc(T, 2u) + wide;
       for (int ks = 0; ks < a.ksteps; ++ks) {
-        if (!wait(&full[s], &peer[s], ph)) {
+        if (!wait(&full[s], ph)) {
           ok = false;
           break;
         }
@@ -602,7 +597,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int h = 0; h < kHeld; ++h) tmem_wait_ld16(held[h]);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_at(&drained[b], 0);
+      if (lane == 0) mbar_arrive(&drained[b]);
 #pragma unroll
       for (int h = 0; h < kHeld; ++h)
         if (p < a.p_rows && c + 2 * h < chunks) store_row<F16>(a, p, q0 + column(c + 2 * h), held[h]);
@@ -618,7 +613,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && abort_flag) st_cluster_u32(map_rank(smem_u32(&abort_flag), rank ^ 1), 1);
   cluster_sync();  // neither CTA's memory goes while the other may read or signal it
+  if (*ctl.abort) {
+    // A wait ran out in one of them: loads may be under way whose other half was never issued. A stage's last fill is
+    // made complete, then awaited: the first CTA's bytes alone lack the second's, the second's alone were not expected.
+    if (rank == 0 && threadIdx.x == 0) {
+      const int g0 = static_cast<int>(fills[0]), g1 = static_cast<int>(fills[1]);
+      for (int s = 0; s < kStages2; ++s) {
+        const int n0 = (g0 - s + kStages2 - 1) / kStages2, n1 = (g1 - s + kStages2 - 1) / kStages2;
+        if (n0 < n1) mbar_arrive_expect_tx(&full[s], kStage2);
+        else if (n0 > n1) asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(kStage2) : "memory");
+        if (n0 || n1) drain_wait(&full[s], (max(n0, n1) - 1) & 1, a.err, kErrDrain);
+      }
+    }
+    cluster_sync();
+  }
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
@@ -681,7 +691,7 @@ cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, 
 
 // Pairs take what would need a second round of 128 x 256 tiles. Measured (us with the launch, one CTA a tile / pairs):
 // 256 x 14336 x 4096 20.5 / 20.6, 1024 x 4096 x 14336 36.9 / 38.9, 1152 x 4096 x 4096 (144 tiles) 18.4 / 24.6;
-// 2048 x 14336 x 4096 78.8 / 66, 4096 x 8192 x 8192 132 / 124, 8192 x 28672 x 8192 852 / 776.
+// 2048 x 14336 x 4096 78.8 / 64, 4096 x 8192 x 8192 132 / 108, 8192 x 28672 x 8192 852 / 671.
 bool pairs_pay(const Mxfp4Matmul& p, int sms) {
   return p.M > kRows && ceil_div(p.M, kRows) * ceil_div(p.N, 256) > sms;
 }
@@ -713,10 +723,14 @@ cudaError_t launch_pairs(const Mxfp4Matmul& p, Args a, bool early, cudaStream_t 
   a.ldy = p.ldy;
   a.vec = (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0 && (p.ldy * (p.f16 ? 2 : 4)) % 16 == 0;
   a.err = p.err;
-  CUtensorMap mp, mq;
+  // Scales as rows of a tile's 512 bytes (as 2-byte elements, of which a row of a copy may have 256), two at a time.
+  CUtensorMap mp, mq, msp, msq;
   const uint64_t row = static_cast<uint64_t>(p.kb) * 16;
-  if (!encode_tensor_map_2d(&mp, 0, p.a, row, a.p_rows, row, kStepBytes, kRows, true) ||
-      !encode_tensor_map_2d(&mq, 0, p.b, row, a.q_rows, row, kStepBytes, kRows, true))
+  const int64_t sp_tiles = a.sp_blocks * a.tiles_k, sq_tiles = a.sq_blocks * a.tiles_k;
+  if (sp_tiles > INT_MAX / 2 || sq_tiles > INT_MAX / 2 || !encode_tensor_map_2d(&mp, 0, p.a, row, a.p_rows, row, kStepBytes, kRows, true) ||
+      !encode_tensor_map_2d(&mq, 0, p.b, row, a.q_rows, row, kStepBytes, kRows, true) ||
+      !encode_tensor_map_2d(&msp, 1, a.sp, kScaleTile / 2, sp_tiles, kScaleTile, kScaleTile / 2, 2, false) ||
+      !encode_tensor_map_2d(&msq, 1, a.sq, kScaleTile / 2, sq_tiles, kScaleTile, kScaleTile / 2, 2, false))
     return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (a.tiles < pairs ? a.tiles : pairs));
@@ -728,7 +742,7 @@ cudaError_t launch_pairs(const Mxfp4Matmul& p, Args a, bool early, cudaStream_t 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = early ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, mxfp4_gemm2_kernel<F16>, mp, mq, a);
+  return cudaLaunchKernelEx(&cfg, mxfp4_gemm2_kernel<F16>, mp, mq, msp, msq, a);
 }
 
 }  // namespace
