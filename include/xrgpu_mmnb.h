@@ -554,7 +554,8 @@ XRGPU_API int xrgpu_kv8_read(const xrgpu_kv8_problem* p, void* stream);
 /* o[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j of the row's sequence that it sees;
  * query head h reads key/value head h / (heads_q / heads_kv). A row that sees nothing gives zeros (cu_seqlens may
  * hold more rows than kv_len tokens here; the first ones then see nothing); so do the rows of a sequence whose
- * kv_len does not fit. Tokens of a bad page id are left out. */
+ * kv_len does not fit. Tokens of a bad page id are left out; pages whose tokens all lie in front of what the call's rows of
+ * the sequence see (a window) are not looked up, so their ids may be anything. */
 XRGPU_API int xrgpu_kv8_attention_workspace_size(const xrgpu_kv8_problem* p, uint64_t* bytes);
 /* workspace as in xrgpu_mxfp4_forward. */
 XRGPU_API int xrgpu_kv8_attention(const xrgpu_kv8_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);

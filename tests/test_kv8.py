@@ -625,3 +625,32 @@ def test_the_largest_windows_see_everything(F, dtype, window, lens, new):
     assert bool((got != 0).any())
     q = torch.randn(sum(new), G * heads, D, generator=torch.Generator().manual_seed(sum(new) + G * heads)).to(dtype)
     assert torch.equal(got, F.attention_kv8(q.cuda(), *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("lens,new", [([200, 90], [1, 3]), ([150 + 7 * i for i in range(40)], [1] * 40), ([333, 300], [150, 140])])
+def test_pages_in_front_of_the_window_may_be_gone(F, dtype, page, lens, new):
+    """Pages whose tokens no row sees any more are released (-1) as a window moves on: nothing is looked up there, nothing
+    recorded, and the results are those with the pages still in place."""
+    G = 4
+    heads = _heads(new, G, 64) if max(new) > 100 else 2
+    for window in (1, 40, 45, 64):
+        c = R.Cache(lens, heads=heads, D=64, page=page, code=INT8)
+        q = torch.randn(sum(new), G * heads, 64, dtype=dtype, device="cuda")
+        want = F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=window)
+        assert F.device_error(0) == 0
+        gone = 0
+        for b, (n, m) in enumerate(zip(lens, new)):
+            first = max(0, n - m - window + 1)
+            c.table[b, :first // page] = -1
+            gone += first // page
+        assert gone > 0
+        got = F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=window)
+        assert F.device_error(0) == 0
+        assert torch.equal(got, want)
+        # a page that a row does see is still missed
+        c.table[0, (lens[0] - 1) // page] = -1
+        F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=window)
+        assert F.device_error(0) == 0x501

@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
     const int all_hi = sees_to(row_first), any_hi = sees_to(row_last), any_lo = sees_from(row_first), all_lo = sees_from(row_last);
 
     // ---- this warp's steps: s0 + warp, + kWarps, ... Page ids come 16 steps at a time: lane i holds the first page
-    // of step i of the batch, lane 16 + i the second one (pages of 16 tokens).
+    // of step i of the batch, lane 16 + i the second one (pages of 16 tokens). A page in front of what the rows see may be
+    // gone from the table, and is not looked up.
     const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kWarps - 1) / kWarps : 0;
     const int64_t head_block = static_cast<int64_t>(head) << p.page_log2;
     int ids = -1;
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
         if ((i & 15) == 0) {
           const int t = (w.first + s0 + warp + (i + (lane & 15)) * kWarps) * kStep + (lane >> 4) * 16;
           ids = -1;
-          if (i + (lane & 15) < mine && t < w.r.len && (lane < 16 || p.page == 16)) ids = page_id(p, b, t >> p.page_log2);
+          if (i + (lane & 15) < mine && t < w.r.len && t + (p.page == 16 ? 16 : kStep) > any_lo && (lane < 16 || p.page == 16)) ids = page_id(p, b, t >> p.page_log2);
         }
         const int t0 = (w.first + s0 + warp + i * kWarps) * kStep;
         const int id0 = __shfl_sync(~0u, ids, i & 15);

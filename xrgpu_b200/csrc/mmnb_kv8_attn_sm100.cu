@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     const uint32_t at0 = line + ((c0 ^ (row0 & 7)) << 4), at1 = line + (((c0 + 1) ^ (row0 & 7)) << 4);
     // Lane c < kChunks knows chunk c of a step: its page id three steps ahead, two steps ahead where its first token's
     // codes lie (-1: nowhere). The first thread of the keys' warps for each chunk also makes the step's factors: scales two
-    // steps ahead, factors one.
+    // steps ahead, factors one. Chunks in front of what any row sees are nowhere too: their pages may be gone from the table.
     const bool factors = keys && ct < kChunks;
     int id_next = -1, ok_raw = 0, ok_now = 0;
     int64_t chunk_base = -1;
@@ -426,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     auto find_page = [&](int j) {
       const int tok = (j0 + j) * kStep + 16 * lane;
       id_next = -1;
-      if (j < n_steps && lane < kChunks && tok < job.t1) id_next = p.page_table[static_cast<int64_t>(job.b) * p.max_pages + (tok >> p.page_log2)];
+      if (j < n_steps && lane < kChunks && tok + 16 > job.t0 && tok < job.t1) id_next = p.page_table[static_cast<int64_t>(job.b) * p.max_pages + (tok >> p.page_log2)];
     };
     auto find = [&](int j) {
       const int tok = (j0 + j) * kStep + 16 * lane;
-      const bool wanted = j < n_steps && lane < kChunks && tok < job.t1, use = wanted && id_next >= 0 && id_next < p.pages;
+      const bool wanted = j < n_steps && lane < kChunks && tok + 16 > job.t0 && tok < job.t1, use = wanted && id_next >= 0 && id_next < p.pages;
       if (wanted && !use) record_device_error(p.err, kErrKv8Page);
       const int64_t block = static_cast<int64_t>(id_next) * p.hkv + head;
       chunk_base = use ? ((block << p.page_log2) + (tok & (p.page - 1))) * D : -1;
