@@ -654,3 +654,45 @@ def test_pages_in_front_of_the_window_may_be_gone(F, dtype, page, lens, new):
         c.table[0, (lens[0] - 1) // page] = -1
         F.attention_kv8(q, *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=window)
         assert F.device_error(0) == 0x501
+
+
+# ------------------------------------------------------------------------------------------ float32 rows
+def _float32_bound(k, v, q, scale):
+    """(o, tolerance) float64 of one float32 row over keys and values [n, D]: float32 sums over D products in a score, each
+    counted once in the values' sum and once in the normaliser, as are an exponential's 2^-21 and the weight's
+    rounding. A weight is a pair of float16 numbers, the second 2^11 times the rest, of 2^7 to 2^15 for the largest: 2^-24 of
+    itself, and steps of 2^-25 2^-11 2^-7 = 2^-43 of the largest where the second number is a subnormal. A
+    query is a pair of float16 numbers below 2^15: 2^-24 of itself (one product's rounding), and steps of 2^-25 2^-14 = 2^-39
+    of the row's largest. n tokens summed in float32 in steps of 32 by at least six warps."""
+    n, D = k.shape
+    x = k @ q * scale
+    w = np.exp(x - x.max())
+    p = w / w.sum()
+    o = p @ v
+    d = (D + 8) * 2.0 ** -24 * (np.abs(k) @ np.abs(q)).max() * abs(scale) + 2.0 ** -39 * np.abs(q).max() * np.abs(k).sum(1).max() * abs(scale)
+    rel = 2 * d + 2.0 ** -20 + 2.0 ** -23 + (64 + n / 64) * 2.0 ** -24
+    return o, rel * (p @ np.abs(v)) + 2.0 ** -43 / w.sum() * np.abs(v).sum(0) + 2.0 ** -24 * np.abs(o)
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("rows,below", [(1, 17.4), (1, 24.0), (9, 17.4), (1, 10.0)])
+def test_float32_small_weights_count(F, code, rows, below):
+    """One token takes nearly all the weight, and 32000 tokens far below it the rest: their values are the result, since the
+    first one's are zero."""
+    n, D, page = 32001, 64, 64
+    c = R.Cache([n], heads=1, D=D, page=page, code=code)
+    at = 12345
+    ids = c.table[0].long()
+    c.k.zero_()
+    c.ks.fill_(0.01)
+    c.k[ids[at // page], 0, at % page] = torch.ones(D).to(code)
+    c.v[:] = (torch.rand(c.v.shape, generator=torch.Generator().manual_seed(1)) * 60 + 60).round().to(code)
+    c.v[ids[at // page], 0, at % page] = torch.zeros(D).to(code)
+    c.vs.fill_(0.01)
+    q = torch.full((rows, 1, D), below / (0.01 * D * D ** -0.5))  # the token's score is `below`, all others' 0
+    got = F.attention_kv8(q.cuda(), *c.cuda(), None, c.lens.cuda(), causal=False).cpu().double().numpy()
+    k, v = c.tokens(0)
+    o, tol = _float32_bound(k[:, 0], v[:, 0], q[0, 0].double().numpy(), D ** -0.5)
+    off = np.abs(got[:, 0] - o) - tol
+    assert (off <= 0).all(), (float(off.max()), float(np.abs(got[:, 0] - o).max() / np.abs(o).max()))

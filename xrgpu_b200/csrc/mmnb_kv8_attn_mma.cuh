@@ -11,10 +11,12 @@
 // more MMA with a constant operand, -128 2^-24 sum(p), for the values. e4m3 codes are float16 numbers by
 // one conversion. Scales multiply the float32 results: the scores of a page by k_scale, each page's O^T by
 // v_scale as it is added to the running one, so pages of very different scales lose nothing against one another.
-// Weights: exp2(x - m) with m the largest score when it was last raised; m is raised only when a score exceeds it by 8
-// (weights then stay below 2^8, far inside float16), so that most steps need one vote instead of a reduction.
-// P is rounded to float16 (2^-11 relative, once, like the result); sums are float32. Float32 rows take q and P
-// as pairs of float16 numbers (22 bits) and signed codes.
+// Weights: 2^7 exp2(x - m) with m the largest score when it was last raised; m is raised only when a score exceeds it by 8,
+// so that most steps need one vote instead of a reduction. Weights then lie below 2^15, inside float16, with steps of 2^-24
+// far below the largest one. P is rounded to float16 (2^-12 relative, once, like the result); sums are float32, of the
+// weights before that rounding. Float32 rows take q and P as pairs of float16 numbers and signed codes: the second one of P
+// holds 2^11 times the rest, and its products are summed first and scaled back, so that a weight has 2^-24 of itself, or of
+// the largest weight 2^-43 (as the rest itself it lost all bits of weights below 2^-25, of which a long sequence has many).
 //
 // Order in memory. A step is 32 tokens of keys and values, copied by a warp with 16-byte cp.async into its own ring
 // of two or three buffers. 16-byte chunk c of row r lies at c ^ f(r), f(r) = (r & 7) ^ 4 (r & 1) for 128-byte rows (two
@@ -41,6 +43,8 @@ namespace {
 
 constexpr int kStep = 32;    // tokens a warp takes at a time
 constexpr float kRaise = 8.0f;
+constexpr float kLift = 7.0f, kDrop = 0.0078125f;  // weights are held times 2^7; 2^-7
+constexpr float kRest = 2048.0f;                   // the second half of a weight: 2^11 times what the first one leaves
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ small pieces
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float top = m[n][e] + kRaise;
+          const float top = m[n][e] + (kRaise + kLift);
           above |= !(x[0][n][e] <= top) | !(x[0][n][e + 2] <= top) | !(x[1][n][e] <= top) | !(x[1][n][e + 2] <= top);
         }
       if (__any_sync(~0u, above)) {
@@ -559,7 +563,7 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
             t = fmaxf(t, __shfl_xor_sync(~0u, t, 4));
             t = fmaxf(t, __shfl_xor_sync(~0u, t, 8));
             t = fmaxf(t, __shfl_xor_sync(~0u, t, 16));
-            t = fmaxf(t, m[n][e]);
+            t = fmaxf(t - kLift, m[n][e]);
             f[e] = m[n][e] == t ? 1.0f : exp2_approx(m[n][e] - t);
             m[n][e] = t;
             l[n][e] *= f[e];
@@ -589,12 +593,13 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
             pb[h][n][k] = transpose8(hw);
             if (F32) {
               const float2 f = unpack_half2(hw);
-              pl[F32 ? h : 0][n][k] = transpose8(pack_half2(w0 - f.x, w1 - f.y));
+              pl[F32 ? h : 0][n][k] = transpose8(pack_half2((w0 - f.x) * kRest, (w1 - f.y) * kRest));
             }
           }
       }
       // O^T += v_scale (V^T P^T), page by page
-      const float unit_v = C::kRaw ? 16777216.0f : 1.0f;
+      // (with the weights' 2^7 taken out; float32 rows take it out of the products, which leaves v_scale its range)
+      const float unit_v = C::kRaw ? 16777216.0f * kDrop : F32 ? 1.0f : kDrop;
       const float vs0 = meta[2] * unit_v, vs1 = meta[3] * unit_v;
       const uint32_t vt = st + C::kTile;
       auto load_v = [&](int t, uint32_t (&v)[D / 32]) {
@@ -632,28 +637,43 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[0][n][e] = t[1][n][e] = base[n][e];
+          uint32_t lo[2][4], hi[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h < h0 || h >= h1) continue;
-            uint32_t lo[4], hi[4];
-            token_pairs<E4M3, C::kRaw>(v[h][0][q], v[h][1][q], lo);
-            token_pairs<E4M3, C::kRaw>(v[h][2][q], v[h][3][q], hi);
+            token_pairs<E4M3, C::kRaw>(v[h][0][q], v[h][1][q], lo[h]);
+            token_pairs<E4M3, C::kRaw>(v[h][2][q], v[h][3][q], hi[h]);
+          }
+          auto products = [&](const uint32_t (&w)[2], int h, int n) {
+            mma_16816(t[0][n], lo[h][0], lo[h][1], hi[h][0], hi[h][1], w[0], w[1]);
+            mma_16816(t[1][n], lo[h][2], lo[h][3], hi[h][2], hi[h][3], w[0], w[1]);
+          };
+          if (F32) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma_16816(t[0][n], lo[0], lo[1], hi[0], hi[1], pb[h][n][0], pb[h][n][1]);
-              mma_16816(t[1][n], lo[2], lo[3], hi[2], hi[3], pb[h][n][0], pb[h][n][1]);
-              if (F32) {
-                mma_16816(t[0][n], lo[0], lo[1], hi[0], hi[1], pl[F32 ? h : 0][n][0], pl[F32 ? h : 0][n][1]);
-                mma_16816(t[1][n], lo[2], lo[3], hi[2], hi[3], pl[F32 ? h : 0][n][0], pl[F32 ? h : 0][n][1]);
-              }
+            for (int h = 0; h < 2; ++h) {
+              if (h < h0 || h >= h1) continue;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) products(pl[F32 ? h : 0][n], h, n);
             }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[k][n][e] *= 1.0f / kRest;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h < h0 || h >= h1) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) products(pb[h][n], h, n);
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) O[2 * q + k][n][e] = fmaf(vs, t[k][n][e], O[2 * q + k][n][e]);
+              for (int e = 0; e < 4; ++e) O[2 * q + k][n][e] = fmaf(vs, F32 ? t[k][n][e] * kDrop : t[k][n][e], O[2 * q + k][n][e]);
         }
         if (bad) {  // rows that see none of the page's tokens stay free of its NaN
 #pragma unroll
@@ -690,7 +710,7 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
         t += __shfl_xor_sync(~0u, t, 16);
         if (g == 0) {
           warp_m[warp * R + n * 8 + 2 * c + e] = m[n][e];
-          warp_l[warp * R + n * 8 + 2 * c + e] = t;
+          warp_l[warp * R + n * 8 + 2 * c + e] = t * kDrop;
         }
       }
     float* mine_o = reinterpret_cast<float*>(ring_ptr);
