@@ -696,3 +696,31 @@ def test_float32_small_weights_count(F, code, rows, below):
     o, tol = _float32_bound(k[:, 0], v[:, 0], q[0, 0].double().numpy(), D ** -0.5)
     off = np.abs(got[:, 0] - o) - tol
     assert (off <= 0).all(), (float(off.max()), float(np.abs(got[:, 0] - o).max() / np.abs(o).max()))
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 12, 2.0 ** 16, 2.0 ** -120, 2.0 ** 127])
+def test_float32_queries_with_an_outlier(F, code, size):
+    """A query's largest number meets keys that are zero there: the scores are those of the small numbers."""
+    n, D, page = 700, 64, 32
+    c = R.Cache([n], heads=1, D=D, page=page, code=code)
+    c.k[..., 5] = torch.zeros(c.k.shape[:-1]).to(code)
+    q = torch.randn(3, 2, D, generator=torch.Generator().manual_seed(2))
+    q[..., 5] = size * 1.3
+    if size > 2.0 ** 100:
+        q[..., 5] = 3.0e38
+        q[..., :5] *= 2.0 ** 100
+        q[..., 6:] *= 2.0 ** 100
+        c.ks *= 2.0 ** -100
+    if size < 2.0 ** -100:
+        q *= 2.0 ** -118
+        q[..., 5] = 2.0 ** -118
+        c.ks *= 2.0 ** 118
+    got = F.attention_kv8(q.cuda(), *c.cuda(), None, c.lens.cuda(), causal=False).cpu().double().numpy()
+    k, v = c.tokens(0)
+    for r in range(3):
+        for h in range(2):
+            o, tol = _float32_bound(k[:, 0], v[:, 0], q[r, h].double().numpy(), D ** -0.5)
+            off = np.abs(got[r, h] - o) - tol
+            assert (off <= 0).all(), (r, h, float(off.max()), float(np.abs(got[r, h] - o).max() / np.abs(o).max()))

@@ -418,9 +418,8 @@ __global__ void __launch_bounds__(Traits<E4M3, D, NT, F32, CL>::kThreads, Traits
         uint32_t a = 0;
         for (int d = lane; d < D; d += 32) a = max(a, real ? __float_as_uint(static_cast<const float*>(p.q)[qat + d]) & 0x7fffffffu : 0u);
         a = __reduce_max_sync(~0u, a);
-        // q / unit lies in [-2, 2]: pairs of float16 numbers hold it to 2^-24 of the largest
-        const uint32_t e = max(a >> 23, 1u);
-        unit = __uint_as_float(min(e, 253u) << 23);
+        // |q / unit| < 2^15: pairs of float16 numbers hold it to 2^-24 of itself and steps of 2^-39 of the row's largest
+        unit = __uint_as_float((max(a >> 23, 15u) - 14u) << 23);
       }
       const float inv = F32 ? 1.0f / unit : 1.0f;
       // lane (s, c) of the fragment's row: k step s takes dims 16 (c + 4 (s / 4)) + 4 (s % 4) + 0..3 of lane c
