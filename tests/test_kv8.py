@@ -724,3 +724,51 @@ def test_float32_queries_with_an_outlier(F, code, size):
             o, tol = _float32_bound(k[:, 0], v[:, 0], q[r, h].double().numpy(), D ** -0.5)
             off = np.abs(got[r, h] - o) - tol
             assert (off <= 0).all(), (r, h, float(off.max()), float(np.abs(got[r, h] - o).max() / np.abs(o).max()))
+
+
+# ------------------------------------------------------------------------------------------ prompts and value scales
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 26, 2.0 ** 32])
+def test_prompts_rows_owe_nothing_to_pages_they_do_not_see(F, code, D, page, window, factor):
+    """One page's values are up to 2^32 times the others': rows before it, and rows whose window has left it, are
+    as exact as without it.
+
+    The rows that do see it: the kernel feeds the products of weight and value scale, p_j s_j, as float16 numbers of 2^7 at
+    least for the row's largest. Where such a number is a subnormal it is off by half a step of 2^-24, which is 2^-32 of
+    the largest; with the codes c_j the sum is off by 2^-32 max_j(p_j s_j) sum_j |c_j| at most, on top of what R.attention
+    counts. That matters for values whose code is zero in the large page. The other rows get none of it.
+    """
+    new, G = [270], 4
+    heads = _heads(new, G, D)
+    c = R.Cache([300], heads=heads, D=D, page=page, code=code)
+    big = 128 // page if not window else 64 // page
+    c.vs[:] = 20000.0 / R.LIMIT[code] / factor
+    c.vs[c.table[0, big]] = 20000.0 / R.LIMIT[code]
+    q = torch.randn(270, G * heads, D, generator=torch.Generator().manual_seed(270 + G * heads)).half()
+    want, tol = R.attention(c, q, _cu(new), window=window)
+    free = np.zeros(270, bool)
+    if window:
+        free[(big + 1) * page + window - 1 - 30:] = True  # rows are the positions from 30 on
+        free[:max(0, big * page - 30)] = True
+    else:
+        free[:big * page - 30] = True
+    ids = c.table[0, :-(-300 // page)].long()
+    codes = np.abs(c.v[ids].float().double().transpose(1, 2).reshape(-1, heads, D)[:300].numpy())
+    scale = c.vs[ids].double().repeat_interleave(page, 0)[:300].numpy()
+    keys, _ = c.tokens(0)
+    for row in np.flatnonzero(~free):
+        pos = row + 30
+        lo = max(0, pos - window + 1) if window else 0
+        for h in range(G * heads):
+            x = keys[lo:pos + 1, h // G] @ q[row, h].double().numpy() * D ** -0.5
+            p = np.exp(x - x.max())
+            p /= p.sum()
+            tol[row, h] += 2.0 ** -32 * (p * scale[lo:pos + 1, h // G]).max() * codes[lo:pos + 1, h // G].sum(0)
+    got = F.attention_kv8(q.cuda(), *c.cuda(), _cu(new).cuda(), c.lens.cuda(), window=window).cpu().double().numpy()
+    assert F.device_error(0) == 0 and np.isfinite(got).all()
+    off = np.abs(got - want) - tol
+    assert (off <= 0).all(), (float(off.max()), float(off[free].max()))
+    assert free.sum() > 60 and (np.abs(got[free]) > 0).any(-1).all()

@@ -6,10 +6,11 @@
 // G, so the group shares every key and value) as two tiles of 128, and passes once over the tokens they see,
 // 64 at a time. Codes are exact float16 numbers: they are widened once a CTA, in registers, on their way
 // to shared memory, and the scales stay out of them: k_scale multiplies the scores a page at a time, and
-// v_scale joins the exponent of the weights: P' = exp2(x - m + log2(v_scale 2^7 / R)), R the power of two above the
-// largest v_scale of the tokens. With m raised only when a score exceeds it by 8, P' stays below 2^15, so
-// float16 holds 2^21 of range below the weight 1 with the largest scale at full precision. The normaliser is the
-// float32 sum of P' divided by the same factor, a page at a time.
+// v_scale joins the exponent of the weights: P' = 2^7 exp2(x + log2(v_scale) - m), m the largest x + log2(v_scale) of
+// what the row sees. With m raised only when one exceeds it by 8, P' stays below 2^15, so float16 holds the products of weight
+// and value scale to 2^-12 of themselves down to 2^-21 of the row's largest, below that in steps of 2^-31 of it, whatever
+// the scales of pages are that other rows see. The normaliser is the float32 sum of P' divided by the same factor, a page
+// at a time.
 //
 // Roles (20 warps, registers moved between them):
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread a row: read S, raise m (and rescale O, rare), write P' over S, at
@@ -51,7 +52,7 @@ constexpr int kChunks = kStep / 16;
 // warpgroups then trade them.
 constexpr int kRegs = 96, kSoftmaxRegs = 112, kWidenRegs = 88, kMmaRegs = 80;
 static_assert(256 * kSoftmaxRegs + 256 * kWidenRegs + 128 * kMmaRegs <= kThreads * kRegs, "more registers than the block has");
-constexpr float kRaise = 8.0f;
+constexpr float kRaise = 8.0f, kLift = 7.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kS = 0, kO = 256;  // tensor memory columns (128 a tile)
 
@@ -66,8 +67,8 @@ struct Smem {
 };
 
 // What the softmax needs of a step's 16-token chunks: the factor of their scores, log2 and inverse of the values'
-// factor, and a bit for each chunk that holds tokens.
-struct Meta {
+// scale, and a bit for each chunk that holds tokens.
+struct alignas(16) Meta {
   float kf[kChunks], lv[kChunks], iv[kChunks];
   int oks;
 };
@@ -155,8 +156,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   using M = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
-  __shared__ __align__(16) Meta meta[2 * kRing];
-  __shared__ uint32_t tmem_slot, vmax_bits;
+  __shared__ Meta meta[2 * kRing];
+  __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, found_b, found_tile;
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const int G = p.hq / p.hkv, head = blockIdx.x % p.hkv, slot = blockIdx.x / p.hkv;
@@ -222,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       mbar_init(&bars.done[i], 1);
     }
     abort_flag = 0;
-    vmax_bits = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   const Ctl ctl{&abort_flag, p.err};
 
-  // ---- queries to shared memory (K-major, 128-byte swizzle), negated for a negative scale; the largest v_scale
+  // ---- queries to shared memory (K-major, 128-byte swizzle), negated for a negative scale
   {
     const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
     const bool vec = (reinterpret_cast<uintptr_t>(p.q) & 15u) == 0 && (p.qs & 7) == 0;
@@ -259,21 +259,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
       const uint32_t at = base + M::kQ + (r / kTile) * M::kQTile + (ch >> 3) * M::kQPanel + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
       sts128(at, v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip);
     }
-    uint32_t vm = 0;
-    for (int pg = (job.t0 >> p.page_log2) + tid; (pg << p.page_log2) < job.t1; pg += kThreads) {
-      const int id = page_id(p, job.b, pg);
-      const uint32_t bits = id < 0 ? 0u : __float_as_uint(p.v_scale[static_cast<int64_t>(id) * p.hkv + head]) & 0x7fffffffu;
-      if (bits < 0x7f800000u) vm = max(vm, bits);
-    }
-    vm = __reduce_max_sync(~0u, vm);
-    if (lane == 0 && vm) atomicMax(&vmax_bits, vm);
     fence_async_shared();
   }
   __syncthreads();
-  // R: the power of two above the largest scale (exponent field + 1), and 2^7 / R
-  const uint32_t r_exp = min(max((vmax_bits >> 23) + 1u, 13u), 253u);
-  const float value_unit = __uint_as_float((r_exp - 7u) << 23);  // R 2^-7
-  const float to_unit = __uint_as_float((261u - r_exp) << 23);
 
   if (warp < kSoftmaxWarps) {
     regs_inc<kSoftmaxRegs>();
@@ -316,11 +304,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         const float* v = reinterpret_cast<const float*>(x + 16 * c);
         const float t = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
                              max3(max3(v[9], v[10], v[11]), max3(v[12], v[13], v[14]), v[15]), -INFINITY);
-        top = fmaxf(top, t > -INFINITY ? t * mt.kf[c] : -INFINITY);
+        top = fmaxf(top, t > -INFINITY ? fmaf(t, mt.kf[c], mt.lv[c]) : -INFINITY);
       }
-      const bool raise = top > m + kRaise;
+      const bool raise = top > m + (kRaise + kLift);
       if (__any_sync(~0u, raise)) {
-        const float fresh = raise ? top : m;
+        const float fresh = raise ? top - kLift : m;
         const float f = raise ? (m == -INFINITY ? 0.0f : exp2_approx(m - fresh)) : 1.0f;
         m = fresh;
         l *= f;
@@ -368,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
     if (ok && n_steps > 0) ok = warp_wait(&bars.odone[a][(n_steps - 1) & 1], ((n_steps - 1) >> 1) & 1, ctl, kErrSoftmax);
     tc_fence_after();
     if (ok) {
-      const float inv = l == 0.0f ? 0.0f : value_unit / l;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       __half* dst = static_cast<__half*>(p.o) + static_cast<int64_t>(job.r.row0 + rr / G) * p.os + (head * G + rr % G) * D;
       const bool vec = (reinterpret_cast<uintptr_t>(p.o) & 15u) == 0 && (p.os & 7) == 0;
 #pragma unroll 1
@@ -443,14 +431,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const Kv8 p) {
         }
       }
     };
-    // Factors that are zero become ones so small that the products vanish all the same: 0 * infinity never meets a
-    // masked score. Of the values' factor 2^-60 is the least: below 2^-40 P' is zero as a float16.
+    // A k_scale of zero becomes a factor so small that the scores vanish all the same: 0 * infinity never meets a masked
+    // score. Value scales below 2^-60 count as 2^-60: with codes of up to 448 either is zero as a float16.
     auto make_factors = [&] {
-      const float f = fmaxf(vs * to_unit, 8.6736174e-19f);
+      const float f = fmaxf(vs, 8.6736174e-19f);
       kf = ks * fabsf(p.scale) * kLog2e;
       if (kf == kf) kf = fmaxf(kf, 1e-30f);
-      lv = vs != vs ? vs : __log2f(f);
-      iv = vs != vs ? vs : __frcp_rn(f);
+      const bool bad = !(fabsf(vs) <= 3.4028234e38f);
+      lv = bad ? __uint_as_float(0x7fc00000u) : __log2f(f);
+      iv = bad ? lv : __frcp_rn(f);
       ok_now = ok_raw;
     };
     auto load = [&](int j, uint4 (&to)[kPer]) {
