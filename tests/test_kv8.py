@@ -772,3 +772,42 @@ def test_prompts_rows_owe_nothing_to_pages_they_do_not_see(F, code, D, page, win
     off = np.abs(got - want) - tol
     assert (off <= 0).all(), (float(off.max()), float(off[free].max()))
     assert free.sum() > 60 and (np.abs(got[free]) > 0).any(-1).all()
+
+
+# ------------------------------------------------------------------------------------------ devices
+def test_workspace_is_asked_for_on_the_tensors_device(F, monkeypatch):
+    """The workspace's size depends on the device's number of SMs: it is asked for, like the launch, with the tensors' device
+    current, whichever was current before."""
+    at, seen = [0], []  # the current device; the tensors' is 3 (CPU tensors stand in for its)
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            at.append(self.index)
+
+        def __exit__(self, *a):
+            at.pop()
+
+    class Library:
+        def xrgpu_kv8_attention_workspace_size(self, p, need):
+            seen.append(("size", at[-1]))
+            need._obj.value = 1000 + at[-1]
+            return 0
+
+        def xrgpu_kv8_attention(self, p, ws, nbytes, stream):
+            seen.append(("launch", at[-1], nbytes, stream))
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[-1])
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 3)
+    monkeypatch.setattr(F, "_current_stream", lambda index: 100 + index)
+    monkeypatch.setattr(F._native, "load", lambda: Library())
+    c = R.Cache([5], heads=1, D=64, page=16, code=INT8)
+    for current in (0, 3):
+        at[:] = [current]
+        seen.clear()
+        F.attention_kv8(torch.zeros(1, 2, 64), c.k, c.v, c.ks, c.vs, c.table, None, c.lens)
+        assert seen == [("size", 3), ("launch", 3, 1003, 103)] and at == [current]

@@ -320,6 +320,17 @@ def _launch(index: int, fn, *args):
             check(fn(*args, _current_stream(index)))
 
 
+def _workspace_bytes(index: int, size, p) -> int:
+    """What `size` asks for the call p on device `index` (it may depend on the current device's number of SMs)."""
+    need = ctypes.c_uint64(0)
+    if torch.cuda.current_device() == index:
+        check(size(ctypes.byref(p), ctypes.byref(need)))
+    else:
+        with torch.cuda.device(index):
+            check(size(ctypes.byref(p), ctypes.byref(need)))
+    return need.value
+
+
 def _device_of(t: torch.Tensor, name: str) -> int:
     index = t.get_device()
     if index < 0:
@@ -587,8 +598,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     p.causal, p.window = int(bool(causal)), int(window)
     p.scale = float(scale) if scale is not None else D ** -0.5
     lib = _native.load()
-    need = ctypes.c_uint64(0)
-    check(lib.xrgpu_kv8_attention_workspace_size(ctypes.byref(p), ctypes.byref(need)))
-    ws = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
-    _launch(index, lib.xrgpu_kv8_attention, ctypes.byref(p), ws.data_ptr() if ws is not None else None, need.value)
+    need = _workspace_bytes(index, lib.xrgpu_kv8_attention_workspace_size, p)
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(index, lib.xrgpu_kv8_attention, ctypes.byref(p), ws.data_ptr() if ws is not None else None, need)
     return out
