@@ -811,3 +811,163 @@ def test_workspace_is_asked_for_on_the_tensors_device(F, monkeypatch):
         seen.clear()
         F.attention_kv8(torch.zeros(1, 2, 64), c.k, c.v, c.ks, c.vs, c.table, None, c.lens)
         assert seen == [("size", 3), ("launch", 3, 1003, 103)] and at == [current]
+
+
+# ------------------------------------------------------------------------------------------ every form of the kernels
+def _form(tokens, seqs, hq, hkv, D, f16, uniform, table_tokens):
+    """The kernels that a call takes, by the rules of mmnb_kv8_attn.cu and mmnb_kv8_attn_mma.cuh."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    G, mean = hq // hkv, -(-tokens // seqs)
+    rows, pairs = mean * G, seqs * hkv
+    prompt = f16 and rows > 64 and pairs * rows * D >= -(-pairs * -(-rows // 256) // sms) * 6500 * 128
+    forms = {"prompt"} if prompt else set()
+    if prompt and uniform:
+        return forms
+    slots = -(-(tokens // seqs * G) // 8) * seqs if uniform else tokens * G // 8 + seqs
+    split = 8
+    while split > 1 and slots * hkv * split > sms:
+        split //= 2
+    if split > 1 and -(-table_tokens // 32) <= 48 * split:
+        return forms | {"cluster"}
+    return forms | {"one tile" if min(rows, 64 if prompt else rows) <= 8 else "two tiles"}
+
+
+def _gpu_cache(lens, hkv, D, page, code, seed):
+    """Tensors of a cache in use, made on the GPU: codes of every value, pages in no order."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    P = sum(need) + 3
+    order = torch.randperm(P, generator=g, device="cuda").int().cpu()
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+
+    def side():
+        codes = torch.randint(-127, 128, (P, hkv, page, D), generator=g, device="cuda", dtype=torch.int8)
+        return (codes if code == INT8 else (codes.float() * 3.5).to(E4M3)), (torch.rand(P, hkv, generator=g, device="cuda") * 1.5 + 0.5) * 3.5 / R.LIMIT[code]
+
+    (k, ks), (v, vs) = side(), side()
+    return k, v, ks, vs, table.cuda()
+
+
+def _check_on_gpu(F, dev, lens, new, hq, dtype, seed):
+    """As _check, with R.attention's values and tolerance (causal, no window) computed on the GPU in float64, and for int8 codes
+    under float16 rows one term more, which matters where every code that a row sees is (next to) zero: the split kernel
+    sums p (c + 128) and takes 128 p out again, in four accumulations a step of 32 tokens, each rounded (or truncated: 2^-23) at
+    no more than 255 times the sum of the step's weights; times the page's scale s and over all steps that is
+    4 * 255 * 2^-23 < 2^-13 of sum_j p_j s_j: 2^-13 of a code."""
+    k, v, ks, vs, table = dev
+    hkv, page, D = k.shape[1], k.shape[2], k.shape[3]
+    G, T = hq // hkv, sum(new)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(T, hq, D, generator=g, device="cuda").to(dtype)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = F.attention_kv8(q, *dev, _cu(new).cuda(), n)
+    again = F.attention_kv8(q, *dev, _cu(new).cuda(), n)
+    assert F.device_error(0) == 0 and torch.equal(got, again)
+    f16, at = dtype == torch.float16, 0
+    for b, (total, m) in enumerate(zip(lens, new)):
+        if m == 0:
+            continue
+        rows = slice(at, at + m)
+        at += m
+        if total == 0:
+            assert not got[rows].any()
+            continue
+        ids = table[b, :-(-total // page)].long()
+        kk, vv = ((c[ids].float().double() * s[ids].double()[..., None, None]).transpose(1, 2).reshape(-1, hkv, D)[:total].transpose(0, 1) for c, s in ((k, ks), (v, vs)))
+        x = q[rows].double().view(m, hkv, G, D).permute(1, 2, 0, 3).reshape(hkv, G * m, D)
+        hide = torch.arange(total, device="cuda") > (total - m + torch.arange(m, device="cuda").repeat(G))[:, None]
+        s = (x @ kk.transpose(1, 2) * D ** -0.5).masked_fill(hide, float("-inf"))
+        blind = torch.isinf(s.amax(-1))
+        w = torch.exp(s - s.amax(-1, keepdim=True)).nan_to_num(0.0)
+        sums = w.sum(-1, keepdim=True).clamp(min=1e-300)
+        o = (w @ vv) / sums
+        d = (D + 8) * 2.0 ** -24 * (x.abs() @ kk.abs().transpose(1, 2)).masked_fill(hide, 0.0).amax(-1, keepdim=True) * D ** -0.5
+        rel = 2 * d + 2.0 ** -20 + 2 * (2.0 ** -11 if f16 else 2.0 ** -21) + (64 + total / 64) * 2.0 ** -24
+        tol = rel * (w @ vv.abs()) / sums + 2.0 ** -25 / sums * ((~hide).double() @ vv.abs()) + (2.0 ** -11 if f16 else 2.0 ** -24) * o.abs() + 2.0 ** -24 * f16
+        if f16 and k.dtype == INT8:
+            tol = tol + 2.0 ** -13 * (w @ vs[ids].double().repeat_interleave(page, 0)[:total].t()[..., None]) / sums
+        mine = got[rows].double().view(m, hkv, G, D).permute(1, 2, 0, 3).reshape(hkv, G * m, D)
+        off = ((mine - o).abs() - tol).masked_fill(blind[..., None], 0.0)
+        assert bool((off <= 0).all()), (b, float(off.max()))
+        assert not mine[blind].any()
+    return got
+
+
+LONG = [("one tile", 1, 4), ("two tiles", 3, 4), ("two tiles", 1, 24)]  # form, rows a sequence, group
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64), (64, 128), (128, 32)])
+@pytest.mark.parametrize("form,rows,G", LONG)
+def test_long_runs_of_the_split_kernel(F, code, dtype, D, page, form, rows, G):
+    """Runs of more than 16 steps a warp (rings used again and again, page ids looked up in several batches), segments cut between
+    CTAs, sequences of very different lengths."""
+    hkv = 8
+    rng = np.random.default_rng(page)
+    lens = [int(n) for n in rng.integers(3000, 9000, 40)] + [rows, 31 + rows, 64]
+    new = [rows] * len(lens)
+    assert _form(sum(new), len(new), G * hkv, hkv, D, dtype == torch.float16, False, -(-max(lens) // page) * page) == {form}
+    assert sum(-(-n // 32) for n in lens) * hkv * -(-rows * G // (8 if form == "one tile" else 16)) > 20 * 6 * 2 * 148
+    _check_on_gpu(F, _gpu_cache(lens, hkv, D, page, code, D + page), lens, new, G * hkv, dtype, 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_forms_are_all_reached(F, dtype):
+    """A few sequences of each form by its rule: the same call shapes as in the tests above, counted."""
+    seen = set()
+    for lens, new, hkv, G, D in (([2000], [1], 2, 4, 128), ([700] * 30, [1] * 30, 8, 4, 64), ([700] * 30, [5] * 30, 8, 4, 64), ([900, 20], [400, 1], 8, 4, 128),
+                                 ([900, 700], [400, 400], 8, 4, 128)):
+        seen |= (form := _form(sum(new), len(new), G * hkv, hkv, D, dtype == torch.float16, False, -(-max(lens) // 64) * 64))
+        assert form
+        _check_on_gpu(F, _gpu_cache(lens, hkv, D, 64, INT8, 3), lens, new, G * hkv, dtype, 2)
+    assert seen == {"cluster", "one tile", "two tiles"} | ({"prompt"} if dtype == torch.float16 else set())
+
+
+def _many(count, most, seed):
+    """(tokens held before, new rows) of `count` short ragged sequences, empty ones among them."""
+    rng = np.random.default_rng(seed)
+    past, new = rng.integers(0, 120, count), rng.integers(0, most + 1, count)
+    past[::7] = 0
+    new[::5] = 0
+    new[count // 2: count // 2 + 40] = 0
+    return past.tolist(), new.tolist()
+
+
+@gpu
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("count,most", [(130, 3), (400, 1), (700, 40)])
+def test_many_sequences_append_and_read(F, code, count, most):
+    """More sequences than a CTA has threads: the searches go on past their first pass."""
+    past, new = _many(count, most, count)
+    c = R.Cache([a + b for a, b in zip(past, new)], heads=2, D=64, page=16, code=code, seed=count)
+    c.poison_tails()
+    T = sum(new)
+    k, v = (torch.randn(T + 3, 2, 64, generator=torch.Generator().manual_seed(i)) * 3 for i in (1, 2))
+    cu, dev = _cu(new), c.cuda()
+    F.kv8_append(k.cuda(), v.cuda(), *dev, cu.cuda(), c.lens.cuda())
+    R.append(c, k, v, cu)
+    used = c.table[c.table >= 0].long()
+    assert torch.equal(dev[2].cpu()[used], c.ks[used]) and torch.equal(dev[3].cpu()[used], c.vs[used])
+    rk, rv = F.kv8_read(*dev, cu.cuda(), c.lens.cuda(), rows=T + 3, dtype=torch.float32)
+    want = [torch.from_numpy(np.concatenate([c.tokens(b)[i][past[b]:] for b in range(count)])).float() for i in (0, 1)]
+    for got, w in ((rk, want[0]), (rv, want[1])):
+        assert torch.equal(got[:T].cpu(), w) and not got[T:].any()
+    assert F.device_error(0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("count,most,hkv,form", [(400, 1, 2, {"one tile"}), (700, 7, 1, {"two tiles"}), (90, 150, 2, {"prompt", "two tiles"})])
+def test_many_sequences_attention(F, dtype, count, most, hkv, form):
+    past, new = _many(count, most, count)
+    lens = [max(1, a + b) if b else a + b for a, b in zip(past, new)]
+    if dtype == torch.float16 or "prompt" not in form:
+        assert _form(sum(new), count, 4 * hkv, hkv, 128, dtype == torch.float16, False, -(-max(lens) // 16) * 16) == form
+    _check_on_gpu(F, _gpu_cache(lens, hkv, 128, 16, INT8, count), lens, new, 4 * hkv, dtype, 3)

@@ -341,3 +341,29 @@ def test_product_of_pairs_is_exact_again_and_again(F, M, N, K):
         a, w = (F.mxfp4_dequantize(held[i], held[i + 1], K=K).double() for i in (0, 2))
         assert torch.equal(out.double(), a @ w.t())  # below 2^24 quarters
     assert F.device_error(0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(256, 14336, 544), (200, 14200, 96), (129, 18900, 4130), (250, 9700, 2080)])
+def test_product_of_single_ctas_with_256_columns(F, dtype, M, N, K):
+    """Tiles of 128 x 256 by one CTA each: more tiles of 128 columns than SMs, no more of 256; sums exact in float32."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert M > 128 and -(-M // 128) * -(-N // 128) > sms >= -(-M // 128) * -(-N // 256)
+    kb = -(-K // 32)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    held = []
+    for rows in (M, N):
+        x = torch.randint(0, 256, (rows, kb, 16), generator=g, dtype=torch.uint8, device="cuda")
+        if K % 32:
+            x[:, -1, K % 32 // 2:] = 0
+        held += [x, F.mxfp4_tile_scales(torch.randint(119, 121, (rows, kb), generator=g, dtype=torch.uint8, device="cuda"))]
+    bias = torch.randn(N, generator=g, device="cuda").to(dtype)
+    a, w = (F.mxfp4_dequantize(held[i], held[i + 1], K=K).double() for i in (0, 2))
+    y = a @ w.t()
+    for _ in range(3):
+        got = F.matmul_mxfp4(held[0], held[2], held[3], a_scales=held[1], K=K, dtype=dtype)
+        assert torch.equal(got, y.to(dtype))
+        got = F.matmul_mxfp4(held[0], held[2], held[3], bias, a_scales=held[1], K=K, dtype=dtype)
+        assert torch.equal(got, (y.float() + bias.float()).to(dtype))  # one float32 sum, rounded once
+    assert F.device_error(0) == 0
