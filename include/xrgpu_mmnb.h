@@ -554,8 +554,12 @@ XRGPU_API int xrgpu_kv8_read(const xrgpu_kv8_problem* p, void* stream);
 /* o[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j of the row's sequence that it sees;
  * query head h reads key/value head h / (heads_q / heads_kv). A row that sees nothing gives zeros (cu_seqlens may
  * hold more rows than kv_len tokens here; the first ones then see nothing); so do the rows of a sequence whose
- * kv_len does not fit. Tokens of a bad page id are left out; pages whose tokens all lie in front of what the call's rows of
- * the sequence see (a window) are not looked up, so their ids may be anything. */
+ * kv_len does not fit. Tokens of a bad page id are left out; pages whose tokens all lie in front of what the call's rows
+ * of the sequence see (a window) are not looked up, so their ids may be anything.
+ * Sums, maxima and normalisers are float32. The softmax's weights are rounded to float16 for float16 rows (2^-12
+ * relative, once; in prompts the products of weight and value scale, those below 2^-21 of the row's largest in steps of 2^-31
+ * of it); for float32 rows they keep 2^-24. Codes are numbers: a NaN among e4m3 codes (append writes none, its blocks with
+ * one have a NaN scale instead) may reach rows of the call that do not see its token. */
 XRGPU_API int xrgpu_kv8_attention_workspace_size(const xrgpu_kv8_problem* p, uint64_t* bytes);
 /* workspace as in xrgpu_mxfp4_forward. */
 XRGPU_API int xrgpu_kv8_attention(const xrgpu_kv8_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);

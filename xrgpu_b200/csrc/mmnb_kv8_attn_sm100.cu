@@ -27,7 +27,8 @@
 // Bounds per 128 tokens and 256 rows at D = 128, in cycles: tensor cores 2048, exponentials (16 a cycle) 2048, shared memory
 // (Q and K read for each S, V for each O, keys and values written: 320 KB) 2560. Measured 6000, the chain of the softmax
 // warps (read S, maximum, exponentials, convert, write P', signal): 2 ragged prompts of up to 4096 rows on as many tokens, 32
-// heads on 8 of 128: 446 us, 761 TFLOP/s; 4 x 1024 rows on 4096 tokens 335 us, 716 TFLOP/s.
+// heads on 8 of 128: 443 us, 766 TFLOP/s; 4 x 1024 rows on 4024 tokens 318 us, 742 TFLOP/s (e4m3 305 us; heads of 64 271 and 268
+// us: the same chain for half the products).
 //
 // Every wait is bounded as in mmnb_gemm_sm100.cu.
 #include <cuda_runtime.h>

@@ -19,8 +19,9 @@
 // its shared-memory buffer has come back, that is when the MMAs that read them are done. Only tiles of up to 128 columns
 // take turns on a CTA (more rows than that go to pairs of CTAs before they need a second round).
 //
-// Measured (codes in, GPU time): 1 x 4096 x 4096 6.3 us (latency), 16 x 14336 x 4096 8.5 us (31 MB, 3.7 TB/s: latency, then the
-// weights' stream), 2048 x 14336 x 4096 59 us (4.1 PFLOP/s), 8192 x 28672 x 8192 671 us (5.7 PFLOP/s, bound by loads from L2).
+// Measured (codes in, GPU time without the launch): 1 x 4096 x 4096 6.3 us (latency), 16 x 14336 x 4096 8.5 us (31 MB, 3.7
+// TB/s: latency, then the weights' stream), 2048 x 14336 x 4096 54 us (4.5 PFLOP/s), 8192 x 28672 x 8192 671 us (5.7 PFLOP/s,
+// bound by loads from L2; 700 us in calls back to back, at the power limit).
 //
 // Every wait is bounded as in mmnb_gemm_sm100.cu.
 #include <cuda.h>
@@ -381,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // of 384 for the same product. What bounds it are these loads from L2, 35 KB a CTA and step (12 TB/s in all): 8192 x
 // 28672 x 8192 takes 671 us (5.7 PFLOP/s); with the loads left out it was 507.
 // Tensor memory: two overlapping accumulators of 256 columns (they and the scales need more than the 512 columns); the
-// drain first takes the shared columns into registers, then the next tile may start (waiting for their stores: 73 -> 66
-// us at 2048 x 14336 x 4096). Each CTA keeps the accumulators of its own rows and all scales it needs.
+// drain first takes the shared columns into registers, then the next tile may start (without waiting for their stores: 73
+// -> 66 us at 2048 x 14336 x 4096 with the launch, before the signals had their present form: 66 -> 61.5). Each CTA keeps the accumulators of its own rows and all scales it needs.
 // Signals between the two. Both CTAs' loads complete on the first one's `full` (the scales too are tensor copies: only those
 // may signal the pair's other CTA), which expects the bytes of both. The MMAs' completion goes to both. The second CTA's
 // epilogue warps meet at its own `drained`, and its warp 1 passes that on with a release at cluster scope. What the
@@ -690,8 +691,8 @@ cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, 
 }
 
 // Pairs take what would need a second round of 128 x 256 tiles. Measured (us with the launch, one CTA a tile / pairs):
-// 256 x 14336 x 4096 20.5 / 20.6, 1024 x 4096 x 14336 36.9 / 38.9, 1152 x 4096 x 4096 (144 tiles) 18.4 / 24.6;
-// 2048 x 14336 x 4096 78.8 / 64, 4096 x 8192 x 8192 132 / 108, 8192 x 28672 x 8192 852 / 671.
+// 256 x 14336 x 4096 20.5 / 20.5, 1152 x 4096 x 4096 (144 tiles) 18.4 / 22.6, 512 x 4096 x 4096 14.3 / 16.4, but 1024 x 4096 x
+// 14336 36.9 / 32.8: many steps along K favour pairs, which the rule leaves out; 2048 x 14336 x 4096 78.8 / 61.5, 4096 x 8192 x 8192 132 / 108, 8192 x 28672 x 8192 852 / 671.
 bool pairs_pay(const Mxfp4Matmul& p, int sms) {
   return p.M > kRows && ceil_div(p.M, kRows) * ceil_div(p.N, 256) > sms;
 }
@@ -708,7 +709,8 @@ cudaError_t launch_pairs(const Mxfp4Matmul& p, Args a, bool early, cudaStream_t 
   a.p_tiles = static_cast<int>(ceil_div(p.M, 256));
   const int64_t tiles = a.p_tiles * ceil_div(p.N, 256);
   if (tiles > INT_MAX / 8) return cudaErrorInvalidValue;
-  // A last round with few tiles takes them in halves (2048 x 14336 x 4096, 448 tiles on 74 pairs: 69.7 -> 67.6 us).
+  // A last round with few tiles takes them in halves (2048 x 14336 x 4096, 448 tiles on 74 pairs: 69.7 -> 67.6 us with the
+  // launch, when it was added).
   const int pairs = device_sm_count() / 2, rest = static_cast<int>(tiles % pairs);
   const bool halve = tiles > pairs && 2 * rest <= pairs;
   a.whole = static_cast<int>(halve ? tiles - rest : tiles);

@@ -583,7 +583,8 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     tokens up to its own position (causal), the last `window` of them if given, or all kv_len (causal=False). Query
     head h reads key/value head h // (query heads // heads). scale defaults to head_dim ** -0.5. Pages in front of every
     row's window are not looked up (released ones may be -1). A row that sees nothing gives zeros; with ``out``, rows
-    behind the last sequence are left as they were (without it they are zero).
+    behind the last sequence are left as they were (without it they are zero). Sums are float32; for float16 rows the softmax's
+    weights are rounded to float16 on their way to the values (2^-12 of each), for float32 rows they keep 2^-24.
     """
     p, index, H, D = _kv8_problem(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, kv_len, q.dtype)
     p.q_stride = _head_rows(q, "q", None, D, index)
