@@ -564,6 +564,95 @@ XRGPU_API int xrgpu_kv8_attention_workspace_size(const xrgpu_kv8_problem* p, uin
 /* workspace as in xrgpu_mxfp4_forward. */
 XRGPU_API int xrgpu_kv8_attention(const xrgpu_kv8_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * 8-bit integer products, dense and grouped by expert, and the router that makes the groups (extensions).
+ * ------------------------------------------------------------------------------------- */
+
+/* Rows as 8-bit codes with one float32 scale: value = code * scale.
+ *   codes  int8 [rows, ldc], 16-byte aligned, ldc a multiple of 16 of at least K (0: K rounded up to 16); a buffer
+ *          of rows * ldc bytes. What lies behind a row's K codes may be written and is never read.
+ *   scales float32 [rows] */
+typedef struct {
+  int32_t dtype;     /* of the unquantised side: XRGPU_FLOAT16 or XRGPU_FLOAT32 */
+  int32_t reserved;
+  int64_t rows, K, ldc;
+  int8_t* codes;
+  float* scales;
+} xrgpu_int8_tensor;
+
+/* x [rows, ldx] (ldx 0: K) -> t->codes, t->scales: s = max|x| / 127 in float32, code = x / s rounded to nearest, ties
+ * to even. A row of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and codes 0. */
+XRGPU_API int xrgpu_int8_quantize(const xrgpu_int8_tensor* t, const void* x, int64_t ldx, void* stream);
+
+/* The values t holds -> out [rows, K] (contiguous, t->dtype). */
+XRGPU_API int xrgpu_int8_dequantize(const xrgpu_int8_tensor* t, void* out, void* stream);
+
+/* Dense (groups 0):  y[m] = act(sum_k a[m, k] b[n, k] * a_scales[m] * b_scales[n] + bias[n]),  M rows.
+ * Grouped: rows offsets[g] .. offsets[g + 1] - 1 of the product take b[g], b_scales[g], bias[g]; its row r reads row
+ * order[r] / top_k of a, or row r without order (then M = rows). Offsets that decrease or leave [0, rows] drop their group
+ * (0x701 in the device error word), an order entry outside [0, M * top_k) counts as a row of zeros (0x702). Rows of no
+ * group are left as they were.
+ * With slots and weights the call returns sums of the product's rows instead: y[t] = sum_j weights[t, j] * row
+ * slots[t, j], j < top_k, for `tokens` rows t, in float32 and in the order of j; slots outside [0, rows) are left out, rows of no
+ * group are zero.
+ * The integer sums are exact (codes -128 .. 127, K <= 131071); what follows is float32, rounded once to y's type.
+ * Activation: XRGPU_ACT_NONE, XRGPU_ACT_RELU, or XRGPU_ACT_SWIGLU over channel pairs (2i gate, 2i + 1 linear; y has N / 2
+ * columns): gate * sigmoid(alpha * gate) * (linear + beta), with has_limit gate clamped to <= limit and linear to
+ * [-limit, limit], as XRGPU_ACT_SWIGLU of xrgpu_qmoe_forward. */
+typedef struct {
+  int32_t dtype;            /* of y and bias: XRGPU_FLOAT16 or XRGPU_FLOAT32 */
+  int32_t a_dtype;          /* XRGPU_INT8: a holds codes; XRGPU_FLOAT16 / XRGPU_FLOAT32: quantised by the call */
+  int32_t activation;
+  int32_t has_limit;
+  float alpha, beta, limit;
+  int32_t zero_rest;        /* nonzero: rows of no group are set to zero */
+  int64_t M, K, N;          /* rows of a; columns of a and b; rows of b (of a group) */
+  int64_t groups;           /* 0: dense; at most 1024 */
+  int64_t rows;             /* grouped: rows of the product */
+  int64_t top_k;            /* with order, or with slots */
+  int64_t tokens;           /* with slots: rows of y */
+  const void* a;            /* codes [M, lda] (16-byte aligned, lda a multiple of 16; 0: K rounded up), or floats [M, lda] (0: K) */
+  const float* a_scales;    /* [M] (a_dtype XRGPU_INT8), else NULL */
+  int64_t lda;
+  const int8_t* b;          /* codes [N, ldb] or [groups, N, ldb], 16-byte aligned, ldb as lda of codes */
+  const float* b_scales;    /* [N] or [groups, N] */
+  int64_t ldb;
+  const void* bias;         /* [N] or [groups, N], or NULL */
+  const int32_t* offsets;   /* [groups + 1] */
+  const int32_t* order;     /* [rows] or NULL */
+  const int32_t* slots;     /* [tokens, top_k] or NULL */
+  const float* weights;     /* [tokens, top_k], with slots */
+  void* y;                  /* [M | rows | tokens, ldy] */
+  int64_t ldy;              /* 0: contiguous */
+} xrgpu_int8_problem;
+
+/* Device scratch bytes of xrgpu_int8_forward (quantised activations; with slots the product's rows in float32). */
+XRGPU_API int xrgpu_int8_workspace_size(const xrgpu_int8_problem* p, uint64_t* bytes);
+/* workspace as in xrgpu_mxfp4_forward. */
+XRGPU_API int xrgpu_int8_forward(const xrgpu_int8_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Router of a mixture of experts. Of each token the top_k experts with the highest scores, best first, ties to the lowest
+ * index (a NaN counts as -infinity); their weights exp(score) over the sum of the chosen ones' (normalize), or of all
+ * experts'; a token whose scores are all -infinity has weights 0. Then all assignments i = token * top_k + rank in
+ * the experts' order, those of an expert ascending: order [tokens * top_k], slots [tokens, top_k] (the place of each in it),
+ * offsets [experts + 1] (the first place of each expert). */
+typedef struct {
+  int32_t dtype;            /* of scores: XRGPU_FLOAT16 or XRGPU_FLOAT32 */
+  int32_t normalize;
+  int64_t tokens, experts, top_k;  /* top_k <= min(experts, 32), experts <= 1024 */
+  int64_t lds;              /* row stride of scores in elements; 0: experts */
+  const void* scores;
+  int32_t* chosen;          /* [tokens, top_k] */
+  float* weights;           /* [tokens, top_k] */
+  int32_t* order;
+  int32_t* slots;
+  int32_t* offsets;
+} xrgpu_moe_route_problem;
+
+XRGPU_API int xrgpu_moe_route_workspace_size(const xrgpu_moe_route_problem* p, uint64_t* bytes);
+/* workspace as in xrgpu_mxfp4_forward. */
+XRGPU_API int xrgpu_moe_route(const xrgpu_moe_route_problem* p, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Library version string. */
 XRGPU_API const char* xrgpu_version(void);
 

@@ -35,6 +35,8 @@ EXPORTED = (
     "xrgpu_mxfp4_scale_bytes", "xrgpu_mxfp4_quantize", "xrgpu_mxfp4_dequantize", "xrgpu_mxfp4_tile_scales",
     "xrgpu_mxfp4_workspace_size", "xrgpu_mxfp4_forward", "xrgpu_kv8_append", "xrgpu_kv8_read",
     "xrgpu_kv8_attention_workspace_size", "xrgpu_kv8_attention",
+    "xrgpu_int8_quantize", "xrgpu_int8_dequantize", "xrgpu_int8_workspace_size", "xrgpu_int8_forward",
+    "xrgpu_moe_route_workspace_size", "xrgpu_moe_route",
 )
 # xrgpu_activation
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_TANH, ACT_SIGMOID, ACT_SWIGLU = range(7)
@@ -145,6 +147,26 @@ class Kv8Problem_(ctypes.Structure):
                 ("page_table", _vp), ("cu_seqlens", _vp), ("kv_len", _vp)]
 
 
+class Int8Tensor_(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("rows", _i64), ("K", _i64), ("ldc", _i64),
+                ("codes", _vp), ("scales", _vp)]
+
+
+class Int8Problem_(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("a_dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("has_limit", ctypes.c_int32), ("alpha", ctypes.c_float), ("beta", ctypes.c_float), ("limit", ctypes.c_float),
+                ("zero_rest", ctypes.c_int32), ("M", _i64), ("K", _i64), ("N", _i64), ("groups", _i64), ("rows", _i64),
+                ("top_k", _i64), ("tokens", _i64), ("a", _vp), ("a_scales", _vp), ("lda", _i64), ("b", _vp), ("b_scales", _vp),
+                ("ldb", _i64), ("bias", _vp), ("offsets", _vp), ("order", _vp), ("slots", _vp), ("weights", _vp), ("y", _vp),
+                ("ldy", _i64)]
+
+
+class MoeRouteProblem_(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("normalize", ctypes.c_int32), ("tokens", _i64), ("experts", _i64), ("top_k", _i64),
+                ("lds", _i64), ("scores", _vp), ("chosen", _vp), ("weights", _vp), ("order", _vp), ("slots", _vp),
+                ("offsets", _vp)]
+
+
 _lib = None
 
 
@@ -211,6 +233,12 @@ def load(path: os.PathLike | None = None):
         "xrgpu_kv8_read": ([P(Kv8Problem_), vp], ctypes.c_int),
         "xrgpu_kv8_attention_workspace_size": ([P(Kv8Problem_), P(u64)], ctypes.c_int),
         "xrgpu_kv8_attention": ([P(Kv8Problem_), vp, u64, vp], ctypes.c_int),
+        "xrgpu_int8_quantize": ([P(Int8Tensor_), vp, _i64, vp], ctypes.c_int),
+        "xrgpu_int8_dequantize": ([P(Int8Tensor_), vp, vp], ctypes.c_int),
+        "xrgpu_int8_workspace_size": ([P(Int8Problem_), P(u64)], ctypes.c_int),
+        "xrgpu_int8_forward": ([P(Int8Problem_), vp, u64, vp], ctypes.c_int),
+        "xrgpu_moe_route_workspace_size": ([P(MoeRouteProblem_), P(u64)], ctypes.c_int),
+        "xrgpu_moe_route": ([P(MoeRouteProblem_), vp, u64, vp], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

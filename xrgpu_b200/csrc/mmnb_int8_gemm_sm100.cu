@@ -1,0 +1,602 @@
+// Product of 8-bit integer operands with scales for each token and channel, dense or grouped by expert (problem:
+// mmnb_int8.h), on tcgen05 tensor cores:
+//   y[r, n] = act((sum_k a[r, k] b[n, k]) sa[r] sb[n] + bias[n]), the sum exact in int32.
+//
+// Orientation. The weights' channels are the MMA's 128-row operand P, the tokens its other one, Q, of any multiple of
+// 16 columns up to 256: a group with few rows pays for few columns, weights stream whole, and an accumulator's 32 lanes are
+// neighbours of a row of y. A tile is 128 channels of a group by up to tmax of its rows (a group's rows are cut evenly).
+//
+// Groups. Offsets are on the device: every CTA counts the groups' tiles itself (a scan in shared memory) and takes tiles
+// of one line, group by group, the tiles of the same channels next to each other. Offsets that do not fit leave out their group
+// and record an error. With `order` the token rows are fetched where they lie (four-row gather copies).
+//
+// Roles (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 drain (lane quadrant warp % 4, alternate 16-column chunks).
+// Few tiles: K is split over a cluster of up to 8 CTAs whose int32 partial tiles meet in shared memory.
+//
+// Every wait is bounded as in mmnb_gemm_sm100.cu.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+
+#include "mmnb_int8.h"
+#include "mmnb_tcgen05.cuh"
+
+namespace xrgpu {
+namespace {
+
+constexpr int kRows = 128;       // channels of a tile
+constexpr int kStepBytes = 128;  // codes of a row per stage: one swizzle row
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = (2 + kEpilogueWarps) * 32;
+constexpr int kSmemBudget = 227 * 1024 - 10 * 1024;  // dynamic: less what is declared
+constexpr int kMaxStages = 12;
+constexpr int kMaxT = 256;
+constexpr int kPitch = kRows;    // int32 values a column of a partial tile in shared memory
+
+constexpr unsigned kErrOffsets = 0x701;
+constexpr unsigned kErrOrder = 0x702;
+constexpr unsigned kErrWaitProducer = 0x711;
+constexpr unsigned kErrWaitMma = 0x712;
+constexpr unsigned kErrWaitEpilogue = 0x713;
+constexpr unsigned kErrDrain = 0x714;
+
+struct Args {
+  int n, p_tiles, groups, rows, a_rows;
+  int tmax, box;               // most rows of Q a tile (a multiple of 16); rows of one copy
+  int ksteps, ksubs;           // stages along K, 32-value MMA steps along K
+  int stages, split;
+  int tmem_cols, acc1;         // acc1: column of the second accumulator
+  int early;                   // the weights may be loaded before the previous kernel has finished
+  uint32_t stage;              // bytes
+  uint32_t tables;             // bytes from the stages' start to the group tables
+  int top_k, act, has_limit, zero_rest, bias_f16;
+  float alpha, beta, limit;
+  const int32_t* offsets;
+  const int32_t* order;
+  const float* a_scales;
+  const float* b_scales;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int vec;                     // pairs of y start on their size
+  unsigned* err;
+};
+
+// D[128 x T] (+)= P (smem, K-major codes) . Q^T in int32.
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: int32 sums of signed 8-bit operands, both K-major, M rows, T columns.
+__device__ __forceinline__ uint32_t instruction_desc(int M, int T) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(T >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Four rows of 128 bytes, at `x` bytes into rows r.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&r)[4], uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// ------------------------------------------------------------------ tiles
+// Tables in shared memory: tile_first [groups + 1] (tiles along the rows before a group), row_first, row_count [groups].
+struct Tables {
+  int* tile_first;
+  int* row_first;
+  int* row_count;
+};
+__device__ __forceinline__ Tables tables_at(uint8_t* at, int groups) {
+  int* t = reinterpret_cast<int*>(at);
+  return {t, t + groups + 1, t + 2 * groups + 1};
+}
+inline uint32_t tables_bytes(int groups) { return static_cast<uint32_t>(align_up(static_cast<uint64_t>(3 * groups + 1) * 4, 16)); }
+
+// All threads; ends with a barrier.
+__device__ __forceinline__ void make_tables(const Args& a, const Tables& t) {
+  __shared__ int chunk_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int base = 32 * warp; base < a.groups; base += kThreads) {
+    const int g = base + lane;
+    int tiles = 0;
+    if (g < a.groups) {
+      int lo = 0, hi = a.rows;
+      if (a.offsets) {
+        lo = a.offsets[g];
+        hi = a.offsets[g + 1];
+        if (lo < 0 || hi < lo || hi > a.rows) {
+          if (blockIdx.x == 0) record_device_error(a.err, kErrOffsets);
+          lo = hi = 0;
+        }
+      }
+      t.row_first[g] = lo;
+      t.row_count[g] = hi - lo;
+      tiles = (hi - lo + a.tmax - 1) / a.tmax;
+    }
+    int s = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(~0u, s, o);
+      if (lane >= o) s += u;
+    }
+    if (g < a.groups) t.tile_first[g + 1] = s;
+    if (lane == 31) chunk_sum[base >> 5] = s;
+  }
+  if (threadIdx.x == 0) t.tile_first[0] = 0;
+  __syncthreads();
+  if (a.groups > 32) {
+    for (int base = 32 * warp; base < a.groups; base += kThreads) {
+      const int chunk = base >> 5;
+      const int before = __reduce_add_sync(~0u, lane < chunk ? chunk_sum[lane] : 0);
+      if (base + lane < a.groups) t.tile_first[base + lane + 1] += before;
+    }
+    __syncthreads();
+  }
+}
+
+struct Tile {
+  int group, pt;   // block of channels
+  int row0, rows;  // rows of the product
+  int width;       // columns of the MMA: a multiple of GRAIN
+};
+template <int GRAIN>
+__device__ __forceinline__ Tile tile_at(const Args& a, const Tables& t, int tile) {
+  const int q = tile / a.p_tiles;
+  int lo = 0, hi = a.groups;  // the last group that begins at or before q
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.tile_first[mid] <= q) lo = mid;
+    else hi = mid;
+  }
+  const int first = t.tile_first[lo], nt = t.tile_first[lo + 1] - first, count = t.row_count[lo];
+  const int local = tile - first * a.p_tiles, pt = local / nt, qt = local - pt * nt;
+  const int even = (count + nt - 1) / nt, width = (even + GRAIN - 1) / GRAIN * GRAIN;
+  return {lo, pt, t.row_first[lo] + qt * width, min(width, count - qt * width), width};
+}
+
+// The row of a that a row of the product reads; -1 where order does not fit.
+__device__ __forceinline__ int source_row(const Args& a, int r) {
+  if (!a.order) return r;
+  const int o = a.order[r], t = o / a.top_k;
+  return o < 0 || t >= a.a_rows ? -1 : t;
+}
+
+// ------------------------------------------------------------------ results
+template <bool F16>
+__device__ __forceinline__ void put(void* y, int64_t at, float v) {
+  if (F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
+  else static_cast<float*>(y)[at] = v;
+}
+
+// (gate, linear) -> gate sigmoid(alpha gate) (linear + beta)
+__device__ __forceinline__ float swiglu(const Args& a, float g, float l) {
+  if (a.has_limit) {
+    g = g > a.limit ? a.limit : g;
+    l = l > a.limit ? a.limit : l < -a.limit ? -a.limit : l;
+  }
+  return g / (1.0f + expf(-a.alpha * g)) * (l + a.beta);
+}
+
+// 16 columns (rows row0 + col0 + j of y) of the lane's channel n, scaled already. All lanes of the warp take part.
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void store_columns(const Args& a, const float (&f)[16], int row0, int col0, int rows, int n, int lane) {
+  const bool odd = lane & 1;
+  if (SWIGLU) {
+    // A channel's neighbour holds the other half of its pair: even lanes take the even columns, odd lanes the odd ones.
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float other = __shfl_xor_sync(~0u, odd ? f[j] : f[j + 1], 1);
+      const float r = odd ? swiglu(a, other, f[j + 1]) : swiglu(a, f[j], other);
+      const int c = col0 + j + (odd ? 1 : 0);
+      if (c < rows && n < a.n) put<F16>(a.y, static_cast<int64_t>(row0 + c) * a.ldy + (n >> 1), r);
+    }
+  } else if (F16) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float other = __shfl_xor_sync(~0u, odd ? f[j] : f[j + 1], 1);
+      const __half2 h = odd ? __floats2half2_rn(other, f[j + 1]) : __floats2half2_rn(f[j], other);
+      const int c = col0 + j + (odd ? 1 : 0), n0 = n & ~1;
+      if (c >= rows || n0 >= a.n) continue;
+      __half* dst = static_cast<__half*>(a.y) + static_cast<int64_t>(row0 + c) * a.ldy + n0;
+      if (a.vec && n0 + 1 < a.n) {
+        *reinterpret_cast<__half2*>(dst) = h;
+      } else {
+        dst[0] = __low2half(h);
+        if (n0 + 1 < a.n) dst[1] = __high2half(h);
+      }
+    }
+  } else if (n < a.n) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (col0 + j >= rows) break;
+      static_cast<float*>(a.y)[static_cast<int64_t>(row0 + col0 + j) * a.ldy + n] = f[j];
+    }
+  }
+}
+
+// Product first with the token's, then with the channel's scale: an int32 and two float32 numbers, each step rounded to 2^-24.
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias, bool relu) {
+  const float r = fmaf(static_cast<float>(acc) * sa, sb, bias);
+  return relu && !(r > 0.0f) && r == r ? 0.0f : r;
+}
+
+// Rows of no group (before the first offset, behind the last) become zero.
+template <bool F16>
+__device__ __forceinline__ void zero_rest(const Args& a, int width) {
+  if (!a.zero_rest || !a.offsets) return;
+  const int lo = min(max(a.offsets[0], 0), a.rows), hi = min(max(a.offsets[a.groups], lo), a.rows);
+  for (int r = blockIdx.x; r < lo + a.rows - hi; r += gridDim.x) {
+    const int64_t row = r < lo ? r : hi + r - lo;
+    for (int n = threadIdx.x; n < width; n += kThreads) put<F16>(a.y, row * a.ldy + n, 0.0f);
+  }
+}
+
+template <bool F16, bool SWIGLU, bool GATHER>
+__global__ void __launch_bounds__(kThreads, 1)
+    int8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int S = a.stages;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  // a stage: [P tile 16 KB][Q tile tmax * 128]
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accfull[2], drained[2], done;
+  __shared__ float row_scale[kEpilogueWarps][kMaxT];  // a copy a warp: no barrier among them
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accfull[b], 1);
+      mbar_init(&drained[b], kEpilogueWarps);
+    }
+    mbar_init(&done, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_slot)), "r"(a.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const Tables tables = tables_at(gbase + a.tables, a.groups);
+  make_tables(a, tables);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+  const Ctl ctl{&abort_flag, a.err};
+  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int tiles = tables.tile_first[a.groups] * a.p_tiles;
+  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
+  const int k0 = static_cast<int>(static_cast<int64_t>(a.ksteps) * rank / a.split);
+  const int k1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.split);
+
+  if (warp == 0) {
+    // One lane loads the weights and counts the bytes, the copies of token rows are spread over the lanes.
+    int g = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true, waited = false;
+    for (int tile = first; ok && tile < tiles; tile += step) {
+      const Tile t = tile_at<16>(a, tables, tile);
+      const int copies = GATHER ? t.width / 4 : (t.width + a.box - 1) / a.box;
+      const uint32_t bytes = kRows * kStepBytes + (GATHER ? t.width : copies * a.box) * kStepBytes;
+      const int p_row = t.group * a.n + t.pt * kRows;
+      auto load_p = [&](int st, int ks) {
+        mbar_arrive_expect_tx(&full[st], bytes);
+        tma_load_2d(base + st * a.stage, &map_p, ks * kStepBytes, p_row, &full[st]);
+      };
+      int from[2][4];  // rows of this lane's gathers
+      if (GATHER) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = 4 * (lane + 32 * h) + i;
+            const int r = c < t.rows ? source_row(a, t.row0 + c) : 0;
+            if (r < 0) record_device_error(a.err, kErrOrder);
+            from[h][i] = max(r, 0);  // what is fetched for a row that does not fit counts as zero (its scale is)
+          }
+      }
+      auto load_q = [&](int st, int ks) {
+        const uint32_t at = base + st * a.stage + kRows * kStepBytes;
+        if (GATHER) {
+          if (lane < copies) tma_gather4(at + lane * 4 * kStepBytes, &map_q, ks * kStepBytes, from[0], &full[st]);
+          if (lane + 32 < copies) tma_gather4(at + (lane + 32) * 4 * kStepBytes, &map_q, ks * kStepBytes, from[1], &full[st]);
+        } else if (lane < copies) {
+          tma_load_2d(at + lane * a.box * kStepBytes, &map_q, ks * kStepBytes, t.row0 + lane * a.box, &full[st]);
+        }
+      };
+      // The weights' first stages do not depend on the kernel before this one; the activations do.
+      int pre = 0;
+      if (!waited) {
+        waited = true;
+        if (a.early) {
+          pre = min(S, k1 - k0);
+          if (lane == 0)
+            for (int i = 0; i < pre; ++i) load_p(i, k0 + i);
+          __syncwarp();
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+      }
+      for (int ks = k0; ks < k1; ++ks, ++g) {
+        if (g >= pre) {
+          if (!warp_spin(&empty[s], ph ^ 1, ctl, kErrWaitProducer)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) load_p(s, ks);
+          __syncwarp();
+        }
+        load_q(s, ks);
+        if (++s == S) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!ok && lane == 0)
+      for (int h = (g > S ? g - S : 0); h < g; ++h) drain_wait(&full[h % S], (h / S) & 1, a.err, kErrDrain);
+  } else if (warp == 1) {
+    // The warp stays converged and elects the issuing lane, so that descriptors stay in uniform registers.
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+    int i = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += step, ++i) {
+      const uint32_t i_desc = instruction_desc(kRows, tile_at<16>(a, tables, tile).width);
+      if (i >= 2 && !warp_spin(&drained[i & 1], ((i - 2) >> 1) & 1, ctl, kErrWaitMma)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
+      for (int ks = k0; ks < k1; ++ks) {
+        if (!warp_spin(&full[s], ph, ctl, kErrWaitMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int subs = a.ksubs - 4 * ks;
+        const uint32_t off = static_cast<uint32_t>(s) * (a.stage >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j > 0 && j >= subs) break;
+            mma_i8(d, p_desc + off + 2 * j, q_desc + off + 2 * j, i_desc, ks > k0 || j > 0);
+          }
+          mma_commit(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == S) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (ok && elect_one()) mma_commit(&accfull[i & 1]);
+      __syncwarp();
+    }
+    if (elect_one()) mma_commit(&done);  // every MMA of this warp has completed once `done` flips
+    __syncwarp();
+    drain_wait(&done, 0, a.err, kErrDrain);
+  } else {
+    const int q = warp & 3, c = (warp - 2) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int i = 0;
+    for (int tile = first; tile < tiles; tile += step, ++i) {
+      const Tile t = tile_at<16>(a, tables, tile);
+      const int b = i & 1, n = t.pt * kRows + 32 * q + lane;
+      float* scale = row_scale[warp - 2];
+#pragma unroll
+      for (int at = lane; at < kMaxT; at += 32) {
+        if (at >= t.width) break;
+        const int r = at < t.rows ? source_row(a, t.row0 + at) : -1;
+        scale[at] = r >= 0 ? a.a_scales[r] : 0.0f;
+      }
+      float sb = 0.0f, bias = 0.0f;
+      if (n < a.n) {
+        const int64_t ch = static_cast<int64_t>(t.group) * a.n + n;
+        sb = a.b_scales[ch];
+        if (a.bias) bias = load_f(a.bias, a.bias_f16, ch);
+      }
+      __syncwarp();
+      if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
+      tc_fence_after();
+      for (int col = 16 * c; col < t.width; col += 32) {
+        uint32_t v[16];
+        tmem_ld16(tmem + lane_addr + (b ? a.acc1 : 0) + col, v);
+        tmem_wait_ld16(v);
+        if (a.split > 1) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) reinterpret_cast<int*>(gbase)[(col + j) * kPitch + 32 * q + lane] = static_cast<int>(v[j]);
+        } else {
+          float f[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f[j] = scaled(static_cast<int>(v[j]), scale[col + j], sb, bias, a.act == XRGPU_ACT_RELU);
+          store_columns<F16, SWIGLU>(a, f, t.row0, col, t.rows, n, lane);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&drained[b]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+  }
+  if (a.split > 1) {
+    // one tile a cluster: every rank sums its share of the columns over the ranks (128 values of a column lie together)
+    cluster_sync();
+    if (first < tiles && !*ctl.abort) {
+      const Tile t = tile_at<16>(a, tables, first);
+      const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, mine = max(0, min(share, t.rows - col0));
+      const bool relu = a.act == XRGPU_ACT_RELU;
+      for (int e = threadIdx.x; e < mine * (kRows / 4); e += kThreads) {
+        const int col = col0 + e / (kRows / 4), row = 4 * (e % (kRows / 4)), n = t.pt * kRows + row;
+        int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < a.split) {
+            const float4 v = ld_cluster_f32x4(map_rank(base + (col * kPitch + row) * 4, k));
+            sum[0] += __float_as_int(v.x);
+            sum[1] += __float_as_int(v.y);
+            sum[2] += __float_as_int(v.z);
+            sum[3] += __float_as_int(v.w);
+          }
+        float f[4];
+        const float sa = row_scale[0][col];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t ch = static_cast<int64_t>(t.group) * a.n + n + i;
+          const bool in = n + i < a.n;
+          f[i] = scaled(sum[i], sa, in ? a.b_scales[ch] : 0.0f, in && a.bias ? load_f(a.bias, a.bias_f16, ch) : 0.0f, relu);
+        }
+        const int64_t at = static_cast<int64_t>(t.row0 + col) * a.ldy;
+        if (SWIGLU) {
+          if (n < a.n) put<F16>(a.y, at + (n >> 1), swiglu(a, f[0], f[1]));
+          if (n + 2 < a.n) put<F16>(a.y, at + (n >> 1) + 1, swiglu(a, f[2], f[3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < a.n) put<F16>(a.y, at + n + i, f[i]);
+        }
+      }
+    }
+    cluster_sync();  // nobody leaves while its partial tile is being read
+  }
+  zero_rest<F16>(a, SWIGLU ? a.n / 2 : a.n);
+}
+
+// ------------------------------------------------------------------ host side
+// Tiles that a call has at the most.
+int64_t most_tiles(const Int8Matmul& p, int64_t tmax, int64_t p_rows) {
+  const int64_t hit = !p.offsets ? 1 : p.groups < p.rows ? p.groups : p.rows;
+  const int64_t along = !p.offsets ? ceil_div(p.rows, tmax) : hit + (p.rows - hit) / tmax;
+  return along * ceil_div(p.N, p_rows);
+}
+
+template <bool F16, bool SWIGLU, bool GATHER>
+cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
+  cudaError_t e = allow_smem<int8_gemm_kernel<F16, SWIGLU, GATHER>>(kSmemBudget);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<F16, SWIGLU, GATHER>, mp, mq, a);
+}
+
+template <bool F16, bool SWIGLU>
+cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
+  return a.order ? launch<F16, SWIGLU, true>(mp, mq, a, grid, smem, early, s) : launch<F16, SWIGLU, false>(mp, mq, a, grid, smem, early, s);
+}
+
+}  // namespace
+
+cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) {
+  const int sms = device_sm_count();
+  Args a{};
+  a.n = static_cast<int>(p.N);
+  a.groups = p.groups;
+  a.rows = static_cast<int>(p.rows);
+  a.a_rows = static_cast<int>(p.a_rows);
+  a.ksubs = static_cast<int>(ceil_div(p.K, 32));
+  a.ksteps = (a.ksubs + 3) / 4;
+  a.early = early;
+  a.top_k = p.top_k;
+  a.act = p.act;
+  a.has_limit = p.has_limit;
+  a.zero_rest = p.zero_rest;
+  a.bias_f16 = p.bias_f16;
+  a.alpha = p.alpha;
+  a.beta = p.beta;
+  a.limit = p.limit;
+  a.offsets = p.offsets;
+  a.order = p.order;
+  a.a_scales = p.a_scales;
+  a.b_scales = p.b_scales;
+  a.bias = p.bias;
+  a.y = p.y;
+  a.ldy = p.ldy;
+  const uintptr_t pair = p.f16 ? 4 : 8;
+  a.vec = reinterpret_cast<uintptr_t>(p.y) % pair == 0 && p.ldy % 2 == 0;
+  a.err = p.err;
+
+  // Columns of a tile: all rows of a dense product with few of them; a group's, when the rows are spread evenly or nearly so.
+  const int64_t mean = ceil_div(p.rows, p.groups), want = p.offsets ? 2 * mean + 8 : mean;
+  a.tmax = static_cast<int>(align_up(want < p.rows ? want : p.rows, 16));
+  if (a.tmax > kMaxT) a.tmax = kMaxT;
+  a.box = p.offsets ? 16 : a.tmax;
+  a.p_tiles = static_cast<int>(ceil_div(p.N, kRows));
+  const int64_t tiles = most_tiles(p, a.tmax, kRows);
+  if (tiles > INT_MAX / 16) return cudaErrorInvalidValue;
+
+  const int64_t most = a.tmax <= 64 ? sms * 8 / 5 : sms;
+  a.split = 1;
+  while (a.split < 8 && tiles * a.split * 2 <= most && a.ksteps >= 4 * a.split) a.split *= 2;
+
+  const uint32_t tables = tables_bytes(p.groups);
+  const int budget = kSmemBudget - 1024 - static_cast<int>(tables);
+  a.stage = static_cast<uint32_t>(kRows + a.tmax) * kStepBytes;
+  const int steps = static_cast<int>(ceil_div(a.ksteps, a.split));
+  const bool one_tile = a.split > 1 || tiles <= sms;
+  int stages = budget / static_cast<int>(a.stage);
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (one_tile && stages > steps) stages = steps;
+  if (a.split > 1) {  // all CTAs at once: those that share an SM share its memory
+    const int together = static_cast<int>(ceil_div(tiles * a.split, sms));
+    const int fit = (budget / together - 11 * 1024) / static_cast<int>(a.stage);
+    if (stages > fit && fit >= 2) stages = fit;
+  }
+  a.stages = stages;
+  size_t smem = static_cast<size_t>(stages) * a.stage;
+  const size_t partial = static_cast<size_t>(a.tmax) * kPitch * 4;
+  if (a.split > 1 && smem < partial) smem = partial;
+  a.tables = static_cast<uint32_t>(smem);
+  smem += tables + 1024;
+  a.acc1 = one_tile ? 0 : a.tmax;
+  a.tmem_cols = 32;
+  while (a.tmem_cols < a.acc1 + a.tmax) a.tmem_cols *= 2;
+  // CTAs that share an SM share its 512 columns: ask for enough shared memory that no more fit than those feed.
+  const size_t least = static_cast<size_t>(227 * 1024) / (512 / a.tmem_cols + 1) + 1024;
+  if (smem < least) smem = least;
+  const int grid = static_cast<int>(a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms));
+
+  CUtensorMap mp, mq;
+  if (!encode_tensor_map_2d(&mp, 0, p.b, p.K, static_cast<uint64_t>(p.groups) * p.N, p.ldb, kStepBytes, kRows, true) ||
+      !encode_tensor_map_2d(&mq, 0, p.a, p.K, p.a_rows, p.lda, kStepBytes, p.order ? 1 : a.box, true))
+    return cudaErrorInvalidValue;
+  if (p.f16) return p.act == XRGPU_ACT_SWIGLU ? launch<true, true>(mp, mq, a, grid, smem, early, s) : launch<true, false>(mp, mq, a, grid, smem, early, s);
+  return p.act == XRGPU_ACT_SWIGLU ? launch<false, true>(mp, mq, a, grid, smem, early, s) : launch<false, false>(mp, mq, a, grid, smem, early, s);
+}
+
+}  // namespace xrgpu

@@ -1,0 +1,274 @@
+// Router of a mixture of experts: each token's top_k experts by score (ties to the lowest index, a NaN counts as -infinity),
+// their weights, and the stable order of all assignments (token * top_k + rank) by expert.
+//
+// Choice: a warp a token; scores are turned into keys that order like the numbers, and top_k times the largest key of
+// the warp (lowest index among equals) is taken out. Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
+// Order: a counting sort. Every warp counts its own tokens' experts, the counts are summed over the warps and CTAs before it, and
+// each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: one CTA does
+// all of it; else a second kernel follows in which every CTA sums the counts of all (G x experts numbers, from L2).
+#include <cuda_fp16.h>
+
+#include "mmnb_common.cuh"
+#include "mmnb_int8.h"
+
+namespace xrgpu {
+namespace {
+
+constexpr int kWarps = 32;
+constexpr int kThreads = kWarps * 32;
+constexpr int64_t kOneCta = 64;  // tokens up to which one CTA does all
+
+struct Args {
+  MoeRoute p;
+  int ctas;
+  int per_warp;   // tokens of a warp, in a row
+  int32_t* counts;  // [ctas, experts]
+};
+
+// A key that orders like the score; 0 is below every score. -0 equals 0, NaN -infinity.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x007fffffu;
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// The choice and weights of the warp's tokens, counted into `mine` [experts]. VPL: scores a lane.
+template <int VPL>
+__device__ __forceinline__ void choose(const Args& a, int64_t t0, int64_t t1, int32_t* mine) {
+  const int lane = threadIdx.x & 31, E = a.p.experts, k = a.p.top_k;
+  for (int64_t t = t0; t < t1; ++t) {
+    uint32_t key[VPL];
+    float x[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) x[i] = lane + 32 * i < E ? load_f(a.p.scores, a.p.f16, t * a.p.lds + lane + 32 * i) : 0.0f;
+    uint32_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      key[i] = lane + 32 * i < E ? key_of(x[i]) : 0u;
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    }
+    const float top = score_of(__reduce_max_sync(~0u, best));
+    float all = 0.0f;
+    if (!a.p.normalize) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) all += key[i] ? expf(score_of(key[i]) - top) : 0.0f;
+      all = warp_sum(all);
+    }
+    int chosen = 0;
+    float score = 0.0f;
+    for (int j = 0; j < k; ++j) {
+      const uint32_t m = __reduce_max_sync(~0u, best);
+      const int e = static_cast<int>(__reduce_min_sync(~0u, best == m ? static_cast<unsigned>(lane + 32 * at) : ~0u));
+      if (lane == j) {
+        chosen = e;
+        score = score_of(m);
+      }
+      if (lane == (e & 31)) {
+        best = 0;
+        at = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          if (i == (e >> 5)) key[i] = 0;
+          if (key[i] > best) {
+            best = key[i];
+            at = i;
+          }
+        }
+      }
+    }
+    // a token whose scores are all -infinity weighs nothing
+    const float w = lane < k && top > -INFINITY ? expf(score - top) : 0.0f;
+    const float sum = a.p.normalize ? warp_sum(w) : all;
+    if (lane < k) {
+      a.p.chosen[t * k + lane] = chosen;
+      a.p.weights[t * k + lane] = top > -INFINITY ? w / sum : 0.0f;
+      mine[chosen] += 1;  // a token's experts differ
+    }
+    __syncwarp();
+  }
+}
+
+// Sum over the threads before, in the order of the threads; *total: of all.
+__device__ __forceinline__ int block_scan(int v, int* part, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(~0u, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) part[warp] = s;
+  __syncthreads();
+  int p = part[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(~0u, p, o);
+    if (lane >= o) p += u;
+  }
+  *total = __shfl_sync(~0u, p, 31);
+  const int before = __shfl_sync(~0u, p, max(warp - 1, 0));
+  return s - v + (warp ? before : 0);
+}
+
+// Places the warp's assignments. hist [kWarps][experts]: the warps' counts; total, before: counts of all CTAs and of those
+// before this one for expert threadIdx.x (experts <= kThreads).
+__device__ __forceinline__ void place(const Args& a, int64_t t0, int64_t t1, int32_t* hist, int total, int before, bool write_offsets) {
+  __shared__ int part[32];
+  const int E = a.p.experts, k = a.p.top_k, e = threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int all;
+  const int first = block_scan(e < E ? total : 0, part, &all);
+  if (e < E) {
+    if (write_offsets) {
+      a.p.offsets[e] = first;
+      if (e == E - 1) a.p.offsets[E] = all;
+    }
+    int at = first + before;
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) {
+      const int c = hist[w * E + e];
+      hist[w * E + e] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  int32_t* mine = hist + warp * E;
+  for (int64_t t = t0; t < t1; ++t) {
+    if (lane < k) {
+      const int c = a.p.chosen[t * k + lane], at = mine[c];
+      mine[c] = at + 1;
+      a.p.slots[t * k + lane] = at;
+      a.p.order[at] = static_cast<int32_t>(t * k + lane);
+    }
+    __syncwarp();
+  }
+}
+
+struct Range {
+  int64_t t0, t1;
+};
+__device__ __forceinline__ Range tokens_of(const Args& a) {
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * a.per_warp;
+  return {min(first, a.p.tokens), min(first + a.per_warp, a.p.tokens)};
+}
+
+template <int VPL, bool ONE>
+__global__ void __launch_bounds__(kThreads, 1) choose_kernel(const Args a) {
+  extern __shared__ int32_t hist[];
+  const int E = a.p.experts;
+  for (int i = threadIdx.x; i < kWarps * E; i += kThreads) hist[i] = 0;
+  __syncthreads();
+  const Range r = tokens_of(a);
+  choose<VPL>(a, r.t0, r.t1, hist + (threadIdx.x >> 5) * E);
+  __syncthreads();
+  int count = 0;
+  if (static_cast<int>(threadIdx.x) < E) {
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) count += hist[w * E + threadIdx.x];
+  }
+  if (ONE) place(a, r.t0, r.t1, hist, count, 0, true);
+  else if (static_cast<int>(threadIdx.x) < E) a.counts[static_cast<int64_t>(blockIdx.x) * E + threadIdx.x] = count;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) place_kernel(const Args a) {
+  extern __shared__ int32_t hist[];
+  __shared__ int sums[2][kThreads];
+  const int E = a.p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < kWarps * E; i += kThreads) hist[i] = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Range r = tokens_of(a);
+  for (int64_t t = r.t0; t < r.t1; ++t) {
+    if (lane < a.p.top_k) hist[warp * E + a.p.chosen[t * a.p.top_k + lane]] += 1;
+    __syncwarp();
+  }
+  // Groups of threads take every groups-th CTA's counts, an expert a thread.
+  const int width = (E + 31) & ~31, groups = kThreads / width, g = threadIdx.x / width, e = threadIdx.x % width;
+  int total = 0, before = 0;
+  if (g < groups && e < E) {
+#pragma unroll 16
+    for (int c = g; c < a.ctas; c += groups) {
+      const int v = a.counts[static_cast<int64_t>(c) * E + e];
+      total += v;
+      before += c < static_cast<int>(blockIdx.x) ? v : 0;
+    }
+  }
+  sums[0][threadIdx.x] = total;
+  sums[1][threadIdx.x] = before;
+  __syncthreads();
+  total = before = 0;
+  if (static_cast<int>(threadIdx.x) < E)
+    for (int i = 0; i < groups; ++i) {
+      total += sums[0][i * width + threadIdx.x];
+      before += sums[1][i * width + threadIdx.x];
+    }
+  place(a, r.t0, r.t1, hist, total, before, blockIdx.x == 0);
+}
+
+int per_warp(const MoeRoute& p) {
+  if (p.tokens <= kOneCta) return static_cast<int>(ceil_div(p.tokens, kWarps));
+  const int64_t ctas = ceil_div(p.tokens, kWarps) < device_sm_count() ? ceil_div(p.tokens, kWarps) : device_sm_count();
+  return static_cast<int>(ceil_div(p.tokens, kWarps * ctas));
+}
+
+template <int VPL>
+cudaError_t launch(const Args& a, cudaStream_t s) {
+  const size_t smem = static_cast<size_t>(kWarps) * a.p.experts * 4;
+  cudaError_t e = allow_smem<choose_kernel<VPL, true>>(kWarps * 32 * VPL * 4);
+  if (e == cudaSuccess) e = allow_smem<choose_kernel<VPL, false>>(kWarps * 32 * VPL * 4);
+  if (e == cudaSuccess) e = allow_smem<place_kernel>(static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  if (a.ctas == 1) {
+    choose_kernel<VPL, true><<<1, kThreads, smem, s>>>(a);
+    return cudaGetLastError();
+  }
+  choose_kernel<VPL, false><<<a.ctas, kThreads, smem, s>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, place_kernel, a);
+}
+
+}  // namespace
+
+uint64_t moe_route_workspace(const MoeRoute& p) {
+  if (p.tokens <= kOneCta) return 0;
+  return static_cast<uint64_t>(ceil_div(p.tokens, static_cast<int64_t>(kWarps) * per_warp(p))) * p.experts * 4;
+}
+
+cudaError_t launch_moe_route(const MoeRoute& p, void* ws, cudaStream_t s) {
+  Args a{};
+  a.p = p;
+  a.per_warp = per_warp(p);
+  a.ctas = static_cast<int>(ceil_div(p.tokens, static_cast<int64_t>(kWarps) * a.per_warp));
+  a.counts = static_cast<int32_t*>(ws);
+  if (p.experts <= 32) return launch<1>(a, s);
+  if (p.experts <= 64) return launch<2>(a, s);
+  if (p.experts <= 128) return launch<4>(a, s);
+  if (p.experts <= 256) return launch<8>(a, s);
+  if (p.experts <= 512) return launch<16>(a, s);
+  return launch<32>(a, s);
+}
+
+}  // namespace xrgpu

@@ -1,4 +1,4 @@
-"""Zero-copy PyTorch entry points over the C ABI (``xrgpu_mmnb_forward``, ``xrgpu_mxfp4_*``, ``xrgpu_kv8_*``, ...).
+"""Zero-copy PyTorch entry points over the C ABI (``xrgpu_mmnb_forward``, ``xrgpu_mxfp4_*``, ``xrgpu_kv8_*``, ``xrgpu_int8_*``, ...).
 
 Tensors stay on the device; the kernels run on the current torch CUDA stream. torch
 supplies device memory and streams only: every numerical step runs in this package's
@@ -7,7 +7,7 @@ CUDA kernels.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -603,3 +603,224 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(index, lib.xrgpu_kv8_attention, ctypes.byref(p), ws.data_ptr() if ws is not None else None, need)
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# 8-bit integer products, dense and grouped by expert, and the router that makes the groups (zero-copy, current CUDA
+# stream of the tensors' device).
+_INT8_ACTIVATIONS = {"none": _native.ACT_NONE, "relu": _native.ACT_RELU, "swiglu": _native.ACT_SWIGLU}
+
+
+def _code_rows(t: torch.Tensor, name: str, index: int) -> int:
+    """Row stride of codes int8 [..., K] on device `index`, whose rows must start on 16 bytes."""
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be a CUDA tensor on cuda:{index}")
+    if t.dtype != torch.int8:
+        raise ValueError(f"{name} must be {torch.int8}")
+    K = t.shape[-1]
+    if t.numel() <= K and (K == 1 or t.stride(-1) == 1):  # one row
+        step = -(-K // 16) * 16
+    else:
+        step = _row_stride(t, name)
+    if step % 16 or t.data_ptr() % 16:
+        raise ValueError(f"{name} must have its rows on 16-byte boundaries (int8_quantize lays them out so)")
+    return step
+
+
+def _small(t: torch.Tensor, name: str, dtype, shape, index: int):
+    _on(t, name, dtype, index)
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}")
+    return t.data_ptr()
+
+
+def int8_quantize(x: torch.Tensor):
+    """x [..., K] (float32 or float16; rows may be strided) as 8-bit codes with one scale a row: (codes, scales).
+
+    codes int8 [..., K] (rows laid out on 16-byte boundaries, as ``matmul_int8`` takes them), scales float32 [...]: scale =
+    max|row| / 127, code = x / scale rounded to nearest, ties to even. A row of zeros has scale 0; the scale of one that holds a NaN
+    or an infinity is NaN, its codes are 0. Weights [N, K] become codes with a scale for each channel by the same call.
+    """
+    dtype = _float_code(x.dtype)
+    index = _device_of(x, "x")
+    K = x.shape[-1] if x.dim() else 0
+    if K < 1:
+        raise ValueError("x must be [..., K] with K >= 1")
+    ld, lead = -(-K // 16) * 16, x.shape[:-1]
+    codes = x.new_empty((*lead, ld), dtype=torch.int8)
+    scales = x.new_empty(lead, dtype=torch.float32)
+    t = _native.Int8Tensor_(dtype, 0, scales.numel(), K, ld, codes.data_ptr(), scales.data_ptr())
+    _launch(index, _native.load().xrgpu_int8_quantize, ctypes.byref(t), x.data_ptr(), _row_stride(x, "x"))
+    return (codes if ld == K else codes[..., :K]), scales
+
+
+def int8_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, dtype=torch.float32) -> torch.Tensor:
+    """The values [..., K] that codes int8 [..., K] and scales float32 [...] hold."""
+    if codes.dim() < 1 or codes.shape[-1] < 1:
+        raise ValueError("codes must be [..., K] with K >= 1")
+    code, index = _float_code(dtype), _device_of(codes, "codes")
+    ld = _code_rows(codes, "codes", index)
+    s = _small(scales, "scales", torch.float32, codes.shape[:-1], index)
+    out = codes.new_empty(codes.shape, dtype=dtype)
+    t = _native.Int8Tensor_(code, 0, scales.numel(), codes.shape[-1], ld, codes.data_ptr(), s)
+    _launch(index, _native.load().xrgpu_int8_dequantize, ctypes.byref(t), out.data_ptr())
+    return out
+
+
+def _int8_problem(a, a_scales, b, b_scales, bias, activation, alpha, beta, limit, dtype):
+    """The operands' part of a call, checked: (problem, device, dtype, columns of y)."""
+    index = _device_of(a, "a")
+    if activation not in _INT8_ACTIVATIONS:
+        raise ValueError("activation must be none, relu or swiglu")
+    if a.dim() < 1 or a.shape[-1] != b.shape[-1] or a.shape[-1] < 1:
+        raise ValueError("a and b differ in K")
+    K, N = a.shape[-1], b.shape[-2]
+    if a_scales is not None:
+        a_code, dtype = _native.INT8, torch.float16 if dtype is None else dtype
+        lda, scales = _code_rows(a, "a", index), _small(a_scales, "a_scales", torch.float32, a.shape[:-1], index)
+    else:
+        if a.dtype == torch.int8:
+            raise ValueError("codes need a_scales")
+        a_code, dtype = _float_code(a.dtype), a.dtype if dtype is None else dtype
+        lda, scales = _row_stride(a, "a"), None
+    code = _float_code(dtype)
+    ldb = _code_rows(b, "b", index)
+    bs = _small(b_scales, "b_scales", torch.float32, b.shape[:-1], index)
+    bias_ptr = None if bias is None else _small(bias, "bias", dtype, b.shape[:-1], index)
+    act = _INT8_ACTIVATIONS[activation]
+    if act == _native.ACT_SWIGLU and N % 2:
+        raise ValueError("swiglu needs pairs of channels")
+    p = _native.Int8Problem_(code, a_code, act, int(limit is not None), float(alpha), float(beta), float(limit or 0.0), 0, a.numel() // K, K, N,
+                             0, 0, 0, 0, a.data_ptr(), scales, lda, b.data_ptr(), bs, ldb, bias_ptr)
+    return p, index, dtype, N // 2 if act == _native.ACT_SWIGLU else N
+
+
+def _int8_forward(p, index: int, out: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
+    lib = _native.load()
+    p.y = out.data_ptr()
+    need = ctypes.c_uint64(0)
+    check(lib.xrgpu_int8_workspace_size(ctypes.byref(p), ctypes.byref(need)))
+    nbytes = need.value
+    ws = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(index, lib.xrgpu_int8_forward, ctypes.byref(p), ws.data_ptr() if nbytes else None, nbytes)
+    return out
+
+
+def _int8_out(p, out, shape, dtype, a, index: int):
+    if out is None:
+        return a.new_empty(shape, dtype=dtype)
+    if out.dtype != dtype or out.get_device() != index or out.shape != shape:
+        raise ValueError(f"out must be {list(shape)} in the output dtype on a's device")
+    p.ldy = _row_stride(out, "out")
+    return out
+
+
+def matmul_int8(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                a_scales: Optional[torch.Tensor] = None, activation: str = "none", alpha: float = 1.0, beta: float = 0.0,
+                limit: Optional[float] = None, dtype=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Y = act(A . B^T (+ bias)) of 8-bit codes with a scale for each row of A (token) and of B (channel).
+
+    b int8 [N, K] with b_scales float32 [N]; a either codes int8 [..., K] with a_scales float32 [...], or float32 /
+    float16 [..., K], which the call quantises first (``int8_quantize``). Rows of codes start on 16-byte boundaries. Y [..., N] in
+    `dtype` (default a's, float16 for codes); bias [N] in it. The sums are exact in 32-bit integers (K <= 131071), the
+    scales and the bias are applied in float32, and Y is rounded once.
+
+    activation "relu", or "swiglu" over channel pairs (2i gate, 2i + 1 linear; Y [..., N / 2]): gate * sigmoid(alpha * gate) *
+    (linear + beta), with `limit` gate clamped to <= limit and linear to [-limit, limit].
+    ``out`` may be a view with unit column stride and rows at one stride.
+    """
+    if b.dim() != 2:
+        raise ValueError("b must be [N, K] codes")
+    p, index, dtype, n = _int8_problem(a, a_scales, b, b_scales, bias, activation, alpha, beta, limit, dtype)
+    out = _int8_out(p, out, (*a.shape[:-1], n), dtype, a, index)
+    return _int8_forward(p, index, out, a)
+
+
+class MoeRoute(NamedTuple):
+    """What ``moe_route`` returns: of T tokens and k experts each, R = T k assignments i = token * k + rank."""
+    experts: torch.Tensor  # int32 [T, k], the best first
+    weights: torch.Tensor  # float32 [T, k]
+    order: torch.Tensor    # int32 [R]: the assignments by expert, those of an expert ascending
+    slots: torch.Tensor    # int32 [T, k]: the place of each assignment in `order`
+    offsets: torch.Tensor  # int32 [experts + 1]: the first place of each expert
+
+
+def moe_route(scores: torch.Tensor, k: int, *, normalize: bool = True) -> MoeRoute:
+    """Chooses each token's k experts by its scores [T, experts] (float32 or float16; rows may be strided) and orders the
+    assignments by expert, for ``matmul_int8_grouped``.
+
+    The highest scores win, ties go to the lowest index (``qmoe`` prefers the highest), a NaN counts as -infinity. Weights:
+    exp(score) over the sum of the chosen experts' (normalize), or of all experts'; a token whose scores are all -infinity
+    weighs nothing. Up to 1024 experts, k up to 32.
+    """
+    code = _float_code(scores.dtype)
+    index = _device_of(scores, "scores")
+    if scores.dim() != 2:
+        raise ValueError("scores must be [tokens, experts]")
+    (T, E), k = scores.shape, int(k)
+    if not 1 <= k <= min(E, 32) or E > 1024:
+        raise ValueError("a router takes up to 1024 experts and a top_k of up to 32 of them")
+    lds = _row_stride(scores, "scores")
+    experts = scores.new_empty((T, k), dtype=torch.int32)
+    weights = scores.new_empty((T, k), dtype=torch.float32)
+    order = scores.new_empty(T * k, dtype=torch.int32)
+    slots = torch.empty_like(experts)
+    offsets = scores.new_empty(E + 1, dtype=torch.int32)
+    p = _native.MoeRouteProblem_(code, int(bool(normalize)), T, E, k, lds, scores.data_ptr(), experts.data_ptr(), weights.data_ptr(),
+                                 order.data_ptr(), slots.data_ptr(), offsets.data_ptr())
+    lib = _native.load()
+    need = _workspace_bytes(index, lib.xrgpu_moe_route_workspace_size, p)
+    ws = scores.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(index, lib.xrgpu_moe_route, ctypes.byref(p), ws.data_ptr() if need else None, need)
+    return MoeRoute(experts, weights, order, slots, offsets)
+
+
+def matmul_int8_grouped(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, offsets: torch.Tensor,
+                        bias: Optional[torch.Tensor] = None, *, a_scales: Optional[torch.Tensor] = None,
+                        order: Optional[torch.Tensor] = None, top_k: int = 1, slots: Optional[torch.Tensor] = None,
+                        weights: Optional[torch.Tensor] = None, activation: str = "none", alpha: float = 1.0, beta: float = 0.0,
+                        limit: Optional[float] = None, dtype=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``matmul_int8`` with a weight matrix for each group of rows: the experts' products of ``moe_route``.
+
+    b int8 [E, N, K], b_scales float32 [E, N], bias [E, N], offsets int32 [E + 1]: rows offsets[e] .. offsets[e + 1] - 1 of the
+    product take b[e] (E up to 1024, groups of any length). a holds the product's rows, or, with order int32 [R], the tokens:
+    row r then reads row order[r] // top_k of it. Returns the R rows in the groups' order, [R, N] (swiglu: [R, N / 2]).
+
+    With slots int32 and weights float32 [T, k] it returns sums instead, [T, N]: y[t] = sum_j weights[t, j] * row slots[t, j], in
+    float32 and in the order of j; a slot outside [0, R) is left out. A mixture of experts over x [T, K] is::
+
+        r = moe_route(scores, k)
+        h = matmul_int8_grouped(x, up, up_scales, r.offsets, order=r.order, top_k=k, activation="swiglu")
+        y = matmul_int8_grouped(h, down, down_scales, r.offsets, slots=r.slots, weights=r.weights)
+
+    With ``out``, rows of no group are left as they were (without it they are zero). Offsets that decrease or leave [0, R] drop
+    their group (``device_error`` 0x701); an order entry that fits no row of a counts as zeros (0x702).
+    """
+    if b.dim() != 3:
+        raise ValueError("b must be [experts, N, K] codes")
+    if a.dim() != 2:
+        raise ValueError("a must be [rows, K]")
+    E = b.shape[0]
+    if not 1 <= E <= 1024:
+        raise ValueError("a product takes 1 to 1024 groups")
+    p, index, dtype, n = _int8_problem(a, a_scales, b, b_scales, bias, activation, alpha, beta, limit, dtype)
+    p.groups, p.offsets, p.rows, p.top_k = E, _small(offsets, "offsets", torch.int32, (E + 1,), index), a.shape[0], int(top_k)
+    if order is not None:
+        if order.dim() != 1:
+            raise ValueError("order must be [rows]")
+        p.order, p.rows = _small(order, "order", torch.int32, order.shape, index), order.shape[0]
+    rows = p.rows
+    if (slots is None) != (weights is None):
+        raise ValueError("slots and weights belong together")
+    if slots is not None:
+        if slots.dim() != 2:
+            raise ValueError("slots must be [tokens, k]")
+        if order is not None and slots.shape[1] != top_k:
+            raise ValueError("slots must have top_k columns")
+        p.slots = _small(slots, "slots", torch.int32, slots.shape, index)
+        p.weights = _small(weights, "weights", torch.float32, slots.shape, index)
+        p.tokens, p.top_k = slots.shape
+        rows = p.tokens
+    p.zero_rest = int(out is None)
+    out = _int8_out(p, out, (rows, n), dtype, a, index)
+    return _int8_forward(p, index, out, a)
