@@ -231,7 +231,7 @@ def _codes(g, rows, K):
 
 
 SIZES = [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (2, 7, 15), (16, 129, 33), (17, 1003, 4100), (33, 2, 127), (64, 640, 2048), (128, 256, 129),
-         (129, 300, 31), (200, 128, 16), (255, 513, 256), (257, 1000, 300), (300, 2049, 128), (1000, 384, 100), (700, 5000, 64), (2049, 700, 257)]
+         (129, 300, 31), (200, 128, 16), (255, 513, 256), (257, 1000, 300), (300, 2049, 128), (1000, 384, 100), (700, 5000, 64), (2049, 700, 257), (2300, 3000, 200), (1030, 9002, 128), (5000, 1500, 96)]
 
 
 @gpu
@@ -395,7 +395,8 @@ def _grouped(F, E, R_, N, K, dtype, bias, act, kind, order=None, top_k=1, M=None
 
 GROUPS = [(1, 40, 130, 70, "even"), (3, 0, 16, 32, "even"), (8, 8, 256, 300, "even"), (5, 33, 7, 100, "ragged"), (33, 64, 128, 2048, "ragged"),
           (64, 500, 384, 96, "ragged"), (12, 2000, 200, 1000, "ragged"), (7, 700, 1030, 64, "one"), (300, 900, 20, 33, "ragged"),
-          (1024, 1500, 4, 16, "ragged"), (4, 1100, 2500, 256, "even"), (2, 1, 4096, 1024, "one")]
+          (1024, 1500, 4, 16, "ragged"), (4, 1100, 2500, 256, "even"), (2, 1, 4096, 1024, "one"),
+          (20, 6000, 1000, 700, "ragged"), (3, 2000, 3000, 130, "one")]
 
 
 @gpu
@@ -408,7 +409,7 @@ def test_grouped_product(F, E, rows, N, K, kind, dtype, bias, act):
 
 
 @gpu
-@pytest.mark.parametrize("T,E,k,N,K", [(1, 64, 8, 256, 512), (3, 8, 8, 130, 33), (70, 16, 2, 200, 100), (333, 12, 3, 100, 250), (700, 6, 4, 2500, 64), (40, 5, 1, 64, 16)])
+@pytest.mark.parametrize("T,E,k,N,K", [(1, 64, 8, 256, 512), (3, 8, 8, 130, 33), (70, 16, 2, 200, 100), (333, 12, 3, 100, 250), (700, 6, 4, 2500, 64), (40, 5, 1, 64, 16), (2000, 10, 3, 700, 1000)])
 @pytest.mark.parametrize("dtype,act", [(HALF, "swiglu"), (FULL, "none")])
 def test_grouped_product_of_gathered_tokens(F, T, E, k, N, K, dtype, act):
     order = np.random.default_rng(T).permutation(T * k)

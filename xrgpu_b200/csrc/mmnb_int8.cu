@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kUnit = 16;                    // values of a thread at a time: 16 bytes of codes
 constexpr int kRowThreads = 512;             // of a row at the most
+constexpr unsigned kErrOrder = 0x702;
 constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: t + kMagic rounds t to a whole number
 constexpr float kNearBorder = 0.49996f;
 constexpr float kSmallScale = 7.9e-31f;      // about 2^-100: below, 1 / s is not used
@@ -112,6 +113,15 @@ struct Unit {
   }
 };
 
+// The row that row r stands for, -1 where it fits none (recorded).
+__device__ __forceinline__ int64_t source_row(const RowOrder& f, int64_t r) {
+  if (!f.order) return r;
+  const int o = f.order[r], t = o / f.top_k;
+  if (o >= 0 && t < f.rows) return t;
+  record_device_error(f.err, kErrOrder);
+  return -1;
+}
+
 // blockDim.x threads (whole warps) a row, blockDim.y rows a CTA. HELD: a row is at most UNITS units a thread, kept in
 // registers between the two passes; else it is read twice.
 template <bool F16, bool VEC, int UNITS, bool HELD>
@@ -120,17 +130,18 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's weights may start to load
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const bool real = row < p.rows;
-  const int64_t row_at = row * p.ldx, units = real ? (p.K + kUnit - 1) / kUnit : 0;
+  const int64_t from = real ? source_row(p.from, row) : 0, row_at = max(from, static_cast<int64_t>(0)) * p.ldx, units = real ? (p.K + kUnit - 1) / kUnit : 0;
+  const int64_t read = real && from >= 0 ? p.K : 0;  // values of x that count
   Unit<F16, VEC> u[UNITS];
   uint32_t amax = 0;
   if (HELD) {
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) u[i].load(p.x, row_at, (threadIdx.x + static_cast<int64_t>(i) * blockDim.x) * kUnit, real ? p.K : 0);
+    for (int i = 0; i < UNITS; ++i) u[i].load(p.x, row_at, (threadIdx.x + static_cast<int64_t>(i) * blockDim.x) * kUnit, read);
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) amax = max(amax, u[i].amax());
   } else {
     for (int64_t at = threadIdx.x; at < units; at += blockDim.x) {
-      u[0].load(p.x, row_at, at * kUnit, p.K);
+      u[0].load(p.x, row_at, at * kUnit, read);
       amax = max(amax, u[0].amax());
     }
   }
@@ -171,10 +182,24 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
       if (threadIdx.x + static_cast<int64_t>(i) * blockDim.x < units) store(u[i], threadIdx.x + static_cast<int64_t>(i) * blockDim.x);
   } else {
     for (int64_t at = threadIdx.x; at < units; at += blockDim.x) {
-      u[0].load(p.x, row_at, at * kUnit, p.K);
+      u[0].load(p.x, row_at, at * kUnit, read);
       store(u[0], at);
     }
   }
+}
+
+__global__ void __launch_bounds__(256) gather_kernel(const Int8Gather p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (row >= p.rows) return;
+  const int64_t from = source_row(p.from, row);
+  if (threadIdx.x == 0) p.scales[row] = from >= 0 ? p.a_scales[from] : 0.0f;
+  const uint4* src = reinterpret_cast<const uint4*>(p.a + max(from, static_cast<int64_t>(0)) * p.lds);
+  uint4* dst = reinterpret_cast<uint4*>(p.codes + row * p.ldc);
+  const int64_t whole = p.K / kUnit;
+#pragma unroll 4
+  for (int64_t at = threadIdx.x; at < whole; at += blockDim.x) dst[at] = src[at];
+  for (int64_t k = whole * kUnit + threadIdx.x; k < p.K; k += blockDim.x) p.codes[row * p.ldc + k] = reinterpret_cast<const int8_t*>(src)[k];
 }
 
 template <bool F16, bool VEC>
@@ -280,6 +305,15 @@ cudaError_t launch_int8_dequantize(const Int8Rows& p, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks)), block(tx, ty);
   if (p.f16) vec ? dequantize_kernel<true, true><<<grid, block, 0, s>>>(p) : dequantize_kernel<true, false><<<grid, block, 0, s>>>(p);
   else vec ? dequantize_kernel<false, true><<<grid, block, 0, s>>>(p) : dequantize_kernel<false, false><<<grid, block, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_int8_gather(const Int8Gather& p, cudaStream_t s) {
+  const int64_t units = ceil_div(p.K, kUnit);
+  const unsigned tx = units >= 256 ? 256 : static_cast<unsigned>(align_up(units, 32)), ty = 256 / tx;
+  const int64_t blocks = ceil_div(p.rows, ty);
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  gather_kernel<<<static_cast<unsigned>(blocks), dim3(tx, ty), 0, s>>>(p);
   return cudaGetLastError();
 }
 

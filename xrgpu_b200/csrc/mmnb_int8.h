@@ -11,6 +11,15 @@
 
 namespace xrgpu {
 
+// Row r stands for row order[r] / top_k of `rows` ones (order nullptr: for row r). An entry that fits none counts as a row of
+// zeros and is recorded.
+struct RowOrder {
+  const int32_t* order;
+  int top_k;
+  int64_t rows;
+  unsigned* err;
+};
+
 struct Int8Rows {
   int f16;          // of the values: 1 float16, 0 float32
   int64_t rows, K;
@@ -19,12 +28,24 @@ struct Int8Rows {
   int8_t* codes;
   float* scales;
   void* out;        // dequantisation: values [rows, K]
+  RowOrder from;    // quantisation: which rows of x
 };
 cudaError_t launch_int8_quantize(const Int8Rows& p, cudaStream_t s);
 cudaError_t launch_int8_dequantize(const Int8Rows& p, cudaStream_t s);
 
-// y[r, :] = act(a[r'] . b[g]^T * a_scale[r'] * b_scale[g, :] + bias[g, :]) for the rows r of group g, offsets[g] <= r <
-// offsets[g + 1] (offsets nullptr: one group of all rows); r' = order[r] / top_k, or r without order.
+// Codes and scales of `rows` rows taken in an order.
+struct Int8Gather {
+  int64_t rows, K, lds, ldc;  // strides of a and codes
+  RowOrder from;
+  const int8_t* a;
+  const float* a_scales;
+  int8_t* codes;
+  float* scales;
+};
+cudaError_t launch_int8_gather(const Int8Gather& p, cudaStream_t s);
+
+// y[r, :] = act(a[r] . b[g]^T * a_scale[r] * b_scale[g, :] + bias[g, :]) for the rows r of group g, offsets[g] <= r <
+// offsets[g + 1] (offsets nullptr: one group of all rows).
 struct Int8Matmul {
   int f16;       // y: 1 float16, 0 float32
   int bias_f16;
@@ -32,15 +53,13 @@ struct Int8Matmul {
   int has_limit, zero_rest;
   float alpha, beta, limit;
   int groups;
-  int64_t rows, a_rows, N, K, lda, ldb, ldy;
-  int top_k;
+  int64_t rows, N, K, lda, ldb, ldy;
   const int8_t* a;
   const float* a_scales;
   const int8_t* b;       // [groups * N, ldb]
   const float* b_scales; // [groups, N]
   const void* bias;      // [groups, N] or nullptr
   const int32_t* offsets;
-  const int32_t* order;
   void* y;
   unsigned* err;
 };

@@ -53,16 +53,17 @@ int rows_of(const xrgpu_int8_tensor* t, Int8Rows* p) {
   return XRGPU_OK;
 }
 
-// Workspace of a product: [codes of a][scales of a][product's rows], the parts it needs.
+// Workspace of a product: [codes of its rows][their scales][its results as float32], the parts it needs.
 struct Layout {
   uint64_t scales, rows, bytes;
-  int64_t ldr;  // row stride of the product's rows
+  int64_t ldr;  // row stride of the results
 };
 Layout layout(const xrgpu_int8_problem& c, int64_t out_n) {
   Layout l{};
-  if (c.a_dtype != XRGPU_INT8) {
-    l.scales = align_up(static_cast<uint64_t>(c.M) * align_up(c.K, 16), 256);
-    l.rows = l.scales + align_up(static_cast<uint64_t>(c.M) * 4, 256);
+  const uint64_t rows = static_cast<uint64_t>(c.groups ? c.rows : c.M);
+  if (c.a_dtype != XRGPU_INT8 || c.order) {
+    l.scales = align_up(rows * align_up(c.K, 16), 256);
+    l.rows = l.scales + align_up(rows * 4, 256);
   }
   l.ldr = static_cast<int64_t>(align_up(out_n, 4));
   l.bytes = l.rows + (c.slots ? static_cast<uint64_t>(c.rows) * l.ldr * 4 : 0);
@@ -100,7 +101,6 @@ int check(const xrgpu_int8_problem* c, Int8Matmul* p, Layout* l) {
     if ((st = code_stride(c->lda, c->K, &p->lda))) return st;
   } else {
     if (c->lda != 0 && c->lda < c->K) return fail("lda must be at least K");
-    p->lda = static_cast<int64_t>(align_up(c->K, 16));
   }
   if ((st = code_stride(c->ldb, c->K, &p->ldb))) return st;
   if (c->ldy != 0 && c->ldy < out_n) return fail("ldy must cover a row of y");
@@ -113,10 +113,8 @@ int check(const xrgpu_int8_problem* c, Int8Matmul* p, Layout* l) {
   p->bias_f16 = p->f16;
   p->groups = c->groups ? static_cast<int>(c->groups) : 1;
   p->rows = c->groups ? c->rows : c->M;
-  p->a_rows = c->M;
   p->N = c->N;
   p->K = c->K;
-  p->top_k = c->order ? static_cast<int>(c->top_k) : 1;
   p->ldy = c->ldy ? c->ldy : out_n;
   p->zero_rest = c->zero_rest != 0;
   return XRGPU_OK;
@@ -148,16 +146,25 @@ int forward(const xrgpu_int8_problem* c, void* ws, uint64_t ws_bytes, cudaStream
   p.b_scales = c->b_scales;
   p.bias = c->bias;
   p.offsets = c->offsets;
-  p.order = c->order;
   p.y = c->y;
   p.err = device_error_word();
   if (p.rows) {
-    if (c->a_dtype != XRGPU_INT8) {
-      Int8Rows q{c->a_dtype == XRGPU_FLOAT16, c->M, c->K, c->lda ? c->lda : c->K, p.lda, c->a, reinterpret_cast<int8_t*>(w),
-                 reinterpret_cast<float*>(w + l.scales), nullptr};
-      if ((st = launched(launch_int8_quantize(q, s)))) return st;
-      p.a = q.codes;
-      p.a_scales = q.scales;
+    const RowOrder from{c->order, c->order ? static_cast<int>(c->top_k) : 1, c->M, p.err};
+    const bool made = c->a_dtype != XRGPU_INT8 || c->order;  // the operand, by a kernel before the product's
+    if (made) {
+      int8_t* codes = reinterpret_cast<int8_t*>(w);
+      float* scales = reinterpret_cast<float*>(w + l.scales);
+      const int64_t ld = static_cast<int64_t>(align_up(c->K, 16));
+      if (c->a_dtype != XRGPU_INT8) {
+        const Int8Rows q{c->a_dtype == XRGPU_FLOAT16, p.rows, c->K, c->lda ? c->lda : c->K, ld, c->a, codes, scales, nullptr, from};
+        st = launched(launch_int8_quantize(q, s));
+      } else {
+        st = launched(launch_int8_gather({p.rows, c->K, p.lda, ld, from, p.a, p.a_scales, codes, scales}, s));
+      }
+      if (st) return st;
+      p.a = codes;
+      p.a_scales = scales;
+      p.lda = ld;
     }
     if (sums) {
       p.f16 = 0;
@@ -165,7 +172,7 @@ int forward(const xrgpu_int8_problem* c, void* ws, uint64_t ws_bytes, cudaStream
       p.ldy = l.ldr;
       p.zero_rest = 1;
     }
-    if ((st = launched(launch_int8_matmul(p, c->a_dtype != XRGPU_INT8, s)))) return st;
+    if ((st = launched(launch_int8_matmul(p, made, s)))) return st;
   }
   if (!sums) return XRGPU_OK;
   const int64_t out_n = c->activation == XRGPU_ACT_SWIGLU ? c->N / 2 : c->N;

@@ -8,7 +8,9 @@
 //
 // Groups. Offsets are on the device: every CTA counts the groups' tiles itself (a scan in shared memory) and takes tiles
 // of one line, group by group, the tiles of the same channels next to each other. Offsets that do not fit leave out their group
-// and record an error. With `order` the token rows are fetched where they lie (four-row gather copies).
+// and record an error. Rows come in the groups' order: fetching them where the tokens lie was slower by far (16384 x 4096 x
+// 4096, 216 us: 483 with 16-byte copies, whose writes need a fence of 2000 cycles a stage before the tensor cores may read
+// them; four-row tensor gathers take 60 cycles each, 3800 a stage of 256 rows).
 //
 // Roles (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 drain (lane quadrant warp % 4, alternate 16-column chunks).
 // Few tiles: K is split over a cluster of up to 8 CTAs whose int32 partial tiles meet in shared memory.
@@ -35,14 +37,13 @@ constexpr int kMaxT = 256;
 constexpr int kPitch = kRows;    // int32 values a column of a partial tile in shared memory
 
 constexpr unsigned kErrOffsets = 0x701;
-constexpr unsigned kErrOrder = 0x702;
 constexpr unsigned kErrWaitProducer = 0x711;
 constexpr unsigned kErrWaitMma = 0x712;
 constexpr unsigned kErrWaitEpilogue = 0x713;
 constexpr unsigned kErrDrain = 0x714;
 
 struct Args {
-  int n, p_tiles, groups, rows, a_rows;
+  int n, p_tiles, groups, rows;
   int tmax, box;               // most rows of Q a tile (a multiple of 16); rows of one copy
   int ksteps, ksubs;           // stages along K, 32-value MMA steps along K
   int stages, split;
@@ -50,10 +51,9 @@ struct Args {
   int early;                   // the weights may be loaded before the previous kernel has finished
   uint32_t stage;              // bytes
   uint32_t tables;             // bytes from the stages' start to the group tables
-  int top_k, act, has_limit, zero_rest, bias_f16;
+  int act, has_limit, zero_rest, bias_f16;
   float alpha, beta, limit;
   const int32_t* offsets;
-  const int32_t* order;
   const float* a_scales;
   const float* b_scales;
   const void* bias;
@@ -76,14 +76,6 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a_desc, uint64_t b_d
 // Instruction descriptor: int32 sums of signed 8-bit operands, both K-major, M rows, T columns.
 __device__ __forceinline__ uint32_t instruction_desc(int M, int T) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(T >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
-}
-
-// Four rows of 128 bytes, at `x` bytes into rows r.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&r)[4], uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
-      : "memory");
 }
 
 // ------------------------------------------------------------------ tiles
@@ -161,13 +153,6 @@ __device__ __forceinline__ Tile tile_at(const Args& a, const Tables& t, int tile
   return {lo, pt, t.row_first[lo] + qt * width, min(width, count - qt * width), width};
 }
 
-// The row of a that a row of the product reads; -1 where order does not fit.
-__device__ __forceinline__ int source_row(const Args& a, int r) {
-  if (!a.order) return r;
-  const int o = a.order[r], t = o / a.top_k;
-  return o < 0 || t >= a.a_rows ? -1 : t;
-}
-
 // ------------------------------------------------------------------ results
 template <bool F16>
 __device__ __forceinline__ void put(void* y, int64_t at, float v) {
@@ -181,7 +166,10 @@ __device__ __forceinline__ float swiglu(const Args& a, float g, float l) {
     g = g > a.limit ? a.limit : g;
     l = l > a.limit ? a.limit : l < -a.limit ? -a.limit : l;
   }
-  return g / (1.0f + expf(-a.alpha * g)) * (l + a.beta);
+  // the reciprocal within one step; of infinity zero
+  float s;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(1.0f + expf(-a.alpha * g)));
+  return g * s * (l + a.beta);
 }
 
 // 16 columns (rows row0 + col0 + j of y) of the lane's channel n, scaled already. All lanes of the warp take part.
@@ -193,7 +181,7 @@ __device__ __forceinline__ void store_columns(const Args& a, const float (&f)[16
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
       const float other = __shfl_xor_sync(~0u, odd ? f[j] : f[j + 1], 1);
-      const float r = odd ? swiglu(a, other, f[j + 1]) : swiglu(a, f[j], other);
+      const float r = swiglu(a, odd ? other : f[j], odd ? f[j + 1] : other);
       const int c = col0 + j + (odd ? 1 : 0);
       if (c < rows && n < a.n) put<F16>(a.y, static_cast<int64_t>(row0 + c) * a.ldy + (n >> 1), r);
     }
@@ -238,7 +226,42 @@ __device__ __forceinline__ void zero_rest(const Args& a, int width) {
   }
 }
 
-template <bool F16, bool SWIGLU, bool GATHER>
+struct ChannelScale {
+  float scale, bias;
+};
+// The scales of a tile's rows into the warp's `row_scale`, and the lane's channel's.
+__device__ __forceinline__ ChannelScale prepare_scales(const Args& a, const Tile& t, int n, float* row_scale, int lane) {
+  ChannelScale ch{0.0f, 0.0f};
+  if (n < a.n) {
+    const int64_t at = static_cast<int64_t>(t.group) * a.n + n;
+    ch.scale = a.b_scales[at];
+    if (a.bias) ch.bias = load_f(a.bias, a.bias_f16, at);
+  }
+  float scale[kMaxT / 32];  // all loads before the first use: one after the other they take 800 cycles each
+#pragma unroll
+  for (int i = 0; i < kMaxT / 32; ++i) scale[i] = 32 * i + lane < t.rows ? a.a_scales[t.row0 + 32 * i + lane] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxT / 32; ++i)
+    if (32 * i < t.width) row_scale[32 * i + lane] = scale[i];
+  __syncwarp();
+  return ch;
+}
+
+// The warp's chunks of a tile's sums, from tensor memory to y.
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_t tmem, int c, int n, const ChannelScale& ch, const float* row_scale, int lane) {
+  for (int col = 16 * c; col < t.width; col += 32) {
+    uint32_t v[16];
+    tmem_ld16(tmem + col, v);
+    tmem_wait_ld16(v);
+    float f[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = scaled(static_cast<int>(v[j]), row_scale[col + j], ch.scale, ch.bias, a.act == XRGPU_ACT_RELU);
+    store_columns<F16, SWIGLU>(a, f, t.row0, col, t.rows, n, lane);
+  }
+}
+
+template <bool F16, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
   extern __shared__ uint8_t smem_raw[];
@@ -284,39 +307,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.split);
 
   if (warp == 0) {
-    // One lane loads the weights and counts the bytes, the copies of token rows are spread over the lanes.
+    // One lane loads the weights and counts the bytes, copies of token rows are spread over the lanes.
     int g = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true, waited = false;
     for (int tile = first; ok && tile < tiles; tile += step) {
       const Tile t = tile_at<16>(a, tables, tile);
-      const int copies = GATHER ? t.width / 4 : (t.width + a.box - 1) / a.box;
-      const uint32_t bytes = kRows * kStepBytes + (GATHER ? t.width : copies * a.box) * kStepBytes;
+      const int copies = (t.width + a.box - 1) / a.box;
+      const uint32_t bytes = (kRows + copies * a.box) * kStepBytes;
       const int p_row = t.group * a.n + t.pt * kRows;
       auto load_p = [&](int st, int ks) {
         mbar_arrive_expect_tx(&full[st], bytes);
         tma_load_2d(base + st * a.stage, &map_p, ks * kStepBytes, p_row, &full[st]);
       };
-      int from[2][4];  // rows of this lane's gathers
-      if (GATHER) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = 4 * (lane + 32 * h) + i;
-            const int r = c < t.rows ? source_row(a, t.row0 + c) : 0;
-            if (r < 0) record_device_error(a.err, kErrOrder);
-            from[h][i] = max(r, 0);  // what is fetched for a row that does not fit counts as zero (its scale is)
-          }
-      }
       auto load_q = [&](int st, int ks) {
         const uint32_t at = base + st * a.stage + kRows * kStepBytes;
-        if (GATHER) {
-          if (lane < copies) tma_gather4(at + lane * 4 * kStepBytes, &map_q, ks * kStepBytes, from[0], &full[st]);
-          if (lane + 32 < copies) tma_gather4(at + (lane + 32) * 4 * kStepBytes, &map_q, ks * kStepBytes, from[1], &full[st]);
-        } else if (lane < copies) {
-          tma_load_2d(at + lane * a.box * kStepBytes, &map_q, ks * kStepBytes, t.row0 + lane * a.box, &full[st]);
-        }
+        if (lane < copies) tma_load_2d(at + lane * a.box * kStepBytes, &map_q, ks * kStepBytes, t.row0 + lane * a.box, &full[st]);
       };
       // The weights' first stages do not depend on the kernel before this one; the activations do.
       int pre = 0;
@@ -396,35 +402,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = first; tile < tiles; tile += step, ++i) {
       const Tile t = tile_at<16>(a, tables, tile);
       const int b = i & 1, n = t.pt * kRows + 32 * q + lane;
-      float* scale = row_scale[warp - 2];
-#pragma unroll
-      for (int at = lane; at < kMaxT; at += 32) {
-        if (at >= t.width) break;
-        const int r = at < t.rows ? source_row(a, t.row0 + at) : -1;
-        scale[at] = r >= 0 ? a.a_scales[r] : 0.0f;
-      }
-      float sb = 0.0f, bias = 0.0f;
-      if (n < a.n) {
-        const int64_t ch = static_cast<int64_t>(t.group) * a.n + n;
-        sb = a.b_scales[ch];
-        if (a.bias) bias = load_f(a.bias, a.bias_f16, ch);
-      }
-      __syncwarp();
+      const ChannelScale ch = prepare_scales(a, t, n, row_scale[warp - 2], lane);
       if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
       tc_fence_after();
-      for (int col = 16 * c; col < t.width; col += 32) {
-        uint32_t v[16];
-        tmem_ld16(tmem + lane_addr + (b ? a.acc1 : 0) + col, v);
-        tmem_wait_ld16(v);
-        if (a.split > 1) {
+      const uint32_t acc = tmem + lane_addr + (b ? a.acc1 : 0);
+      if (a.split > 1) {
+        for (int col = 16 * c; col < t.width; col += 32) {
+          uint32_t v[16];
+          tmem_ld16(acc + col, v);
+          tmem_wait_ld16(v);
 #pragma unroll
           for (int j = 0; j < 16; ++j) reinterpret_cast<int*>(gbase)[(col + j) * kPitch + 32 * q + lane] = static_cast<int>(v[j]);
-        } else {
-          float f[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) f[j] = scaled(static_cast<int>(v[j]), scale[col + j], sb, bias, a.act == XRGPU_ACT_RELU);
-          store_columns<F16, SWIGLU>(a, f, t.row0, col, t.rows, n, lane);
         }
+      } else {
+        drain_tile<F16, SWIGLU>(a, t, acc, c, n, ch, row_scale[warp - 2], lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -481,6 +472,199 @@ __global__ void __launch_bounds__(kThreads, 1)
   zero_rest<F16>(a, SWIGLU ? a.n / 2 : a.n);
 }
 
+// ------------------------------------------------------------------ pairs of CTAs
+// For many rows: a cluster of two CTAs on 256 channels by up to 256 rows. Each holds 128 of the channels and half of the rows; the
+// first one's MMAs (cta_group::2) read both halves from both shared memories, so that a CTA loads 256 rows a step instead of
+// 384 for the same product. Each CTA keeps the sums of its own channels, two accumulators of 256 columns, and drains them as
+// the kernel above does.
+// Signals between the two. Both CTAs' loads complete on the first one's `full`, which expects the bytes of both; the MMAs' completion goes to both. The second CTA's epilogue warps meet at its own `drained`,
+// and its warp 1 passes that on with a release at cluster scope. What the first CTA waits for it acquires at cluster scope.
+constexpr int kStages2 = 6;
+constexpr uint32_t kStage2 = 2 * kRows * kStepBytes;  // a CTA's bytes: channels, half of the rows
+
+__device__ __forceinline__ void mma2_i8(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <bool F16, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    int8_gemm2_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kStages2], empty[kStages2], accfull[2], drained[2], done;
+  __shared__ float row_scale[kEpilogueWarps][kMaxT];
+  __shared__ uint32_t tmem_slot, fills[2];  // stages that each CTA's loads were issued for (in the first CTA)
+  __shared__ int abort_flag;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  const int rank = static_cast<int>(cluster_rank());
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages2; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accfull[b], 1);
+      mbar_init(&drained[b], kEpilogueWarps + (rank == 0));  // the first CTA's: and the second CTA
+    }
+    mbar_init(&done, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  const Tables tables = tables_at(smem_raw + (base - raw) + a.tables, a.groups);
+  make_tables(a, tables);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are there
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+  const Ctl ctl{&abort_flag, a.err};
+  const int tiles = tables.tile_first[a.groups] * a.p_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    int g = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true, waited = false;
+    for (int tile = first; ok && tile < tiles; tile += step) {
+      const Tile t = tile_at<32>(a, tables, tile);
+      const int copies = (t.width / 2 + a.box - 1) / a.box, q_row = t.row0 + rank * (t.width / 2);
+      const uint32_t bytes = 2 * (kRows + copies * a.box) * kStepBytes;
+      const int p_row = t.group * a.n + (2 * t.pt + rank) * kRows;
+      auto load_p = [&](int st, int ks) {
+        if (rank == 0) mbar_arrive_expect_tx(&full[st], bytes);
+        tma2_load_2d(base + st * kStage2, &map_p, ks * kStepBytes, p_row, map_rank(smem_u32(&full[st]), 0));
+      };
+      // The weights' first stages do not depend on the kernel before this one; the activations do.
+      int pre = 0;
+      if (!waited) {
+        waited = true;
+        if (a.early) {
+          pre = min(kStages2, a.ksteps);
+          if (lane == 0)
+            for (int i = 0; i < pre; ++i) load_p(i, i);
+          __syncwarp();
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+      }
+      for (int ks = 0; ks < a.ksteps; ++ks, ++g) {
+        if (g >= pre) {
+          if (!warp_spin(&empty[s], ph ^ 1, ctl, kErrWaitProducer)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) load_p(s, ks);
+          __syncwarp();
+        }
+        if (lane < copies)
+          tma2_load_2d(base + s * kStage2 + (kRows + lane * a.box) * kStepBytes, &map_q, ks * kStepBytes, q_row + lane * a.box,
+                       map_rank(smem_u32(&full[s]), 0));
+        if (++s == kStages2) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (lane == 0) st_cluster_u32(map_rank(smem_u32(&fills[rank]), 0), g);
+  } else if (warp == 1 && rank == 1) {
+    // passes on that this CTA's accumulators have been read
+    int i = 0;
+    for (int tile = first; tile < tiles; tile += step, ++i) {
+      if (!warp_spin(&drained[i & 1], (i >> 1) & 1, ctl, kErrWaitMma)) break;
+      if (lane == 0) arrive_at(&drained[i & 1], 0);
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+    int i = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    // both CTAs' loads, or both CTAs' drains
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return warp_spin(bar, parity, ctl, kErrWaitMma) && __all_sync(~0u, acquire_cluster(bar, parity));
+    };
+    for (int tile = first; ok && tile < tiles; tile += step, ++i) {
+      const uint32_t i_desc = instruction_desc(2 * kRows, tile_at<32>(a, tables, tile).width);
+      if (i >= 2 && !wait(&drained[i & 1], ((i - 2) >> 1) & 1)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + ((i & 1) ? kMaxT : 0);
+      for (int ks = 0; ks < a.ksteps; ++ks) {
+        if (!wait(&full[s], ph)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int subs = a.ksubs - 4 * ks;
+        const uint32_t off = static_cast<uint32_t>(s) * (kStage2 >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j > 0 && j >= subs) break;
+            mma2_i8(d, p_desc + off + 2 * j, q_desc + off + 2 * j, i_desc, ks > 0 || j > 0);
+          }
+          mma2_commit(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == kStages2) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (ok && elect_one()) mma2_commit(&accfull[i & 1]);
+      __syncwarp();
+    }
+    if (elect_one()) mma2_commit(&done);
+    __syncwarp();
+    drain_wait(&done, 0, a.err, kErrDrain);
+  } else {
+    const int q = warp & 3, c = (warp - 2) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int i = 0;
+    for (int tile = first; tile < tiles; tile += step, ++i) {
+      const Tile t = tile_at<32>(a, tables, tile);
+      const int b = i & 1, n = (2 * t.pt + rank) * kRows + 32 * q + lane;
+      const ChannelScale ch = prepare_scales(a, t, n, row_scale[warp - 2], lane);
+      if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
+      tc_fence_after();
+      drain_tile<F16, SWIGLU>(a, t, tmem + lane_addr + (b ? kMaxT : 0), c, n, ch, row_scale[warp - 2], lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&drained[b]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && abort_flag) st_cluster_u32(map_rank(smem_u32(&abort_flag), rank ^ 1), 1);
+  cluster_sync();  // neither CTA's memory goes while the other may read or signal it
+  if (*ctl.abort) {
+    // A wait ran out in one of them: tensor copies may be under way. A stage's last fill is awaited (its phase may lack the
+    // other CTA's part; then the wait ends by its limit, long after the copies).
+    if (rank == 0 && threadIdx.x == 0) {
+      const int g = static_cast<int>(max(fills[0], fills[1]));
+      for (int s = 0; s < kStages2; ++s) {
+        const int n = (g - s + kStages2 - 1) / kStages2;
+        if (n > 0) drain_wait(&full[s], (n - 1) & 1, a.err, kErrDrain);
+      }
+    }
+    cluster_sync();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+  zero_rest<F16>(a, SWIGLU ? a.n / 2 : a.n);
+}
+
 // ------------------------------------------------------------------ host side
 // Tiles that a call has at the most.
 int64_t most_tiles(const Int8Matmul& p, int64_t tmax, int64_t p_rows) {
@@ -489,81 +673,50 @@ int64_t most_tiles(const Int8Matmul& p, int64_t tmax, int64_t p_rows) {
   return along * ceil_div(p.N, p_rows);
 }
 
-template <bool F16, bool SWIGLU, bool GATHER>
-cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
-  cudaError_t e = allow_smem<int8_gemm_kernel<F16, SWIGLU, GATHER>>(kSmemBudget);
+struct Launch {
+  CUtensorMap p, q;
+  int grid, split;
+  bool pairs, early;
+  size_t smem;
+};
+
+template <auto Kernel>
+cudaError_t launch_kernel(const Launch& l, const Args& a, cudaStream_t s) {
+  cudaError_t e = allow_smem<Kernel>(kSmemBudget);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(l.grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = l.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (early) {
+  if (l.early) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (a.split > 1) {
+  if (!l.pairs && l.split > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = a.split;
+    attr[n].val.clusterDim.x = l.split;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<F16, SWIGLU, GATHER>, mp, mq, a);
+  return cudaLaunchKernelEx(&cfg, Kernel, l.p, l.q, a);
 }
 
 template <bool F16, bool SWIGLU>
-cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const Args& a, int grid, size_t smem, bool early, cudaStream_t s) {
-  return a.order ? launch<F16, SWIGLU, true>(mp, mq, a, grid, smem, early, s) : launch<F16, SWIGLU, false>(mp, mq, a, grid, smem, early, s);
+cudaError_t launch(const Launch& l, const Args& a, cudaStream_t s) {
+  return l.pairs ? launch_kernel<int8_gemm2_kernel<F16, SWIGLU>>(l, a, s) : launch_kernel<int8_gemm_kernel<F16, SWIGLU>>(l, a, s);
 }
 
-}  // namespace
-
-cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) {
-  const int sms = device_sm_count();
-  Args a{};
-  a.n = static_cast<int>(p.N);
-  a.groups = p.groups;
-  a.rows = static_cast<int>(p.rows);
-  a.a_rows = static_cast<int>(p.a_rows);
-  a.ksubs = static_cast<int>(ceil_div(p.K, 32));
-  a.ksteps = (a.ksubs + 3) / 4;
-  a.early = early;
-  a.top_k = p.top_k;
-  a.act = p.act;
-  a.has_limit = p.has_limit;
-  a.zero_rest = p.zero_rest;
-  a.bias_f16 = p.bias_f16;
-  a.alpha = p.alpha;
-  a.beta = p.beta;
-  a.limit = p.limit;
-  a.offsets = p.offsets;
-  a.order = p.order;
-  a.a_scales = p.a_scales;
-  a.b_scales = p.b_scales;
-  a.bias = p.bias;
-  a.y = p.y;
-  a.ldy = p.ldy;
-  const uintptr_t pair = p.f16 ? 4 : 8;
-  a.vec = reinterpret_cast<uintptr_t>(p.y) % pair == 0 && p.ldy % 2 == 0;
-  a.err = p.err;
-
-  // Columns of a tile: all rows of a dense product with few of them; a group's, when the rows are spread evenly or nearly so.
-  const int64_t mean = ceil_div(p.rows, p.groups), want = p.offsets ? 2 * mean + 8 : mean;
-  a.tmax = static_cast<int>(align_up(want < p.rows ? want : p.rows, 16));
-  if (a.tmax > kMaxT) a.tmax = kMaxT;
-  a.box = p.offsets ? 16 : a.tmax;
-  a.p_tiles = static_cast<int>(ceil_div(p.N, kRows));
-  const int64_t tiles = most_tiles(p, a.tmax, kRows);
-  if (tiles > INT_MAX / 16) return cudaErrorInvalidValue;
-
+// Shared memory, stages, split of K and grid of single CTAs.
+void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& l) {
+  // K is split while the CTAs find an SM each (narrow tiles: 1.6 CTAs an SM, they run side by side).
   const int64_t most = a.tmax <= 64 ? sms * 8 / 5 : sms;
   a.split = 1;
   while (a.split < 8 && tiles * a.split * 2 <= most && a.ksteps >= 4 * a.split) a.split *= 2;
-
   const uint32_t tables = tables_bytes(p.groups);
   const int budget = kSmemBudget - 1024 - static_cast<int>(tables);
   a.stage = static_cast<uint32_t>(kRows + a.tmax) * kStepBytes;
@@ -589,14 +742,75 @@ cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) 
   // CTAs that share an SM share its 512 columns: ask for enough shared memory that no more fit than those feed.
   const size_t least = static_cast<size_t>(227 * 1024) / (512 / a.tmem_cols + 1) + 1024;
   if (smem < least) smem = least;
-  const int grid = static_cast<int>(a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms));
+  l.smem = smem;
+  l.split = a.split;
+  l.grid = static_cast<int>(a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms));
+}
 
-  CUtensorMap mp, mq;
-  if (!encode_tensor_map_2d(&mp, 0, p.b, p.K, static_cast<uint64_t>(p.groups) * p.N, p.ldb, kStepBytes, kRows, true) ||
-      !encode_tensor_map_2d(&mq, 0, p.a, p.K, p.a_rows, p.lda, kStepBytes, p.order ? 1 : a.box, true))
+// Pairs take what needs a second round of single CTAs and has tiles wide enough.
+bool pairs_pay(const Int8Matmul& p, int64_t tiles, int tmax, int sms) { return tmax >= 128 && tiles > sms; }
+
+}  // namespace
+
+cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) {
+  const int sms = device_sm_count();
+  Args a{};
+  a.n = static_cast<int>(p.N);
+  a.groups = p.groups;
+  a.rows = static_cast<int>(p.rows);
+  a.ksubs = static_cast<int>(ceil_div(p.K, 32));
+  a.ksteps = (a.ksubs + 3) / 4;
+  a.early = early;
+  a.act = p.act;
+  a.has_limit = p.has_limit;
+  a.zero_rest = p.zero_rest;
+  a.bias_f16 = p.bias_f16;
+  a.alpha = p.alpha;
+  a.beta = p.beta;
+  a.limit = p.limit;
+  a.offsets = p.offsets;
+  a.a_scales = p.a_scales;
+  a.b_scales = p.b_scales;
+  a.bias = p.bias;
+  a.y = p.y;
+  a.ldy = p.ldy;
+  a.vec = reinterpret_cast<uintptr_t>(p.y) % 4 == 0 && p.ldy % 2 == 0;
+  a.err = p.err;
+
+  // Rows of a tile at the most: all of a dense product with few of them; twice a group's mean, so that most groups take one.
+  const int64_t mean = ceil_div(p.rows, p.groups), want = p.offsets ? 2 * mean + 8 : mean;
+  a.tmax = static_cast<int>(align_up(want < p.rows ? want : p.rows, 16));
+  if (p.offsets && a.tmax > 96) a.tmax = static_cast<int>(align_up(a.tmax, 64));
+  if (a.tmax > kMaxT) a.tmax = kMaxT;
+  // Rows of one copy: all of a dense tile; of a ragged one, whose last copy may reach into the next group's rows, large
+  // ones too (16 rows a copy: 39 cycles each, 620 a stage of 256 rows).
+  a.box = !p.offsets ? a.tmax : a.tmax % 64 == 0 ? 64 : 16;
+
+  Launch l{};
+  l.early = early;
+  int64_t tiles = most_tiles(p, a.tmax, kRows);
+  l.pairs = pairs_pay(p, tiles, a.tmax, sms);
+  const int channels = l.pairs ? 2 * kRows : kRows;
+  a.p_tiles = static_cast<int>(ceil_div(p.N, channels));
+  if (l.pairs) {
+    a.tmax = kMaxT;
+    a.box = p.offsets ? 64 : kRows;
+    tiles = most_tiles(p, a.tmax, channels);
+    a.split = 1;
+    a.stages = kStages2;
+    a.tables = kStages2 * kStage2;
+    l.smem = a.tables + tables_bytes(p.groups) + 1024;
+    l.grid = static_cast<int>(2 * (tiles < sms / 2 ? tiles : sms / 2));
+  } else {
+    if (tiles <= INT_MAX / 16) single_shape(p, tiles, sms, a, l);
+  }
+  if (tiles > INT_MAX / 16) return cudaErrorInvalidValue;
+
+  if (!encode_tensor_map_2d(&l.p, 0, p.b, p.K, static_cast<uint64_t>(p.groups) * p.N, p.ldb, kStepBytes, kRows, true) ||
+      !encode_tensor_map_2d(&l.q, 0, p.a, p.K, p.rows, p.lda, kStepBytes, a.box, true))
     return cudaErrorInvalidValue;
-  if (p.f16) return p.act == XRGPU_ACT_SWIGLU ? launch<true, true>(mp, mq, a, grid, smem, early, s) : launch<true, false>(mp, mq, a, grid, smem, early, s);
-  return p.act == XRGPU_ACT_SWIGLU ? launch<false, true>(mp, mq, a, grid, smem, early, s) : launch<false, false>(mp, mq, a, grid, smem, early, s);
+  if (p.f16) return p.act == XRGPU_ACT_SWIGLU ? launch<true, true>(l, a, s) : launch<true, false>(l, a, s);
+  return p.act == XRGPU_ACT_SWIGLU ? launch<false, true>(l, a, s) : launch<false, false>(l, a, s);
 }
 
 }  // namespace xrgpu
