@@ -1,9 +1,10 @@
 // Rows as 8-bit codes with one scale, and sums of rows by weights (format: mmnb_int8.h).
 //
-// Quantisation of a row: s = max|x| / 127 in float32, code = x / s rounded to nearest, ties to even. The quotient is
-// not computed: t = x * (1 / s) is off by less than 3e-5 (|t| <= 127, one rounding each of 1 / s and the product), so
-// round(t) is the code unless t lies that near to a border; there the border itself is compared, 2 |x| with (2 m + 1) s, exactly
-// in 64 bits (24 + 8 bits). A row with a NaN or an infinity has scale NaN and codes 0.
+// Quantisation of a row: s = max|x| / 127 in float32, code = x / s rounded to nearest, ties to even. The quotient is not
+// computed: r = round(x * (1 / s)) is the code or, next to a border, one off it. What is left, x - r s, is exact in one fused step
+// (it has no bit below both numbers' last ones and is at most about s / 2), so comparing it with s / 2 decides, and with r's
+// last bit a tie. Float32 rows of scales under 2^-60 are brought up by 2^100 first (exact as well); where s has
+// only a few bits left (subnormal), codes saturate. A row with a NaN or an infinity has scale NaN and codes 0.
 #include <cuda_fp16.h>
 
 #include "mmnb_common.cuh"
@@ -12,103 +13,89 @@
 namespace xrgpu {
 namespace {
 
-constexpr int kUnit = 16;                    // values of a thread at a time: 16 bytes of codes
-constexpr int kRowThreads = 512;             // of a row at the most
+constexpr int kUnit = 16;                    // codes of 16 bytes
+constexpr int kRowThreads = 1024;            // of a row at the most
 constexpr unsigned kErrOrder = 0x702;
 constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: t + kMagic rounds t to a whole number
-constexpr float kNearBorder = 0.49996f;
-constexpr float kSmallScale = 7.9e-31f;      // about 2^-100: below, 1 / s is not used
+constexpr float kSmallScale = 8.7e-19f;      // about 2^-60
 
-// code of x for scale s, from the exact quotient.
-__device__ __forceinline__ int exact_code(float x, float s) {
-  const double a = 2.0 * fabs(static_cast<double>(x)), d = static_cast<double>(s);
-  double m = floor(a / (2.0 * d));
-  m = m > 127.0 ? 127.0 : m;
-  const double border = (2.0 * m + 1.0) * d;  // of m and m + 1
-  int c = static_cast<int>(m);
-  if (a > border || (a == border && (c & 1))) ++c;
-  c = min(c, 127);
-  return x < 0.0f ? -c : c;
-}
+__device__ __forceinline__ uint32_t pack4(const uint32_t* b) { return prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410); }
 
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return prmt(prmt(a, b, 0x0040), prmt(c, d, 0x0040), 0x5410);
-}
+struct Scale {
+  float s, inv, up;  // of values times `up`
+};
 
-// The 16 codes of a thread.
-__device__ __forceinline__ uint4 codes16(const float (&v)[kUnit], float s, float inv) {
-  uint32_t b[kUnit];
+// Codes of a thread's N values, in the low bytes of b.
+template <int N, bool F16>
+__device__ __forceinline__ void codes_of(const float (&v)[N], const Scale& c, uint32_t (&b)[N]) {
   float worst = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kUnit; ++i) {
-    const float t = v[i] * inv, r = t + kMagic;
-    b[i] = __float_as_uint(r);
-    worst = fmaxf(worst, fabsf(t - (r - kMagic)));
+  for (int i = 0; i < N; ++i) {
+    const float x = F16 ? v[i] : v[i] * c.up;
+    const float t = fmaf(x, c.inv, kMagic), r = t - kMagic;
+    b[i] = __float_as_uint(t);
+    worst = fmaxf(worst, fabsf(fmaf(-r, c.s, x)));
   }
-  if (worst > kNearBorder) {
+  if (worst >= 0.5f * c.s) {  // hardly ever: a tie, a code one off, or one that saturates
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) {
-      const float t = v[i] * inv, r = t + kMagic;
-      if (fabsf(t - (r - kMagic)) > kNearBorder) b[i] = static_cast<uint32_t>(exact_code(v[i], s));
+    for (int i = 0; i < N; ++i) {
+      const float x = F16 ? v[i] : v[i] * c.up, r = __uint_as_float(b[i]) - kMagic, left = fmaf(-r, c.s, x);
+      int code = static_cast<int>(r);
+      if (fabsf(left) > 0.5f * c.s || (fabsf(left) == 0.5f * c.s && (code & 1))) code += left > 0.0f ? 1 : -1;
+      b[i] = static_cast<uint32_t>(max(-127, min(127, code)));
     }
   }
-  return make_uint4(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]), pack4(b[8], b[9], b[10], b[11]),
-                    pack4(b[12], b[13], b[14], b[15]));
 }
 
-// 16 values from k0 on of a row, zeros behind K, as they are held (raw) and as floats.
+// 16 bytes of a row from value k0 on, zeros behind K, as they are held and as floats.
 template <bool F16, bool VEC>
 struct Unit {
-  uint4 raw[F16 ? 2 : 4];
+  static constexpr int kValues = F16 ? 8 : 4;
+  uint32_t u[4];
   __device__ __forceinline__ void load(const void* x, int64_t row_at, int64_t k0, int64_t K) {
-    constexpr int es = F16 ? 2 : 4;
-    if (k0 >= K) {
+    if (VEC && k0 + kValues <= K) {
+      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + (row_at + k0) * (F16 ? 2 : 4));
+      u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+      return;
+    }
 #pragma unroll
-      for (int i = 0; i < (F16 ? 2 : 4); ++i) raw[i] = make_uint4(0, 0, 0, 0);
-    } else if (VEC && k0 + kUnit <= K) {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + (row_at + k0) * es);
-#pragma unroll
-      for (int i = 0; i < (F16 ? 2 : 4); ++i) raw[i] = src[i];
-    } else {
-      uint32_t u[F16 ? 8 : 16];
-#pragma unroll
-      for (int i = 0; i < (F16 ? 8 : 16); ++i) {
-        if (F16) {
-          const uint16_t* h = static_cast<const uint16_t*>(x) + row_at + k0;
-          const uint32_t lo = k0 + 2 * i < K ? h[2 * i] : 0, hi = k0 + 2 * i + 1 < K ? h[2 * i + 1] : 0;
-          u[i] = lo | hi << 16;
-        } else {
-          u[i] = k0 + i < K ? static_cast<const uint32_t*>(x)[row_at + k0 + i] : 0;
-        }
+    for (int i = 0; i < 4; ++i) {
+      if (F16) {
+        const uint16_t* h = static_cast<const uint16_t*>(x) + row_at + k0;
+        const uint32_t lo = k0 + 2 * i < K ? h[2 * i] : 0, hi = k0 + 2 * i + 1 < K ? h[2 * i + 1] : 0;
+        u[i] = lo | hi << 16;
+      } else {
+        u[i] = k0 + i < K ? static_cast<const uint32_t*>(x)[row_at + k0 + i] : 0;
       }
-#pragma unroll
-      for (int i = 0; i < (F16 ? 2 : 4); ++i) raw[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
     }
   }
   // the bits of the largest magnitude as float32 (NaN > infinity > numbers)
   __device__ __forceinline__ uint32_t amax() const {
-    const uint32_t* u = reinterpret_cast<const uint32_t*>(raw);
     if (F16) {
-      __half2 m = __float2half2_rn(0.0f);
+      __half2 m = __habs2(*reinterpret_cast<const __half2*>(&u[0]));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
+      for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
       return __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))) & 0x7fffffffu;
     }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < (F16 ? 8 : 16); ++i) m = max(m, u[i] & 0x7fffffffu);
-    return m;
+    return max(max(u[0] & 0x7fffffffu, u[1] & 0x7fffffffu), max(u[2] & 0x7fffffffu, u[3] & 0x7fffffffu));
   }
-  __device__ __forceinline__ void floats(float (&v)[kUnit]) const {
-    const uint32_t* u = reinterpret_cast<const uint32_t*>(raw);
+  __device__ __forceinline__ void store(int8_t* codes, int64_t at, const Scale& c, bool none) const {
+    float v[kValues];
+    uint32_t b[kValues];
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) {
+    for (int i = 0; i < kValues; ++i) {
       if (F16) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i >> 1]));
         v[i] = (i & 1) ? f.y : f.x;
       } else {
-        v[i] = __uint_as_float(u[F16 ? 0 : i]);
+        v[i] = __uint_as_float(u[i & 3]);
       }
+    }
+    codes_of<kValues, F16>(v, c, b);
+    if (F16) {
+      reinterpret_cast<uint2*>(codes)[at] = none ? make_uint2(0, 0) : make_uint2(pack4(b), pack4(b + (F16 ? 4 : 0)));
+    } else {
+      reinterpret_cast<uint32_t*>(codes)[at] = none ? 0 : pack4(b);
     }
   }
 };
@@ -126,32 +113,33 @@ __device__ __forceinline__ int64_t source_row(const RowOrder& f, int64_t r) {
 // registers between the two passes; else it is read twice.
 template <bool F16, bool VEC, int UNITS, bool HELD>
 __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p) {
+  using U = Unit<F16, VEC>;
   __shared__ uint32_t part[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's weights may start to load
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const bool real = row < p.rows;
-  const int64_t from = real ? source_row(p.from, row) : 0, row_at = max(from, static_cast<int64_t>(0)) * p.ldx, units = real ? (p.K + kUnit - 1) / kUnit : 0;
-  const int64_t read = real && from >= 0 ? p.K : 0;  // values of x that count
-  Unit<F16, VEC> u[UNITS];
+  const int64_t from = real ? source_row(p.from, row) : -1, row_at = max(from, static_cast<int64_t>(0)) * p.ldx;
+  const int64_t read = from >= 0 ? p.K : 0;  // values of x that count
+  const int units = real ? static_cast<int>((p.K + U::kValues - 1) / U::kValues) : 0;
+  U u[UNITS];
   uint32_t amax = 0;
   if (HELD) {
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) u[i].load(p.x, row_at, (threadIdx.x + static_cast<int64_t>(i) * blockDim.x) * kUnit, read);
+    for (int i = 0; i < UNITS; ++i) u[i].load(p.x, row_at, (threadIdx.x + i * blockDim.x) * static_cast<int64_t>(U::kValues), read);
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) amax = max(amax, u[i].amax());
   } else {
-    for (int64_t at = threadIdx.x; at < units; at += blockDim.x) {
-      u[0].load(p.x, row_at, at * kUnit, read);
+    for (int at = threadIdx.x; at < units; at += blockDim.x) {
+      u[0].load(p.x, row_at, at * static_cast<int64_t>(U::kValues), read);
       amax = max(amax, u[0].amax());
     }
   }
   amax = __reduce_max_sync(~0u, amax);
   const int warps = blockDim.x >> 5;
   if (warps > 1) {
-    const int w = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) part[threadIdx.y * warps + w] = amax;
-    __syncthreads();
     const int lane = threadIdx.x & 31;
+    if (lane == 0) part[threadIdx.y * warps + (threadIdx.x >> 5)] = amax;
+    __syncthreads();
     amax = __reduce_max_sync(~0u, lane < warps ? part[threadIdx.y * warps + lane] : 0u);
   }
   if (!real) return;
@@ -159,31 +147,21 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
   const float s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(amax), 127.0f);
   if (threadIdx.x == 0) p.scales[row] = s;
   const bool none = bad || s == 0.0f;
-  const float inv = none ? 0.0f : __fdiv_rn(1.0f, s);
-  uint4* dst = reinterpret_cast<uint4*>(p.codes + row * p.ldc);
-  auto store = [&](const Unit<F16, VEC>& x, int64_t at) {
-    float v[kUnit];
-    x.floats(v);
-    if (none) {
-      dst[at] = make_uint4(0, 0, 0, 0);
-    } else if (!F16 && s < kSmallScale) {
-      uint32_t b[kUnit];
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i) b[i] = static_cast<uint32_t>(exact_code(v[i], s));
-      dst[at] = make_uint4(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]), pack4(b[8], b[9], b[10], b[11]),
-                           pack4(b[12], b[13], b[14], b[15]));
-    } else {
-      dst[at] = codes16(v, s, inv);
-    }
-  };
+  Scale c;
+  c.up = !F16 && s < kSmallScale ? 0x1p100f : 1.0f;
+  c.s = none ? 1.0f : s * c.up;
+  c.inv = __fdiv_rn(1.0f, c.s);
+  int8_t* codes = p.codes + row * p.ldc;
   if (HELD) {
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i)
-      if (threadIdx.x + static_cast<int64_t>(i) * blockDim.x < units) store(u[i], threadIdx.x + static_cast<int64_t>(i) * blockDim.x);
+    for (int i = 0; i < UNITS; ++i) {
+      const int at = threadIdx.x + i * blockDim.x;
+      if (at < units) u[i].store(codes, at, c, none);
+    }
   } else {
-    for (int64_t at = threadIdx.x; at < units; at += blockDim.x) {
-      u[0].load(p.x, row_at, at * kUnit, read);
-      store(u[0], at);
+    for (int at = threadIdx.x; at < units; at += blockDim.x) {
+      u[0].load(p.x, row_at, at * static_cast<int64_t>(U::kValues), read);
+      u[0].store(codes, at, c, none);
     }
   }
 }
@@ -202,34 +180,37 @@ __global__ void __launch_bounds__(256) gather_kernel(const Int8Gather p) {
   for (int64_t k = whole * kUnit + threadIdx.x; k < p.K; k += blockDim.x) p.codes[row * p.ldc + k] = reinterpret_cast<const int8_t*>(src)[k];
 }
 
+// VEC: 16 bytes of values a thread at a time (K a multiple of 16).
 template <bool F16, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_kernel(const Int8Rows p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if (row >= p.rows) return;
   const float s = p.scales[row];
   const int8_t* src = p.codes + row * p.ldc;
-  if (VEC) {  // K a multiple of 16
-    for (int64_t at = threadIdx.x; at < p.K / kUnit; at += blockDim.x) {
-      const uint4 c = reinterpret_cast<const uint4*>(src)[at];
-      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-      float v[kUnit];
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)))) * s;
+  if (VEC) {
+    const int items = static_cast<int>(p.K / (F16 ? 8 : 4));
+#pragma unroll 4
+    for (int at = threadIdx.x; at < items; at += blockDim.x) {
+      uint32_t w[2];
       if (F16) {
-        uint32_t h[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-          h[i] = *reinterpret_cast<const uint32_t*>(&x);
-        }
-        uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + row * p.K + at * kUnit);
-        d[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        d[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        const uint2 c = reinterpret_cast<const uint2*>(src)[at];
+        w[0] = c.x;
+        w[1] = c.y;
       } else {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.K + at * kUnit);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        w[0] = reinterpret_cast<const uint32_t*>(src)[at];
       }
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (F16) {
+          const uint32_t pair = w[i >> 1] >> (16 * (i & 1));
+          const __half2 h = __floats2half2_rn(static_cast<float>(static_cast<int8_t>(pair)) * s, static_cast<float>(static_cast<int8_t>(pair >> 8)) * s);
+          o[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          o[i] = __float_as_uint(static_cast<float>(static_cast<int8_t>(w[0] >> (8 * i))) * s);
+        }
+      }
+      reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + row * p.K * (F16 ? 2 : 4))[at] = make_uint4(o[0], o[1], o[2], o[3]);
     }
   } else {
     for (int64_t k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -270,9 +251,9 @@ __global__ void __launch_bounds__(kSumThreads) weighted_rows_kernel(const Weight
 
 template <bool F16, bool VEC>
 cudaError_t quantize(const Int8Rows& p, cudaStream_t s) {
-  // Units a thread: a row has about 256 threads, and it stays in registers (8 or 16 of them a unit).
-  const int64_t units = ceil_div(p.K, kUnit);
-  const int64_t per = units <= 256 ? 1 : units <= 512 ? 2 : 4;
+  // A row has about 256 threads of up to 8 units, and stays in registers while it has no more than 1024 of them.
+  const int64_t units = ceil_div(p.K, Unit<F16, VEC>::kValues);
+  const int64_t per = units <= 256 ? 1 : units <= 512 ? 2 : units <= 1024 ? 4 : 8;
   const int64_t threads = align_up(ceil_div(units, per), 32);
   const bool held = threads <= kRowThreads;
   const unsigned tx = static_cast<unsigned>(held ? threads : kRowThreads), ty = tx < 256 ? 256 / tx : 1;
@@ -282,7 +263,8 @@ cudaError_t quantize(const Int8Rows& p, cudaStream_t s) {
   if (!held) quantize_kernel<F16, VEC, 1, false><<<grid, block, 0, s>>>(p);
   else if (per == 1) quantize_kernel<F16, VEC, 1, true><<<grid, block, 0, s>>>(p);
   else if (per == 2) quantize_kernel<F16, VEC, 2, true><<<grid, block, 0, s>>>(p);
-  else quantize_kernel<F16, VEC, 4, true><<<grid, block, 0, s>>>(p);
+  else if (per == 4) quantize_kernel<F16, VEC, 4, true><<<grid, block, 0, s>>>(p);
+  else quantize_kernel<F16, VEC, 8, true><<<grid, block, 0, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -298,7 +280,7 @@ cudaError_t launch_int8_quantize(const Int8Rows& p, cudaStream_t s) {
 
 cudaError_t launch_int8_dequantize(const Int8Rows& p, cudaStream_t s) {
   const bool vec = p.K % kUnit == 0 && aligned16(p.out);
-  const int64_t items = vec ? p.K / kUnit : p.K;
+  const int64_t items = vec ? p.K / (p.f16 ? 8 : 4) : p.K;
   const unsigned tx = items >= 256 ? 256 : static_cast<unsigned>(align_up(items, 32)), ty = 256 / tx;
   const int64_t blocks = ceil_div(p.rows, ty);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;

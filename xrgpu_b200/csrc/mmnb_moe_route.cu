@@ -1,22 +1,28 @@
 // Router of a mixture of experts: each token's top_k experts by score (ties to the lowest index, a NaN counts as -infinity),
 // their weights, and the stable order of all assignments (token * top_k + rank) by expert.
 //
-// Choice: a warp a token; scores are turned into keys that order like the numbers, and top_k times the largest key of
-// the warp (lowest index among equals) is taken out. Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
+// Choice: a warp a token. Scores become numbers of 32 bits that order like them: the upper 22 bits of a key of the
+// score, then the index counted down, and the largest of the warp is taken out top_k times. That is exact for float16 (16
+// bits); for float32 two neighbours of the result that agree in the 22 bits send the token to the exact form (whole keys, then the
+// lowest index among equals). What bounds it is instructions: about 25 a choice instead of 50 for whole keys.
+// Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
 // Order: a counting sort. Every warp counts its own tokens' experts, the counts are summed over the warps and CTAs before it, and
-// each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: one CTA does
-// all of it; else a second kernel follows in which every CTA sums the counts of all (G x experts numbers, from L2).
+// each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: the CTAs of one
+// cluster read each other's counts; else a second kernel follows in which every CTA sums the counts of all (from L2).
 #include <cuda_fp16.h>
 
 #include "mmnb_common.cuh"
 #include "mmnb_int8.h"
+#include "mmnb_tcgen05.cuh"
 
 namespace xrgpu {
 namespace {
 
 constexpr int kWarps = 32;
 constexpr int kThreads = kWarps * 32;
-constexpr int64_t kOneCta = 64;  // tokens up to which one CTA does all
+constexpr int kClusterCtas = 8;
+// Tokens that a cluster takes, one a warp (128 experts, 8 of them; us, cluster / two kernels: 64 tokens 6.4 / 8.4, 256 7.2 / 8.4, 512 9.3 / 8.4).
+constexpr int64_t kClusterTokens = 256;
 
 struct Args {
   MoeRoute p;
@@ -41,60 +47,85 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The choice and weights of the warp's tokens, counted into `mine` [experts]. VPL: scores a lane.
+// The chosen experts by whole keys: lane j returns the j-th.
 template <int VPL>
-__device__ __forceinline__ void choose(const Args& a, int64_t t0, int64_t t1, int32_t* mine) {
-  const int lane = threadIdx.x & 31, E = a.p.experts, k = a.p.top_k;
-  for (int64_t t = t0; t < t1; ++t) {
-    uint32_t key[VPL];
-    float x[VPL];
+__device__ __noinline__ int choose_exact(const float* scores, int E, int k) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[VPL], best = 0;
+  int at = 0, chosen = 0;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) x[i] = lane + 32 * i < E ? load_f(a.p.scores, a.p.f16, t * a.p.lds + lane + 32 * i) : 0.0f;
-    uint32_t best = 0;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      key[i] = lane + 32 * i < E ? key_of(x[i]) : 0u;
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
-      }
+  for (int i = 0; i < VPL; ++i) {
+    key[i] = lane + 32 * i < E ? key_of(scores[lane + 32 * i]) : 0u;
+    if (key[i] > best) {
+      best = key[i];
+      at = i;
     }
-    const float top = score_of(__reduce_max_sync(~0u, best));
-    float all = 0.0f;
-    if (!a.p.normalize) {
+  }
+  for (int j = 0; j < k; ++j) {
+    const uint32_t m = __reduce_max_sync(~0u, best);
+    const int e = static_cast<int>(__reduce_min_sync(~0u, best == m ? static_cast<unsigned>(lane + 32 * at) : ~0u));
+    if (lane == j) chosen = e;
+    if (lane == (e & 31)) {
+      best = 0;
+      at = 0;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) all += key[i] ? expf(score_of(key[i]) - top) : 0.0f;
-      all = warp_sum(all);
-    }
-    int chosen = 0;
-    float score = 0.0f;
-    for (int j = 0; j < k; ++j) {
-      const uint32_t m = __reduce_max_sync(~0u, best);
-      const int e = static_cast<int>(__reduce_min_sync(~0u, best == m ? static_cast<unsigned>(lane + 32 * at) : ~0u));
-      if (lane == j) {
-        chosen = e;
-        score = score_of(m);
-      }
-      if (lane == (e & 31)) {
-        best = 0;
-        at = 0;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          if (i == (e >> 5)) key[i] = 0;
-          if (key[i] > best) {
-            best = key[i];
-            at = i;
-          }
+      for (int i = 0; i < VPL; ++i) {
+        if (i == (e >> 5)) key[i] = 0;
+        if (key[i] > best) {
+          best = key[i];
+          at = i;
         }
       }
     }
+  }
+  return chosen;
+}
+
+// The choice and weights of the warp's tokens, counted into `mine` [experts]. VPL: scores a lane.
+template <int VPL, bool F16>
+__device__ __forceinline__ void choose(const Args& a, int64_t t0, int64_t t1, int32_t* mine) {
+  const int lane = threadIdx.x & 31, E = a.p.experts, k = a.p.top_k;
+  for (int64_t t = t0; t < t1; ++t) {
+    float x[VPL];
+    uint32_t c[VPL], top = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) x[i] = lane + 32 * i < E ? load_f(a.p.scores, F16, t * a.p.lds + lane + 32 * i) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      c[i] = lane + 32 * i < E ? (key_of(x[i]) & ~1023u) | (1023u - (lane + 32 * i)) : 0u;
+      top = max(top, c[i]);
+    }
+    int chosen = 0;
+    uint32_t last = 0;
+    bool close = false;
+    const int picks = F16 ? k : min(k + 1, E);
+    for (int j = 0; j < picks; ++j) {
+      const uint32_t m = __reduce_max_sync(~0u, top);
+      if (lane == j) chosen = static_cast<int>(1023u - (m & 1023u));
+      close |= (m ^ last) < 1024u;
+      last = m;
+      top = 0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        c[i] = c[i] == m ? 0u : c[i];
+        top = max(top, c[i]);
+      }
+    }
+    if (!F16 && close) chosen = choose_exact<VPL>(static_cast<const float*>(a.p.scores) + t * a.p.lds, E, k);
+    const float score = lane < k ? score_of(key_of(load_f(a.p.scores, F16, t * a.p.lds + chosen))) : 0.0f;
+    const float best = __shfl_sync(~0u, score, 0);
     // a token whose scores are all -infinity weighs nothing
-    const float w = lane < k && top > -INFINITY ? expf(score - top) : 0.0f;
-    const float sum = a.p.normalize ? warp_sum(w) : all;
+    const float w = lane < k && best > -INFINITY ? expf(score - best) : 0.0f;
+    float sum = w;
+    if (!a.p.normalize) {
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) sum += lane + 32 * i < E && x[i] == x[i] ? expf(x[i] - best) : 0.0f;
+    }
+    sum = warp_sum(sum);
     if (lane < k) {
       a.p.chosen[t * k + lane] = chosen;
-      a.p.weights[t * k + lane] = top > -INFINITY ? w / sum : 0.0f;
+      a.p.weights[t * k + lane] = best > -INFINITY ? w / sum : 0.0f;
       mine[chosen] += 1;  // a token's experts differ
     }
     __syncwarp();
@@ -164,22 +195,42 @@ __device__ __forceinline__ Range tokens_of(const Args& a) {
   return {min(first, a.p.tokens), min(first + a.per_warp, a.p.tokens)};
 }
 
-template <int VPL, bool ONE>
+// CLUSTER: all CTAs are one cluster, and the kernel does the whole call.
+template <int VPL, bool F16, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1) choose_kernel(const Args a) {
   extern __shared__ int32_t hist[];
-  const int E = a.p.experts;
+  __shared__ int32_t counts[kThreads];
+  const int E = a.p.experts, e = threadIdx.x;
   for (int i = threadIdx.x; i < kWarps * E; i += kThreads) hist[i] = 0;
   __syncthreads();
   const Range r = tokens_of(a);
-  choose<VPL>(a, r.t0, r.t1, hist + (threadIdx.x >> 5) * E);
+  choose<VPL, F16>(a, r.t0, r.t1, hist + (threadIdx.x >> 5) * E);
   __syncthreads();
   int count = 0;
-  if (static_cast<int>(threadIdx.x) < E) {
+  if (e < E) {
 #pragma unroll 8
-    for (int w = 0; w < kWarps; ++w) count += hist[w * E + threadIdx.x];
+    for (int w = 0; w < kWarps; ++w) count += hist[w * E + e];
   }
-  if (ONE) place(a, r.t0, r.t1, hist, count, 0, true);
-  else if (static_cast<int>(threadIdx.x) < E) a.counts[static_cast<int64_t>(blockIdx.x) * E + threadIdx.x] = count;
+  if (!CLUSTER) {
+    if (e < E) a.counts[static_cast<int64_t>(blockIdx.x) * E + e] = count;
+    return;
+  }
+  int total = count, before = 0;
+  if (a.ctas > 1) {
+    counts[e] = count;
+    cluster_sync();
+    total = 0;
+    int c[kClusterCtas];
+#pragma unroll
+    for (int i = 0; i < kClusterCtas; ++i) c[i] = i < a.ctas ? ld_cluster_s32(map_rank(smem_u32(&counts[e]), i)) : 0;
+#pragma unroll
+    for (int i = 0; i < kClusterCtas; ++i) {
+      total += c[i];
+      before += i < static_cast<int>(blockIdx.x) ? c[i] : 0;
+    }
+    cluster_sync();  // nobody leaves while its counts are being read
+  }
+  place(a, r.t0, r.t1, hist, total, before, blockIdx.x == 0);
 }
 
 __global__ void __launch_bounds__(kThreads, 1) place_kernel(const Args a) {
@@ -217,25 +268,17 @@ __global__ void __launch_bounds__(kThreads, 1) place_kernel(const Args a) {
   place(a, r.t0, r.t1, hist, total, before, blockIdx.x == 0);
 }
 
+// Tokens that one cluster takes: one or two a warp.
+bool one_cluster(const MoeRoute& p) { return p.tokens <= kClusterTokens; }
+
 int per_warp(const MoeRoute& p) {
-  if (p.tokens <= kOneCta) return static_cast<int>(ceil_div(p.tokens, kWarps));
-  const int64_t ctas = ceil_div(p.tokens, kWarps) < device_sm_count() ? ceil_div(p.tokens, kWarps) : device_sm_count();
-  return static_cast<int>(ceil_div(p.tokens, kWarps * ctas));
+  const int64_t warps = ceil_div(p.tokens, kWarps), most = one_cluster(p) ? kClusterCtas : device_sm_count();
+  return static_cast<int>(ceil_div(p.tokens, kWarps * (warps < most ? warps : most)));
 }
 
-template <int VPL>
-cudaError_t launch(const Args& a, cudaStream_t s) {
-  const size_t smem = static_cast<size_t>(kWarps) * a.p.experts * 4;
-  cudaError_t e = allow_smem<choose_kernel<VPL, true>>(kWarps * 32 * VPL * 4);
-  if (e == cudaSuccess) e = allow_smem<choose_kernel<VPL, false>>(kWarps * 32 * VPL * 4);
-  if (e == cudaSuccess) e = allow_smem<place_kernel>(static_cast<int>(smem));
-  if (e != cudaSuccess) return e;
-  if (a.ctas == 1) {
-    choose_kernel<VPL, true><<<1, kThreads, smem, s>>>(a);
-    return cudaGetLastError();
-  }
-  choose_kernel<VPL, false><<<a.ctas, kThreads, smem, s>>>(a);
-  e = cudaGetLastError();
+template <auto Kernel>
+cudaError_t launch_kernel(const Args& a, size_t smem, int cluster, bool early, cudaStream_t s) {
+  cudaError_t e = allow_smem<Kernel>(static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.ctas);
@@ -243,17 +286,35 @@ cudaError_t launch(const Args& a, cudaStream_t s) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  if (early) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, place_kernel, a);
+  cfg.numAttrs = early || cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, Kernel, a);
+}
+
+template <int VPL, bool F16>
+cudaError_t launch(const Args& a, cudaStream_t s) {
+  const size_t smem = static_cast<size_t>(kWarps) * a.p.experts * 4;
+  if (one_cluster(a.p)) return launch_kernel<choose_kernel<VPL, F16, true>>(a, smem, a.ctas, false, s);
+  const cudaError_t e = launch_kernel<choose_kernel<VPL, F16, false>>(a, smem, 1, false, s);
+  return e != cudaSuccess ? e : launch_kernel<place_kernel>(a, smem, 1, true, s);
+}
+template <int VPL>
+cudaError_t launch(const Args& a, cudaStream_t s) {
+  return a.p.f16 ? launch<VPL, true>(a, s) : launch<VPL, false>(a, s);
 }
 
 }  // namespace
 
 uint64_t moe_route_workspace(const MoeRoute& p) {
-  if (p.tokens <= kOneCta) return 0;
+  if (one_cluster(p)) return 0;
   return static_cast<uint64_t>(ceil_div(p.tokens, static_cast<int64_t>(kWarps) * per_warp(p))) * p.experts * 4;
 }
 
