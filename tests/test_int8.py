@@ -64,12 +64,14 @@ def test_product_workspace(cuda_lib):
     need = ctypes.c_uint64()
     size = lambda **kw: (cuda_lib.xrgpu_int8_workspace_size(ctypes.byref(_problem(**kw)), ctypes.byref(need)), need.value)  # noqa: E731
     assert size() == (0, 0)
-    assert size(a_dtype=_native.FLOAT16) == (0, 512)  # codes, scales
+    assert size(a_dtype=_native.FLOAT16) == (0, 0)  # few rows are quantised in place
+    assert size(a_dtype=_native.FLOAT16, M=17) == (0, 1280 + 256)  # codes, scales
+    assert size(**GROUPED, order=4096, top_k=1) == (0, 512 + 256)  # rows in the groups' order
     assert size(**GROUPED, slots=4096, weights=4096, tokens=3, top_k=2) == (0, 6 * 8 * 4)
-    p = _problem(a_dtype=_native.FLOAT16)
-    assert cuda_lib.xrgpu_int8_forward(ctypes.byref(p), 4096, 511, None) == _native.INVALID_ARGUMENT
+    p = _problem(a_dtype=_native.FLOAT16, M=17)
+    assert cuda_lib.xrgpu_int8_forward(ctypes.byref(p), 4096, 1535, None) == _native.INVALID_ARGUMENT
     assert "workspace too small" in cuda_lib.xrgpu_last_error().decode()
-    assert cuda_lib.xrgpu_int8_forward(ctypes.byref(p), 4100, 512, None) == _native.INVALID_ARGUMENT
+    assert cuda_lib.xrgpu_int8_forward(ctypes.byref(p), 4100, 1536, None) == _native.INVALID_ARGUMENT
     assert cuda_lib.xrgpu_int8_forward(ctypes.byref(_problem(M=0)), None, 0, None) == 0  # no rows: nothing to do
     assert cuda_lib.xrgpu_int8_forward(None, None, 0, None) == _native.INVALID_ARGUMENT
 
@@ -262,6 +264,30 @@ def test_product_quantises_floats(F, M, N, K, dtype):
     want, err = R.product(a, sa, b, sb.double().numpy())
     R.close(F.matmul_int8(x.cuda(), bd, sb.cuda()), want, err, dtype)
     R.close(F.matmul_int8(x.cuda(), bd, sb.cuda(), dtype=FULL), want, err, FULL)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (2, 130, 33), (16, 2000, 600), (7, 14336, 1000), (3, 256, 9001), (1, 4096, 4096), (13, 700, 28672), (16, 24000, 100), (4, 29000, 520)])
+@pytest.mark.parametrize("dtype,out,act", [(HALF, HALF, "none"), (FULL, FULL, "swiglu"), (HALF, FULL, "relu"), (FULL, HALF, "none")])
+def test_product_of_few_float_rows(F, M, N, K, dtype, out, act):
+    """Rows that the product's own kernel quantises: strided, with zeros, NaN, infinities and tiny numbers among them."""
+    N += N % 2 if act == "swiglu" else 0
+    g = torch.Generator().manual_seed(M * N + K)
+    x = _values(M, K, dtype, K + M)
+    if M > 4:
+        x[0], x[1, K // 2], x[2, -1] = 0.0, float("nan"), float("-inf")
+        x[3] *= 2.0 ** -120 if dtype == FULL else 2.0 ** -13
+    b, bd, sb = _codes(g, N, K)
+    v = torch.randn(N, generator=g).to(out)
+    a, sa = R.quantize(x.double().numpy())
+    want, err = R.product(a, np.nan_to_num(sa), b, sb.double().numpy(), v.double().numpy(), act)
+    want[np.isnan(sa)] = np.nan
+    wide = torch.randn(M, K + 24, generator=g).to(dtype).cuda()
+    for lead in (8, 3):  # rows on 16 bytes (for some K), and rows that are not
+        view = wide[:, lead:lead + K]
+        view.copy_(x)
+        R.close(F.matmul_int8(view, bd, sb.cuda(), v.cuda(), activation=act, dtype=out), want, err, out)
+    assert F.device_error() == 0
 
 
 @gpu

@@ -1,13 +1,7 @@
 // Rows as 8-bit codes with one scale, and sums of rows by weights (format: mmnb_int8.h).
-//
-// Quantisation of a row: s = max|x| / 127 in float32, code = x / s rounded to nearest, ties to even. The quotient is not
-// computed: r = round(x * (1 / s)) is the code or, next to a border, one off it. What is left, x - r s, is exact in one fused step
-// (it has no bit below both numbers' last ones and is at most about s / 2), so comparing it with s / 2 decides, and with r's
-// last bit a tie. Float32 rows of scales under 2^-60 are brought up by 2^100 first (exact as well); where s has
-// only a few bits left (subnormal), codes saturate. A row with a NaN or an infinity has scale NaN and codes 0.
 #include <cuda_fp16.h>
 
-#include "mmnb_common.cuh"
+#include "mmnb_int8.cuh"
 #include "mmnb_int8.h"
 
 namespace xrgpu {
@@ -16,89 +10,6 @@ namespace {
 constexpr int kUnit = 16;                    // codes of 16 bytes
 constexpr int kRowThreads = 1024;            // of a row at the most
 constexpr unsigned kErrOrder = 0x702;
-constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: t + kMagic rounds t to a whole number
-constexpr float kSmallScale = 8.7e-19f;      // about 2^-60
-
-__device__ __forceinline__ uint32_t pack4(const uint32_t* b) { return prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410); }
-
-struct Scale {
-  float s, inv, up;  // of values times `up`
-};
-
-// Codes of a thread's N values, in the low bytes of b.
-template <int N, bool F16>
-__device__ __forceinline__ void codes_of(const float (&v)[N], const Scale& c, uint32_t (&b)[N]) {
-  float worst = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = F16 ? v[i] : v[i] * c.up;
-    const float t = fmaf(x, c.inv, kMagic), r = t - kMagic;
-    b[i] = __float_as_uint(t);
-    worst = fmaxf(worst, fabsf(fmaf(-r, c.s, x)));
-  }
-  if (worst >= 0.5f * c.s) {  // hardly ever: a tie, a code one off, or one that saturates
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float x = F16 ? v[i] : v[i] * c.up, r = __uint_as_float(b[i]) - kMagic, left = fmaf(-r, c.s, x);
-      int code = static_cast<int>(r);
-      if (fabsf(left) > 0.5f * c.s || (fabsf(left) == 0.5f * c.s && (code & 1))) code += left > 0.0f ? 1 : -1;
-      b[i] = static_cast<uint32_t>(max(-127, min(127, code)));
-    }
-  }
-}
-
-// 16 bytes of a row from value k0 on, zeros behind K, as they are held and as floats.
-template <bool F16, bool VEC>
-struct Unit {
-  static constexpr int kValues = F16 ? 8 : 4;
-  uint32_t u[4];
-  __device__ __forceinline__ void load(const void* x, int64_t row_at, int64_t k0, int64_t K) {
-    if (VEC && k0 + kValues <= K) {
-      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + (row_at + k0) * (F16 ? 2 : 4));
-      u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (F16) {
-        const uint16_t* h = static_cast<const uint16_t*>(x) + row_at + k0;
-        const uint32_t lo = k0 + 2 * i < K ? h[2 * i] : 0, hi = k0 + 2 * i + 1 < K ? h[2 * i + 1] : 0;
-        u[i] = lo | hi << 16;
-      } else {
-        u[i] = k0 + i < K ? static_cast<const uint32_t*>(x)[row_at + k0 + i] : 0;
-      }
-    }
-  }
-  // the bits of the largest magnitude as float32 (NaN > infinity > numbers)
-  __device__ __forceinline__ uint32_t amax() const {
-    if (F16) {
-      __half2 m = __habs2(*reinterpret_cast<const __half2*>(&u[0]));
-#pragma unroll
-      for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
-      return __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))) & 0x7fffffffu;
-    }
-    return max(max(u[0] & 0x7fffffffu, u[1] & 0x7fffffffu), max(u[2] & 0x7fffffffu, u[3] & 0x7fffffffu));
-  }
-  __device__ __forceinline__ void store(int8_t* codes, int64_t at, const Scale& c, bool none) const {
-    float v[kValues];
-    uint32_t b[kValues];
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) {
-      if (F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i >> 1]));
-        v[i] = (i & 1) ? f.y : f.x;
-      } else {
-        v[i] = __uint_as_float(u[i & 3]);
-      }
-    }
-    codes_of<kValues, F16>(v, c, b);
-    if (F16) {
-      reinterpret_cast<uint2*>(codes)[at] = none ? make_uint2(0, 0) : make_uint2(pack4(b), pack4(b + (F16 ? 4 : 0)));
-    } else {
-      reinterpret_cast<uint32_t*>(codes)[at] = none ? 0 : pack4(b);
-    }
-  }
-};
 
 // The row that row r stands for, -1 where it fits none (recorded).
 __device__ __forceinline__ int64_t source_row(const RowOrder& f, int64_t r) {
@@ -143,25 +54,27 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
     amax = __reduce_max_sync(~0u, lane < warps ? part[threadIdx.y * warps + lane] : 0u);
   }
   if (!real) return;
-  const bool bad = amax >= 0x7f800000u;
-  const float s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(amax), 127.0f);
-  if (threadIdx.x == 0) p.scales[row] = s;
-  const bool none = bad || s == 0.0f;
   Scale c;
-  c.up = !F16 && s < kSmallScale ? 0x1p100f : 1.0f;
-  c.s = none ? 1.0f : s * c.up;
-  c.inv = __fdiv_rn(1.0f, c.s);
+  bool none;
+  const float s = row_scale_of<F16>(amax, &c, &none);
+  if (threadIdx.x == 0) p.scales[row] = s;
   int8_t* codes = p.codes + row * p.ldc;
+  auto store = [&](const U& x, int at) {
+    uint32_t w[2];
+    x.codes(c, w);
+    if (F16) reinterpret_cast<uint2*>(codes)[at] = none ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
+    else reinterpret_cast<uint32_t*>(codes)[at] = none ? 0 : w[0];
+  };
   if (HELD) {
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
       const int at = threadIdx.x + i * blockDim.x;
-      if (at < units) u[i].store(codes, at, c, none);
+      if (at < units) store(u[i], at);
     }
   } else {
     for (int at = threadIdx.x; at < units; at += blockDim.x) {
       u[0].load(p.x, row_at, at * static_cast<int64_t>(U::kValues), read);
-      u[0].store(codes, at, c, none);
+      store(u[0], at);
     }
   }
 }

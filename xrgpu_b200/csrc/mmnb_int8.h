@@ -65,6 +65,10 @@ struct Int8Matmul {
 };
 // early: the kernel before it on the stream writes a and a_scales only and announces its end early.
 cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s);
+// The product of a few float rows x [p.rows, ldx], quantised by the same kernel (p.a and p.a_scales are not used), and whether a
+// call takes this form.
+bool int8_few_rows(const Int8Matmul& p);
+cudaError_t launch_int8_few(const Int8Matmul& p, const void* x, bool x_f16, int64_t ldx, cudaStream_t s);
 
 // out[t] = sum_j weights[t, j] y[slots[t, j]], float32 sums in the order of j; slots outside [0, rows) are left out.
 struct WeightedRows {

@@ -58,10 +58,10 @@ struct Layout {
   uint64_t scales, rows, bytes;
   int64_t ldr;  // row stride of the results
 };
-Layout layout(const xrgpu_int8_problem& c, int64_t out_n) {
+Layout layout(const xrgpu_int8_problem& c, int64_t out_n, bool in_place) {
   Layout l{};
   const uint64_t rows = static_cast<uint64_t>(c.groups ? c.rows : c.M);
-  if (c.a_dtype != XRGPU_INT8 || c.order) {
+  if ((c.a_dtype != XRGPU_INT8 && !in_place) || c.order) {
     l.scales = align_up(rows * align_up(c.K, 16), 256);
     l.rows = l.scales + align_up(rows * 4, 256);
   }
@@ -71,7 +71,7 @@ Layout layout(const xrgpu_int8_problem& c, int64_t out_n) {
 }
 
 // Everything but the pointers of tensors.
-int check(const xrgpu_int8_problem* c, Int8Matmul* p, Layout* l) {
+int check(const xrgpu_int8_problem* c, Int8Matmul* p, Layout* l, bool* in_place) {
   if (!c) return fail("Null problem");
   int st = t1_code(c->dtype, &p->f16);
   if (st) return st;
@@ -104,7 +104,6 @@ int check(const xrgpu_int8_problem* c, Int8Matmul* p, Layout* l) {
   }
   if ((st = code_stride(c->ldb, c->K, &p->ldb))) return st;
   if (c->ldy != 0 && c->ldy < out_n) return fail("ldy must cover a row of y");
-  *l = layout(*c, out_n);
   p->act = c->activation;
   p->has_limit = c->has_limit != 0;
   p->alpha = c->alpha;
@@ -117,6 +116,9 @@ int check(const xrgpu_int8_problem* c, Int8Matmul* p, Layout* l) {
   p->K = c->K;
   p->ldy = c->ldy ? c->ldy : out_n;
   p->zero_rest = c->zero_rest != 0;
+  p->offsets = c->offsets;
+  *in_place = c->a_dtype != XRGPU_INT8 && !c->groups && int8_few_rows(*p);
+  *l = layout(*c, out_n, *in_place);
   return XRGPU_OK;
 }
 
@@ -131,7 +133,8 @@ int workspace(void** ws, uint64_t given, uint64_t need) {
 int forward(const xrgpu_int8_problem* c, void* ws, uint64_t ws_bytes, cudaStream_t s) {
   Int8Matmul p{};
   Layout l{};
-  int st = check(c, &p, &l);
+  bool in_place;
+  int st = check(c, &p, &l, &in_place);
   if (st) return st;
   const bool sums = c->slots != nullptr;
   if (sums ? c->tokens == 0 : p.rows == 0) return XRGPU_OK;
@@ -145,9 +148,9 @@ int forward(const xrgpu_int8_problem* c, void* ws, uint64_t ws_bytes, cudaStream
   p.b = c->b;
   p.b_scales = c->b_scales;
   p.bias = c->bias;
-  p.offsets = c->offsets;
   p.y = c->y;
   p.err = device_error_word();
+  if (in_place) return launched(launch_int8_few(p, c->a, c->a_dtype == XRGPU_FLOAT16, c->lda ? c->lda : c->K, s));
   if (p.rows) {
     const RowOrder from{c->order, c->order ? static_cast<int>(c->top_k) : 1, c->M, p.err};
     const bool made = c->a_dtype != XRGPU_INT8 || c->order;  // the operand, by a kernel before the product's
@@ -224,7 +227,8 @@ int xrgpu_int8_dequantize(const xrgpu_int8_tensor* t, void* out, void* stream) {
 int xrgpu_int8_workspace_size(const xrgpu_int8_problem* c, uint64_t* bytes) {
   xrgpu::Int8Matmul p{};
   xrgpu::Layout l{};
-  const int st = xrgpu::check(c, &p, &l);
+  bool in_place;
+  const int st = xrgpu::check(c, &p, &l, &in_place);
   if (st) return st;
   if (bytes) *bytes = l.bytes;
   return XRGPU_OK;

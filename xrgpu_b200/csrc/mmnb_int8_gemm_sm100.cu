@@ -21,6 +21,7 @@
 
 #include <climits>
 
+#include "mmnb_int8.cuh"
 #include "mmnb_int8.h"
 #include "mmnb_tcgen05.cuh"
 
@@ -261,6 +262,44 @@ __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_
   }
 }
 
+// A split tile's sums over the cluster's ranks (128 values of a column lie together at `base` of each): every rank takes its
+// share of the columns. All threads.
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t base, int rank, const float* row_scale) {
+  const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, mine = max(0, min(share, t.rows - col0));
+  const bool relu = a.act == XRGPU_ACT_RELU;
+  for (int e = threadIdx.x; e < mine * (kRows / 4); e += kThreads) {
+    const int col = col0 + e / (kRows / 4), row = 4 * (e % (kRows / 4)), n = t.pt * kRows + row;
+    int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < a.split) {
+        const float4 v = ld_cluster_f32x4(map_rank(base + (col * kPitch + row) * 4, k));
+        sum[0] += __float_as_int(v.x);
+        sum[1] += __float_as_int(v.y);
+        sum[2] += __float_as_int(v.z);
+        sum[3] += __float_as_int(v.w);
+      }
+    float f[4];
+    const float sa = row_scale[col];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t ch = static_cast<int64_t>(t.group) * a.n + n + i;
+      const bool in = n + i < a.n;
+      f[i] = scaled(sum[i], sa, in ? a.b_scales[ch] : 0.0f, in && a.bias ? load_f(a.bias, a.bias_f16, ch) : 0.0f, relu);
+    }
+    const int64_t at = static_cast<int64_t>(t.row0 + col) * a.ldy;
+    if (SWIGLU) {
+      if (n < a.n) put<F16>(a.y, at + (n >> 1), swiglu(a, f[0], f[1]));
+      if (n + 2 < a.n) put<F16>(a.y, at + (n >> 1) + 1, swiglu(a, f[2], f[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.n) put<F16>(a.y, at + n + i, f[i]);
+    }
+  }
+}
+
 template <bool F16, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
@@ -432,44 +471,269 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (a.split > 1) {
     // one tile a cluster: every rank sums its share of the columns over the ranks (128 values of a column lie together)
     cluster_sync();
-    if (first < tiles && !*ctl.abort) {
-      const Tile t = tile_at<16>(a, tables, first);
-      const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, mine = max(0, min(share, t.rows - col0));
-      const bool relu = a.act == XRGPU_ACT_RELU;
-      for (int e = threadIdx.x; e < mine * (kRows / 4); e += kThreads) {
-        const int col = col0 + e / (kRows / 4), row = 4 * (e % (kRows / 4)), n = t.pt * kRows + row;
-        int sum[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < a.split) {
-            const float4 v = ld_cluster_f32x4(map_rank(base + (col * kPitch + row) * 4, k));
-            sum[0] += __float_as_int(v.x);
-            sum[1] += __float_as_int(v.y);
-            sum[2] += __float_as_int(v.z);
-            sum[3] += __float_as_int(v.w);
-          }
-        float f[4];
-        const float sa = row_scale[0][col];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t ch = static_cast<int64_t>(t.group) * a.n + n + i;
-          const bool in = n + i < a.n;
-          f[i] = scaled(sum[i], sa, in ? a.b_scales[ch] : 0.0f, in && a.bias ? load_f(a.bias, a.bias_f16, ch) : 0.0f, relu);
-        }
-        const int64_t at = static_cast<int64_t>(t.row0 + col) * a.ldy;
-        if (SWIGLU) {
-          if (n < a.n) put<F16>(a.y, at + (n >> 1), swiglu(a, f[0], f[1]));
-          if (n + 2 < a.n) put<F16>(a.y, at + (n >> 1) + 1, swiglu(a, f[2], f[3]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < a.n) put<F16>(a.y, at + n + i, f[i]);
-        }
-      }
-    }
+    if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, tile_at<16>(a, tables, first), base, rank, row_scale[0]);
     cluster_sync();  // nobody leaves while its partial tile is being read
   }
   zero_rest<F16>(a, SWIGLU ? a.n / 2 : a.n);
+}
+
+// ------------------------------------------------------------------ few rows, quantised in place
+// A few float rows (decoded tokens) of a dense product, one tile a CTA: the CTA quantises its part of the rows itself, straight into
+// the swizzled layout that the MMAs read, while the weights' first stages arrive. No kernel before it, and no trip of the codes
+// through memory. Each CTA reads whole rows for their largest magnitudes (ranks that told each other theirs waited 6000 cycles
+// for the signal, behind the weights), so this is for few values: a part of 512 a warp and time, four times.
+// Roles: warp 0 loads weights, warp 1 issues the MMAs, warps 2-9 quantise, then drain.
+constexpr int kFewRows = 16;
+constexpr int kFewStep = kFewRows * kStepBytes;  // codes of all rows, a stage's part of K
+constexpr int kFewPart = 32 * 16;                // values of a row that a warp takes at a time
+constexpr int kFewHeld = 4;                      // of these a warp
+constexpr uint32_t kFewStage = kRows * kStepBytes;
+constexpr unsigned kErrWaitRanks = 0x715;
+
+struct FewRows {
+  const void* x;
+  int64_t ldx, K;
+  int vec;         // rows of x start on 16 bytes
+  uint32_t codes, sums;  // bytes from the stages' start to the rows' codes, and to the sums sent by the ranks
+};
+
+template <bool XF16, bool VEC>
+struct Part {  // 16 values of a lane
+  static constexpr int kUnits = XF16 ? 2 : 4;
+  Unit<XF16, VEC> u[kUnits];
+  __device__ __forceinline__ void load(const FewRows& f, int64_t row, int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) u[i].load(f.x, row * f.ldx, k0 + i * Unit<XF16, VEC>::kValues, f.K);
+  }
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) m = max(m, u[i].amax());
+    return m;
+  }
+  __device__ __forceinline__ uint4 codes(const Scale& c, bool none) const {
+    uint32_t w[4 + 2];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) u[i].codes(c, w + i * (XF16 ? 2 : 1));
+    return none ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+struct FewShared {
+  uint64_t full[kMaxStages], empty[kMaxStages], ready, summed, accfull, done;
+  uint32_t largest[kFewRows];             // magnitudes of the rows, as bits
+  Scale scale[kEpilogueWarps][kFewRows];  // a copy a warp
+  float row_scale[kEpilogueWarps][kFewRows];
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+
+// The eight warps 2-9: the rows' scales, and the codes of the steps k0 .. k1 - 1.
+template <bool XF16, bool VEC>
+__device__ __forceinline__ void quantise_rows(const Args& a, const FewRows& f, int k0, int k1, FewShared& sh, uint32_t codes) {
+  const int warp = (threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
+  const int parts = (static_cast<int>(f.K) + kFewPart - 1) / kFewPart, items = a.rows * parts;
+  Part<XF16, VEC> held[kFewHeld];
+#pragma unroll
+  for (int i = 0; i < kFewHeld; ++i) {
+    const int item = warp + 8 * i, row = item / parts;
+    if (item < items) held[i].load(f, row, (item - row * parts) * kFewPart + lane * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < kFewHeld; ++i) {
+    const int item = warp + 8 * i;
+    if (item >= items) break;
+    const uint32_t m = __reduce_max_sync(~0u, held[i].amax());
+    if (lane == 0) atomicMax(&sh.largest[item / parts], m);
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");  // these eight warps, none of which leaves before
+  if (lane < kFewRows) {
+    Scale c;
+    bool none;
+    sh.row_scale[warp][lane] = row_scale_of<XF16>(sh.largest[lane], &c, &none);
+    if (none) c.up = 0.0f;  // marks rows whose codes are 0
+    sh.scale[warp][lane] = c;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kFewHeld; ++i) {
+    const int item = warp + 8 * i, row = item / parts, k = (item - row * parts) * kFewPart + lane * 16 - k0 * kStepBytes;
+    if (item >= items) break;
+    if (k < 0 || k >= (k1 - k0) * kStepBytes) continue;
+    const Scale c = sh.scale[warp][row];
+    const uint4 w = held[i].codes(c, c.up == 0.0f);
+    const uint32_t dst = codes + (k / kStepBytes) * kFewStep + row * kStepBytes + ((((k / 16) & 7) ^ (row & 7)) << 4);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+  }
+  fence_async_shared();
+  __syncwarp();
+}
+
+// A split tile's sums: every rank owns `share` of the rows. The warp that read 32 channels of this rank's sums sends each owner
+// its part, in the owner's order, waits for the parts of its own rows and adds them up. No rank waits for another to read.
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void exchange_sums(const Args& a, const Tile& t, const uint32_t (&v)[16], uint32_t sums, int rank, int q, int n,
+                                              const ChannelScale& ch, FewShared& sh, const float* row_scale, int lane, const Ctl& ctl) {
+  const int share = (t.rows + a.split - 1) / a.split, owners = (t.rows + share - 1) / share;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if (j >= t.rows) break;
+    const int owner = j / share;  // at [rank][row of the owner][channel]
+    st_cluster_u32(map_rank(sums + ((rank * share + j - owner * share) * kRows + 32 * q + lane) * 4, owner), v[j]);
+  }
+  __syncwarp();
+  if (lane < owners) arrive_at(&sh.summed, lane);
+  if (rank >= owners) return;
+  if (!warp_wait(&sh.summed, 0, ctl, kErrWaitRanks) || !__all_sync(~0u, acquire_cluster(&sh.summed, 0))) return;
+  float f[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) f[j] = 0.0f;
+  const int mine = min(share, t.rows - rank * share);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if (j >= mine) break;
+    int sum = 0;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      uint32_t x = 0;
+      if (r < a.split) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(sums + ((r * share + j) * kRows + 32 * q + lane) * 4) : "memory");
+      sum += static_cast<int>(x);
+    }
+    f[j] = scaled(sum, row_scale[rank * share + j], ch.scale, ch.bias, a.act == XRGPU_ACT_RELU);
+  }
+  store_columns<F16, SWIGLU>(a, f, rank * share, 0, mine, n, lane);
+}
+
+template <bool F16, bool SWIGLU, bool XF16>
+__global__ void __launch_bounds__(kThreads, 1) int8_few_kernel(const __grid_constant__ CUtensorMap map_p, const Args a, const FewRows f) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ FewShared sh;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int S = a.stages;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0, pt = blockIdx.x / a.split;
+  const Tile t{0, pt, 0, a.rows, kFewRows};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], 1);
+    }
+    mbar_init(&sh.ready, kEpilogueWarps);
+    mbar_init(&sh.summed, 4 * a.split);
+    mbar_init(&sh.accfull, 1);
+    mbar_init(&sh.done, 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x < kFewRows) sh.largest[threadIdx.x] = 0;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)), "r"(32) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_slot);
+  const Ctl ctl{&sh.abort_flag, a.err};
+  const int k0 = static_cast<int>(static_cast<int64_t>(a.ksteps) * rank / a.split);
+  const int k1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.split), steps = k1 - k0;
+  const uint32_t codes = base + f.codes, sums = base + f.sums;
+  bool waited = false;  // for the cluster's barrier
+  // All ranks' barriers have to be there before the first signal, which comes from the draining warps.
+  if (a.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load = [&](int i, int s) {
+        mbar_arrive_expect_tx(&sh.full[s], kRows * kStepBytes);
+        tma_load_2d(base + s * kFewStage, &map_p, (k0 + i) * kStepBytes, pt * kRows, &sh.full[s]);
+      };
+      int i = 0, s = 0;
+      uint32_t ph = 1;
+      for (; i < steps; ++i) {
+        if (!thread_wait(&sh.empty[s], ph, ctl, kErrWaitProducer)) break;
+        load(i, s);
+        if (++s == S) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (i < steps)
+        for (int h = (i > S ? i - S : 0); h < i; ++h) drain_wait(&sh.full[h % S], (h / S) & 1, a.err, kErrDrain);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(codes);
+    const uint32_t i_desc = instruction_desc(kRows, kFewRows);
+    bool ok = warp_spin(&sh.ready, 0, ctl, kErrWaitMma);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = 0; ok && i < steps; ++i) {
+      if (!warp_spin(&sh.full[s], ph, ctl, kErrWaitMma)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int subs = a.ksubs - 4 * (k0 + i);
+      const uint32_t p_off = static_cast<uint32_t>(s) * (kFewStage >> 4), q_off = static_cast<uint32_t>(i) * (kFewStep >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j > 0 && j >= subs) break;
+          mma_i8(tmem, p_desc + p_off + 2 * j, q_desc + q_off + 2 * j, i_desc, i > 0 || j > 0);
+        }
+        mma_commit(&sh.empty[s]);
+      }
+      __syncwarp();
+      if (++s == S) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    if (ok && elect_one()) mma_commit(&sh.accfull);
+    __syncwarp();
+    if (elect_one()) mma_commit(&sh.done);
+    __syncwarp();
+    drain_wait(&sh.done, 0, a.err, kErrDrain);
+  } else {
+    const int q = warp & 3, c = (warp - 2) >> 2, n = pt * kRows + 32 * q + lane;
+    if (f.vec) quantise_rows<XF16, true>(a, f, k0, k1, sh, codes);
+    else quantise_rows<XF16, false>(a, f, k0, k1, sh, codes);
+    if (lane == 0) mbar_arrive(&sh.ready);
+    __syncwarp();
+    if (c == 0) {
+      ChannelScale ch{0.0f, 0.0f};
+      if (n < a.n) {
+        ch.scale = a.b_scales[n];
+        if (a.bias) ch.bias = load_f(a.bias, a.bias_f16, n);
+      }
+      const float* scale = sh.row_scale[warp - 2];
+      if (warp_wait(&sh.accfull, 0, ctl, kErrWaitEpilogue)) {
+        tc_fence_after();
+        const uint32_t acc = tmem + (static_cast<uint32_t>(32 * q) << 16);
+        if (a.split > 1) {
+          uint32_t v[16];
+          tmem_ld16(acc, v);
+          tmem_wait_ld16(v);
+          waited = true;
+          asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+          exchange_sums<F16, SWIGLU>(a, t, v, sums, rank, q, n, ch, sh, scale, lane, ctl);
+        } else {
+          drain_tile<F16, SWIGLU>(a, t, acc, 0, n, ch, scale, lane);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (a.split > 1 && !waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(32) : "memory");
+  }
+  // After a wait that ran out another rank may still send to this one: stay until the others have left, or are here too.
+  if (a.split > 1 && *ctl.abort) cluster_sync();
 }
 
 // ------------------------------------------------------------------ pairs of CTAs
@@ -747,20 +1011,56 @@ void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& 
   l.grid = static_cast<int>(a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms));
 }
 
-// Pairs take what needs a second round of single CTAs and has tiles wide enough.
-bool pairs_pay(const Int8Matmul& p, int64_t tiles, int tmax, int sms) { return tmax >= 128 && tiles > sms; }
+// Split of K and stages of the kernel for few float rows; false where it does not take the call: one tile a CTA, rows that its warps
+// hold at once.
+bool few_shape(const Int8Matmul& p, int sms, Args& a, FewRows& f, Launch& l) {
+  if (p.offsets || p.rows > kFewRows || p.rows * ceil_div(p.K, kFewPart) > kEpilogueWarps * kFewHeld) return false;
+  const int64_t tiles = ceil_div(p.N, kRows);
+  if (tiles > sms) return false;
+  a.split = 1;
+  while (a.split < 8 && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2;
+  const int64_t steps = ceil_div(a.ksteps, a.split), rows = steps * kFewStep;
+  // a rank's sums: [ranks][its share of the rows][channels]
+  const int64_t sums = a.split > 1 ? a.split * ceil_div(p.rows, a.split) * kRows * 4 : 0;
+  int64_t stages = (kSmemBudget - 1024 - rows - sums) / kFewStage;
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (stages > steps) stages = steps;
+  if (stages < steps && stages < 6) return false;  // long rows: their codes leave too little for the weights
+  a.stages = static_cast<int>(stages);
+  a.p_tiles = static_cast<int>(tiles);
+  f.codes = static_cast<uint32_t>(stages) * kFewStage;
+  f.sums = f.codes + static_cast<uint32_t>(rows);
+  l.smem = f.sums + static_cast<size_t>(sums) + 1024;
+  l.split = a.split;
+  l.grid = static_cast<int>(tiles * a.split);
+  return true;
+}
 
-}  // namespace
+template <bool F16, bool SWIGLU, bool XF16>
+cudaError_t launch_few(const Launch& l, const Args& a, const FewRows& f, cudaStream_t s) {
+  cudaError_t e = allow_smem<int8_few_kernel<F16, SWIGLU, XF16>>(kSmemBudget);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(l.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = l.smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = l.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = l.split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, int8_few_kernel<F16, SWIGLU, XF16>, l.p, a, f);
+}
 
-cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) {
-  const int sms = device_sm_count();
+Args arguments(const Int8Matmul& p) {
   Args a{};
   a.n = static_cast<int>(p.N);
   a.groups = p.groups;
   a.rows = static_cast<int>(p.rows);
   a.ksubs = static_cast<int>(ceil_div(p.K, 32));
   a.ksteps = (a.ksubs + 3) / 4;
-  a.early = early;
   a.act = p.act;
   a.has_limit = p.has_limit;
   a.zero_rest = p.zero_rest;
@@ -776,6 +1076,39 @@ cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) 
   a.ldy = p.ldy;
   a.vec = reinterpret_cast<uintptr_t>(p.y) % 4 == 0 && p.ldy % 2 == 0;
   a.err = p.err;
+  return a;
+}
+
+// Pairs take what needs a second round of single CTAs and has tiles wide enough.
+bool pairs_pay(const Int8Matmul& p, int64_t tiles, int tmax, int sms) { return tmax >= 128 && tiles > sms; }
+
+}  // namespace
+
+bool int8_few_rows(const Int8Matmul& p) {
+  Args a = arguments(p);
+  FewRows f{};
+  Launch l{};
+  return few_shape(p, device_sm_count(), a, f, l);
+}
+
+cudaError_t launch_int8_few(const Int8Matmul& p, const void* x, bool x_f16, int64_t ldx, cudaStream_t s) {
+  Args a = arguments(p);
+  FewRows f{x, ldx, p.K, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_f16 ? 2 : 4) % 16 == 0, 0, 0};
+  Launch l{};
+  if (!few_shape(p, device_sm_count(), a, f, l) || !encode_tensor_map_2d(&l.p, 0, p.b, p.K, p.N, p.ldb, kStepBytes, kRows, true)) return cudaErrorInvalidValue;
+  const bool swiglu = p.act == XRGPU_ACT_SWIGLU;
+  if (p.f16) {
+    if (swiglu) return x_f16 ? launch_few<true, true, true>(l, a, f, s) : launch_few<true, true, false>(l, a, f, s);
+    return x_f16 ? launch_few<true, false, true>(l, a, f, s) : launch_few<true, false, false>(l, a, f, s);
+  }
+  if (swiglu) return x_f16 ? launch_few<false, true, true>(l, a, f, s) : launch_few<false, true, false>(l, a, f, s);
+  return x_f16 ? launch_few<false, false, true>(l, a, f, s) : launch_few<false, false, false>(l, a, f, s);
+}
+
+cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) {
+  const int sms = device_sm_count();
+  Args a = arguments(p);
+  a.early = early;
 
   // Rows of a tile at the most: all of a dense product with few of them; twice a group's mean, so that most groups take one.
   const int64_t mean = ceil_div(p.rows, p.groups), want = p.offsets ? 2 * mean + 8 : mean;

@@ -627,6 +627,15 @@ def _code_rows(t: torch.Tensor, name: str, index: int) -> int:
     return step
 
 
+def _empty(shape, dtype, like: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor beside `like` (``empty_strided`` takes 0.5 us less than ``new_empty``)."""
+    stride, step = [0] * len(shape), 1
+    for d in range(len(shape) - 1, -1, -1):
+        stride[d] = step
+        step *= shape[d] or 1
+    return torch.empty_strided(shape, stride, dtype=dtype, device=like.device)
+
+
 def _small(t: torch.Tensor, name: str, dtype, shape, index: int):
     _on(t, name, dtype, index)
     if t.shape != shape:
@@ -647,8 +656,8 @@ def int8_quantize(x: torch.Tensor):
     if K < 1:
         raise ValueError("x must be [..., K] with K >= 1")
     ld, lead = -(-K // 16) * 16, x.shape[:-1]
-    codes = x.new_empty((*lead, ld), dtype=torch.int8)
-    scales = x.new_empty(lead, dtype=torch.float32)
+    codes = _empty((*lead, ld), torch.int8, x)
+    scales = _empty(lead, torch.float32, x)
     t = _native.Int8Tensor_(dtype, 0, scales.numel(), K, ld, codes.data_ptr(), scales.data_ptr())
     _launch(index, _native.load().xrgpu_int8_quantize, ctypes.byref(t), x.data_ptr(), _row_stride(x, "x"))
     return (codes if ld == K else codes[..., :K]), scales
@@ -661,7 +670,7 @@ def int8_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, dtype=torch.fl
     code, index = _float_code(dtype), _device_of(codes, "codes")
     ld = _code_rows(codes, "codes", index)
     s = _small(scales, "scales", torch.float32, codes.shape[:-1], index)
-    out = codes.new_empty(codes.shape, dtype=dtype)
+    out = _empty(codes.shape, dtype, codes)
     t = _native.Int8Tensor_(code, 0, scales.numel(), codes.shape[-1], ld, codes.data_ptr(), s)
     _launch(index, _native.load().xrgpu_int8_dequantize, ctypes.byref(t), out.data_ptr())
     return out
@@ -698,17 +707,15 @@ def _int8_problem(a, a_scales, b, b_scales, bias, activation, alpha, beta, limit
 def _int8_forward(p, index: int, out: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
     lib = _native.load()
     p.y = out.data_ptr()
-    need = ctypes.c_uint64(0)
-    check(lib.xrgpu_int8_workspace_size(ctypes.byref(p), ctypes.byref(need)))
-    nbytes = need.value
-    ws = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch(index, lib.xrgpu_int8_forward, ctypes.byref(p), ws.data_ptr() if nbytes else None, nbytes)
+    need = _workspace_bytes(index, lib.xrgpu_int8_workspace_size, p)
+    ws = _empty((need,), torch.uint8, a) if need else None
+    _launch(index, lib.xrgpu_int8_forward, ctypes.byref(p), ws.data_ptr() if need else None, need)
     return out
 
 
 def _int8_out(p, out, shape, dtype, a, index: int):
     if out is None:
-        return a.new_empty(shape, dtype=dtype)
+        return _empty(shape, dtype, a)
     if out.dtype != dtype or out.get_device() != index or out.shape != shape:
         raise ValueError(f"out must be {list(shape)} in the output dtype on a's device")
     p.ldy = _row_stride(out, "out")
@@ -761,16 +768,13 @@ def moe_route(scores: torch.Tensor, k: int, *, normalize: bool = True) -> MoeRou
     if not 1 <= k <= min(E, 32) or E > 1024:
         raise ValueError("a router takes up to 1024 experts and a top_k of up to 32 of them")
     lds = _row_stride(scores, "scores")
-    experts = scores.new_empty((T, k), dtype=torch.int32)
-    weights = scores.new_empty((T, k), dtype=torch.float32)
-    order = scores.new_empty(T * k, dtype=torch.int32)
-    slots = torch.empty_like(experts)
-    offsets = scores.new_empty(E + 1, dtype=torch.int32)
+    experts, weights, slots = _empty((T, k), torch.int32, scores), _empty((T, k), torch.float32, scores), _empty((T, k), torch.int32, scores)
+    order, offsets = _empty((T * k,), torch.int32, scores), _empty((E + 1,), torch.int32, scores)
     p = _native.MoeRouteProblem_(code, int(bool(normalize)), T, E, k, lds, scores.data_ptr(), experts.data_ptr(), weights.data_ptr(),
                                  order.data_ptr(), slots.data_ptr(), offsets.data_ptr())
     lib = _native.load()
     need = _workspace_bytes(index, lib.xrgpu_moe_route_workspace_size, p)
-    ws = scores.new_empty(need, dtype=torch.uint8) if need else None
+    ws = _empty((need,), torch.uint8, scores) if need else None
     _launch(index, lib.xrgpu_moe_route, ctypes.byref(p), ws.data_ptr() if need else None, need)
     return MoeRoute(experts, weights, order, slots, offsets)
 
