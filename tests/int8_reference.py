@@ -35,7 +35,8 @@ def swiglu(g, l, alpha=1.0, beta=0.0, limit=None):
 
 def product(a, sa, b, sb, bias=None, act="none", alpha=1.0, beta=0.0, limit=None):
     """Codes a [M, K], b [N, K] with scales -> (y, bound of the float32 steps before the last rounding), float64."""
-    t = (np.asarray(a, np.int64) @ np.asarray(b, np.int64).T).astype(np.float64) * np.asarray(sa, np.float64)[:, None] * np.asarray(sb, np.float64)
+    # whole numbers below 2^53: exact in any order
+    t = (np.asarray(a, np.float64) @ np.asarray(b, np.float64).T) * np.asarray(sa, np.float64)[:, None] * np.asarray(sb, np.float64)
     y = t if bias is None else t + np.asarray(bias, np.float64)
     # the sum, two scales and the bias: three roundings of the term, one of the result
     err = 3 * EPS * np.abs(t) + EPS * np.abs(y) + 2.0 ** -148

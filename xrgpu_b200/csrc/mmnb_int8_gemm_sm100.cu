@@ -20,6 +20,7 @@
 #include <cuda_fp16.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "mmnb_int8.cuh"
 #include "mmnb_int8.h"
@@ -60,7 +61,6 @@ struct Args {
   const void* bias;
   void* y;
   int64_t ldy;
-  int vec;                     // pairs of y start on their size
   unsigned* err;
 };
 
@@ -150,8 +150,8 @@ __device__ __forceinline__ Tile tile_at(const Args& a, const Tables& t, int tile
   }
   const int first = t.tile_first[lo], nt = t.tile_first[lo + 1] - first, count = t.row_count[lo];
   const int local = tile - first * a.p_tiles, pt = local / nt, qt = local - pt * nt;
-  const int even = (count + nt - 1) / nt, width = (even + GRAIN - 1) / GRAIN * GRAIN;
-  return {lo, pt, t.row_first[lo] + qt * width, min(width, count - qt * width), width};
+  const int even = ((count + nt - 1) / nt + GRAIN - 1) / GRAIN * GRAIN, rows = min(even, count - qt * even);
+  return {lo, pt, t.row_first[lo] + qt * even, rows, (rows + GRAIN - 1) / GRAIN * GRAIN};
 }
 
 // ------------------------------------------------------------------ results
@@ -173,48 +173,9 @@ __device__ __forceinline__ float swiglu(const Args& a, float g, float l) {
   return g * s * (l + a.beta);
 }
 
-// 16 columns (rows row0 + col0 + j of y) of the lane's channel n, scaled already. All lanes of the warp take part.
-template <bool F16, bool SWIGLU>
-__device__ __forceinline__ void store_columns(const Args& a, const float (&f)[16], int row0, int col0, int rows, int n, int lane) {
-  const bool odd = lane & 1;
-  if (SWIGLU) {
-    // A channel's neighbour holds the other half of its pair: even lanes take the even columns, odd lanes the odd ones.
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const float other = __shfl_xor_sync(~0u, odd ? f[j] : f[j + 1], 1);
-      const float r = swiglu(a, odd ? other : f[j], odd ? f[j + 1] : other);
-      const int c = col0 + j + (odd ? 1 : 0);
-      if (c < rows && n < a.n) put<F16>(a.y, static_cast<int64_t>(row0 + c) * a.ldy + (n >> 1), r);
-    }
-  } else if (F16) {
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const float other = __shfl_xor_sync(~0u, odd ? f[j] : f[j + 1], 1);
-      const __half2 h = odd ? __floats2half2_rn(other, f[j + 1]) : __floats2half2_rn(f[j], other);
-      const int c = col0 + j + (odd ? 1 : 0), n0 = n & ~1;
-      if (c >= rows || n0 >= a.n) continue;
-      __half* dst = static_cast<__half*>(a.y) + static_cast<int64_t>(row0 + c) * a.ldy + n0;
-      if (a.vec && n0 + 1 < a.n) {
-        *reinterpret_cast<__half2*>(dst) = h;
-      } else {
-        dst[0] = __low2half(h);
-        if (n0 + 1 < a.n) dst[1] = __high2half(h);
-      }
-    }
-  } else if (n < a.n) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if (col0 + j >= rows) break;
-      static_cast<float*>(a.y)[static_cast<int64_t>(row0 + col0 + j) * a.ldy + n] = f[j];
-    }
-  }
-}
-
 // Product first with the token's, then with the channel's scale: an int32 and two float32 numbers, each step rounded to 2^-24.
-__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias, bool relu) {
-  const float r = fmaf(static_cast<float>(acc) * sa, sb, bias);
-  return relu && !(r > 0.0f) && r == r ? 0.0f : r;
-}
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias) { return fmaf(static_cast<float>(acc) * sa, sb, bias); }
+__device__ __forceinline__ float relu(float r) { return r < 0.0f ? 0.0f : r; }  // a NaN stays
 
 // Rows of no group (before the first offset, behind the last) become zero.
 template <bool F16>
@@ -230,14 +191,18 @@ __device__ __forceinline__ void zero_rest(const Args& a, int width) {
 struct ChannelScale {
   float scale, bias;
 };
-// The scales of a tile's rows into the warp's `row_scale`, and the lane's channel's.
-__device__ __forceinline__ ChannelScale prepare_scales(const Args& a, const Tile& t, int n, float* row_scale, int lane) {
+__device__ __forceinline__ ChannelScale channel_scale(const Args& a, int group, int n) {
   ChannelScale ch{0.0f, 0.0f};
   if (n < a.n) {
-    const int64_t at = static_cast<int64_t>(t.group) * a.n + n;
+    const int64_t at = static_cast<int64_t>(group) * a.n + n;
     ch.scale = a.b_scales[at];
     if (a.bias) ch.bias = load_f(a.bias, a.bias_f16, at);
   }
+  return ch;
+}
+// The scales of a tile's rows into the warp's `row_scale`, and the lane's channel's.
+__device__ __forceinline__ ChannelScale prepare_scales(const Args& a, const Tile& t, int n, float* row_scale, int lane) {
+  const ChannelScale ch = channel_scale(a, t.group, n);
   float scale[kMaxT / 32];  // all loads before the first use: one after the other they take 800 cycles each
 #pragma unroll
   for (int i = 0; i < kMaxT / 32; ++i) scale[i] = 32 * i + lane < t.rows ? a.a_scales[t.row0 + 32 * i + lane] : 0.0f;
@@ -248,6 +213,68 @@ __device__ __forceinline__ ChannelScale prepare_scales(const Args& a, const Tile
   return ch;
 }
 
+// Results of 16 columns of the lane's channel, as y holds them: float16 two a word, in the order of the columns. With swiglu a lane has
+// every other column of its pair of channels: even lanes the even columns, odd lanes the odd ones.
+template <bool F16, bool SWIGLU>
+constexpr int kWords = (SWIGLU ? 8 : 16) / (F16 ? 2 : 1);
+
+// All lanes of the warp take part; the columns' row scales are at `row_scale`.
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void results(const Args& a, const uint32_t (&v)[16], const ChannelScale& ch, const float* row_scale, int lane, uint32_t (&w)[kWords<F16, SWIGLU>]) {
+  float f[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) f[j] = scaled(static_cast<int>(v[j]), row_scale[j], ch.scale, ch.bias);
+  if (SWIGLU) {
+    const bool odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float other = __shfl_xor_sync(~0u, odd ? f[j] : f[j + 1], 1);
+      f[j / 2] = swiglu(a, odd ? other : f[j], odd ? f[j + 1] : other);
+    }
+  } else if (a.act == XRGPU_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = relu(f[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kWords<F16, SWIGLU>; ++j) {
+    if (F16) {
+      const __half2 h = __floats2half2_rn(f[2 * j], f[(2 * j + 1) & 15]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      w[j] = __float_as_uint(f[j]);
+    }
+  }
+}
+
+// They go to rows row0 + col0 + j of y, each by itself, 64 or 128 bytes a warp. (Pairs of channels, joined by shuffles, would make
+// half as many stores of as many rows of y each: 11700 cycles for 128 channels by 256 rows, 6400 by single ones; 4000 of these are
+// the stores' own.)
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void store_results(const Args& a, const uint32_t (&w)[kWords<F16, SWIGLU>], int row0, int col0, int rows, int n, int lane) {
+  using T = typename std::conditional<F16, uint16_t, uint32_t>::type;
+  constexpr int kStep = SWIGLU ? 2 : 1;
+  if (n >= a.n) return;
+  const int odd = SWIGLU ? lane & 1 : 0, left = rows - col0 - odd;
+  T* y = static_cast<T*>(a.y) + static_cast<int64_t>(row0 + col0 + odd) * a.ldy + (SWIGLU ? n >> 1 : n);
+  auto value = [&](int i) { return static_cast<T>(F16 ? w[i >> 1] >> (16 * (i & 1)) : w[i & (kWords<F16, SWIGLU> - 1)]); };
+  if (left > 15) {
+#pragma unroll
+    for (int j = 0; j < 16; j += kStep, y += kStep * a.ldy) *y = value(j / kStep);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j += kStep, y += kStep * a.ldy)
+      if (j < left) *y = value(j / kStep);
+  }
+}
+
+// 16 columns of a tile's sums, from column `col` on with the rows' scales at `row_scale`, to y.
+template <bool F16, bool SWIGLU>
+__device__ __forceinline__ void store_chunk(const Args& a, const Tile& t, const uint32_t (&v)[16], int col, int n, const ChannelScale& ch, const float* row_scale, int lane) {
+  uint32_t w[kWords<F16, SWIGLU>];
+  results<F16, SWIGLU>(a, v, ch, row_scale, lane, w);
+  store_results<F16, SWIGLU>(a, w, t.row0, col, t.rows, n, lane);
+}
+
 // The warp's chunks of a tile's sums, from tensor memory to y.
 template <bool F16, bool SWIGLU>
 __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_t tmem, int c, int n, const ChannelScale& ch, const float* row_scale, int lane) {
@@ -255,10 +282,7 @@ __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_
     uint32_t v[16];
     tmem_ld16(tmem + col, v);
     tmem_wait_ld16(v);
-    float f[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = scaled(static_cast<int>(v[j]), row_scale[col + j], ch.scale, ch.bias, a.act == XRGPU_ACT_RELU);
-    store_columns<F16, SWIGLU>(a, f, t.row0, col, t.rows, n, lane);
+    store_chunk<F16, SWIGLU>(a, t, v, col, n, ch, row_scale + col, lane);
   }
 }
 
@@ -267,7 +291,6 @@ __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_
 template <bool F16, bool SWIGLU>
 __device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t base, int rank, const float* row_scale) {
   const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, mine = max(0, min(share, t.rows - col0));
-  const bool relu = a.act == XRGPU_ACT_RELU;
   for (int e = threadIdx.x; e < mine * (kRows / 4); e += kThreads) {
     const int col = col0 + e / (kRows / 4), row = 4 * (e % (kRows / 4)), n = t.pt * kRows + row;
     int sum[4] = {0, 0, 0, 0};
@@ -286,7 +309,8 @@ __device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t
     for (int i = 0; i < 4; ++i) {
       const int64_t ch = static_cast<int64_t>(t.group) * a.n + n + i;
       const bool in = n + i < a.n;
-      f[i] = scaled(sum[i], sa, in ? a.b_scales[ch] : 0.0f, in && a.bias ? load_f(a.bias, a.bias_f16, ch) : 0.0f, relu);
+      f[i] = scaled(sum[i], sa, in ? a.b_scales[ch] : 0.0f, in && a.bias ? load_f(a.bias, a.bias_f16, ch) : 0.0f);
+      if (a.act == XRGPU_ACT_RELU) f[i] = relu(f[i]);
     }
     const int64_t at = static_cast<int64_t>(t.row0 + col) * a.ldy;
     if (SWIGLU) {
@@ -523,7 +547,7 @@ struct FewShared {
   uint64_t full[kMaxStages], empty[kMaxStages], ready, summed, accfull, done;
   uint32_t largest[kFewRows];             // magnitudes of the rows, as bits
   Scale scale[kEpilogueWarps][kFewRows];  // a copy a warp
-  float row_scale[kEpilogueWarps][kFewRows];
+  float row_scale[kEpilogueWarps][2 * kFewRows];  // a rank reads 16 from its first row on
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -551,6 +575,7 @@ __device__ __forceinline__ void quantise_rows(const Args& a, const FewRows& f, i
     Scale c;
     bool none;
     sh.row_scale[warp][lane] = row_scale_of<XF16>(sh.largest[lane], &c, &none);
+    sh.row_scale[warp][kFewRows + lane] = 0.0f;
     if (none) c.up = 0.0f;  // marks rows whose codes are 0
     sh.scale[warp][lane] = c;
   }
@@ -585,23 +610,20 @@ __device__ __forceinline__ void exchange_sums(const Args& a, const Tile& t, cons
   if (lane < owners) arrive_at(&sh.summed, lane);
   if (rank >= owners) return;
   if (!warp_wait(&sh.summed, 0, ctl, kErrWaitRanks) || !__all_sync(~0u, acquire_cluster(&sh.summed, 0))) return;
-  float f[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) f[j] = 0.0f;
   const int mine = min(share, t.rows - rank * share);
+  uint32_t sum[16] = {};
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     if (j >= mine) break;
-    int sum = 0;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       uint32_t x = 0;
       if (r < a.split) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(sums + ((r * share + j) * kRows + 32 * q + lane) * 4) : "memory");
-      sum += static_cast<int>(x);
+      sum[j] += x;
     }
-    f[j] = scaled(sum, row_scale[rank * share + j], ch.scale, ch.bias, a.act == XRGPU_ACT_RELU);
   }
-  store_columns<F16, SWIGLU>(a, f, rank * share, 0, mine, n, lane);
+  // this rank's rows, as a tile of their own (scales behind them are those of no row)
+  store_chunk<F16, SWIGLU>(a, {0, t.pt, rank * share, mine, kFewRows}, sum, 0, n, ch, row_scale + rank * share, lane);
 }
 
 template <bool F16, bool SWIGLU, bool XF16>
@@ -702,11 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_few_kernel(const __grid_cons
     if (lane == 0) mbar_arrive(&sh.ready);
     __syncwarp();
     if (c == 0) {
-      ChannelScale ch{0.0f, 0.0f};
-      if (n < a.n) {
-        ch.scale = a.b_scales[n];
-        if (a.bias) ch.bias = load_f(a.bias, a.bias_f16, n);
-      }
+      const ChannelScale ch = channel_scale(a, 0, n);
       const float* scale = sh.row_scale[warp - 2];
       if (warp_wait(&sh.accfull, 0, ctl, kErrWaitEpilogue)) {
         tc_fence_after();
@@ -739,12 +757,17 @@ __global__ void __launch_bounds__(kThreads, 1) int8_few_kernel(const __grid_cons
 // ------------------------------------------------------------------ pairs of CTAs
 // For many rows: a cluster of two CTAs on 256 channels by up to 256 rows. Each holds 128 of the channels and half of the rows; the
 // first one's MMAs (cta_group::2) read both halves from both shared memories, so that a CTA loads 256 rows a step instead of
-// 384 for the same product. Each CTA keeps the sums of its own channels, two accumulators of 256 columns, and drains them as
-// the kernel above does.
-// Signals between the two. Both CTAs' loads complete on the first one's `full`, which expects the bytes of both; the MMAs' completion goes to both. The second CTA's epilogue warps meet at its own `drained`,
-// and its warp 1 passes that on with a release at cluster scope. What the first CTA waits for it acquires at cluster scope.
+// 384 for the same product. Each CTA keeps the sums of its own channels, two accumulators that it drains in turns, under the next
+// tile's MMAs. The tiles of a last round that has too few for all pairs are cut into two or four.
+// What bounds these products are the loads from L2, about 49 bytes a cycle and SM: a stage, 32 KB a CTA, takes 670 to 700 cycles of the
+// 512 of its MMAs. Tiles of 512 rows (48 KB a stage, 1024 cycles, then bound by the MMAs) need both accumulators at once, and lost
+// in waiting for the drain what they won: 2048 x 14336 x 4096 91 us against 89 to 96, with swiglu 104 against 94 to 101.
+// Signals between the two. Both CTAs' loads complete on the first one's `full`, which expects the bytes of both; the MMAs'
+// completion goes to both. The second CTA's epilogue warps meet at its own `drained`, and its warp 1 passes that on with a release at
+// cluster scope. What the first CTA waits for it acquires at cluster scope.
 constexpr int kStages2 = 6;
-constexpr uint32_t kStage2 = 2 * kRows * kStepBytes;  // a CTA's bytes: channels, half of the rows
+constexpr uint32_t kPart2 = kRows * kStepBytes;  // a CTA's channels, or its rows
+constexpr uint32_t kStage2 = 2 * kPart2;
 
 __device__ __forceinline__ void mma2_i8(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -753,6 +776,26 @@ __device__ __forceinline__ void mma2_i8(uint32_t d, uint64_t a_desc, uint64_t b_
       "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// The line of tiles of `pairs` pairs: whole ones, then the pieces of the rest.
+struct Line {
+  int whole, cut, end;
+};
+__device__ __forceinline__ Line line_of(int tiles, int pairs) {
+  const int rest = tiles % pairs, cut = rest == 0 ? 1 : 4 * rest <= pairs ? 4 : 2 * rest <= pairs ? 2 : 1;
+  return {tiles - rest, cut, tiles - rest + rest * cut};
+}
+__device__ __forceinline__ Tile tile2_at(const Args& a, const Tables& tables, const Line& l, int i) {
+  const bool piece = i >= l.whole && l.cut > 1;
+  Tile t = tile_at<32>(a, tables, piece ? l.whole + (i - l.whole) / l.cut : i);
+  if (piece) {  // possibly an empty one
+    const int at = (i - l.whole) % l.cut, rows = ((t.rows + l.cut - 1) / l.cut + 31) / 32 * 32;
+    t.row0 += at * rows;
+    t.rows = max(0, min(rows, t.rows - at * rows));
+    t.width = (t.rows + 31) / 32 * 32;
+  }
+  return t;
 }
 
 template <bool F16, bool SWIGLU>
@@ -791,16 +834,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   const Ctl ctl{&abort_flag, a.err};
-  const int tiles = tables.tile_first[a.groups] * a.p_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const Line line = line_of(tables.tile_first[a.groups] * a.p_tiles, step);
 
   if (warp == 0) {
     int g = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true, waited = false;
-    for (int tile = first; ok && tile < tiles; tile += step) {
-      const Tile t = tile_at<32>(a, tables, tile);
-      const int copies = (t.width / 2 + a.box - 1) / a.box, q_row = t.row0 + rank * (t.width / 2);
-      const uint32_t bytes = 2 * (kRows + copies * a.box) * kStepBytes;
+    for (int tile = first; ok && tile < line.end; tile += step) {
+      const Tile t = tile2_at(a, tables, line, tile);
+      if (!t.rows) continue;
+      const int copies = (t.width / 2 + a.box - 1) / a.box, q_row = t.row0 + rank * (t.width / 2) + lane * a.box;
+      const uint32_t bytes = 2 * (kRows + copies * a.box) * kStepBytes, q_at = kPart2 + lane * a.box * kStepBytes;
       const int p_row = t.group * a.n + (2 * t.pt + rank) * kRows;
       auto load_p = [&](int st, int ks) {
         if (rank == 0) mbar_arrive_expect_tx(&full[st], bytes);
@@ -827,9 +872,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (lane == 0) load_p(s, ks);
           __syncwarp();
         }
-        if (lane < copies)
-          tma2_load_2d(base + s * kStage2 + (kRows + lane * a.box) * kStepBytes, &map_q, ks * kStepBytes, q_row + lane * a.box,
-                       map_rank(smem_u32(&full[s]), 0));
+        if (lane < copies) tma2_load_2d(base + s * kStage2 + q_at, &map_q, ks * kStepBytes, q_row, map_rank(smem_u32(&full[s]), 0));
         if (++s == kStages2) {
           s = 0;
           ph ^= 1;
@@ -841,13 +884,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1 && rank == 1) {
     // passes on that this CTA's accumulators have been read
     int i = 0;
-    for (int tile = first; tile < tiles; tile += step, ++i) {
+    for (int tile = first; tile < line.end; tile += step) {
+      if (!tile2_at(a, tables, line, tile).rows) continue;
       if (!warp_spin(&drained[i & 1], (i >> 1) & 1, ctl, kErrWaitMma)) break;
       if (lane == 0) arrive_at(&drained[i & 1], 0);
       __syncwarp();
+      ++i;
     }
   } else if (warp == 1) {
-    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kPart2);
     int i = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -855,8 +900,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return warp_spin(bar, parity, ctl, kErrWaitMma) && __all_sync(~0u, acquire_cluster(bar, parity));
     };
-    for (int tile = first; ok && tile < tiles; tile += step, ++i) {
-      const uint32_t i_desc = instruction_desc(2 * kRows, tile_at<32>(a, tables, tile).width);
+    for (int tile = first; ok && tile < line.end; tile += step) {
+      const Tile t = tile2_at(a, tables, line, tile);
+      if (!t.rows) continue;
+      const uint32_t i_desc = instruction_desc(2 * kRows, t.width);
       if (i >= 2 && !wait(&drained[i & 1], ((i - 2) >> 1) & 1)) break;
       tc_fence_after();
       const uint32_t d = tmem + ((i & 1) ? kMaxT : 0);
@@ -884,6 +931,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (ok && elect_one()) mma2_commit(&accfull[i & 1]);
       __syncwarp();
+      ++i;
     }
     if (elect_one()) mma2_commit(&done);
     __syncwarp();
@@ -893,8 +941,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int i = 0;
-    for (int tile = first; tile < tiles; tile += step, ++i) {
-      const Tile t = tile_at<32>(a, tables, tile);
+    for (int tile = first; tile < line.end; tile += step) {
+      const Tile t = tile2_at(a, tables, line, tile);
+      if (!t.rows) continue;
       const int b = i & 1, n = (2 * t.pt + rank) * kRows + 32 * q + lane;
       const ChannelScale ch = prepare_scales(a, t, n, row_scale[warp - 2], lane);
       if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
@@ -903,6 +952,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&drained[b]);
+      ++i;
     }
   }
 
@@ -946,7 +996,7 @@ struct Launch {
 
 template <auto Kernel>
 cudaError_t launch_kernel(const Launch& l, const Args& a, cudaStream_t s) {
-  cudaError_t e = allow_smem<Kernel>(kSmemBudget);
+  cudaError_t e = allow_smem<Kernel>(static_cast<int>(l.smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(l.grid);
@@ -977,10 +1027,12 @@ cudaError_t launch(const Launch& l, const Args& a, cudaStream_t s) {
 
 // Shared memory, stages, split of K and grid of single CTAs.
 void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& l) {
-  // K is split while the CTAs find an SM each (narrow tiles: 1.6 CTAs an SM, they run side by side).
-  const int64_t most = a.tmax <= 64 ? sms * 8 / 5 : sms;
+  // K is split while the CTAs find an SM each, over 8 only for narrow tiles. Measured (us, split 1 / 2 / 4 / 8): 16 x 4096 x 14336
+  // 35.4 / 21.9 / 16.1 / 15.7, 16 x 14336 x 4096 (112 tiles) 14.8 / 15.9 / 21.5, 128 x 4096 x 4096 16.1 / 14.5 / 12.0, 333 x 1003 x 4100 in
+  // tiles of 128 rows - / 15.1 / 11.2 / 13.2, of 256 - / 17.9 / 13.9 / 20.4.
+  const int most = a.tmax <= 32 ? 8 : 4;
   a.split = 1;
-  while (a.split < 8 && tiles * a.split * 2 <= most && a.ksteps >= 4 * a.split) a.split *= 2;
+  while (a.split < most && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2;
   const uint32_t tables = tables_bytes(p.groups);
   const int budget = kSmemBudget - 1024 - static_cast<int>(tables);
   a.stage = static_cast<uint32_t>(kRows + a.tmax) * kStepBytes;
@@ -1074,13 +1126,23 @@ Args arguments(const Int8Matmul& p) {
   a.bias = p.bias;
   a.y = p.y;
   a.ldy = p.ldy;
-  a.vec = reinterpret_cast<uintptr_t>(p.y) % 4 == 0 && p.ldy % 2 == 0;
   a.err = p.err;
   return a;
 }
 
-// Pairs take what needs a second round of single CTAs and has tiles wide enough.
-bool pairs_pay(const Int8Matmul& p, int64_t tiles, int tmax, int sms) { return tmax >= 128 && tiles > sms; }
+// Rows of a tile of single CTAs at the most: all of a dense product with few of them, else 256, or 128 where one round holds the
+// narrower ones too (512 x 4096 x 4096: 16.9 us against 19.4); twice a group's mean, so that most groups take one.
+int single_rows(const Int8Matmul& p, int sms) {
+  const int64_t mean = ceil_div(p.rows, p.groups), want = p.offsets ? 2 * mean + 8 : mean;
+  int64_t t = align_up(want < p.rows ? want : p.rows, 16);
+  if (p.offsets) return static_cast<int>(t > kMaxT ? kMaxT : t > 96 ? align_up(t, 64) : t);
+  if (t > 128 && most_tiles(p, 128, kRows) <= sms) t = 128;
+  return static_cast<int>(t > kMaxT ? kMaxT : t);
+}
+
+// Pairs take what fills most of the SMs with tiles of 128 channels by 256 rows. Measured (us, single CTAs / pairs): 256 x 14336 x 4096
+// (112 tiles) 22.5 / 20.7, 1024 x 4096 x 4096 (128) 20.8 / 20.0, 512 x 4096 x 4096 (64) 16.9 / 19.4.
+bool pairs_pay(const Int8Matmul& p, int tmax, int sms) { return tmax >= 128 && 10 * most_tiles(p, kMaxT, kRows) >= 7 * sms; }
 
 }  // namespace
 
@@ -1110,35 +1172,28 @@ cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) 
   Args a = arguments(p);
   a.early = early;
 
-  // Rows of a tile at the most: all of a dense product with few of them; twice a group's mean, so that most groups take one.
-  const int64_t mean = ceil_div(p.rows, p.groups), want = p.offsets ? 2 * mean + 8 : mean;
-  a.tmax = static_cast<int>(align_up(want < p.rows ? want : p.rows, 16));
-  if (p.offsets && a.tmax > 96) a.tmax = static_cast<int>(align_up(a.tmax, 64));
-  if (a.tmax > kMaxT) a.tmax = kMaxT;
-  // Rows of one copy: all of a dense tile; of a ragged one, whose last copy may reach into the next group's rows, large
-  // ones too (16 rows a copy: 39 cycles each, 620 a stage of 256 rows).
-  a.box = !p.offsets ? a.tmax : a.tmax % 64 == 0 ? 64 : 16;
-
   Launch l{};
   l.early = early;
-  int64_t tiles = most_tiles(p, a.tmax, kRows);
-  l.pairs = pairs_pay(p, tiles, a.tmax, sms);
+  a.tmax = single_rows(p, sms);
+  l.pairs = pairs_pay(p, a.tmax, sms);
+  if (l.pairs) a.tmax = kMaxT;
   const int channels = l.pairs ? 2 * kRows : kRows;
+  const int64_t tiles = most_tiles(p, a.tmax, channels);
+  if (tiles > INT_MAX / 16) return cudaErrorInvalidValue;
   a.p_tiles = static_cast<int>(ceil_div(p.N, channels));
   if (l.pairs) {
-    a.tmax = kMaxT;
-    a.box = p.offsets ? 64 : kRows;
-    tiles = most_tiles(p, a.tmax, channels);
+    a.box = 64;  // of the rows of a narrow tile or piece no more than needed
     a.split = 1;
     a.stages = kStages2;
     a.tables = kStages2 * kStage2;
     l.smem = a.tables + tables_bytes(p.groups) + 1024;
-    l.grid = static_cast<int>(2 * (tiles < sms / 2 ? tiles : sms / 2));
+    l.grid = sms / 2 * 2;
   } else {
-    if (tiles <= INT_MAX / 16) single_shape(p, tiles, sms, a, l);
+    // Rows of one copy: all of a dense tile; of a ragged one, whose last copy may reach into the next group's rows, large ones
+    // too (16 rows a copy: 39 cycles each, 620 a stage of 256 rows).
+    a.box = !p.offsets ? a.tmax : a.tmax % 64 == 0 ? 64 : 16;
+    single_shape(p, tiles, sms, a, l);
   }
-  if (tiles > INT_MAX / 16) return cudaErrorInvalidValue;
-
   if (!encode_tensor_map_2d(&l.p, 0, p.b, p.K, static_cast<uint64_t>(p.groups) * p.N, p.ldb, kStepBytes, kRows, true) ||
       !encode_tensor_map_2d(&l.q, 0, p.a, p.K, p.rows, p.lda, kStepBytes, a.box, true))
     return cudaErrorInvalidValue;
