@@ -174,7 +174,7 @@ def _values(rows, K, dtype, seed):
 
 @gpu
 @pytest.mark.parametrize("dtype", [HALF, FULL])
-@pytest.mark.parametrize("rows,K", [(1, 1), (1, 4096), (3, 15), (17, 16), (70, 33), (2, 4100), (5, 8192), (3, 16384), (2, 28672), (2, 40000), (300, 64), (33, 250)])
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 4096), (3, 15), (17, 16), (70, 33), (2, 4100), (5, 8192), (3, 16384), (2, 28672), (2, 40000), (300, 64), (33, 250), (700, 1024), (1500, 4096), (1000, 5000), (600, 9008), (650, 24000), (593, 6000), (3000, 9000), (5000, 1024), (2500, 14336)])
 def test_quantize_is_exact(F, dtype, rows, K):
     x = _values(rows, K, dtype, rows * 1000 + K)
     if rows > 2:
@@ -436,7 +436,7 @@ def test_grouped_product(F, E, rows, N, K, kind, dtype, bias, act):
 
 
 @gpu
-@pytest.mark.parametrize("T,E,k,N,K", [(1, 64, 8, 256, 512), (3, 8, 8, 130, 33), (70, 16, 2, 200, 100), (333, 12, 3, 100, 250), (700, 6, 4, 2500, 64), (40, 5, 1, 64, 16), (2000, 10, 3, 700, 1000)])
+@pytest.mark.parametrize("T,E,k,N,K", [(1, 64, 8, 256, 512), (3, 8, 8, 130, 33), (70, 16, 2, 200, 100), (333, 12, 3, 100, 250), (700, 6, 4, 2500, 64), (40, 5, 1, 64, 16), (2000, 10, 3, 700, 1000), (1500, 16, 4, 256, 2048), (1200, 6, 2, 130, 4100)])
 @pytest.mark.parametrize("dtype,act", [(HALF, "swiglu"), (FULL, "none")])
 def test_grouped_product_of_gathered_tokens(F, T, E, k, N, K, dtype, act):
     order = np.random.default_rng(T).permutation(T * k)

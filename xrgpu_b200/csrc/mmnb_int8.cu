@@ -79,18 +79,38 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
   }
 }
 
+// blockDim.x threads take kGatherRows rows at a time, blockDim.y such sets a CTA: their entries of the order, then their codes, are
+// loaded side by side (one row at a time: 45 us for 16384 rows of 4096 codes).
+constexpr int kGatherRows = 4;
 __global__ void __launch_bounds__(256) gather_kernel(const Int8Gather p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;
-  const int64_t from = source_row(p.from, row);
-  if (threadIdx.x == 0) p.scales[row] = from >= 0 ? p.a_scales[from] : 0.0f;
-  const uint4* src = reinterpret_cast<const uint4*>(p.a + max(from, static_cast<int64_t>(0)) * p.lds);
-  uint4* dst = reinterpret_cast<uint4*>(p.codes + row * p.ldc);
-  const int64_t whole = p.K / kUnit;
-#pragma unroll 4
-  for (int64_t at = threadIdx.x; at < whole; at += blockDim.x) dst[at] = src[at];
-  for (int64_t k = whole * kUnit + threadIdx.x; k < p.K; k += blockDim.x) p.codes[row * p.ldc + k] = reinterpret_cast<const int8_t*>(src)[k];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y) * kGatherRows;
+  const int rows = static_cast<int>(min(p.rows - row, static_cast<int64_t>(kGatherRows)));
+  int64_t from[kGatherRows];
+#pragma unroll
+  for (int i = 0; i < kGatherRows; ++i) from[i] = i < rows ? source_row(p.from, row + i) : -1;
+  if (static_cast<int>(threadIdx.x) < rows) {
+    int64_t f = from[0];
+#pragma unroll
+    for (int i = 1; i < kGatherRows; ++i) f = threadIdx.x == i ? from[i] : f;
+    p.scales[row + threadIdx.x] = f >= 0 ? p.a_scales[f] : 0.0f;
+  }
+  const int whole = static_cast<int>(p.K / kUnit);
+  for (int at = threadIdx.x; at < whole; at += blockDim.x) {
+    uint4 v[kGatherRows];
+#pragma unroll
+    for (int i = 0; i < kGatherRows; ++i)  // a row that fits none: any codes, its scale is 0
+      if (i < rows) v[i] = reinterpret_cast<const uint4*>(p.a + max(from[i], static_cast<int64_t>(0)) * p.lds)[at];
+#pragma unroll
+    for (int i = 0; i < kGatherRows; ++i)
+      if (i < rows) reinterpret_cast<uint4*>(p.codes + (row + i) * p.ldc)[at] = v[i];
+  }
+  for (int64_t k = static_cast<int64_t>(whole) * kUnit + threadIdx.x; k < p.K; k += blockDim.x) {  // the last row may end with its codes
+#pragma unroll
+    for (int i = 0; i < kGatherRows; ++i)
+      if (i < rows) p.codes[(row + i) * p.ldc + k] = p.a[max(from[i], static_cast<int64_t>(0)) * p.lds + k];
+  }
 }
 
 // VEC: 16 bytes of values a thread at a time (K a multiple of 16).
@@ -203,13 +223,21 @@ cudaError_t launch_int8_dequantize(const Int8Rows& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_int8_gather(const Int8Gather& p, cudaStream_t s) {
+cudaError_t launch_int8_gather(const Int8Gather& p, bool early, cudaStream_t s) {
   const int64_t units = ceil_div(p.K, kUnit);
   const unsigned tx = units >= 256 ? 256 : static_cast<unsigned>(align_up(units, 32)), ty = 256 / tx;
-  const int64_t blocks = ceil_div(p.rows, ty);
+  const int64_t blocks = ceil_div(p.rows, ty * kGatherRows);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  gather_kernel<<<static_cast<unsigned>(blocks), dim3(tx, ty), 0, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(tx, ty);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gather_kernel, p);
 }
 
 cudaError_t launch_weighted_rows(const WeightedRows& p, cudaStream_t s) {

@@ -42,7 +42,8 @@ struct Int8Gather {
   int8_t* codes;
   float* scales;
 };
-cudaError_t launch_int8_gather(const Int8Gather& p, cudaStream_t s);
+// early: a is what the kernel before it on the stream writes.
+cudaError_t launch_int8_gather(const Int8Gather& p, bool early, cudaStream_t s);
 
 // y[r, :] = act(a[r] . b[g]^T * a_scale[r] * b_scale[g, :] + bias[g, :]) for the rows r of group g, offsets[g] <= r <
 // offsets[g + 1] (offsets nullptr: one group of all rows).
