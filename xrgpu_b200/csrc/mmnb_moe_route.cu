@@ -2,7 +2,7 @@
 // their weights, and the stable order of all assignments (token * top_k + rank) by expert.
 //
 // Choice: a warp a token. Scores become numbers of 32 bits that order like them: the upper 22 bits of a key of the
-// score, then the index counted down, and the largest of the warp is taken out top_k times. That is exact for float16 (16
+// score, then the index counted down, and the largest of the warp is taken out top_k times, from lanes that hold theirs sorted. That is exact for float16 (16
 // bits); for float32 two neighbours of the result that agree in the 22 bits send the token to the exact form (whole keys, then the
 // lowest index among equals). What bounds it is instructions: about 25 a choice instead of 50 for whole keys.
 // Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
@@ -33,9 +33,8 @@ struct Args {
 
 // A key that orders like the score; 0 is below every score. -0 equals 0, NaN -infinity.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x007fffffu;
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const int u = __float_as_int(x == x ? x + 0.0f : -INFINITY);
+  return static_cast<uint32_t>(u ^ ((u >> 31) | static_cast<int>(0x80000000u)));
 }
 __device__ __forceinline__ float score_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
@@ -81,35 +80,50 @@ __device__ __noinline__ int choose_exact(const float* scores, int E, int k) {
   return chosen;
 }
 
+// Descending order, by Batcher's merges of odd and even places.
+template <int N>
+__device__ __forceinline__ void sort_descending(uint32_t (&c)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2) {
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2) {
+#pragma unroll
+      for (int i = 0; i + k < N; ++i) {
+        if (i >= k % p && (i - k % p) / k % 2 == 0 && i / (2 * p) == (i + k) / (2 * p)) {
+          const uint32_t a = c[i], b = c[i + k];
+          c[i] = max(a, b);
+          c[i + k] = min(a, b);
+        }
+      }
+    }
+  }
+}
+
 // The choice and weights of the warp's tokens, counted into `mine` [experts]. VPL: scores a lane.
 template <int VPL, bool F16>
 __device__ __forceinline__ void choose(const Args& a, int64_t t0, int64_t t1, int32_t* mine) {
   const int lane = threadIdx.x & 31, E = a.p.experts, k = a.p.top_k;
   for (int64_t t = t0; t < t1; ++t) {
     float x[VPL];
-    uint32_t c[VPL], top = 0;
+    uint32_t c[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) x[i] = lane + 32 * i < E ? load_f(a.p.scores, F16, t * a.p.lds + lane + 32 * i) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      c[i] = lane + 32 * i < E ? (key_of(x[i]) & ~1023u) | (1023u - (lane + 32 * i)) : 0u;
-      top = max(top, c[i]);
-    }
+    for (int i = 0; i < VPL; ++i) c[i] = lane + 32 * i < E ? (key_of(x[i]) & ~1023u) | (1023u - (lane + 32 * i)) : 0u;
+    sort_descending<VPL>(c);
     int chosen = 0;
     uint32_t last = 0;
     bool close = false;
     const int picks = F16 ? k : min(k + 1, E);
     for (int j = 0; j < picks; ++j) {
-      const uint32_t m = __reduce_max_sync(~0u, top);
+      const uint32_t m = __reduce_max_sync(~0u, c[0]);
       if (lane == j) chosen = static_cast<int>(1023u - (m & 1023u));
       close |= (m ^ last) < 1024u;
       last = m;
-      top = 0;
+      const bool taken = c[0] == m;  // one lane's
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        c[i] = c[i] == m ? 0u : c[i];
-        top = max(top, c[i]);
-      }
+      for (int i = 0; i + 1 < VPL; ++i) c[i] = taken ? c[i + 1] : c[i];
+      if (taken) c[VPL - 1] = 0u;
     }
     if (!F16 && close) chosen = choose_exact<VPL>(static_cast<const float*>(a.p.scores) + t * a.p.lds, E, k);
     const float score = lane < k ? score_of(key_of(load_f(a.p.scores, F16, t * a.p.lds + chosen))) : 0.0f;
