@@ -504,13 +504,23 @@ def test_grouped_offsets_and_order_that_do_not_fit(F):
     args, kw, want, err = _grouped(F, 4, 50, 60, 64, FULL, False, "none", "even")
     good = F.matmul_int8_grouped(*args, **kw)
     first = args[3].tolist()
-    for off in ([0, first[1], first[2], first[3], 51], [-1] + first[1:], [0, first[1], first[2], 1 << 30, first[4]], [0, first[2], first[1], first[3], first[4]]):
-        y = torch.zeros_like(good)
+    for off, keep in (([0, first[1], first[2], first[3], 51], 3), ([-1] + first[1:], 0), ([0, first[1], first[2], 1 << 30, first[4]], 2),
+                      ([0, first[2], first[1], first[3], first[4]], 1)):
+        y = torch.full_like(good, 7.0)
         F.matmul_int8_grouped(*args[:3], torch.tensor(off, dtype=torch.int32, device="cuda"), **kw, out=y)
-        assert F.device_error() == 0x701 and torch.isfinite(y).all()
-        for e in range(4):  # groups whose offsets are as they were
-            if off[e:e + 2] == first[e:e + 2]:
-                assert torch.equal(y[first[e]:first[e + 1]], good[first[e]:first[e + 1]]) or off == [0, first[2], first[1], first[3], first[4]]
+        assert F.device_error() == 0x701
+        end = off[keep]  # the groups before the first bad offset; nothing behind them is written
+        assert (y[end:] == 7).all() and torch.equal(y[:first[1]] if keep else y[:0], good[:first[1]] if keep else good[:0])
+    many, kwm, want, err = _grouped(F, 300, 900, 20, 33, FULL, False, "none", "ragged")
+    off = many[3].tolist()
+    whole = F.matmul_int8_grouped(*many, **kwm)
+    for bad in (5, 31, 32, 33, 100, 299):
+        broken = many[3].clone()
+        broken[bad + 1:] = -5
+        y = torch.full_like(whole, 7.0)
+        F.matmul_int8_grouped(*many[:3], broken, **kwm, out=y)
+        assert F.device_error() == 0x701
+        assert torch.equal(y[:off[bad]], whole[:off[bad]]) and (y[off[bad]:] == 7).all()
     order = torch.arange(50, dtype=torch.int32, device="cuda")
     order[3], order[40] = -1, 50
     y = F.matmul_int8_grouped(*args, **kw, order=order)

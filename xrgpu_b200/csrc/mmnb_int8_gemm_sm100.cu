@@ -7,8 +7,8 @@
 // neighbours of a row of y. A tile is 128 channels of a group by up to tmax of its rows (a group's rows are cut evenly).
 //
 // Groups. Offsets are on the device: every CTA counts the groups' tiles itself (a scan in shared memory) and takes tiles
-// of one line, group by group, the tiles of the same channels next to each other. Offsets that do not fit leave out their group
-// and record an error. Rows come in the groups' order: fetching them where the tokens lie was slower by far (16384 x 4096 x
+// of one line, group by group, the tiles of the same channels next to each other. Offsets that do not fit leave out the groups
+// from there on and record an error. Rows come in the groups' order: fetching them where the tokens lie was slower by far (16384 x 4096 x
 // 4096, 216 us: 483 with 16-byte copies, whose writes need a fence of 2000 cycles a stage before the tensor cores may read
 // them; four-row tensor gathers take 60 cycles each, 3800 a stage of 256 rows).
 //
@@ -92,46 +92,52 @@ __device__ __forceinline__ Tables tables_at(uint8_t* at, int groups) {
 }
 inline uint32_t tables_bytes(int groups) { return static_cast<uint32_t>(align_up(static_cast<uint64_t>(3 * groups + 1) * 4, 16)); }
 
-// All threads; ends with a barrier.
-__device__ __forceinline__ void make_tables(const Args& a, const Tables& t) {
-  __shared__ int chunk_sum[32];
+// All threads; ends with a barrier. From the first offset on that decreases or leaves [0, rows] no group has tiles: what comes
+// before it is in order, so no two groups share a row. Returns whether all offsets fit.
+__device__ __forceinline__ bool make_tables(const Args& a, const Tables& t) {
+  __shared__ int chunk_sum[32], chunk_bad[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int base = 32 * warp; base < a.groups; base += kThreads) {
     const int g = base + lane;
-    int tiles = 0;
+    int lo = 0, hi = g < a.groups ? a.rows : 0;
+    if (a.offsets && g < a.groups) {
+      lo = a.offsets[g];
+      hi = a.offsets[g + 1];
+    }
+    const unsigned bad = __ballot_sync(~0u, lo < 0 || hi < lo || hi > a.rows);
+    if (bad && (bad & (2u << lane) - 1)) lo = hi = 0;  // this group, or one before it
     if (g < a.groups) {
-      int lo = 0, hi = a.rows;
-      if (a.offsets) {
-        lo = a.offsets[g];
-        hi = a.offsets[g + 1];
-        if (lo < 0 || hi < lo || hi > a.rows) {
-          if (blockIdx.x == 0) record_device_error(a.err, kErrOffsets);
-          lo = hi = 0;
-        }
-      }
       t.row_first[g] = lo;
       t.row_count[g] = hi - lo;
-      tiles = (hi - lo + a.tmax - 1) / a.tmax;
     }
-    int s = tiles;
+    int s = (hi - lo + a.tmax - 1) / a.tmax;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(~0u, s, o);
       if (lane >= o) s += u;
     }
     if (g < a.groups) t.tile_first[g + 1] = s;
-    if (lane == 31) chunk_sum[base >> 5] = s;
+    if (lane == 31) {
+      chunk_sum[base >> 5] = s;
+      chunk_bad[base >> 5] = bad != 0;
+      if (bad && blockIdx.x == 0) record_device_error(a.err, kErrOffsets);
+    }
   }
   if (threadIdx.x == 0) t.tile_first[0] = 0;
   __syncthreads();
+  bool fit = !chunk_bad[0];
   if (a.groups > 32) {
+    const int chunks = (a.groups + 31) / 32, sum = lane < chunks ? chunk_sum[lane] : 0;
+    const unsigned bad = __ballot_sync(~0u, lane < chunks && chunk_bad[lane]);
+    const int last = bad ? __ffs(bad) - 1 : chunks;  // the last chunk that counts
+    fit = !bad;
     for (int base = 32 * warp; base < a.groups; base += kThreads) {
-      const int chunk = base >> 5;
-      const int before = __reduce_add_sync(~0u, lane < chunk ? chunk_sum[lane] : 0);
-      if (base + lane < a.groups) t.tile_first[base + lane + 1] += before;
+      const int chunk = base >> 5, before = __reduce_add_sync(~0u, lane < chunk && lane <= last ? sum : 0);
+      if (base + lane < a.groups) t.tile_first[base + lane + 1] = before + (chunk <= last ? t.tile_first[base + lane + 1] : 0);
     }
     __syncthreads();
   }
+  return fit;
 }
 
 struct Tile {
@@ -179,9 +185,9 @@ __device__ __forceinline__ float relu(float r) { return r < 0.0f ? 0.0f : r; }  
 
 // Rows of no group (before the first offset, behind the last) become zero.
 template <bool F16>
-__device__ __forceinline__ void zero_rest(const Args& a, int width) {
-  if (!a.zero_rest || !a.offsets) return;
-  const int lo = min(max(a.offsets[0], 0), a.rows), hi = min(max(a.offsets[a.groups], lo), a.rows);
+__device__ __forceinline__ void zero_rest(const Args& a, bool fit, int width) {
+  if (!a.zero_rest || !a.offsets || !fit) return;
+  const int lo = a.offsets[0], hi = a.offsets[a.groups];
   for (int r = blockIdx.x; r < lo + a.rows - hi; r += gridDim.x) {
     const int64_t row = r < lo ? r : hi + r - lo;
     for (int n = threadIdx.x; n < width; n += kThreads) put<F16>(a.y, row * a.ldy + n, 0.0f);
@@ -283,6 +289,7 @@ __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_
     tmem_ld16(tmem + col, v);
     tmem_wait_ld16(v);
     store_chunk<F16, SWIGLU>(a, t, v, col, n, ch, row_scale + col, lane);
+    __syncwarp();
   }
 }
 
@@ -357,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const Tables tables = tables_at(gbase + a.tables, a.groups);
-  make_tables(a, tables);
+  const bool fit = make_tables(a, tables);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -498,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, tile_at<16>(a, tables, first), base, rank, row_scale[0]);
     cluster_sync();  // nobody leaves while its partial tile is being read
   }
-  zero_rest<F16>(a, SWIGLU ? a.n / 2 : a.n);
+  zero_rest<F16>(a, fit, SWIGLU ? a.n / 2 : a.n);
 }
 
 // ------------------------------------------------------------------ few rows, quantised in place
@@ -827,7 +834,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   const Tables tables = tables_at(smem_raw + (base - raw) + a.tables, a.groups);
-  make_tables(a, tables);
+  const bool fit = make_tables(a, tables);
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are there
@@ -976,7 +983,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
-  zero_rest<F16>(a, SWIGLU ? a.n / 2 : a.n);
+  zero_rest<F16>(a, fit, SWIGLU ? a.n / 2 : a.n);
 }
 
 // ------------------------------------------------------------------ host side
