@@ -29,23 +29,24 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's weights may start to load
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const bool real = row < p.rows;
-  const int64_t from = real ? source_row(p.from, row) : -1, row_at = max(from, static_cast<int64_t>(0)) * p.ldx;
-  const int64_t read = from >= 0 ? p.K : 0;  // values of x that count
+  const int64_t from = real ? source_row(p.from, row) : -1;
+  const uint8_t* x = static_cast<const uint8_t*>(p.x) + max(from, static_cast<int64_t>(0)) * p.ldx * (F16 ? 2 : 4);
+  const int read = from >= 0 ? static_cast<int>(p.K) : 0;  // values of x that count
   const int units = real ? static_cast<int>((p.K + U::kValues - 1) / U::kValues) : 0;
   U u[UNITS];
-  uint32_t amax = 0;
+  Largest<F16> largest;
   if (HELD) {
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) u[i].load(p.x, row_at, (threadIdx.x + i * blockDim.x) * static_cast<int64_t>(U::kValues), read);
+    for (int i = 0; i < UNITS; ++i) u[i].load(x, (threadIdx.x + i * blockDim.x) * U::kValues, read);
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) amax = max(amax, u[i].amax());
+    for (int i = 0; i < UNITS; ++i) u[i].largest(largest);
   } else {
     for (int at = threadIdx.x; at < units; at += blockDim.x) {
-      u[0].load(p.x, row_at, at * static_cast<int64_t>(U::kValues), read);
-      amax = max(amax, u[0].amax());
+      u[0].load(x, at * U::kValues, read);
+      u[0].largest(largest);
     }
   }
-  amax = __reduce_max_sync(~0u, amax);
+  uint32_t amax = __reduce_max_sync(~0u, largest.bits());
   const int warps = blockDim.x >> 5;
   if (warps > 1) {
     const int lane = threadIdx.x & 31;
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p)
     }
   } else {
     for (int at = threadIdx.x; at < units; at += blockDim.x) {
-      u[0].load(p.x, row_at, at * static_cast<int64_t>(U::kValues), read);
+      u[0].load(x, at * U::kValues, read);
       store(u[0], at);
     }
   }
@@ -206,7 +207,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 }  // namespace
 
 cudaError_t launch_int8_quantize(const Int8Rows& p, cudaStream_t s) {
-  const bool vec = aligned16(p.x) && (p.ldx * (p.f16 ? 2 : 4)) % 16 == 0;
+  const bool vec = aligned16(p.x) && (p.ldx * (p.f16 ? 2 : 4)) % 16 == 0 && p.K % (p.f16 ? 8 : 4) == 0;
   if (p.f16) return vec ? quantize<true, true>(p, s) : quantize<true, false>(p, s);
   return vec ? quantize<false, true>(p, s) : quantize<false, false>(p, s);
 }

@@ -34,16 +34,47 @@ __device__ __forceinline__ float row_scale_of(uint32_t amax, Scale* c, bool* non
   return s;
 }
 
+// Two float32 numbers in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Codes of a thread's N values, in the low bytes of b.
 template <int N, bool F16>
 __device__ __forceinline__ void codes_of(const float (&v)[N], const Scale& c, uint32_t (&b)[N]) {
+  const uint64_t inv = pair(c.inv, c.inv), magic = pair(kMagic, kMagic), back = pair(-kMagic, -kMagic), s = pair(-c.s, -c.s), up = pair(c.up, c.up);
   float worst = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = F16 ? v[i] : v[i] * c.up;
-    const float t = fmaf(x, c.inv, kMagic), r = t - kMagic;
-    b[i] = __float_as_uint(t);
-    worst = fmaxf(worst, fabsf(fmaf(-r, c.s, x)));
+  for (int i = 0; i < N; i += 2) {
+    uint64_t x = pair(v[i], v[i + 1]);
+    if (!F16) x = mul2(x, up);
+    const uint64_t t = fma2(x, inv, magic);
+    const float2 code = unpair(t), left = unpair(fma2(add2(t, back), s, x));
+    b[i] = __float_as_uint(code.x);
+    b[i + 1] = __float_as_uint(code.y);
+    worst = fmaxf(fmaxf(worst, fabsf(left.x)), fabsf(left.y));
   }
   if (worst >= 0.5f * c.s) {  // hardly ever: a tie, a code one off, or one that saturates
 #pragma unroll
@@ -56,37 +87,50 @@ __device__ __forceinline__ void codes_of(const float (&v)[N], const Scale& c, ui
   }
 }
 
-// 16 bytes of a row from value k0 on, zeros behind K, as they are held and as floats.
+// The largest magnitude of values, as the bits of a float32 (NaN > infinity > numbers). Pairs of halves as they are.
+template <bool F16>
+struct Largest {
+  uint32_t m = 0;
+  __device__ __forceinline__ void add(uint32_t u) {
+    if (F16) {
+      const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2*>(&m), __habs2(*reinterpret_cast<const __half2*>(&u)));
+      m = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      m = max(m, u & 0x7fffffffu);
+    }
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    if (!F16) return m;
+    const __half2 h = *reinterpret_cast<const __half2*>(&m);
+    return __float_as_uint(__half2float(__hmax_nan(__low2half(h), __high2half(h)))) & 0x7fffffffu;
+  }
+};
+
+// 16 bytes of a row from value k0 on, zeros behind K. VEC: rows start on 16 bytes and hold whole units.
 template <bool F16, bool VEC>
 struct Unit {
   static constexpr int kValues = F16 ? 8 : 4;
   uint32_t u[4];
-  __device__ __forceinline__ void load(const void* x, int64_t row_at, int64_t k0, int64_t K) {
-    if (VEC && k0 + kValues <= K) {
-      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + (row_at + k0) * (F16 ? 2 : 4));
+  __device__ __forceinline__ void load(const void* row, int k0, int K) {
+    if (VEC) {
+      const uint4 v = k0 < K ? *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + k0 * (F16 ? 2ll : 4ll)) : make_uint4(0, 0, 0, 0);
       u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
       return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (F16) {
-        const uint16_t* h = static_cast<const uint16_t*>(x) + row_at + k0;
+        const uint16_t* h = static_cast<const uint16_t*>(row) + k0;
         const uint32_t lo = k0 + 2 * i < K ? h[2 * i] : 0, hi = k0 + 2 * i + 1 < K ? h[2 * i + 1] : 0;
         u[i] = lo | hi << 16;
       } else {
-        u[i] = k0 + i < K ? static_cast<const uint32_t*>(x)[row_at + k0 + i] : 0;
+        u[i] = k0 + i < K ? static_cast<const uint32_t*>(row)[k0 + i] : 0;
       }
     }
   }
-  // the bits of the largest magnitude as float32 (NaN > infinity > numbers)
-  __device__ __forceinline__ uint32_t amax() const {
-    if (F16) {
-      __half2 m = __habs2(*reinterpret_cast<const __half2*>(&u[0]));
+  __device__ __forceinline__ void largest(Largest<F16>& l) const {
 #pragma unroll
-      for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&u[i])));
-      return __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))) & 0x7fffffffu;
-    }
-    return max(max(u[0] & 0x7fffffffu, u[1] & 0x7fffffffu), max(u[2] & 0x7fffffffu, u[3] & 0x7fffffffu));
+    for (int i = 0; i < 4; ++i) l.add(u[i]);
   }
   // Codes, four a word: kValues / 4 words of `word`.
   __device__ __forceinline__ void codes(const Scale& c, uint32_t* word) const {

@@ -524,7 +524,7 @@ constexpr unsigned kErrWaitRanks = 0x715;
 struct FewRows {
   const void* x;
   int64_t ldx, K;
-  int vec;         // rows of x start on 16 bytes
+  int vec;         // rows of x start on 16 bytes and hold whole units of them
   uint32_t codes, sums;  // bytes from the stages' start to the rows' codes, and to the sums sent by the ranks
 };
 
@@ -532,15 +532,16 @@ template <bool XF16, bool VEC>
 struct Part {  // 16 values of a lane
   static constexpr int kUnits = XF16 ? 2 : 4;
   Unit<XF16, VEC> u[kUnits];
-  __device__ __forceinline__ void load(const FewRows& f, int64_t row, int64_t k0) {
+  __device__ __forceinline__ void load(const FewRows& f, int64_t row, int k0) {
+    const uint8_t* x = static_cast<const uint8_t*>(f.x) + row * f.ldx * (XF16 ? 2 : 4);
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) u[i].load(f.x, row * f.ldx, k0 + i * Unit<XF16, VEC>::kValues, f.K);
+    for (int i = 0; i < kUnits; ++i) u[i].load(x, k0 + i * Unit<XF16, VEC>::kValues, static_cast<int>(f.K));
   }
   __device__ __forceinline__ uint32_t amax() const {
-    uint32_t m = 0;
+    Largest<XF16> l;
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) m = max(m, u[i].amax());
-    return m;
+    for (int i = 0; i < kUnits; ++i) u[i].largest(l);
+    return l.bits();
   }
   __device__ __forceinline__ uint4 codes(const Scale& c, bool none) const {
     uint32_t w[4 + 2];
@@ -1162,7 +1163,7 @@ bool int8_few_rows(const Int8Matmul& p) {
 
 cudaError_t launch_int8_few(const Int8Matmul& p, const void* x, bool x_f16, int64_t ldx, cudaStream_t s) {
   Args a = arguments(p);
-  FewRows f{x, ldx, p.K, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_f16 ? 2 : 4) % 16 == 0, 0, 0};
+  FewRows f{x, ldx, p.K, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_f16 ? 2 : 4) % 16 == 0 && p.K % (x_f16 ? 8 : 4) == 0, 0, 0};
   Launch l{};
   if (!few_shape(p, device_sm_count(), a, f, l) || !encode_tensor_map_2d(&l.p, 0, p.b, p.K, p.N, p.ldb, kStepBytes, kRows, true)) return cudaErrorInvalidValue;
   const bool swiglu = p.act == XRGPU_ACT_SWIGLU;
