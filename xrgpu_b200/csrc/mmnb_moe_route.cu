@@ -2,13 +2,16 @@
 // their weights, and the stable order of all assignments (token * top_k + rank) by expert.
 //
 // Choice: a warp a token. Scores become numbers of 32 bits that order like them: the upper 22 bits of a key of the
-// score, then the index counted down, and the largest of the warp is taken out top_k times, from lanes that hold theirs sorted. That is exact for float16 (16
-// bits); for float32 two neighbours of the result that agree in the 22 bits send the token to the exact form (whole keys, then the
-// lowest index among equals). What bounds it is instructions: about 25 a choice instead of 50 for whole keys.
+// score, then the index counted down, and the largest of the warp is taken out top_k times, from lanes that hold theirs
+// sorted. That is exact for float16 (16 bits); for float32 two neighbours of the result that agree in the 22 bits send the token
+// to the exact form (whole keys, then the lowest index among equals). What bounds it is instructions, about 20 a choice (50
+// with whole keys), and where tokens are few the latency of its steps.
 // Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
 // Order: a counting sort. Every warp counts its own tokens' experts, the counts are summed over the warps and CTAs before it, and
 // each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: the CTAs of one
 // cluster read each other's counts; else a second kernel follows in which every CTA sums the counts of all (from L2).
+// Measured (8 experts a token): 64 tokens x 128 experts 5.6 us, 1024 7.9, 32768 20.1; 8192 x 256 of float32 with weights of all 16.4
+// (9.5 MB: 1.4 us at the copy rate; the choice takes 10 of them, the order 6).
 #include <cuda_fp16.h>
 
 #include "mmnb_common.cuh"
