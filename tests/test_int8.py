@@ -529,6 +529,74 @@ def test_grouped_offsets_and_order_that_do_not_fit(F):
     assert torch.equal(y[keep], good[keep]) and (y[3] == 0).all() and (y[40] == 0).all()
 
 
+@gpu
+def test_no_tokens_at_all(F):
+    x, scores = torch.zeros(0, 64, dtype=HALF, device="cuda"), torch.zeros(0, 6, device="cuda")
+    up, down = (F.int8_quantize(torch.ones(6, 64, 64, device="cuda")) for _ in range(2))
+    r = F.moe_route(scores, 2)
+    h = F.matmul_int8_grouped(x, *up, r.offsets, order=r.order, top_k=2)
+    assert h.shape == (0, 64) and F.matmul_int8_grouped(h, *down, r.offsets, slots=r.slots, weights=r.weights).shape == (0, 64)
+    assert F.matmul_int8(x, up[0][0], up[1][0]).shape == (0, 64)
+
+
+@gpu
+def test_c_calls_with_the_librarys_workspace(F, cuda_lib):
+    """NULL workspaces: quantised rows, gathered rows, rows to be summed, a router's counts."""
+    g = torch.Generator().manual_seed(8)
+    E, T, k, N, K = 6, 300, 2, 130, 200
+    x = torch.randn(T, K, generator=g, dtype=HALF).cuda()
+    w, ws = F.int8_quantize(torch.randn(E, N, K, generator=g).cuda())
+    scores = torch.randn(T, E, generator=g).cuda()
+    r = F.moe_route(scores, k)
+    own = [torch.empty_like(t) for t in r]
+    p = _native.MoeRouteProblem_(_native.FLOAT32, 1, T, E, k, 0, scores.data_ptr(), *(t.data_ptr() for t in own))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert cuda_lib.xrgpu_moe_route(ctypes.byref(p), None, 0, stream) == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(own, r))
+    y, s = torch.empty(T * k, N, dtype=HALF, device="cuda"), torch.empty(T, N, dtype=HALF, device="cuda")
+    q = _native.Int8Problem_()
+    q.dtype = q.a_dtype = _native.FLOAT16
+    q.M, q.K, q.N, q.groups, q.rows, q.top_k = T, K, N, E, T * k, k
+    q.a, q.b, q.b_scales, q.ldb, q.offsets, q.order, q.y = x.data_ptr(), w.data_ptr(), ws.data_ptr(), w.stride(1), r.offsets.data_ptr(), r.order.data_ptr(), y.data_ptr()
+    assert cuda_lib.xrgpu_int8_forward(ctypes.byref(q), None, 0, stream) == 0
+    assert torch.equal(y, F.matmul_int8_grouped(x, w, ws, r.offsets, order=r.order, top_k=k))
+    q.slots, q.weights, q.tokens, q.y = r.slots.data_ptr(), r.weights.data_ptr(), T, s.data_ptr()
+    assert cuda_lib.xrgpu_int8_forward(ctypes.byref(q), None, 0, stream) == 0
+    assert torch.equal(s, F.matmul_int8_grouped(x, w, ws, r.offsets, order=r.order, top_k=k, slots=r.slots, weights=r.weights))
+    assert F.device_error() == 0
+
+
+@gpu
+def test_sizes_beyond_32_bits(F):
+    """More than 2^31 values of a result, of an operand's codes and of a row quantisation: the last rows are right."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    M, N, K = 66000, 33000, 32
+    a = torch.randint(-127, 128, (M, K), generator=g, device="cuda", dtype=torch.int8)
+    b = torch.randint(-127, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    sa, sb = torch.full((M,), 2.0 ** -6, device="cuda"), torch.full((N,), 2.0 ** -6, device="cuda")
+    y = F.matmul_int8(a, b, sb, a_scales=sa)
+    for rows in (slice(0, 3), slice(M // 2, M // 2 + 3), slice(M - 3, M)):  # sums below 2^20, scaled by 2^-12: one rounding
+        assert torch.equal(y[rows], (a[rows].double() @ b.double().t() * 2.0 ** -12).to(HALF))
+    del a, b, y
+    E, N, K = 5, 30000, 16400  # 2.46e9 codes; the last expert's begin at 1.97e9
+    w = torch.zeros(E, N, K, dtype=torch.int8, device="cuda")
+    w[3:, -300:] = torch.randint(-127, 128, (2, 300, K), generator=g, device="cuda", dtype=torch.int8)
+    x = torch.randint(-9, 10, (20, K), generator=g, device="cuda", dtype=torch.int8)
+    off = torch.tensor([0, 0, 3, 3, 9, 20], dtype=torch.int32, device="cuda")
+    y = F.matmul_int8_grouped(x, w, torch.ones(E, N, device="cuda"), off, a_scales=torch.ones(20, device="cuda"), dtype=FULL)
+    assert torch.equal(y[9:, -300:].double(), x[9:].double() @ w[4, -300:].double().t()) and (y[9:, :-300] == 0).all()
+    assert torch.equal(y[3:9, -300:].double(), x[3:9].double() @ w[3, -300:].double().t()) and (y[:3] == 0).all()
+    del w, y
+    h = torch.zeros(70000, 31000, dtype=HALF, device="cuda")
+    h[-2:] = torch.randn(2, 31000, generator=g, device="cuda", dtype=HALF)
+    c, s = F.int8_quantize(h)
+    codes, scales = R.quantize(h[-2:].cpu().double().numpy())
+    assert np.array_equal(c[-2:].cpu().numpy(), codes) and np.array_equal(s[-2:].cpu().double().numpy(), scales) and not c[:-2].any()
+    assert torch.equal(F.int8_dequantize(c, s, dtype=HALF)[-2:].cpu(), (torch.from_numpy(codes).float() * torch.from_numpy(scales).float()[:, None]).to(HALF))
+    assert F.device_error() == 0
+
+
 # ------------------------------------------------------------------------------------------ together
 def _layer(F, x, scores, k, up, down, **kw):
     r = F.moe_route(scores, k)
