@@ -590,8 +590,8 @@ XRGPU_API int xrgpu_int8_dequantize(const xrgpu_int8_tensor* t, void* out, void*
 /* Dense (groups 0):  y[m] = act(sum_k a[m, k] b[n, k] * a_scales[m] * b_scales[n] + bias[n]),  M rows.
  * Grouped: rows offsets[g] .. offsets[g + 1] - 1 of the product take b[g], b_scales[g], bias[g]; its row r reads row
  * order[r] / top_k of a, or row r without order (then M = rows). From the first offset on that decreases or leaves
- * [0, rows] the groups are dropped, their rows not written (0x701 in the device error word); an order entry outside [0, M * top_k) counts as a row of zeros (0x702). Rows of no
- * group are left as they were.
+ * [0, rows] there are no groups (0x701 in the device error word); an order entry outside [0, M * top_k) counts as a row of
+ * zeros (0x702). Rows of no group are left as they were.
  * With slots and weights the call returns sums of the product's rows instead: y[t] = sum_j weights[t, j] * row
  * slots[t, j], j < top_k, for `tokens` rows t, in float32 and in the order of j; slots outside [0, rows) are left out, rows of no
  * group are zero.

@@ -521,6 +521,15 @@ def test_grouped_offsets_and_order_that_do_not_fit(F):
         F.matmul_int8_grouped(*many[:3], broken, **kwm, out=y)
         assert F.device_error() == 0x701
         assert torch.equal(y[:off[bad]], whole[:off[bad]]) and (y[off[bad]:] == 7).all()
+        y = F.matmul_int8_grouped(*many[:3], broken, **kwm)  # without out they are zero, in the sums too
+        assert torch.equal(y[:off[bad]], whole[:off[bad]]) and (y[off[bad]:] == 0).all()
+        slots = torch.randperm(900, device="cuda").int().view(450, 2)
+        s = F.matmul_int8_grouped(*many[:3], broken, **kwm, slots=slots, weights=torch.ones(450, 2, device="cuda"))
+        assert torch.equal(s, y[slots[:, 0].long()] + y[slots[:, 1].long()])
+        assert F.device_error() == 0x701
+    for off in ([-1] * 5, [51] * 5, [20, 10, 30, 40, 50], [7, 7, 7, 7, 51], [-1, 10, 20, 30, 50], [60, 10, 20, 30, 50]):
+        y = F.matmul_int8_grouped(*args[:3], torch.tensor(off, dtype=torch.int32, device="cuda"), **kw)
+        assert (y == 0).all() and F.device_error() == 0x701
     order = torch.arange(50, dtype=torch.int32, device="cuda")
     order[3], order[40] = -1, 50
     y = F.matmul_int8_grouped(*args, **kw, order=order)

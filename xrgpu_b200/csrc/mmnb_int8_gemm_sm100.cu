@@ -7,8 +7,8 @@
 // neighbours of a row of y. A tile is 128 channels of a group by up to tmax of its rows (a group's rows are cut evenly).
 //
 // Groups. Offsets are on the device: every CTA counts the groups' tiles itself (a scan in shared memory) and takes tiles
-// of one line, group by group, the tiles of the same channels next to each other. Offsets that do not fit leave out the groups
-// from there on and record an error. Rows come in the groups' order: fetching them where the tokens lie was slower by far (16384 x 4096 x
+// of one line, group by group, the tiles of the same channels next to each other. From the first offset that does not
+// fit on there are no groups, and an error is recorded. Rows come in the groups' order: fetching them where the tokens lie was slower by far (16384 x 4096 x
 // 4096, 216 us: 483 with 16-byte copies, whose writes need a fence of 2000 cycles a stage before the tensor cores may read
 // them; four-row tensor gathers take 60 cycles each, 3800 a stage of 256 rows).
 //
@@ -189,11 +189,20 @@ __device__ __forceinline__ float swiglu(const Args& a, float g, float l) {
 __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias) { return fmaf(static_cast<float>(acc) * sa, sb, bias); }
 __device__ __forceinline__ float relu(float r) { return r < 0.0f ? 0.0f : r; }  // a NaN stays
 
-// Rows of no group (before the first offset, behind the last) become zero.
+// Rows of no group (before the first offset, behind the last one that counts) become zero.
 template <bool F16>
 __device__ __forceinline__ void zero_rest(const Args& a, bool fit, int width) {
-  if (!a.zero_rest || !a.offsets || !fit) return;
-  const int lo = a.offsets[0], hi = a.offsets[a.groups];
+  if (!a.zero_rest || !a.offsets) return;
+  int lo = a.offsets[0], hi = a.offsets[a.groups];
+  if (!fit) {
+    const bool none = lo < 0 || lo > a.rows;
+    hi = lo = none ? 0 : lo;
+    for (int g = 1; !none && g <= a.groups; ++g) {
+      const int o = a.offsets[g];
+      if (o < hi || o > a.rows) break;
+      hi = o;
+    }
+  }
   for (int r = blockIdx.x; r < lo + a.rows - hi; r += gridDim.x) {
     const int64_t row = r < lo ? r : hi + r - lo;
     for (int n = threadIdx.x; n < width; n += kThreads) put<F16>(a.y, row * a.ldy + n, 0.0f);

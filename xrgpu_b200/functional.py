@@ -806,8 +806,8 @@ def matmul_int8_grouped(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor
         y = matmul_int8_grouped(h, down, down_scales, r.offsets, slots=r.slots, weights=r.weights)
 
     With ``out``, rows of no group are left as they were (without it they are zero). From the first offset on that
-    decreases or leaves [0, R] the groups are dropped and their rows not written (``device_error`` 0x701); an order entry that fits
-    no row of a counts as zeros (0x702).
+    decreases or leaves [0, R] there are no groups (``device_error`` 0x701); an order entry that fits no row of a counts as
+    zeros (0x702).
     """
     if b.dim() != 3:
         raise ValueError("b must be [experts, N, K] codes")
