@@ -369,6 +369,31 @@ def test_route(F, dtype, T, E, k, normalize):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [HALF, FULL])
+@pytest.mark.parametrize("E,k", [(32, 32), (64, 8), (128, 32), (160, 32), (200, 7), (256, 8), (256, 32), (512, 16), (999, 32), (1024, 8)])
+def test_route_of_distinct_and_nearly_equal_scores(F, dtype, E, k):
+    """Distinct scores; favourites at every 32nd place; neighbours one step apart around the k-th; all of this in one call."""
+    g = torch.Generator().manual_seed(E + k)
+    x = torch.randn(400, E, generator=g).to(dtype)
+    for t in range(100, 200):  # the best of all share a place modulo 32
+        at = torch.arange(t % 32, E, 32)
+        x[t, at] = (10 + torch.randn(len(at), generator=g)).to(dtype)
+    for t in range(200, 300):  # the k-th and the next one step apart, the later one the higher
+        rank = torch.argsort(-x[t].double(), stable=True)
+        if k < E:
+            i, j = sorted((int(rank[k - 1]), int(rank[k])))
+            v = x[t, rank[k - 1]]
+            x[t, i], x[t, j] = v, torch.nextafter(v, torch.tensor(float("inf"), dtype=dtype))
+    for t in range(300, 400):  # many within a few steps of one value
+        x[t] = (1 + torch.randint(0, 40, (E,), generator=g) * torch.finfo(dtype).eps).to(dtype)
+    experts, weights, order, slots, offsets, bound = R.route(x.double().numpy(), k)
+    r = F.moe_route(x.cuda(), k)
+    assert np.array_equal(r.experts.cpu().numpy(), experts)
+    assert np.array_equal(r.order.cpu().numpy(), order) and np.array_equal(r.slots.cpu().numpy(), slots) and np.array_equal(r.offsets.cpu().numpy(), offsets)
+    R.close(r.weights, weights, weights * bound, FULL)
+
+
+@gpu
 def test_route_strides_empty_and_infinite(F):
     x = torch.randn(70, 50, device="cuda")
     a, b = F.moe_route(x[:, 5:45], 4), F.moe_route(x[:, 5:45].contiguous(), 4)

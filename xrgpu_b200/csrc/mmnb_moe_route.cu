@@ -2,16 +2,17 @@
 // their weights, and the stable order of all assignments (token * top_k + rank) by expert.
 //
 // Choice: a warp a token. Scores become numbers of 32 bits that order like them: the upper 22 bits of a key of the
-// score, then the index counted down, and the largest of the warp is taken out top_k times, from lanes that hold theirs
-// sorted. That is exact for float16 (16 bits); for float32 two neighbours of the result that agree in the 22 bits send the token
-// to the exact form (whole keys, then the lowest index among equals). What bounds it is instructions, about 20 a choice (50
-// with whole keys), and where tokens are few the latency of its steps.
+// score, then the index counted down, and the largest of the warp is taken out top_k times, from lanes that hold their best four
+// sorted. That is exact for float16 (16 bits); for float32 two neighbours of the result that agree in the 22 bits, and a lane
+// whose four were all taken while it has more, send the token to the exact form (whole keys, then the lowest index among equals).
+// What bounds it is instructions, about 14 a choice (50 with whole keys), and where tokens are few the latency of its steps. Four
+// held instead of all: 8192 x 256 16.4 -> 15.5 us, 2000 x 1024 27.9 -> 24.8.
 // Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
 // Order: a counting sort. Every warp counts its own tokens' experts, the counts are summed over the warps and CTAs before it, and
 // each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: the CTAs of one
 // cluster read each other's counts; else a second kernel follows in which every CTA sums the counts of all (from L2).
-// Measured (8 experts a token): 64 tokens x 128 experts 5.6 us, 1024 7.9, 32768 20.1; 8192 x 256 of float32 with weights of all 16.4
-// (9.5 MB: 1.4 us at the copy rate; the choice takes 10 of them, the order 6).
+// Measured (8 experts a token): 64 tokens x 128 experts 5.6 us, 1024 7.9, 32768 20.1; 8192 x 256 of float32 with weights of all 15.5
+// (9.5 MB: 1.4 us at the copy rate; the choice takes 9 of them, the order 6).
 #include <cuda_fp16.h>
 
 #include "mmnb_common.cuh"
@@ -50,14 +51,14 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // The chosen experts by whole keys: lane j returns the j-th.
-template <int VPL>
-__device__ __noinline__ int choose_exact(const float* scores, int E, int k) {
+template <int VPL, bool F16>
+__device__ __noinline__ int choose_exact(const void* scores, int64_t at0, int E, int k) {
   const int lane = threadIdx.x & 31;
   uint32_t key[VPL], best = 0;
   int at = 0, chosen = 0;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    key[i] = lane + 32 * i < E ? key_of(scores[lane + 32 * i]) : 0u;
+    key[i] = lane + 32 * i < E ? key_of(load_f(scores, F16, at0 + lane + 32 * i)) : 0u;
     if (key[i] > best) {
       best = key[i];
       at = i;
@@ -83,52 +84,76 @@ __device__ __noinline__ int choose_exact(const float* scores, int E, int k) {
   return chosen;
 }
 
-// Descending order, by Batcher's merges of odd and even places.
-template <int N>
-__device__ __forceinline__ void sort_descending(uint32_t (&c)[N]) {
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b) {
+  const uint32_t m = max(a, b);
+  b = min(a, b);
+  a = m;
+}
+__device__ __forceinline__ void sort_descending(uint32_t (&c)[1]) {}
+__device__ __forceinline__ void sort_descending(uint32_t (&c)[2]) { exchange(c[0], c[1]); }
+__device__ __forceinline__ void sort_descending(uint32_t (&c)[4]) {
+  exchange(c[0], c[1]);
+  exchange(c[2], c[3]);
+  exchange(c[0], c[2]);
+  exchange(c[1], c[3]);
+  exchange(c[1], c[2]);
+}
+// The four largest of `c` and `more`, both in descending order.
+__device__ __forceinline__ void keep_four(uint32_t (&c)[4], const uint32_t (&more)[4]) {
 #pragma unroll
-  for (int p = 1; p < N; p *= 2) {
-#pragma unroll
-    for (int k = p; k >= 1; k /= 2) {
-#pragma unroll
-      for (int i = 0; i + k < N; ++i) {
-        if (i >= k % p && (i - k % p) / k % 2 == 0 && i / (2 * p) == (i + k) / (2 * p)) {
-          const uint32_t a = c[i], b = c[i + k];
-          c[i] = max(a, b);
-          c[i + k] = min(a, b);
-        }
-      }
-    }
-  }
+  for (int i = 0; i < 4; ++i) c[i] = max(c[i], more[3 - i]);  // they rise, then fall, or the other way round
+  exchange(c[0], c[2]);
+  exchange(c[1], c[3]);
+  exchange(c[0], c[1]);
+  exchange(c[2], c[3]);
 }
 
 // The choice and weights of the warp's tokens, counted into `mine` [experts]. VPL: scores a lane.
 template <int VPL, bool F16>
 __device__ __forceinline__ void choose(const Args& a, int64_t t0, int64_t t1, int32_t* mine) {
+  constexpr int kHeld = VPL < 4 ? VPL : 4;
   const int lane = threadIdx.x & 31, E = a.p.experts, k = a.p.top_k;
   for (int64_t t = t0; t < t1; ++t) {
     float x[VPL];
-    uint32_t c[VPL];
+    uint32_t c[kHeld];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) x[i] = lane + 32 * i < E ? load_f(a.p.scores, F16, t * a.p.lds + lane + 32 * i) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) c[i] = lane + 32 * i < E ? (key_of(x[i]) & ~1023u) | (1023u - (lane + 32 * i)) : 0u;
-    sort_descending<VPL>(c);
-    int chosen = 0;
-    uint32_t last = 0;
-    bool close = false;
+    for (int b = 0; b < VPL; b += kHeld) {
+      uint32_t more[kHeld];
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int e = lane + 32 * (b + i);
+        more[i] = e < E ? (key_of(x[b + i]) & ~1023u) | (1023u - e) : 0u;
+      }
+      sort_descending(more);
+      if constexpr (VPL > kHeld) {
+        if (b > 0) {
+          keep_four(c, more);
+          continue;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) c[i] = more[i];
+    }
+    uint32_t pick = 0, last = 0;  // lane j: the j-th
     const int picks = F16 ? k : min(k + 1, E);
     for (int j = 0; j < picks; ++j) {
       const uint32_t m = __reduce_max_sync(~0u, c[0]);
-      if (lane == j) chosen = static_cast<int>(1023u - (m & 1023u));
-      close |= (m ^ last) < 1024u;
+      if (lane == j) pick = m;
       last = m;
       const bool taken = c[0] == m;  // one lane's
 #pragma unroll
-      for (int i = 0; i + 1 < VPL; ++i) c[i] = taken ? c[i + 1] : c[i];
-      if (taken) c[VPL - 1] = 0u;
+      for (int i = 0; i + 1 < kHeld; ++i) c[i] = taken ? c[i + 1] : c[i];
+      if (taken) c[kHeld - 1] = 0u;
     }
-    if (!F16 && close) chosen = choose_exact<VPL>(static_cast<const float*>(a.p.scores) + t * a.p.lds, E, k);
+    int chosen = static_cast<int>(1023u - (pick & 1023u));
+    bool close = VPL > kHeld && c[0] == 0u && lane + 32 * kHeld < E;  // the lane may hold more of the chosen than it kept
+    if (!F16) {
+      const uint32_t next = __shfl_down_sync(~0u, pick, 1);
+      close |= lane + 1 < k ? (pick ^ next) < 1024u : lane + 1 == k && picks > k && (pick ^ last) < 1024u;
+    }
+    if ((!F16 || VPL > kHeld) && __any_sync(~0u, close)) chosen = choose_exact<VPL, F16>(a.p.scores, t * a.p.lds, E, k);
     const float score = lane < k ? score_of(key_of(load_f(a.p.scores, F16, t * a.p.lds + chosen))) : 0.0f;
     const float best = __shfl_sync(~0u, score, 0);
     // a token whose scores are all -infinity weighs nothing
