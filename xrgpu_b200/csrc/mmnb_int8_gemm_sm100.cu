@@ -309,12 +309,16 @@ __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_
 }
 
 // A split tile's sums over the cluster's ranks (128 values of a column lie together at `base` of each): every rank takes its
-// share of the columns. All threads.
+// share of the columns, a thread the same four channels (`ch`) of each. Little code, once through: 333 x 1003 x 4100 14.3 us with the
+// channels' scales loaded a column at a time, 13.8 so, 14.8 with two columns at a time, unrolled. All threads.
 template <bool F16, bool SWIGLU>
-__device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t base, int rank, const float* row_scale) {
-  const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, mine = max(0, min(share, t.rows - col0));
-  for (int e = threadIdx.x; e < mine * (kRows / 4); e += kThreads) {
-    const int col = col0 + e / (kRows / 4), row = 4 * (e % (kRows / 4)), n = t.pt * kRows + row;
+__device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t base, int rank, const float* row_scale, const ChannelScale (&ch)[4]) {
+  constexpr int kLanes = kRows / 4, kColumns = kThreads / kLanes;  // threads a column, columns at a time
+  const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, end = min(t.rows, col0 + share);
+  const int row = 4 * (threadIdx.x % kLanes), n = t.pt * kRows + row;
+  if (n >= a.n) return;
+#pragma unroll 1
+  for (int col = col0 + threadIdx.x / kLanes; col < end; col += kColumns) {
     int sum[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -329,14 +333,12 @@ __device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t
     const float sa = row_scale[col];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t ch = static_cast<int64_t>(t.group) * a.n + n + i;
-      const bool in = n + i < a.n;
-      f[i] = scaled(sum[i], sa, in ? a.b_scales[ch] : 0.0f, in && a.bias ? load_f(a.bias, a.bias_f16, ch) : 0.0f);
+      f[i] = scaled(sum[i], sa, ch[i].scale, ch[i].bias);
       if (a.act == XRGPU_ACT_RELU) f[i] = relu(f[i]);
     }
     const int64_t at = static_cast<int64_t>(t.row0 + col) * a.ldy;
     if (SWIGLU) {
-      if (n < a.n) put<F16>(a.y, at + (n >> 1), swiglu(a, f[0], f[1]));
+      put<F16>(a.y, at + (n >> 1), swiglu(a, f[0], f[1]));
       if (n + 2 < a.n) put<F16>(a.y, at + (n >> 1) + 1, swiglu(a, f[2], f[3]));
     } else {
 #pragma unroll
@@ -508,6 +510,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  Tile t{};
+  ChannelScale ch[4];  // of the four channels whose sums this thread takes
+  if (a.split > 1 && first < tiles) {
+    t = tile_at<16>(a, tables, first);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ch[i] = channel_scale(a, t.group, t.pt * kRows + 4 * (threadIdx.x % (kRows / 4)) + i);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (a.split > 1) {
     // one tile a cluster: every rank sums its share of the columns over the ranks (128 values of a column lie together)
     cluster_sync();
-    if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, tile_at<16>(a, tables, first), base, rank, row_scale[0]);
+    if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, t, base, rank, row_scale[0], ch);
     cluster_sync();  // nobody leaves while its partial tile is being read
   }
   zero_rest<F16>(a, fit, SWIGLU ? a.n / 2 : a.n);
