@@ -16,8 +16,8 @@
 // Few tiles: K is split over a cluster of up to 8 CTAs whose int32 partial tiles meet in shared memory.
 //
 // Measured (GPU time of the call, weights from memory): 1 x 4096 x 4096 float rows 7.7 us (16.8 MB, 2.2 TB/s: latency), 16 x 4096 x
-// 14336 17.6 us with the rows' quantisation (59 MB, 3.3 TB/s: start and end, then the stream), one token by 8 of 64 experts of
-// 4096 x 4096 28.8 us (134 MB, 4.7 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 94 us (540 MB, 5.7 TB/s), 2048 x
+// 14336 16.7 us with the rows' quantisation (59 MB, 3.5 TB/s: start and end, then the stream), one token by 8 of 64 experts of
+// 4096 x 4096 27.5 us (134 MB, 4.9 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 89.5 us (540 MB, 6.0 TB/s), 2048 x
 // 14336 x 4096 85.6 us (2.8 PFLOP/s; tensor cores 78 % of the cycles, at 1.4 GHz under the power limit from the first launch on;
 // 99.6 us in calls back to back for seconds), 8192 x 8192 x 8192 372 us, 428 us for seconds (2.6 PFLOP/s at 1.24 GHz).
 //
@@ -39,7 +39,8 @@ constexpr int kRows = 128;       // channels of a tile
 constexpr int kStepBytes = 128;  // codes of a row per stage: one swizzle row
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = (2 + kEpilogueWarps) * 32;
-constexpr int kSmemBudget = 227 * 1024 - 10 * 1024;  // dynamic: less what is declared
+constexpr int kSmemMost = 227 * 1024;
+constexpr int kSmemBudget = kSmemMost - 10 * 1024;  // dynamic: less what is declared
 constexpr int kMaxStages = 12;
 constexpr int kMaxT = 256;
 constexpr int kPitch = kRows;    // int32 values a column of a partial tile in shared memory
@@ -58,7 +59,7 @@ struct Args {
   int tmem_cols, acc1;         // acc1: column of the second accumulator
   int early;                   // the weights may be loaded before the previous kernel has finished
   uint32_t stage;              // bytes
-  uint32_t tables;             // bytes from the stages' start to the group tables
+  uint32_t tables, scales;     // bytes from the stages' start to the group tables, and to the rows' scales
   int act, has_limit, zero_rest, bias_f16;
   float alpha, beta, limit;
   const int32_t* offsets;
@@ -348,7 +349,19 @@ __device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t
   }
 }
 
-template <bool F16, bool SWIGLU>
+// The order of a tile's stages along K: tiles begin at different ones, so that CTAs side by side do not read the same part of rows
+// that lie a power of two apart.
+struct Walk {
+  int k1, turn, steps;
+  __device__ __forceinline__ Walk(int k0, int k1, int tile) : k1(k1), turn(tile % (k1 - k0)), steps(k1 - k0) {}
+  __device__ __forceinline__ int at(int ks) const { return ks + turn < k1 ? ks + turn : ks + turn - steps; }
+};
+
+// STEPS: 128-byte steps along K of a stage. Two where four such stages fit (narrow tiles), and no more stages than these: fewer waits,
+// copies and signals a byte, 256 bytes of a row at a time, and with more loads under way than 128 KB an SM memory is slower. With the
+// walk: 64 tokens by 8 of 64 experts of 4096 x 2048 (six stages / five / four / and the walk) 95 / 94 / 91.5 / 89.8 us, 94.5 with 10
+// stages of one step; one token by 8 of 64 of 4096 x 4096 29.1 -> 27.5; 16 x 14336 x 4096 15.6 -> 14.5, 64 rows 16.4 -> 15.1.
+template <bool F16, bool SWIGLU, int STEPS>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Args a) {
   extern __shared__ uint8_t smem_raw[];
@@ -356,13 +369,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int S = a.stages;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  // a stage: [P tile 16 KB][Q tile tmax * 128]
+  // a stage: STEPS P tiles of 16 KB, then as many Q tiles of tmax * 128 bytes
+  constexpr uint32_t kPartP = kRows * kStepBytes;
+  const uint32_t part_q = static_cast<uint32_t>(a.tmax) * kStepBytes;
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], accfull[2], drained[2], done;
-  __shared__ float row_scale[kEpilogueWarps][kMaxT];  // a copy a warp: no barrier among them
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == kThreads - 32) {  // not warp 0, which reads the offsets
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -381,6 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const Tables tables = tables_at(gbase + a.tables, a.groups);
+  const int scale_pitch = (a.tmax + 31) & ~31;
+  float* const scales = reinterpret_cast<float*>(gbase + a.scales);  // of a tile's rows, a copy a warp: no barrier among them
   const bool fit = make_tables(a, tables);
   tc_fence_before();
   __syncthreads();
@@ -401,15 +417,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = first; ok && tile < tiles; tile += step) {
       const Tile t = tile_at<16>(a, tables, tile);
       const int copies = (t.width + a.box - 1) / a.box;
-      const uint32_t bytes = (kRows + copies * a.box) * kStepBytes;
+      const uint32_t bytes = STEPS * (kRows + copies * a.box) * kStepBytes;
       const int p_row = t.group * a.n + t.pt * kRows;
-      auto load_p = [&](int st, int ks) {
+      const Walk walk(k0, k1, tile);
+      auto load_p = [&](int st, int i_k) {
+        const int ks = walk.at(i_k);
         mbar_arrive_expect_tx(&full[st], bytes);
-        tma_load_2d(base + st * a.stage, &map_p, ks * kStepBytes, p_row, &full[st]);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) tma_load_2d(base + st * a.stage + i * kPartP, &map_p, (STEPS * ks + i) * kStepBytes, p_row, &full[st]);
       };
-      auto load_q = [&](int st, int ks) {
-        const uint32_t at = base + st * a.stage + kRows * kStepBytes;
-        if (lane < copies) tma_load_2d(at + lane * a.box * kStepBytes, &map_q, ks * kStepBytes, t.row0 + lane * a.box, &full[st]);
+      auto load_q = [&](int st, int i_k) {
+        const int ks = walk.at(i_k);
+        const uint32_t at = base + st * a.stage + STEPS * kPartP + lane * a.box * kStepBytes;
+        if (lane < copies) {
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) tma_load_2d(at + i * part_q, &map_q, (STEPS * ks + i) * kStepBytes, t.row0 + lane * a.box, &full[st]);
+        }
       };
       // The weights' first stages do not depend on the kernel before this one; the activations do.
       int pre = 0;
@@ -444,13 +467,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int h = (g > S ? g - S : 0); h < g; ++h) drain_wait(&full[h % S], (h / S) & 1, a.err, kErrDrain);
   } else if (warp == 1) {
     // The warp stays converged and elects the issuing lane, so that descriptors stay in uniform registers.
-    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + kRows * kStepBytes);
+    const uint64_t p_desc = umma_desc_sw128(base), q_desc = umma_desc_sw128(base + STEPS * kPartP);
     int i = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += step, ++i) {
       const uint32_t i_desc = instruction_desc(kRows, tile_at<16>(a, tables, tile).width);
       if (i >= 2 && !warp_spin(&drained[i & 1], ((i - 2) >> 1) & 1, ctl, kErrWaitMma)) break;
+      const Walk walk(k0, k1, tile);
       tc_fence_after();
       const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
       for (int ks = k0; ks < k1; ++ks) {
@@ -459,13 +483,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
-        const int subs = a.ksubs - 4 * ks;
+        const int subs = a.ksubs - 4 * STEPS * walk.at(ks);
         const uint32_t off = static_cast<uint32_t>(s) * (a.stage >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 4 * STEPS; ++j) {
             if (j > 0 && j >= subs) break;
-            mma_i8(d, p_desc + off + 2 * j, q_desc + off + 2 * j, i_desc, ks > k0 || j > 0);
+            mma_i8(d, p_desc + off + (j / 4) * (kPartP >> 4) + 2 * (j % 4), q_desc + off + (j / 4) * (part_q >> 4) + 2 * (j % 4), i_desc, ks > k0 || j > 0);
           }
           mma_commit(&empty[s]);
         }
@@ -484,12 +508,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int q = warp & 3, c = (warp - 2) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(32 * q) << 16;
+    float* const row_scale = scales + (warp - 2) * scale_pitch;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int i = 0;
     for (int tile = first; tile < tiles; tile += step, ++i) {
       const Tile t = tile_at<16>(a, tables, tile);
       const int b = i & 1, n = t.pt * kRows + 32 * q + lane;
-      const ChannelScale ch = prepare_scales(a, t, n, row_scale[warp - 2], lane);
+      const ChannelScale ch = prepare_scales(a, t, n, row_scale, lane);
       if (!warp_wait(&accfull[b], (i >> 1) & 1, ctl, kErrWaitEpilogue)) break;
       tc_fence_after();
       const uint32_t acc = tmem + lane_addr + (b ? a.acc1 : 0);
@@ -502,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 16; ++j) reinterpret_cast<int*>(gbase)[(col + j) * kPitch + 32 * q + lane] = static_cast<int>(v[j]);
         }
       } else {
-        drain_tile<F16, SWIGLU>(a, t, acc, c, n, ch, row_scale[warp - 2], lane);
+        drain_tile<F16, SWIGLU>(a, t, acc, c, n, ch, row_scale, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -526,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (a.split > 1) {
     // one tile a cluster: every rank sums its share of the columns over the ranks (128 values of a column lie together)
     cluster_sync();
-    if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, t, base, rank, row_scale[0], ch);
+    if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, t, base, rank, scales, ch);
     cluster_sync();  // nobody leaves while its partial tile is being read
   }
   zero_rest<F16>(a, fit, SWIGLU ? a.n / 2 : a.n);
@@ -1022,7 +1047,7 @@ int64_t most_tiles(const Int8Matmul& p, int64_t tmax, int64_t p_rows) {
 
 struct Launch {
   CUtensorMap p, q;
-  int grid, split;
+  int grid, split, steps;
   bool pairs, early;
   size_t smem;
 };
@@ -1055,7 +1080,8 @@ cudaError_t launch_kernel(const Launch& l, const Args& a, cudaStream_t s) {
 
 template <bool F16, bool SWIGLU>
 cudaError_t launch(const Launch& l, const Args& a, cudaStream_t s) {
-  return l.pairs ? launch_kernel<int8_gemm2_kernel<F16, SWIGLU>>(l, a, s) : launch_kernel<int8_gemm_kernel<F16, SWIGLU>>(l, a, s);
+  if (l.pairs) return launch_kernel<int8_gemm2_kernel<F16, SWIGLU>>(l, a, s);
+  return l.steps == 2 ? launch_kernel<int8_gemm_kernel<F16, SWIGLU, 2>>(l, a, s) : launch_kernel<int8_gemm_kernel<F16, SWIGLU, 1>>(l, a, s);
 }
 
 // Shared memory, stages, split of K and grid of single CTAs.
@@ -1067,12 +1093,17 @@ void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& 
   a.split = 1;
   while (a.split < most && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2;
   const uint32_t tables = tables_bytes(p.groups);
-  const int budget = kSmemBudget - 1024 - static_cast<int>(tables);
-  a.stage = static_cast<uint32_t>(kRows + a.tmax) * kStepBytes;
+  const uint32_t scales = static_cast<uint32_t>(kEpilogueWarps) * ((a.tmax + 31) & ~31) * 4;
+  const int budget = kSmemMost - 1024 - 1024 - static_cast<int>(tables + scales);  // what is declared; up to the first 1024-byte boundary
+  const uint32_t step = static_cast<uint32_t>(kRows + a.tmax) * kStepBytes;
+  l.steps = 8 * step <= static_cast<uint32_t>(budget) ? 2 : 1;  // (figures at the kernel)
+  a.ksteps = (a.ksteps + l.steps - 1) / l.steps;
+  a.stage = step * l.steps;
   const int steps = static_cast<int>(ceil_div(a.ksteps, a.split));
   const bool one_tile = a.split > 1 || tiles <= sms;
   int stages = budget / static_cast<int>(a.stage);
-  if (stages > kMaxStages) stages = kMaxStages;
+  const int most_stages = l.steps == 2 ? 4 : kMaxStages;
+  if (stages > most_stages) stages = most_stages;
   if (one_tile && stages > steps) stages = steps;
   if (a.split > 1) {  // all CTAs at once: those that share an SM share its memory
     const int together = static_cast<int>(ceil_div(tiles * a.split, sms));
@@ -1084,7 +1115,8 @@ void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& 
   const size_t partial = static_cast<size_t>(a.tmax) * kPitch * 4;
   if (a.split > 1 && smem < partial) smem = partial;
   a.tables = static_cast<uint32_t>(smem);
-  smem += tables + 1024;
+  a.scales = a.tables + tables;
+  smem += tables + scales + 1024;
   a.acc1 = one_tile ? 0 : a.tmax;
   a.tmem_cols = 32;
   while (a.tmem_cols < a.acc1 + a.tmax) a.tmem_cols *= 2;
