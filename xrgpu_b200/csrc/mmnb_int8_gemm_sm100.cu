@@ -17,7 +17,7 @@
 //
 // Measured (GPU time of the call, weights from memory): 1 x 4096 x 4096 float rows 7.7 us (16.8 MB, 2.2 TB/s: latency), 16 x 4096 x
 // 14336 16.7 us with the rows' quantisation (59 MB, 3.5 TB/s: start and end, then the stream), one token by 8 of 64 experts of
-// 4096 x 4096 27.5 us (134 MB, 4.9 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 89.5 us (540 MB, 6.0 TB/s), 2048 x
+// 4096 x 4096 26.9 us (134 MB, 5.0 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 89.5 us (540 MB, 6.0 TB/s), 2048 x
 // 14336 x 4096 85.6 us (2.8 PFLOP/s; tensor cores 78 % of the cycles, at 1.4 GHz under the power limit from the first launch on;
 // 99.6 us in calls back to back for seconds), 8192 x 8192 x 8192 372 us, 428 us for seconds (2.6 PFLOP/s at 1.24 GHz).
 //
@@ -51,8 +51,24 @@ constexpr unsigned kErrWaitMma = 0x712;
 constexpr unsigned kErrWaitEpilogue = 0x713;
 constexpr unsigned kErrDrain = 0x714;
 
+// n / d for n < 2^31 by a multiplication with ceil(2^p / d), p = 31 + ceil(log2 d) (Granlund and Montgomery, 1994).
+struct Divide {
+  uint32_t mul;  // 0: d = 1
+  int shift;
+};
+Divide divide_by(int d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  if (!l) return {0, 0};
+  return {static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1};
+}
+__device__ __forceinline__ int operator/(int n, const Divide& d) {
+  return d.mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.mul) >> d.shift) : n;
+}
+
 struct Args {
   int n, p_tiles, groups, rows;
+  Divide by_p, by_tmax;        // p_tiles, tmax
   int tmax, box;               // most rows of Q a tile (a multiple of 16); rows of one copy
   int ksteps, ksubs;           // stages along K, 32-value MMA steps along K
   int stages, split;
@@ -117,7 +133,7 @@ __device__ __forceinline__ bool make_tables(const Args& a, const Tables& t) {
       t.row_first[g] = lo;
       t.row_count[g] = hi - lo;
     }
-    int s = (hi - lo + a.tmax - 1) / a.tmax;
+    int s = (hi - lo + a.tmax - 1) / a.by_tmax;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(~0u, s, o);
@@ -152,19 +168,19 @@ struct Tile {
   int row0, rows;  // rows of the product
   int width;       // columns of the MMA: a multiple of GRAIN
 };
+// Whole warps. Little code: what every CTA runs before its first load comes from memory.
 template <int GRAIN>
 __device__ __forceinline__ Tile tile_at(const Args& a, const Tables& t, int tile) {
-  const int q = tile / a.p_tiles;
-  int lo = 0, hi = a.groups;  // the last group that begins at or before q
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (t.tile_first[mid] <= q) lo = mid;
-    else hi = mid;
-  }
-  const int first = t.tile_first[lo], nt = t.tile_first[lo + 1] - first, count = t.row_count[lo];
-  const int local = tile - first * a.p_tiles, pt = local / nt, qt = local - pt * nt;
+  const int q = tile / a.by_p, lane = threadIdx.x & 31;
+  // the last group that begins at or before q: among every 32nd, then among 32
+  int g = 0;
+  if (a.groups > 32) g = 32 * (__popc(__ballot_sync(~0u, 32 * lane < a.groups && t.tile_first[min(32 * lane, a.groups)] <= q)) - 1);
+  g += __popc(__ballot_sync(~0u, g + lane < a.groups && t.tile_first[min(g + lane, a.groups)] <= q)) - 1;
+  const int first = t.tile_first[g], nt = t.tile_first[g + 1] - first, count = t.row_count[g], local = tile - first * a.p_tiles;
+  if (nt == 1) return {g, local, t.row_first[g], count, (count + GRAIN - 1) / GRAIN * GRAIN};
+  const int pt = local / nt, qt = local - pt * nt;
   const int even = ((count + nt - 1) / nt + GRAIN - 1) / GRAIN * GRAIN, rows = min(even, count - qt * even);
-  return {lo, pt, t.row_first[lo] + qt * even, rows, (rows + GRAIN - 1) / GRAIN * GRAIN};
+  return {g, pt, t.row_first[g] + qt * even, rows, (rows + GRAIN - 1) / GRAIN * GRAIN};
 }
 
 // ------------------------------------------------------------------ results
@@ -397,9 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Tables tables = tables_at(gbase + a.tables, a.groups);
   const int scale_pitch = (a.tmax + 31) & ~31;
   float* const scales = reinterpret_cast<float*>(gbase + a.scales);  // of a tile's rows, a copy a warp: no barrier among them
-  const bool fit = make_tables(a, tables);
   tc_fence_before();
-  __syncthreads();
+  const bool fit = make_tables(a, tables);  // and a barrier
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   const Ctl ctl{&abort_flag, a.err};
@@ -885,9 +900,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   const Tables tables = tables_at(smem_raw + (base - raw) + a.tables, a.groups);
-  const bool fit = make_tables(a, tables);
   tc_fence_before();
-  __syncthreads();
+  const bool fit = make_tables(a, tables);
   cluster_sync();  // both CTAs' barriers are there
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
@@ -1242,10 +1256,12 @@ cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) 
   a.tmax = single_rows(p, sms);
   l.pairs = pairs_pay(p, a.tmax, sms);
   if (l.pairs) a.tmax = kMaxT;
+  a.by_tmax = divide_by(a.tmax);
   const int channels = l.pairs ? 2 * kRows : kRows;
   const int64_t tiles = most_tiles(p, a.tmax, channels);
   if (tiles > INT_MAX / 16) return cudaErrorInvalidValue;
   a.p_tiles = static_cast<int>(ceil_div(p.N, channels));
+  a.by_p = divide_by(a.p_tiles);
   if (l.pairs) {
     a.box = kRows;  // one copy a stage, of more rows than a narrow tile needs: a copy takes 28 cycles of its own (64 rows: 89.7 us, 128: 86.8)
     a.split = 1;
