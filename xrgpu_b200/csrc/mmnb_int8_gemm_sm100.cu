@@ -15,9 +15,9 @@
 // Roles (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 drain (lane quadrant warp % 4, alternate 16-column chunks).
 // Few tiles: K is split over a cluster of up to 8 CTAs whose int32 partial tiles meet in shared memory.
 //
-// Measured (GPU time of the call, weights from memory): 1 x 4096 x 4096 float rows 7.7 us (16.8 MB, 2.2 TB/s: latency), 16 x 4096 x
-// 14336 16.7 us with the rows' quantisation (59 MB, 3.5 TB/s: start and end, then the stream), one token by 8 of 64 experts of
-// 4096 x 4096 26.9 us (134 MB, 5.0 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 89.5 us (540 MB, 6.0 TB/s), 2048 x
+// Measured (GPU time of the call, weights from memory): 1 x 4096 x 4096 float rows 7.2 us (16.8 MB, 2.3 TB/s: latency), 16 x 4096 x
+// 14336 16.2 us with the rows' quantisation (59 MB, 3.6 TB/s: start and end, then the stream), one token by 8 of 64 experts of
+// 4096 x 4096 26.4 us (134 MB, 5.1 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 89.5 us (540 MB, 6.0 TB/s), 2048 x
 // 14336 x 4096 85.6 us (2.8 PFLOP/s; tensor cores 78 % of the cycles, at 1.4 GHz under the power limit from the first launch on;
 // 99.6 us in calls back to back for seconds), 8192 x 8192 x 8192 372 us, 428 us for seconds (2.6 PFLOP/s at 1.24 GHz).
 //
@@ -69,9 +69,9 @@ __device__ __forceinline__ int operator/(int n, const Divide& d) {
 struct Args {
   int n, p_tiles, groups, rows;
   Divide by_p, by_tmax;        // p_tiles, tmax
-  int tmax, box;               // most rows of Q a tile (a multiple of 16); rows of one copy
+  int tmax, box, box_log;      // most rows of Q a tile (a multiple of 16); rows of one copy (30: one copy takes all of a tile's)
   int ksteps, ksubs;           // stages along K, 32-value MMA steps along K
-  int stages, split;
+  int stages, split, split_log;
   int tmem_cols, acc1;         // acc1: column of the second accumulator
   int early;                   // the weights may be loaded before the previous kernel has finished
   uint32_t stage;              // bytes
@@ -96,6 +96,8 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a_desc, uint64_t b_d
       ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 
 // Instruction descriptor: int32 sums of signed 8-bit operands, both K-major, M rows, T columns.
 __device__ __forceinline__ uint32_t instruction_desc(int M, int T) {
@@ -168,7 +170,8 @@ struct Tile {
   int row0, rows;  // rows of the product
   int width;       // columns of the MMA: a multiple of GRAIN
 };
-// Whole warps. Little code: what every CTA runs before its first load comes from memory.
+// Whole warps. Little code, and no division for a group of one tile: what every CTA runs before its first load comes from memory, and
+// cost 5000 cycles (1 x 4096 x 4096 7.7 -> 7.2 us without, 333 x 1003 x 4100 13.8 -> 12.8).
 template <int GRAIN>
 __device__ __forceinline__ Tile tile_at(const Args& a, const Tables& t, int tile) {
   const int q = tile / a.by_p, lane = threadIdx.x & 31;
@@ -331,7 +334,7 @@ __device__ __forceinline__ void drain_tile(const Args& a, const Tile& t, uint32_
 template <bool F16, bool SWIGLU>
 __device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t base, int rank, const float* row_scale, const ChannelScale (&ch)[4]) {
   constexpr int kLanes = kRows / 4, kColumns = kThreads / kLanes;  // threads a column, columns at a time
-  const int share = (t.rows + a.split - 1) / a.split, col0 = rank * share, end = min(t.rows, col0 + share);
+  const int share = (t.rows + a.split - 1) >> a.split_log, col0 = rank * share, end = min(t.rows, col0 + share);
   const int row = 4 * (threadIdx.x % kLanes), n = t.pt * kRows + row;
   if (n >= a.n) return;
 #pragma unroll 1
@@ -365,13 +368,16 @@ __device__ __forceinline__ void sum_ranks(const Args& a, const Tile& t, uint32_t
   }
 }
 
-// The order of a tile's stages along K: tiles begin at different ones, so that CTAs side by side do not read the same part of rows
+// The order of a tile's stages along K: tiles next to each other begin at different ones, so that CTAs side by side do not read the same part of rows
 // that lie a power of two apart.
 struct Walk {
-  int k1, turn, steps;
-  __device__ __forceinline__ Walk(int k0, int k1, int tile) : k1(k1), turn(tile % (k1 - k0)), steps(k1 - k0) {}
+  int k1, steps, turn;
   __device__ __forceinline__ int at(int ks) const { return ks + turn < k1 ? ks + turn : ks + turn - steps; }
 };
+__device__ __forceinline__ Walk walk_of(int k0, int k1, int tile) {
+  const int steps = k1 - k0;
+  return {k1, steps, tile & ((1 << (31 - __clz(steps))) - 1)};
+}
 
 // STEPS: 128-byte steps along K of a stage. Two where four such stages fit (narrow tiles), and no more stages than these: fewer waits,
 // copies and signals a byte, 256 bytes of a row at a time, and with more loads under way than 128 KB an SM memory is slower. With the
@@ -393,6 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int abort_flag;
 
   if (threadIdx.x == kThreads - 32) {  // not warp 0, which reads the offsets
+    prefetch_map(&map_p);
+    prefetch_map(&map_q);
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -420,9 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Ctl ctl{&abort_flag, a.err};
   const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int tiles = tables.tile_first[a.groups] * a.p_tiles;
-  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
-  const int k0 = static_cast<int>(static_cast<int64_t>(a.ksteps) * rank / a.split);
-  const int k1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.split);
+  const int first = blockIdx.x >> a.split_log, step = gridDim.x >> a.split_log;
+  const int k0 = a.ksteps * rank >> a.split_log, k1 = a.ksteps * (rank + 1) >> a.split_log;
 
   if (warp == 0) {
     // One lane loads the weights and counts the bytes, copies of token rows are spread over the lanes.
@@ -431,10 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true, waited = false;
     for (int tile = first; ok && tile < tiles; tile += step) {
       const Tile t = tile_at<16>(a, tables, tile);
-      const int copies = (t.width + a.box - 1) / a.box;
+      const int copies = (t.width + (1 << a.box_log) - 1) >> a.box_log;
       const uint32_t bytes = STEPS * (kRows + copies * a.box) * kStepBytes;
       const int p_row = t.group * a.n + t.pt * kRows;
-      const Walk walk(k0, k1, tile);
+      const Walk walk = walk_of(k0, k1, tile);
       auto load_p = [&](int st, int i_k) {
         const int ks = walk.at(i_k);
         mbar_arrive_expect_tx(&full[st], bytes);
@@ -489,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = first; ok && tile < tiles; tile += step, ++i) {
       const uint32_t i_desc = instruction_desc(kRows, tile_at<16>(a, tables, tile).width);
       if (i >= 2 && !warp_spin(&drained[i & 1], ((i - 2) >> 1) & 1, ctl, kErrWaitMma)) break;
-      const Walk walk(k0, k1, tile);
+      const Walk walk = walk_of(k0, k1, tile);
       tc_fence_after();
       const uint32_t d = tmem + ((i & 1) ? a.acc1 : 0);
       for (int ks = k0; ks < k1; ++ks) {
@@ -589,6 +596,8 @@ struct FewRows {
   const void* x;
   int64_t ldx, K;
   int vec;         // rows of x start on 16 bytes and hold whole units of them
+  int parts;       // of a row
+  Divide by_parts;
   uint32_t codes, sums;  // bytes from the stages' start to the rows' codes, and to the sums sent by the ranks
 };
 
@@ -628,11 +637,11 @@ struct FewShared {
 template <bool XF16, bool VEC>
 __device__ __forceinline__ void quantise_rows(const Args& a, const FewRows& f, int k0, int k1, FewShared& sh, uint32_t codes) {
   const int warp = (threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
-  const int parts = (static_cast<int>(f.K) + kFewPart - 1) / kFewPart, items = a.rows * parts;
+  const int parts = f.parts, items = a.rows * parts;
   Part<XF16, VEC> held[kFewHeld];
 #pragma unroll
   for (int i = 0; i < kFewHeld; ++i) {
-    const int item = warp + 8 * i, row = item / parts;
+    const int item = warp + 8 * i, row = item / f.by_parts;
     if (item < items) held[i].load(f, row, (item - row * parts) * kFewPart + lane * 16);
   }
 #pragma unroll
@@ -640,7 +649,7 @@ __device__ __forceinline__ void quantise_rows(const Args& a, const FewRows& f, i
     const int item = warp + 8 * i;
     if (item >= items) break;
     const uint32_t m = __reduce_max_sync(~0u, held[i].amax());
-    if (lane == 0) atomicMax(&sh.largest[item / parts], m);
+    if (lane == 0) atomicMax(&sh.largest[item / f.by_parts], m);
   }
   asm volatile("bar.sync 1, 256;" ::: "memory");  // these eight warps, none of which leaves before
   if (lane < kFewRows) {
@@ -654,7 +663,7 @@ __device__ __forceinline__ void quantise_rows(const Args& a, const FewRows& f, i
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < kFewHeld; ++i) {
-    const int item = warp + 8 * i, row = item / parts, k = (item - row * parts) * kFewPart + lane * 16 - k0 * kStepBytes;
+    const int item = warp + 8 * i, row = item / f.by_parts, k = (item - row * parts) * kFewPart + lane * 16 - k0 * kStepBytes;
     if (item >= items) break;
     if (k < 0 || k >= (k1 - k0) * kStepBytes) continue;
     const Scale c = sh.scale[warp][row];
@@ -671,13 +680,18 @@ __device__ __forceinline__ void quantise_rows(const Args& a, const FewRows& f, i
 template <bool F16, bool SWIGLU>
 __device__ __forceinline__ void exchange_sums(const Args& a, const Tile& t, const uint32_t (&v)[16], uint32_t sums, int rank, int q, int n,
                                               const ChannelScale& ch, FewShared& sh, const float* row_scale, int lane, const Ctl& ctl) {
-  const int share = (t.rows + a.split - 1) / a.split, owners = (t.rows + share - 1) / share;
+  const int share = (t.rows + a.split - 1) >> a.split_log;
+  int owner = 0, at = 0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     if (j >= t.rows) break;
-    const int owner = j / share;  // at [rank][row of the owner][channel]
-    st_cluster_u32(map_rank(sums + ((rank * share + j - owner * share) * kRows + 32 * q + lane) * 4, owner), v[j]);
+    if (at == share) {
+      at = 0;
+      ++owner;
+    }
+    st_cluster_u32(map_rank(sums + ((rank * share + at++) * kRows + 32 * q + lane) * 4, owner), v[j]);  // at [rank][row of the owner][channel]
   }
+  const int owners = owner + 1;
   __syncwarp();
   if (lane < owners) arrive_at(&sh.summed, lane);
   if (rank >= owners) return;
@@ -705,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_few_kernel(const __grid_cons
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int S = a.stages;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0, pt = blockIdx.x / a.split;
+  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0, pt = blockIdx.x >> a.split_log;
   const Tile t{0, pt, 0, a.rows, kFewRows};
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -729,8 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_few_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_slot);
   const Ctl ctl{&sh.abort_flag, a.err};
-  const int k0 = static_cast<int>(static_cast<int64_t>(a.ksteps) * rank / a.split);
-  const int k1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.split), steps = k1 - k0;
+  const int k0 = a.ksteps * rank >> a.split_log, k1 = a.ksteps * (rank + 1) >> a.split_log, steps = k1 - k0;
   const uint32_t codes = base + f.codes, sums = base + f.sums;
   bool waited = false;  // for the cluster's barrier
   // All ranks' barriers have to be there before the first signal, which comes from the draining warps.
@@ -916,11 +929,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int tile = first; ok && tile < line.end; tile += step) {
       const Tile t = tile2_at(a, tables, line, tile);
       if (!t.rows) continue;
-      const int copies = (t.width / 2 + a.box - 1) / a.box, q_row = t.row0 + rank * (t.width / 2) + lane * a.box;
-      const uint32_t bytes = 2 * (kRows + copies * a.box) * kStepBytes, q_at = kPart2 + lane * a.box * kStepBytes;
+      const int q_row = t.row0 + rank * (t.width / 2);
       const int p_row = t.group * a.n + (2 * t.pt + rank) * kRows;
       auto load_p = [&](int st, int ks) {
-        if (rank == 0) mbar_arrive_expect_tx(&full[st], bytes);
+        if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kStage2);
         tma2_load_2d(base + st * kStage2, &map_p, ks * kStepBytes, p_row, map_rank(smem_u32(&full[st]), 0));
       };
       // The weights' first stages do not depend on the kernel before this one; the activations do.
@@ -944,7 +956,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (lane == 0) load_p(s, ks);
           __syncwarp();
         }
-        if (lane < copies) tma2_load_2d(base + s * kStage2 + q_at, &map_q, ks * kStepBytes, q_row, map_rank(smem_u32(&full[s]), 0));
+        if (lane == 0) tma2_load_2d(base + s * kStage2 + kPart2, &map_q, ks * kStepBytes, q_row, map_rank(smem_u32(&full[s]), 0));
         if (++s == kStages2) {
           s = 0;
           ph ^= 1;
@@ -1105,7 +1117,7 @@ void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& 
   // tiles of 128 rows - / 15.1 / 11.2 / 13.2, of 256 - / 17.9 / 13.9 / 20.4.
   const int most = a.tmax <= 32 ? 8 : 4;
   a.split = 1;
-  while (a.split < most && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2;
+  while (a.split < most && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2, ++a.split_log;
   const uint32_t tables = tables_bytes(p.groups);
   const uint32_t scales = static_cast<uint32_t>(kEpilogueWarps) * ((a.tmax + 31) & ~31) * 4;
   const int budget = kSmemMost - 1024 - 1024 - static_cast<int>(tables + scales);  // what is declared; up to the first 1024-byte boundary
@@ -1149,7 +1161,7 @@ bool few_shape(const Int8Matmul& p, int sms, Args& a, FewRows& f, Launch& l) {
   const int64_t tiles = ceil_div(p.N, kRows);
   if (tiles > sms) return false;
   a.split = 1;
-  while (a.split < 8 && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2;
+  while (a.split < 8 && tiles * a.split * 2 <= sms && a.ksteps >= 4 * a.split) a.split *= 2, ++a.split_log;
   const int64_t steps = ceil_div(a.ksteps, a.split), rows = steps * kFewStep;
   // a rank's sums: [ranks][its share of the rows][channels]
   const int64_t sums = a.split > 1 ? a.split * ceil_div(p.rows, a.split) * kRows * 4 : 0;
@@ -1157,6 +1169,8 @@ bool few_shape(const Int8Matmul& p, int sms, Args& a, FewRows& f, Launch& l) {
   if (stages > kMaxStages) stages = kMaxStages;
   if (stages > steps) stages = steps;
   if (stages < steps && stages < 6) return false;  // long rows: their codes leave too little for the weights
+  f.parts = static_cast<int>(ceil_div(p.K, kFewPart));
+  f.by_parts = divide_by(f.parts);
   a.stages = static_cast<int>(stages);
   a.p_tiles = static_cast<int>(tiles);
   f.codes = static_cast<uint32_t>(stages) * kFewStage;
@@ -1234,7 +1248,7 @@ bool int8_few_rows(const Int8Matmul& p) {
 
 cudaError_t launch_int8_few(const Int8Matmul& p, const void* x, bool x_f16, int64_t ldx, cudaStream_t s) {
   Args a = arguments(p);
-  FewRows f{x, ldx, p.K, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_f16 ? 2 : 4) % 16 == 0 && p.K % (x_f16 ? 8 : 4) == 0, 0, 0};
+  FewRows f{x, ldx, p.K, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (x_f16 ? 2 : 4) % 16 == 0 && p.K % (x_f16 ? 8 : 4) == 0, 0, {}, 0, 0};
   Launch l{};
   if (!few_shape(p, device_sm_count(), a, f, l) || !encode_tensor_map_2d(&l.p, 0, p.b, p.K, p.N, p.ldb, kStepBytes, kRows, true)) return cudaErrorInvalidValue;
   const bool swiglu = p.act == XRGPU_ACT_SWIGLU;
@@ -1273,6 +1287,7 @@ cudaError_t launch_int8_matmul(const Int8Matmul& p, bool early, cudaStream_t s) 
     // Rows of one copy: all of a dense tile; of a ragged one, whose last copy may reach into the next group's rows, large ones
     // too (16 rows a copy: 39 cycles each, 620 a stage of 256 rows).
     a.box = !p.offsets ? a.tmax : a.tmax % 64 == 0 ? 64 : 16;
+    a.box_log = !p.offsets ? 30 : a.tmax % 64 == 0 ? 6 : 4;
     single_shape(p, tiles, sms, a, l);
   }
   if (!encode_tensor_map_2d(&l.p, 0, p.b, p.K, static_cast<uint64_t>(p.groups) * p.N, p.ldb, kStepBytes, kRows, true) ||
