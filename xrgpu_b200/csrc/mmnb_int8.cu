@@ -14,7 +14,7 @@ constexpr unsigned kErrOrder = 0x702;
 // The row that row r stands for, -1 where it fits none (recorded).
 __device__ __forceinline__ int64_t source_row(const RowOrder& f, int64_t r) {
   if (!f.order) return r;
-  const int o = f.order[r], t = o / f.top_k;
+  const int o = f.order[r], t = o / f.by_top_k;
   if (o >= 0 && t < f.rows) return t;
   record_device_error(f.err, kErrOrder);
   return -1;

@@ -11,11 +11,29 @@
 
 namespace xrgpu {
 
+// n / d for 0 <= n < 2^31 by a multiplication with ceil(2^p / d), p = 31 + ceil(log2 d) (Granlund and Montgomery, 1994): kernels of a
+// few microseconds feel the code of a division, which comes from memory before the first load.
+struct Divide {
+  uint32_t mul;  // 0: d = 1
+  int shift;
+};
+inline Divide divide_by(int d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  if (!l) return {0, 0};
+  return {static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1};
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ int operator/(int n, const Divide& d) {
+  return d.mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.mul) >> d.shift) : n;
+}
+#endif
+
 // Row r stands for row order[r] / top_k of `rows` ones (order nullptr: for row r). An entry that fits none counts as a row of
 // zeros and is recorded.
 struct RowOrder {
   const int32_t* order;
-  int top_k;
+  Divide by_top_k;
   int64_t rows;
   unsigned* err;
 };

@@ -162,7 +162,7 @@ int forward(const xrgpu_int8_problem* c, void* ws, uint64_t ws_bytes, cudaStream
   p.err = device_error_word();
   if (in_place) return launched(launch_int8_few(p, c->a, c->a_dtype == XRGPU_FLOAT16, c->lda ? c->lda : c->K, s));
   if (p.rows) {
-    const RowOrder from{c->order, c->order ? static_cast<int>(c->top_k) : 1, c->M, p.err};
+    const RowOrder from{c->order, divide_by(c->order ? static_cast<int>(c->top_k) : 1), c->M, p.err};
     const bool made = c->a_dtype != XRGPU_INT8 || c->order;  // the operand, by a kernel before the product's
     if (made) {
       int8_t* codes = reinterpret_cast<int8_t*>(w);
@@ -173,7 +173,7 @@ int forward(const xrgpu_int8_problem* c, void* ws, uint64_t ws_bytes, cudaStream
       if (quantise_once(*c)) {
         int8_t* tokens = reinterpret_cast<int8_t*>(w + l.tokens);
         float* token_scales = reinterpret_cast<float*>(w + l.token_scales);
-        st = launched(launch_int8_quantize({f16, c->M, c->K, ldx, ld, c->a, tokens, token_scales, nullptr, {nullptr, 1, c->M, p.err}}, s));
+        st = launched(launch_int8_quantize({f16, c->M, c->K, ldx, ld, c->a, tokens, token_scales, nullptr, {nullptr, {}, c->M, p.err}}, s));
         if (!st) st = launched(launch_int8_gather({p.rows, c->K, ld, ld, from, tokens, token_scales, codes, scales}, true, s));
       } else if (c->a_dtype != XRGPU_INT8) {
         st = launched(launch_int8_quantize({f16, p.rows, c->K, ldx, ld, c->a, codes, scales, nullptr, from}, s));

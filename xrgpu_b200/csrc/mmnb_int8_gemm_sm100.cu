@@ -51,21 +51,6 @@ constexpr unsigned kErrWaitMma = 0x712;
 constexpr unsigned kErrWaitEpilogue = 0x713;
 constexpr unsigned kErrDrain = 0x714;
 
-// n / d for n < 2^31 by a multiplication with ceil(2^p / d), p = 31 + ceil(log2 d) (Granlund and Montgomery, 1994).
-struct Divide {
-  uint32_t mul;  // 0: d = 1
-  int shift;
-};
-Divide divide_by(int d) {
-  int l = 0;
-  while ((int64_t(1) << l) < d) ++l;
-  if (!l) return {0, 0};
-  return {static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1};
-}
-__device__ __forceinline__ int operator/(int n, const Divide& d) {
-  return d.mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.mul) >> d.shift) : n;
-}
-
 struct Args {
   int n, p_tiles, groups, rows;
   Divide by_p, by_tmax;        // p_tiles, tmax

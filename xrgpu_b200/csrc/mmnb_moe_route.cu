@@ -11,7 +11,7 @@
 // Order: a counting sort. Every warp counts its own tokens' experts, the counts are summed over the warps and CTAs before it, and
 // each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: the CTAs of one
 // cluster read each other's counts; else a second kernel follows in which every CTA sums the counts of all (from L2).
-// Measured (8 experts a token): 64 tokens x 128 experts 5.6 us, 1024 7.9, 32768 20.1; 8192 x 256 of float32 with weights of all 15.5
+// Measured (8 experts a token): 64 tokens x 128 experts 5.6 us, 1024 7.9, 32768 20.1; 8192 x 256 of float32 with weights of all 15.0
 // (9.5 MB: 1.4 us at the copy rate; the choice takes 9 of them, the order 6).
 #include <cuda_fp16.h>
 
@@ -33,6 +33,7 @@ struct Args {
   int ctas;
   int per_warp;   // tokens of a warp, in a row
   int32_t* counts;  // [ctas, experts]
+  Divide by_width;  // experts up to whole warps
 };
 
 // A key that orders like the score; 0 is below every score. -0 equals 0, NaN -infinity.
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) place_kernel(const Args a) {
     __syncwarp();
   }
   // Groups of threads take every groups-th CTA's counts, an expert a thread.
-  const int width = (E + 31) & ~31, groups = kThreads / width, g = threadIdx.x / width, e = threadIdx.x % width;
+  const int width = (E + 31) & ~31, groups = kThreads / a.by_width, g = static_cast<int>(threadIdx.x) / a.by_width, e = threadIdx.x - g * width;
   int total = 0, before = 0;
   if (g < groups && e < E) {
 #pragma unroll 16
@@ -366,6 +367,7 @@ cudaError_t launch_moe_route(const MoeRoute& p, void* ws, cudaStream_t s) {
   a.per_warp = per_warp(p);
   a.ctas = static_cast<int>(ceil_div(p.tokens, static_cast<int64_t>(kWarps) * a.per_warp));
   a.counts = static_cast<int32_t*>(ws);
+  a.by_width = divide_by((p.experts + 31) & ~31);
   if (p.experts <= 32) return launch<1>(a, s);
   if (p.experts <= 64) return launch<2>(a, s);
   if (p.experts <= 128) return launch<4>(a, s);
