@@ -234,7 +234,8 @@ def _codes(g, rows, K):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (2, 7, 15), (16, 129, 33), (17, 1003, 4100), (33, 2, 127), (64, 640, 2048), (128, 256, 129),
          (129, 300, 31), (200, 128, 16), (255, 513, 256), (257, 1000, 300), (300, 2049, 128), (1000, 384, 100), (700, 5000, 64), (2049, 700, 257), (2300, 3000, 200), (1030, 9002, 128), (5000, 1500, 96),
-         (2048, 5000, 100), (1600, 6500, 700), (4000, 2600, 1300), (260, 15000, 515), (3100, 11000, 140)]
+         (2048, 5000, 100), (1600, 6500, 700), (4000, 2600, 1300), (260, 15000, 515), (3100, 11000, 140),
+         (2300, 3001, 1057), (260, 15000, 1100), (1030, 9002, 1130), (530, 7000, 1025), (9000, 4000, 96)]
 
 
 @gpu
@@ -448,7 +449,8 @@ def _grouped(F, E, R_, N, K, dtype, bias, act, kind, order=None, top_k=1, M=None
 GROUPS = [(1, 40, 130, 70, "even"), (3, 0, 16, 32, "even"), (8, 8, 256, 300, "even"), (5, 33, 7, 100, "ragged"), (33, 64, 128, 2048, "ragged"),
           (64, 500, 384, 96, "ragged"), (12, 2000, 200, 1000, "ragged"), (7, 700, 1030, 64, "one"), (300, 900, 20, 33, "ragged"),
           (1024, 1500, 4, 16, "ragged"), (4, 1100, 2500, 256, "even"), (2, 1, 4096, 1024, "one"),
-          (20, 6000, 1000, 700, "ragged"), (3, 2000, 3000, 130, "one"), (9, 9000, 1500, 900, "ragged"), (16, 4096, 2048, 640, "even")]
+          (20, 6000, 1000, 700, "ragged"), (3, 2000, 3000, 130, "one"), (9, 9000, 1500, 900, "ragged"), (16, 4096, 2048, 640, "even"),
+          (20, 3000, 1000, 1100, "ragged"), (3, 2000, 1502, 1030, "one"), (40, 9000, 1300, 100, "ragged")]
 
 
 @gpu

@@ -1218,9 +1218,14 @@ int single_rows(const Int8Matmul& p, int sms) {
   return static_cast<int>(t > kMaxT ? kMaxT : t);
 }
 
-// Pairs take what fills most of the SMs with tiles of 128 channels by 256 rows. Measured (us, single CTAs / pairs): 256 x 14336 x 4096
-// (112 tiles) 22.5 / 20.7, 1024 x 4096 x 4096 (128) 20.8 / 20.0, 512 x 4096 x 4096 (64) 16.9 / 19.4.
-bool pairs_pay(const Int8Matmul& p, int tmax, int sms) { return tmax >= 128 && 10 * most_tiles(p, kMaxT, kRows) >= 7 * sms; }
+// Pairs take what fills most of the SMs with tiles of 128 channels by 256 rows, but for short rows only what fills them several
+// times. Measured (us, single CTAs / pairs): 256 x 14336 x 4096 (112 tiles) 22.5 / 20.7, 1024 x 4096 x 4096 (128) 20.8 / 20.0, 512 x 4096 x
+// 4096 (64) 16.9 / 19.4; 512 x 8192 x 512 (128) 8.2 / 9.3, 2000 x 4096 x 1024 (256) 13.9 / 14.1, 1000 tokens by 4 of 16 experts of 1500 x
+// 768 (372 at the most) 24.9 / 25.7, 1500 by 4 of 16 of 2048 x 2048 (608) 43.3 / 40.4.
+bool pairs_pay(const Int8Matmul& p, int tmax, int sms) {
+  const int64_t tiles = most_tiles(p, kMaxT, kRows);
+  return tmax >= 128 && 10 * tiles >= (p.K > 1024 ? 7 : 25) * sms;
+}
 
 }  // namespace
 
