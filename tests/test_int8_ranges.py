@@ -1,0 +1,46 @@
+"""8-bit integer operators at the ends of their ranges: subnormal scales."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import int8_reference as R
+from test_int8 import F, gpu  # noqa: F401
+
+
+# ------------------------------------------------------------------------------------------ subnormal scales
+def _units(u):
+    """Multiples of 2^-149, the smallest float32 step, as they are."""
+    u = np.asarray(u, np.int64)
+    return torch.from_numpy((np.abs(u) | np.where(u < 0, 1 << 31, 0)).astype(np.uint32).view(np.float32).copy())
+
+
+@gpu
+@pytest.mark.parametrize("K", [5, 8, 100, 9000])
+def test_codes_of_subnormal_scales_saturate(F, K):
+    """A scale of few bits may lie a third under max|x| / 127: quotients up to 190, also those that leave no remainder. Every
+    largest magnitude up to the one where the scale has all its quotients within 127, and beyond."""
+    most = 17000 if K < 100 else 700
+    u = np.zeros((most, K), np.int64)
+    top = np.arange(most)
+    for i, v in enumerate((top, -top, top // 2, -(top // 3), top - 1)):
+        u[:, (i * 7) % K] = np.where(top > 0, v, 0)
+    x = _units(u)
+    codes, scales = R.quantize(x.double().numpy())
+    c, s = F.int8_quantize(x.cuda())
+    assert np.array_equal(s.cpu().double().numpy(), scales) and np.array_equal(c.cpu().numpy(), codes)
+
+
+@gpu
+@pytest.mark.parametrize("M", [12, 40])
+def test_products_of_subnormal_rows_saturate(F, M):
+    """Rows quantised by the product (12: in the product's own kernel), by weights that pick out one code each."""
+    K = 64
+    top = np.resize([128, 130, 190, 191, 5000, 127, 254, 71, 317, 1, 63, 64], M)
+    u = np.zeros((M, K), np.int64)
+    u[:, 0], u[:, 1], u[:, 9], u[:, 40] = top, -top, top // 2, -(top // 4)
+    x = _units(u)
+    codes, scales = R.quantize(x.double().numpy())
+    w = torch.eye(K, dtype=torch.int8, device="cuda")
+    y = F.matmul_int8(x.cuda(), w, torch.full((K,), 2.0 ** 40, device="cuda"))
+    assert np.array_equal(y.cpu().double().numpy(), codes * scales[:, None] * 2.0 ** 40)  # a code by a scale of few bits: exact

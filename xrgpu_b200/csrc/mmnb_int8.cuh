@@ -4,7 +4,7 @@
 // computed: r = round(x * (1 / s)) is the code or, next to a border, one off it. What is left, x - r s, is exact in one fused step
 // (it has no bit below both numbers' last ones and is at most about s / 2), so comparing it with s / 2 decides, and with r's
 // last bit a tie. Float32 rows of scales under 2^-60 are brought up by 2^100 first (exact as well); where s has
-// only a few bits left (subnormal), codes saturate. A row with a NaN or an infinity has scale NaN and codes 0.
+// only a few bits left (subnormal), x / s may be up to 190, and codes saturate. A row with a NaN or an infinity has scale NaN and codes 0.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -76,7 +76,9 @@ __device__ __forceinline__ void codes_of(const float (&v)[N], const Scale& c, ui
     b[i + 1] = __float_as_uint(code.y);
     worst = fmaxf(fmaxf(worst, fabsf(left.x)), fabsf(left.y));
   }
-  if (worst >= 0.5f * c.s) {  // hardly ever: a tie, a code one off, or one that saturates
+  // Hardly ever: a tie or a code one off; small scales, whose quotients may exceed 127 and leave nothing (the last bits of a word that
+  // was not clamped are another code: 128 units of 2^-149 by a scale of one came out as -128).
+  if (worst >= 0.5f * c.s || (!F16 && c.up != 1.0f)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float x = F16 ? v[i] : v[i] * c.up, r = __uint_as_float(b[i]) - kMagic, left = fmaf(-r, c.s, x);
