@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <atomic>
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include "xrgpu_mmnb.h"
@@ -30,16 +31,22 @@ struct Problem {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t align_up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
 
-// Lets `Kernel` use up to `bytes` of dynamic shared memory on the current device (asked of the runtime once a device).
+// Lets `Kernel` use up to `bytes` of dynamic shared memory on the current device (asked of the runtime once a device and size).
+// Calls of different sizes may come from several threads: the limit is only raised, by one of them at a time, so that it is never below
+// what a call was promised.
 template <auto Kernel>
 cudaError_t allow_smem(int bytes) {
   static std::atomic<int> allowed[64];
+  static std::mutex raising;
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && allowed[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  const std::lock_guard<std::mutex> one(raising);
+  if (known && allowed[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
   const cudaError_t f = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (f == cudaSuccess && dev >= 0 && dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
+  if (f == cudaSuccess && known) allowed[dev].store(bytes, std::memory_order_release);
   return f;
 }
 
