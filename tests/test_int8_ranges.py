@@ -1,11 +1,11 @@
-"""8-bit integer operators at the ends of their ranges: subnormal scales."""
+"""8-bit integer operators at the ends of their ranges: subnormal scales, empty orders and sums."""
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import int8_reference as R
-from test_int8 import F, gpu  # noqa: F401
+from test_int8 import F, FULL, gpu  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------ subnormal scales
@@ -44,3 +44,25 @@ def test_products_of_subnormal_rows_saturate(F, M):
     w = torch.eye(K, dtype=torch.int8, device="cuda")
     y = F.matmul_int8(x.cuda(), w, torch.full((K,), 2.0 ** 40, device="cuda"))
     assert np.array_equal(y.cpu().double().numpy(), codes * scales[:, None] * 2.0 ** 40)  # a code by a scale of few bits: exact
+
+
+# ------------------------------------------------------------------------------------------ nothing to do
+@gpu
+@pytest.mark.parametrize("floats", [True, False])
+def test_no_rows_of_some_tokens(F, floats):
+    """Tokens of which none chose one of these experts, and sums for no tokens."""
+    w, ws = F.int8_quantize(torch.ones(4, 48, 64, device="cuda"))
+    x, kw = torch.ones(6, 64, device="cuda"), dict(dtype=FULL)
+    if not floats:
+        x, kw["a_scales"] = F.int8_quantize(x)
+    off = torch.zeros(5, dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert F.matmul_int8_grouped(x, w, ws, off, order=none, top_k=2, **kw).shape == (0, 48)
+    slots, weights = torch.full((6, 2), -1, dtype=torch.int32, device="cuda"), torch.ones(6, 2, device="cuda")
+    y = F.matmul_int8_grouped(x, w, ws, off, order=none, top_k=2, slots=slots, weights=weights, **kw)
+    assert y.shape == (6, 48) and (y == 0).all()
+    off[1:] = 6
+    assert F.matmul_int8_grouped(x, w, ws, off, slots=slots[:0], weights=weights[:0], **kw).shape == (0, 48)
+    out = torch.full((3, 48), 5.0, device="cuda")
+    assert F.matmul_int8_grouped(x, w, ws, off, slots=slots[:0], weights=weights[:0], out=out[:0], **kw).shape == (0, 48)
+    assert (out == 5).all() and F.device_error() == 0

@@ -818,10 +818,11 @@ def matmul_int8_grouped(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor
         raise ValueError("a product takes 1 to 1024 groups")
     p, index, dtype, n = _int8_problem(a, a_scales, b, b_scales, bias, activation, alpha, beta, limit, dtype)
     p.groups, p.offsets, p.rows, p.top_k = E, _small(offsets, "offsets", torch.int32, (E + 1,), index), a.shape[0], int(top_k)
+    some = p.offsets  # stands for the address of an empty tensor, which has none: it is given, and not read
     if order is not None:
         if order.dim() != 1:
             raise ValueError("order must be [rows]")
-        p.order, p.rows = _small(order, "order", torch.int32, order.shape, index), order.shape[0]
+        p.order, p.rows = _small(order, "order", torch.int32, order.shape, index) or some, order.shape[0]
     rows = p.rows
     if (slots is None) != (weights is None):
         raise ValueError("slots and weights belong together")
@@ -830,8 +831,8 @@ def matmul_int8_grouped(a: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor
             raise ValueError("slots must be [tokens, k]")
         if order is not None and slots.shape[1] != top_k:
             raise ValueError("slots must have top_k columns")
-        p.slots = _small(slots, "slots", torch.int32, slots.shape, index)
-        p.weights = _small(weights, "weights", torch.float32, slots.shape, index)
+        p.slots = _small(slots, "slots", torch.int32, slots.shape, index) or some
+        p.weights = _small(weights, "weights", torch.float32, slots.shape, index) or some
         p.tokens, p.top_k = slots.shape
         rows = p.tokens
     p.zero_rest = int(out is None)
