@@ -1,11 +1,12 @@
-"""8-bit integer operators at the ends of their ranges: subnormal scales, empty orders and sums."""
+"""8-bit integer operators at the ends of their ranges: subnormal scales, scales whose products leave float32 on the way,
+empty orders and sums."""
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import int8_reference as R
-from test_int8 import F, FULL, gpu  # noqa: F401
+from test_int8 import F, FULL, _codes, _groups, _summed, gpu  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------ subnormal scales
@@ -44,6 +45,68 @@ def test_products_of_subnormal_rows_saturate(F, M):
     w = torch.eye(K, dtype=torch.int8, device="cuda")
     y = F.matmul_int8(x.cuda(), w, torch.full((K,), 2.0 ** 40, device="cuda"))
     assert np.array_equal(y.cpu().double().numpy(), codes * scales[:, None] * 2.0 ** 40)  # a code by a scale of few bits: exact
+
+
+# ------------------------------------------------------------------------------------------ scales far apart
+def _far_scales(g, M, N):
+    """Rows of ordinary scales, of ones whose product with a sum leaves float32, and channels that bring it back."""
+    sa = torch.exp2(torch.randint(-20, 6, (M,), generator=g).float())
+    far = torch.rand(M, generator=g) < 0.5
+    sa[far] = torch.exp2(96 + 31 * torch.rand(int(far.sum()), generator=g))
+    sa[0] = 2.0 ** 127
+    sign = lambda n: torch.where(torch.rand(n, generator=g) < 0.2, -1.0, 1.0)  # noqa: E731
+    return sa * sign(M), torch.exp2(-100 - 20 * torch.rand(N, generator=g)) * sign(N)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 130, 4096), (40, 130, 70), (16, 4096, 2048), (333, 1004, 1100), (700, 5000, 300), (2300, 3000, 1057)])
+@pytest.mark.parametrize("act,bias", [("none", False), ("relu", True), ("swiglu", True)])
+def test_scales_far_apart(F, M, N, K, act, bias):
+    g = torch.Generator().manual_seed(M + K)
+    a, ad, _ = _codes(g, M, K)
+    b, bd, _ = _codes(g, N, K)
+    if M > 3:
+        a[3], ad[3] = 0, 0
+    sa, sb = _far_scales(g, M, N)
+    v = torch.randn(N, generator=g) if bias else None
+    want, err = R.product(a, sa.double().numpy(), b, sb.double().numpy(), v.double().numpy() if bias else None, act)
+    y = F.matmul_int8(ad, bd, sb.cuda(), v.cuda() if bias else None, a_scales=sa.cuda(), activation=act, dtype=FULL)
+    R.close(y, want, err, FULL)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(3, 256, 1024), (16, 2000, 600), (50, 200, 1000)])
+def test_float_rows_of_large_numbers(F, M, N, K):
+    g = torch.Generator().manual_seed(M)
+    x = torch.rand(M, K, generator=g) * 3e38
+    x[1] *= 2.0 ** -120
+    b, bd, _ = _codes(g, N, K)
+    sb = torch.rand(N, generator=g) * 2.0 ** -60
+    a, sa = R.quantize(x.double().numpy())
+    want, err = R.product(a, sa, b, sb.double().numpy())
+    R.close(F.matmul_int8(x.cuda(), bd, sb.cuda()), want, err, FULL)
+
+
+@gpu
+def test_grouped_rows_of_large_scales(F):
+    g = torch.Generator().manual_seed(2)
+    E, rows, N, K, k = 5, 300, 150, 200, 3
+    a, ad, _ = _codes(g, rows, K)
+    b, bd, _ = _codes(g, E * N, K)
+    sa, sb = _far_scales(g, rows, E * N)
+    off = _groups(E, rows, 1, "ragged")
+    want, err = np.zeros((rows, N)), np.zeros((rows, N))
+    for e in range(E):
+        lo, hi = off[e], off[e + 1]
+        if lo < hi:
+            want[lo:hi], err[lo:hi] = R.product(a[lo:hi], sa[lo:hi].double().numpy(), b.reshape(E, N, K)[e], sb.view(E, N)[e].double().numpy())
+    args = (ad, bd.unflatten(0, (E, N)), sb.view(E, N).cuda(), torch.from_numpy(off).int().cuda())
+    kw = dict(a_scales=sa.cuda(), dtype=FULL)
+    R.close(F.matmul_int8_grouped(*args, **kw), want, err, FULL)
+    slots = torch.randperm(rows, generator=g).view(-1, k)
+    weights = torch.rand(slots.shape, generator=g)
+    y = F.matmul_int8_grouped(*args, **kw, slots=slots.int().cuda(), weights=weights.cuda())
+    R.close(y, *_summed(want, err, slots.numpy(), weights.numpy()), FULL)
 
 
 # ------------------------------------------------------------------------------------------ nothing to do
