@@ -1,5 +1,5 @@
 """8-bit integer operators at the ends of their ranges: subnormal scales, scales whose products leave float32 on the way,
-empty orders and sums."""
+empty orders and sums, K split over a cluster."""
 import numpy as np
 import pytest
 
@@ -107,6 +107,19 @@ def test_grouped_rows_of_large_scales(F):
     weights = torch.rand(slots.shape, generator=g)
     y = F.matmul_int8_grouped(*args, **kw, slots=slots.int().cuda(), weights=weights.cuda())
     R.close(y, *_summed(want, err, slots.numpy(), weights.numpy()), FULL)
+
+
+# ------------------------------------------------------------------------------------------ K split over a cluster
+@gpu
+@pytest.mark.parametrize("M", [20, 40, 67, 75, 90, 107, 128, 139, 155, 250])
+@pytest.mark.parametrize("N,K", [(130, 4096), (1000, 2050)])
+def test_split_products_of_every_width(F, M, N, K):
+    g = torch.Generator().manual_seed(M + N)
+    a, ad, sa = _codes(g, M, K)
+    b, bd, sb = _codes(g, N, K)
+    want, err = R.product(a, sa.double().numpy(), b, sb.double().numpy())
+    R.close(F.matmul_int8(ad, bd, sb.cuda(), a_scales=sa.cuda(), dtype=FULL), want, err, FULL)
+    assert F.device_error() == 0
 
 
 # ------------------------------------------------------------------------------------------ nothing to do

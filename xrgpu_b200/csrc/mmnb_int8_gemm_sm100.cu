@@ -1136,11 +1136,6 @@ void single_shape(const Int8Matmul& p, int64_t tiles, int sms, Args& a, Launch& 
   const int most_stages = l.steps == 2 ? 4 : kMaxStages;
   if (stages > most_stages) stages = most_stages;
   if (one_tile && stages > steps) stages = steps;
-  if (a.split > 1) {  // all CTAs at once: those that share an SM share its memory
-    const int together = static_cast<int>(ceil_div(tiles * a.split, sms));
-    const int fit = (budget / together - 11 * 1024) / static_cast<int>(a.stage);
-    if (stages > fit && fit >= 2) stages = fit;
-  }
   a.stages = stages;
   size_t smem = static_cast<size_t>(stages) * a.stage;
   const size_t partial = static_cast<size_t>(a.tmax) * kPitch * 4;

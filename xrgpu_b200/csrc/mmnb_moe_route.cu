@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) place_kernel(const Args a) {
   place(a, r.t0, r.t1, hist, total, before, blockIdx.x == 0);
 }
 
-// Tokens that one cluster takes: one or two a warp.
+// Tokens that one cluster takes: one a warp.
 bool one_cluster(const MoeRoute& p) { return p.tokens <= kClusterTokens; }
 
 int per_warp(const MoeRoute& p) {
