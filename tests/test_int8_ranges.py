@@ -1,12 +1,12 @@
 """8-bit integer operators at the ends of their ranges: subnormal scales, scales whose products leave float32 on the way,
-empty orders and sums, K split over a cluster."""
+empty orders and sums, K split over a cluster, float rows read several times."""
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import int8_reference as R
-from test_int8 import F, FULL, _codes, _groups, _summed, gpu  # noqa: F401
+from test_int8 import F, FULL, HALF, _codes, _groups, _summed, _values, gpu  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------ subnormal scales
@@ -142,3 +142,71 @@ def test_no_rows_of_some_tokens(F, floats):
     out = torch.full((3, 48), 5.0, device="cuda")
     assert F.matmul_int8_grouped(x, w, ws, off, slots=slots[:0], weights=weights[:0], out=out[:0], **kw).shape == (0, 48)
     assert (out == 5).all() and F.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------ float rows read several times
+@gpu
+@pytest.mark.parametrize("T,E,k,N,K", [(1100, 7, 4, 130, 2048), (1100, 5, 4, 66, 2050), (1000, 9, 4, 96, 2050), (300, 3, 32, 64, 1000)])
+@pytest.mark.parametrize("dtype,act", [(HALF, "swiglu"), (FULL, "none")])
+def test_float_tokens_read_several_times(F, dtype, act, T, E, k, N, K):
+    """Gathered float rows on both sides of the size from which tokens are quantised once: strided, in turn with new ones, entries
+    that fit no row among them, as rows and as sums."""
+    rng = np.random.default_rng(T + K)
+    rows = T * k
+    g = torch.Generator().manual_seed(K)
+    b, bd, sb = _codes(g, E * N, K)
+    bd, sb = bd.unflatten(0, (E, N)), (sb / K ** 0.5).view(E, N)
+    wide = torch.zeros(T, K + 13, dtype=dtype, device="cuda")
+    slots, weights = rng.permutation(rows).reshape(T, k), rng.normal(size=(T, k)).astype(np.float32)
+    sums = dict(slots=torch.from_numpy(slots).int().cuda(), weights=torch.from_numpy(weights).cuda())
+    calls = []
+    for turn, lead in enumerate((0, 8, 3)):
+        x = _values(T, K, dtype, turn + K)
+        x[5], x[6, K - 1] = 0.0, float("nan")
+        order = rng.permutation(rows) if turn else np.repeat(rng.permutation(T), k) * k
+        if turn == 2:
+            order[[0, 7, rows - 1]] = [-1, rows, 2 ** 31 - 1]
+        off = _groups(E, rows, turn, "ragged")
+        wide[:, lead:lead + K].copy_(x)
+        args = (wide[:, lead:lead + K], bd, sb.cuda(), torch.from_numpy(off).int().cuda())
+        kw = dict(order=torch.from_numpy(order).int().cuda(), top_k=k, activation=act)
+        calls.append((x, order, off, F.matmul_int8_grouped(*args, **kw), F.matmul_int8_grouped(*args, **kw, **sums)))
+    assert F.device_error() == 0x702
+    for x, order, off, y, s in calls:
+        codes, scales = R.quantize(x.double().numpy())
+        fits = (order >= 0) & (order < rows)
+        token = np.where(fits, order // k, 0)
+        a, sa = np.where(fits[:, None], codes[token], 0), np.where(fits, scales[token], 0.0)
+        want, err = np.zeros((rows, N // 2 if act == "swiglu" else N)), np.zeros((rows, N // 2 if act == "swiglu" else N))
+        for e in range(E):
+            lo, hi = off[e], off[e + 1]
+            if lo < hi:
+                want[lo:hi], err[lo:hi] = R.product(a[lo:hi], np.nan_to_num(sa[lo:hi]), b.reshape(E, N, K)[e], sb[e].double().numpy(), None, act)
+        want[np.isnan(sa)] = np.nan
+        R.close(y, want, err, dtype)
+        R.close(s, *_summed(want, err, slots, weights), dtype)
+
+
+@gpu
+def test_captured_tokens_read_several_times(F):
+    """The chain of quantisation, copies and product in a graph, replayed with new tokens and another order."""
+    g = torch.Generator().manual_seed(1)
+    T, E, k, N, K = 1100, 6, 4, 128, 2048
+    w, ws = F.int8_quantize(torch.randn(E, N, K, generator=g).cuda())
+    x, scores = torch.randn(T, K, generator=g, dtype=HALF).cuda(), torch.randn(T, E, generator=g).cuda()
+
+    def layer():
+        r = F.moe_route(scores, k)
+        return F.matmul_int8_grouped(x, w, ws, r.offsets, order=r.order, top_k=k, slots=r.slots, weights=r.weights)
+
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer()
+    for turn in range(4):
+        x.copy_(torch.randn(T, K, generator=g, dtype=HALF))
+        scores.copy_(torch.randn(T, E, generator=g))
+        graph.replay()
+        assert torch.equal(y, layer())
+    assert F.device_error() == 0

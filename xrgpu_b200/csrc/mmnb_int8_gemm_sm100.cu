@@ -1234,9 +1234,12 @@ int single_rows(const Int8Matmul& p, int sms) {
 }
 
 // Pairs take what fills most of the SMs with tiles of 128 channels by 256 rows, but for short rows only what fills them several
-// times. Measured (us, single CTAs / pairs): 256 x 14336 x 4096 (112 tiles) 22.5 / 20.7, 1024 x 4096 x 4096 (128) 20.8 / 20.0, 512 x 4096 x
-// 4096 (64) 16.9 / 19.4; 512 x 8192 x 512 (128) 8.2 / 9.3, 2000 x 4096 x 1024 (256) 13.9 / 14.1, 1000 tokens by 4 of 16 experts of 1500 x
-// 768 (372 at the most) 24.9 / 25.7, 1500 by 4 of 16 of 2048 x 2048 (608) 43.3 / 40.4.
+// times. Measured (us, single CTAs / pairs; tiles as counted here): 512 x 4096 x 4096 (64) 14.7 / 17.2, 512 x 6144 x 2048 (96) 13.1 / 13.3, 256 x
+// 14336 x 4096 (112) 21.0 / 20.2, 1024 x 4096 x 4096 (128) 18.9 / 18.5, 1500 tokens by 4 of 16 experts of 2048 x 2048 (624) 43.0 / 40.8. Short
+// rows: 512 x 8192 x 512 (128) 8.1 / 9.1, 2000 x 4096 x 1024 (256) 14.1 / 14.3, 2560 x 5120 x 768 (400) 17.7 / 17.7, 2560 x 6400 x 1024 (500)
+// 23.4 / 21.4. Around the borders, 104 and 370 tiles on 148 SMs, the last round decides and either wins by up to 5 %: 1024 x 3328 x 2048 (104)
+// 12.6 / 13.1, 900 x 3400 x 1100 (108) 12.2 / 11.5, 1000 tokens by 4 of 16 experts of 1500 x 768 (372) 23.3 / 24.4, 2000 x 6000 x 1024 (376) 19.0 /
+// 18.6, 2304 x 5504 x 768 (387) 17.2 / 17.6.
 bool pairs_pay(const Int8Matmul& p, int tmax, int sms) {
   const int64_t tiles = most_tiles(p, kMaxT, kRows);
   return tmax >= 128 && 10 * tiles >= (p.K > 1024 ? 7 : 25) * sms;
