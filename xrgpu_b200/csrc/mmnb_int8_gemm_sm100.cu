@@ -15,10 +15,10 @@
 // Roles (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 drain (lane quadrant warp % 4, alternate 16-column chunks).
 // Few tiles: K is split over a cluster of up to 8 CTAs whose int32 partial tiles meet in shared memory.
 //
-// Measured (GPU time of the call, weights from memory): 1 x 4096 x 4096 float rows 7.2 us (16.8 MB, 2.3 TB/s: latency), 16 x 4096 x
-// 14336 16.2 us with the rows' quantisation (59 MB, 3.6 TB/s: start and end, then the stream), one token by 8 of 64 experts of
+// Measured (GPU time of the call, weights from memory): 1 x 4096 x 4096 float rows 7.4 us (16.8 MB, 2.3 TB/s: latency), 16 x 4096 x
+// 14336 16.3 us with the rows' quantisation (59 MB, 3.6 TB/s: start and end, then the stream), one token by 8 of 64 experts of
 // 4096 x 4096 26.4 us (134 MB, 5.1 TB/s), 64 tokens by 64 experts of 4096 x 2048 with their sums 89.5 us (540 MB, 6.0 TB/s), 2048 x
-// 14336 x 4096 85.6 us (2.8 PFLOP/s; tensor cores 78 % of the cycles, at 1.4 GHz under the power limit from the first launch on;
+// 14336 x 4096 86.5 us (2.8 PFLOP/s; tensor cores 78 % of the cycles, at 1.4 GHz under the power limit from the first launch on;
 // 99.6 us in calls back to back for seconds), 8192 x 8192 x 8192 372 us, 428 us for seconds (2.6 PFLOP/s at 1.24 GHz).
 //
 // Every wait is bounded as in mmnb_gemm_sm100.cu.

@@ -5,8 +5,8 @@
 // score, then the index counted down, and the largest of the warp is taken out top_k times, from lanes that hold their best four
 // sorted. That is exact for float16 (16 bits); for float32 two neighbours of the result that agree in the 22 bits, and a lane
 // whose four were all taken while it has more, send the token to the exact form (whole keys, then the lowest index among equals).
-// What bounds it is instructions, about 14 a choice (50 with whole keys), and where tokens are few the latency of its steps. Four
-// held instead of all: 8192 x 256 16.4 -> 15.5 us, 2000 x 1024 27.9 -> 24.8.
+// What bounds it is the latency of a token's chain of choices, about 14 instructions each (50 with whole keys): 1.3 instructions a cycle
+// of 4, with 32 warps an SM. Four held instead of all: 8192 x 256 16.4 -> 15.5 us, 2000 x 1024 27.9 -> 24.8.
 // Weights: exp(s - s_max) over their sum, or over the sum of all experts'.
 // Order: a counting sort. Every warp counts its own tokens' experts, the counts are summed over the warps and CTAs before it, and
 // each warp writes its assignments in turn from there: no atomics, so the order is always the same. Few tokens: the CTAs of one
