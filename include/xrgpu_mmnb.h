@@ -581,7 +581,7 @@ typedef struct {
 } xrgpu_int8_tensor;
 
 /* x [rows, ldx] (ldx 0: K) -> t->codes, t->scales: s = max|x| / 127 in float32, code = x / s rounded to nearest, ties
- * to even. A row of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and codes 0. */
+ * to even, at most 127 in magnitude (where s is subnormal, x / s may be more). A row of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and codes 0. */
 XRGPU_API int xrgpu_int8_quantize(const xrgpu_int8_tensor* t, const void* x, int64_t ldx, void* stream);
 
 /* The values t holds -> out [rows, K] (contiguous, t->dtype). */

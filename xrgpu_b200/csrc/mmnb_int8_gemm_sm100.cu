@@ -574,7 +574,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // one tile a cluster: every rank sums its share of the columns over the ranks (128 values of a column lie together)
     cluster_sync();
     if (first < tiles && !*ctl.abort) sum_ranks<F16, SWIGLU>(a, t, base, rank, scales, ch);
-    __syncwarp();  // lanes come from there one by one, the barrier takes whole warps
     cluster_sync();  // nobody leaves while its partial tile is being read
   }
   zero_rest<F16>(a, fit, SWIGLU ? a.n / 2 : a.n);
@@ -1046,7 +1045,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && abort_flag) st_cluster_u32(map_rank(smem_u32(&abort_flag), rank ^ 1), 1);
-  __syncwarp();
   cluster_sync();  // neither CTA's memory goes while the other may read or signal it
   if (*ctl.abort) {
     // A wait ran out in one of them: tensor copies may be under way. A stage's last fill is awaited (its phase may lack the
@@ -1058,7 +1056,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (n > 0) drain_wait(&full[s], (n - 1) & 1, a.err, kErrDrain);
       }
     }
-    __syncwarp();
     cluster_sync();
   }
   if (warp == 1) {

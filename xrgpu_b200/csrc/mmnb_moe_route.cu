@@ -261,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 1) choose_kernel(const Args a) {
   int total = count, before = 0;
   if (a.ctas > 1) {
     counts[e] = count;
-    __syncwarp();  // lanes without an expert come first, the barrier takes whole warps
     cluster_sync();
     total = 0;
     int c[kClusterCtas];

@@ -231,8 +231,10 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_de
       : "memory");
 }
 
-// Cluster barrier over all threads of all CTAs (release / acquire of shared memory).
+// Cluster barrier over all threads of all CTAs (release / acquire of shared memory). Its instructions take whole warps, whose lanes may
+// come one by one.
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

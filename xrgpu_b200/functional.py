@@ -651,7 +651,7 @@ def int8_quantize(x: torch.Tensor):
     """x [..., K] (float32 or float16; rows may be strided) as 8-bit codes with one scale a row: (codes, scales).
 
     codes int8 [..., K] (rows laid out on 16-byte boundaries, as ``matmul_int8`` takes them), scales float32 [...]: scale =
-    max|row| / 127, code = x / scale rounded to nearest, ties to even. A row of zeros has scale 0; the scale of one that holds a NaN
+    max|row| / 127, code = x / scale rounded to nearest, ties to even, within +-127. A row of zeros has scale 0; the scale of one that holds a NaN
     or an infinity is NaN, its codes are 0. Weights [N, K] become codes with a scale for each channel by the same call.
     """
     dtype = _float_code(x.dtype)
